@@ -132,6 +132,15 @@ SIGNATURES: dict[str, tuple] = {
     "gfxinfer_qwen38_launch_gdn_recurrent_decode_block": (I32, [P] * 13 + [U32, P]),
     "gfxinfer_qwen38_launch_gdn_recurrent_decode": (I32, [P] * 10),
     "gfxinfer_launch_argmax": (I32, [P, P, SZ, P]),
+    "gfxinfer_kv_pages_workspace_bytes": (SZ, [P]),
+    "gfxinfer_launch_kv_pages_reset": (I32, [P, P]),
+    "gfxinfer_launch_kv_pages_fork": (I32, [P, U32, P, U32, P]),
+    "gfxinfer_launch_kv_pages_reserve": (I32, [P, P, U32, U32, P, P, SZ, P]),
+    "gfxinfer_launch_kv_pages_append": (I32, [P, U32, P, P, P, U32, U32, P]),
+    "gfxinfer_launch_kv_pages_advance": (I32, [P, P, U32, U32, P, P]),
+    "gfxinfer_launch_kv_pages_free": (I32, [P, P, P, U32, P]),
+    "gfxinfer_launch_kv_pages_copy": (I32, [P, P, P, U32, P]),
+    "gfxinfer_launch_kv_pages_compact": (I32, [P, P, P, SZ, P]),
     # include/gfxinfer_runtime.h
     "gfxinfer_model_spec_qwen38_27b": (None, [P]),
     "gfxinfer_model_spec_qwen38_reference": (None, [P]),
@@ -331,6 +340,92 @@ def launch_row_gather_tiled_batch(fmt, w, ws, out, host_rows, first_row, rest_ro
 
 def launch_row_gather_tiled_indirect(fmt, w, ws, out, row_ptr, rows, columns, stream=None):
     check(lib().gfxinfer_launch_lowbit_row_gather_tiled_indirect(fmt, _p(w), _p(ws), _p(out), _p(row_ptr), rows, columns, _stream(stream)))
+
+
+# ---- pages of a K/V cache ------------------------------------------------------
+
+class KvPages(ctypes.Structure):
+    """gfxinfer_kv_pages.  `of` describes tensors (fp16 pools, int32 state) and keeps them alive."""
+    _fields_ = [("key_pages", P), ("value_pages", P), ("page_table", P), ("lengths", P), ("references", P),
+                ("layers", U32), ("page_count", U32), ("page_tokens", U32), ("kv_heads", U32), ("head_size", U32),
+                ("sequences", U32), ("table_stride", U32)]
+
+    @classmethod
+    def of(cls, key_pages, value_pages, page_table, lengths, references):
+        """key_pages, value_pages [layers, pages, page_tokens, kv_heads, head_size]; page_table
+        [sequences, pages per sequence]; lengths [sequences]; references [pages].  All contiguous."""
+        tensors = (key_pages, value_pages, page_table, lengths, references)
+        layers, pages, page_tokens, kv_heads, head_size = key_pages.shape
+        sequences, stride = page_table.shape
+        if (tuple(value_pages.shape) != tuple(key_pages.shape) or tuple(lengths.shape) != (sequences,)
+                or tuple(references.shape) != (pages,) or not all(t.is_contiguous() for t in tensors)
+                or any(t.element_size() != size for t, size in zip(tensors, (2, 2, 4, 4, 4)))):
+            raise ValueError("K/V pages: pools of one shape in 16 bits, 32-bit state, all contiguous")
+        self = cls(*(_p(t) for t in tensors), layers, pages, page_tokens, kv_heads, head_size, sequences, stride)
+        self.tensors = tensors
+        return self
+
+
+def _bytes(workspace) -> int:
+    return 0 if workspace is None else workspace.numel() * workspace.element_size()
+
+
+def _host_ids(values):
+    """A host list of uint32 (None stays None); a ctypes array is passed as it is."""
+    if values is None or isinstance(values, ctypes.Array):
+        return values
+    return (U32 * len(values))(*values)
+
+
+def kv_pages_workspace_bytes(pages) -> int:
+    return int(lib().gfxinfer_kv_pages_workspace_bytes(ctypes.byref(pages)))
+
+
+def launch_kv_pages_reset(pages, stream=None):
+    check(lib().gfxinfer_launch_kv_pages_reset(ctypes.byref(pages), _stream(stream)))
+
+
+def launch_kv_pages_fork(pages, parent, children, stream=None):
+    ids = _host_ids(children)
+    check(lib().gfxinfer_launch_kv_pages_fork(ctypes.byref(pages), parent, ids, len(ids), _stream(stream)))
+
+
+def launch_kv_pages_reserve(pages, sequences, tokens, status, workspace, stream=None):
+    ids = _host_ids(sequences)
+    check(lib().gfxinfer_launch_kv_pages_reserve(ctypes.byref(pages), ids, len(ids), tokens, _p(status), _p(workspace),
+                                                 _bytes(workspace), _stream(stream)))
+
+
+def launch_kv_pages_append(pages, layer, key, value, sequences, tokens, stream=None):
+    ids = _host_ids(sequences)
+    check(lib().gfxinfer_launch_kv_pages_append(ctypes.byref(pages), layer, _p(key), _p(value), ids, len(ids), tokens,
+                                                _stream(stream)))
+
+
+def launch_kv_pages_advance(pages, sequences, tokens, token_counts=None, stream=None):
+    """token_counts: device uint32 per listed sequence, or None for `tokens` each."""
+    ids = _host_ids(sequences)
+    check(lib().gfxinfer_launch_kv_pages_advance(ctypes.byref(pages), ids, len(ids), tokens, _p(token_counts),
+                                                 _stream(stream)))
+
+
+def launch_kv_pages_free(pages, sequences, keep_tokens=None, stream=None):
+    ids, keep = _host_ids(sequences), _host_ids(keep_tokens)
+    if keep is not None and len(keep) != len(ids):
+        raise ValueError("one length to keep per sequence")
+    check(lib().gfxinfer_launch_kv_pages_free(ctypes.byref(pages), ids, keep, len(ids), _stream(stream)))
+
+
+def launch_kv_pages_copy(pages, sources, destinations, stream=None):
+    a, b = _host_ids(sources), _host_ids(destinations)
+    if len(a) != len(b):
+        raise ValueError("as many destinations as sources")
+    check(lib().gfxinfer_launch_kv_pages_copy(ctypes.byref(pages), a, b, len(a), _stream(stream)))
+
+
+def launch_kv_pages_compact(pages, live_pages, workspace, stream=None):
+    check(lib().gfxinfer_launch_kv_pages_compact(ctypes.byref(pages), _p(live_pages), _p(workspace), _bytes(workspace),
+                                                 _stream(stream)))
 
 
 # ---- host-side layout (numpy) -------------------------------------------------

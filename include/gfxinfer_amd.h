@@ -598,6 +598,88 @@ size_t gfxinfer_rope_table_bytes(size_t positions, size_t rotary_size);
 int32_t gfxinfer_launch_rope_table(float* table, size_t positions, size_t rotary_size, float rope_theta,
                                    void* stream);
 
+/* ---- pages of a K/V cache: sequences that share prefixes --------------------------------
+ * No reference counterpart (the reference decodes one sequence from one contiguous cache).
+ * A pool of pages holds the K and V rows of many sequences, all layers of a position under
+ * one page number; a sequence is a row of the page table and a length.  Sequences forked
+ * from one parent name the same pages until one of them needs room in a shared page.
+ *
+ * A page is free exactly when references[page] is 0; allocation takes the lowest free
+ * pages first, so the state after a call is the same on every run.  The calls of one cache
+ * run in stream order: two of them at the same time on different streams race.  Lists of
+ * sequences are host memory, read at call time (1..512 entries; a captured call replays
+ * with the list it was recorded with); lengths and tables stay on the device, so a decode
+ * step can be captured into a graph.  A table entry that names no page of the pool is
+ * treated as a missing one: nothing is read or written there. */
+typedef struct gfxinfer_kv_pages {
+  uint16_t* key_pages;   /* fp16 [layers][page_count][page_tokens][kv_heads][head_size], 16-byte aligned */
+  uint16_t* value_pages; /* the same */
+  int32_t* page_table;   /* [sequences][table_stride], -1 past a sequence's pages */
+  uint32_t* lengths;     /* [sequences]: committed tokens */
+  uint32_t* references;  /* [page_count]: table entries that name the page; 16-byte aligned */
+  uint32_t layers;
+  uint32_t page_count;   /* at most 2^24 */
+  uint32_t page_tokens;  /* a power of two, 16..4096 */
+  uint32_t kv_heads;
+  uint32_t head_size;    /* 128 or 256 */
+  uint32_t sequences;    /* at most 65536 */
+  uint32_t table_stride; /* pages per sequence; table_stride * page_tokens at most 2^31 */
+} gfxinfer_kv_pages;
+
+/* Bytes of device workspace (16-byte aligned) that reserve and compact need; 0 for an
+ * invalid description.  Its contents need not be kept between calls. */
+size_t gfxinfer_kv_pages_workspace_bytes(const gfxinfer_kv_pages* pages);
+
+/* Every page free, every sequence empty (the pools are left as they are). */
+int32_t gfxinfer_launch_kv_pages_reset(const gfxinfer_kv_pages* pages, void* stream);
+
+/* children[0..count) (host, distinct, none of them the parent) give back what they hold and
+ * become copies of the parent's committed tokens: same pages, same length.  No K/V row
+ * moves; rows the parent appended past its length stay the parent's. */
+int32_t gfxinfer_launch_kv_pages_fork(const gfxinfer_kv_pages* pages, uint32_t parent, const uint32_t* children,
+                                      uint32_t count, void* stream);
+
+/* Makes room for `tokens` (1..2^24) more tokens of each listed sequence (distinct; NULL:
+ * 0..count-1): new pages for positions the sequence has no page for, and a private copy of
+ * a partly filled last page that other sequences hold too (its committed rows, all layers;
+ * where all holders are in the list the last of them keeps the page).  Pages are taken
+ * lowest first, sequence by sequence in list order, a copy before new pages.  *status
+ * (device) = 0, or 1 when the pool or a table row is too small: then nothing changed. */
+int32_t gfxinfer_launch_kv_pages_reserve(const gfxinfer_kv_pages* pages, const uint32_t* sequences, uint32_t count,
+                                         uint32_t tokens, int32_t* status, void* workspace, size_t workspace_bytes,
+                                         void* stream);
+
+/* gfxinfer_launch_kv_append_block for pages: K (fp16) and V (fp32 -> fp16) rows
+ * [count][tokens][kv_heads * head_size] (16-byte aligned) of one layer at positions length +
+ * 0..tokens-1 of each listed sequence (distinct; NULL: 0..count-1).  Positions no page was
+ * reserved for are skipped; lengths stay as they are. */
+int32_t gfxinfer_launch_kv_pages_append(const gfxinfer_kv_pages* pages, uint32_t layer, const uint16_t* key,
+                                        const float* value, const uint32_t* sequences, uint32_t count,
+                                        uint32_t tokens, void* stream);
+
+/* Commits appended tokens: length += tokens, or += min(token_counts[i], tokens) for the
+ * i-th listed sequence when token_counts (device, the accepted tokens of a verify block) is
+ * not NULL.  A length never passes table_stride * page_tokens. */
+int32_t gfxinfer_launch_kv_pages_advance(const gfxinfer_kv_pages* pages, const uint32_t* sequences, uint32_t count,
+                                         uint32_t tokens, const uint32_t* token_counts, void* stream);
+
+/* Cuts each listed sequence (distinct; NULL: 0..count-1) to its first keep_tokens[i] tokens
+ * (host; NULL: none) and gives back the pages past them. */
+int32_t gfxinfer_launch_kv_pages_free(const gfxinfer_kv_pages* pages, const uint32_t* sequences,
+                                      const uint32_t* keep_tokens, uint32_t count, void* stream);
+
+/* Copies whole pages, all layers, K and V: sources[i] to destinations[i] (host, 1..256
+ * pairs; a destination occurs once and is no source).  Tables and references stay as they
+ * are: for a caller that keeps its own tables. */
+int32_t gfxinfer_launch_kv_pages_copy(const gfxinfer_kv_pages* pages, const uint32_t* sources,
+                                      const uint32_t* destinations, uint32_t count, void* stream);
+
+/* Moves the used pages into [0, live) (live = their number; used pages at or past live go,
+ * in order, to the free pages before it, in order) and renames them in every table entry.
+ * live_pages (device) may be NULL. */
+int32_t gfxinfer_launch_kv_pages_compact(const gfxinfer_kv_pages* pages, uint32_t* live_pages, void* workspace,
+                                         size_t workspace_bytes, void* stream);
+
 /* ---- single-token launchers: the one-token calls of greedy_step and the MTP proposal ---
  * Each is its block launcher at batch 1 (same kernels, bit-identical results). */
 
