@@ -141,6 +141,8 @@ SIGNATURES: dict[str, tuple] = {
     "gfxinfer_launch_kv_pages_free": (I32, [P, P, P, U32, P]),
     "gfxinfer_launch_kv_pages_copy": (I32, [P, P, P, U32, P]),
     "gfxinfer_launch_kv_pages_compact": (I32, [P, P, P, SZ, P]),
+    "gfxinfer_logit_rules_workspace_bytes": (SZ, [SZ, U32]),
+    "gfxinfer_launch_logit_rules": (I32, [P, SZ, SZ, U32, P, P, SZ, P, P, SZ, P]),
     # include/gfxinfer_runtime.h
     "gfxinfer_model_spec_qwen38_27b": (None, [P]),
     "gfxinfer_model_spec_qwen38_reference": (None, [P]),
@@ -426,6 +428,60 @@ def launch_kv_pages_copy(pages, sources, destinations, stream=None):
 def launch_kv_pages_compact(pages, live_pages, workspace, stream=None):
     check(lib().gfxinfer_launch_kv_pages_compact(ctypes.byref(pages), _p(live_pages), _p(workspace), _bytes(workspace),
                                                  _stream(stream)))
+
+
+# ---- rules on logits -------------------------------------------------------------
+
+class LogitRules(ctypes.Structure):
+    """gfxinfer_logit_rules.  `of` describes tensors and keeps them alive."""
+    _fields_ = [(n, P) for n in ("history", "history_rows", "history_lengths", "prompt_lengths", "repetition", "presence",
+                                 "frequency", "bias_tokens", "bias_values", "bias_counts", "allowed", "allowed_rows")]
+    _fields_ += [(n, U32) for n in ("history_row_count", "history_stride", "bias_stride", "allowed_row_count",
+                                    "allowed_stride")]
+
+    @classmethod
+    def of(cls, **tensors):
+        """Contiguous 32-bit tensors by the names of the fields: history [rows, tokens], bias_tokens and
+        bias_values [batch, entries], allowed [masks, words], the others [batch]."""
+        self = cls()
+        wide = ("history", "bias_tokens", "bias_values", "allowed")
+        for name, t in tensors.items():
+            if name not in dict(cls._fields_[:12]):
+                raise TypeError(f"no logit rule is called {name}")
+            if t is None:
+                continue
+            if not t.is_contiguous() or t.element_size() != 4 or t.dim() != (2 if name in wide else 1):
+                raise ValueError(f"logit rules: {name} is a contiguous 32-bit {'matrix' if name in wide else 'vector'}")
+            setattr(self, name, _p(t))
+        shape = lambda name: tuple(tensors[name].shape) if tensors.get(name) is not None else (0, 0)  # noqa: E731
+        if shape("bias_tokens") != shape("bias_values"):
+            raise ValueError("logit rules: as many bias values as tokens")
+        (self.history_row_count, self.history_stride), self.bias_stride = shape("history"), shape("bias_tokens")[1]
+        self.allowed_row_count, self.allowed_stride = shape("allowed")
+        vectors = {tuple(t.shape)[0] for n, t in tensors.items() if t is not None and n not in wide}
+        vectors |= {shape("bias_tokens")[0]} - {0}
+        if len(vectors) > 1:
+            raise ValueError("logit rules: one entry per row of the logits")
+        self.batch = next(iter(vectors), None)
+        self.tensors = tensors
+        return self
+
+
+def logit_rules_workspace_bytes(vocabulary, batch) -> int:
+    return int(lib().gfxinfer_logit_rules_workspace_bytes(vocabulary, batch))
+
+
+def launch_logit_rules(logits, rules, output, tokens, workspace, vocabulary=None, stream=None):
+    """logits, output: fp32 [batch, columns] (the last dimension dense); output, tokens and workspace may be None."""
+    batch, columns = logits.shape
+    if rules.batch not in (None, batch):
+        raise ValueError("logit rules: made for another number of rows")
+    for t in (logits,) if output is None else (logits, output):
+        if t.stride(1) != 1 or t.element_size() != 4 or t.shape[0] != batch:
+            raise ValueError("logit rules: logits are fp32 [batch, columns] with dense rows")
+    check(lib().gfxinfer_launch_logit_rules(_p(logits), logits.stride(0), columns if vocabulary is None else vocabulary, batch,
+                                            ctypes.byref(rules), _p(output), 0 if output is None else output.stride(0),
+                                            _p(tokens), _p(workspace), _bytes(workspace), _stream(stream)))
 
 
 # ---- host-side layout (numpy) -------------------------------------------------

@@ -680,6 +680,51 @@ int32_t gfxinfer_launch_kv_pages_copy(const gfxinfer_kv_pages* pages, const uint
 int32_t gfxinfer_launch_kv_pages_compact(const gfxinfer_kv_pages* pages, uint32_t* live_pages, void* workspace,
                                          size_t workspace_bytes, void* stream);
 
+/* ---- rules on logits -------------------------------------------------------------------
+ * No reference counterpart (the reference picks the plain argmax).  For row b and token v of
+ * fp32 logits, with c = how often v occurs among the row's generated tokens and r = whether
+ * it occurs among its prompt or generated tokens:
+ *     x = r ? (x > 0 ? x / repetition[b] : x * repetition[b]) : x
+ *     x = x - frequency[b] * c, then x - presence[b] if c > 0
+ *     x = x + bias value of the row's last entry that names v, if any
+ *     x = v allowed ? x : -inf
+ * A NULL member leaves its rule out.  Tokens of a list that are no token of the vocabulary
+ * are passed over.  All pointers are device memory; the struct itself is host memory read
+ * at call time. */
+typedef struct gfxinfer_logit_rules {
+  const uint32_t* history;         /* [history_row_count][history_stride] token ids, prompt first */
+  const int32_t* history_rows;     /* [batch]: the history row of a logits row (several may share one, as the
+                                      rows of a verify block do), none if outside; NULL: row b */
+  const uint32_t* history_lengths; /* [batch]: tokens of the row that count, needed with history */
+  const uint32_t* prompt_lengths;  /* [batch]: how many of them are the prompt's; NULL: 0 */
+  const float* repetition;         /* [batch]; NULL: 1 */
+  const float* presence;           /* [batch]; NULL: 0 */
+  const float* frequency;          /* [batch]; NULL: 0 */
+  const uint32_t* bias_tokens;     /* [batch][bias_stride] */
+  const float* bias_values;        /* [batch][bias_stride] */
+  const uint32_t* bias_counts;     /* [batch]; NULL: bias_stride each */
+  const uint32_t* allowed;         /* [allowed_row_count][allowed_stride] words, bit v % 32 of word v / 32 */
+  const int32_t* allowed_rows;     /* [batch]: the mask of a logits row, none if outside; NULL: row b */
+  uint32_t history_row_count;
+  uint32_t history_stride;         /* at most 524287 */
+  uint32_t bias_stride;            /* at most 4095 */
+  uint32_t allowed_row_count;
+  uint32_t allowed_stride;         /* at least vocabulary_size / 32, rounded up */
+} gfxinfer_logit_rules;
+
+/* Bytes of device workspace (8-byte aligned) the greedy pick needs; 0 for invalid sizes. */
+size_t gfxinfer_logit_rules_workspace_bytes(size_t vocabulary_size, uint32_t batch);
+
+/* Applies the rules to logits [batch][row_stride], of which the first vocabulary_size of a
+ * row count.  output [batch][output_stride] receives the result (it may be the logits
+ * themselves, with the same stride; otherwise the two must not overlap), tokens [batch] the
+ * lowest index of each row's largest value as gfxinfer_launch_argmax_batch finds it (NaN and
+ * -inf never win; 0 when nothing wins).  Either may be NULL; without tokens no workspace is
+ * needed.  Columns of the output past vocabulary_size are left as they are. */
+int32_t gfxinfer_launch_logit_rules(const float* logits, size_t row_stride, size_t vocabulary_size, uint32_t batch,
+                                    const gfxinfer_logit_rules* rules, float* output, size_t output_stride,
+                                    uint32_t* tokens, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- single-token launchers: the one-token calls of greedy_step and the MTP proposal ---
  * Each is its block launcher at batch 1 (same kernels, bit-identical results). */
 
