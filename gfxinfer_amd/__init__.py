@@ -141,6 +141,8 @@ SIGNATURES: dict[str, tuple] = {
     "gfxinfer_launch_kv_pages_free": (I32, [P, P, P, U32, P]),
     "gfxinfer_launch_kv_pages_copy": (I32, [P, P, P, U32, P]),
     "gfxinfer_launch_kv_pages_compact": (I32, [P, P, P, SZ, P]),
+    "gfxinfer_kv_pages_attention_workspace_bytes": (SZ, [P, U32, U32, U32, SZ]),
+    "gfxinfer_launch_kv_pages_gated_attention": (I32, [P, U32, P, P, P, P, U32, U32, U32, SZ, P, SZ, P]),
     "gfxinfer_logit_rules_workspace_bytes": (SZ, [SZ, U32]),
     "gfxinfer_launch_logit_rules": (I32, [P, SZ, SZ, U32, P, P, SZ, P, P, SZ, P]),
     # include/gfxinfer_runtime.h
@@ -428,6 +430,19 @@ def launch_kv_pages_copy(pages, sources, destinations, stream=None):
 def launch_kv_pages_compact(pages, live_pages, workspace, stream=None):
     check(lib().gfxinfer_launch_kv_pages_compact(ctypes.byref(pages), _p(live_pages), _p(workspace), _bytes(workspace),
                                                  _stream(stream)))
+
+
+def kv_pages_attention_workspace_bytes(pages, count, tokens, q_heads, shared_tokens) -> int:
+    return int(lib().gfxinfer_kv_pages_attention_workspace_bytes(ctypes.byref(pages), count, tokens, q_heads, shared_tokens))
+
+
+def launch_kv_pages_gated_attention(pages, layer, query, gate, output, sequences, tokens, q_heads, shared_tokens, workspace,
+                                    stream=None):
+    """gate may be None."""
+    ids = _host_ids(sequences)
+    check(lib().gfxinfer_launch_kv_pages_gated_attention(ctypes.byref(pages), layer, _p(query), _p(gate), _p(output), ids,
+                                                         len(ids), tokens, q_heads, shared_tokens, _p(workspace),
+                                                         _bytes(workspace), _stream(stream)))
 
 
 # ---- rules on logits -------------------------------------------------------------

@@ -680,6 +680,30 @@ int32_t gfxinfer_launch_kv_pages_copy(const gfxinfer_kv_pages* pages, const uint
 int32_t gfxinfer_launch_kv_pages_compact(const gfxinfer_kv_pages* pages, uint32_t* live_pages, void* workspace,
                                          size_t workspace_bytes, void* stream);
 
+/* Bytes of device workspace (16-byte aligned) of gfxinfer_launch_kv_pages_gated_attention; 0
+ * for invalid arguments. */
+size_t gfxinfer_kv_pages_attention_workspace_bytes(const gfxinfer_kv_pages* pages, uint32_t count, uint32_t tokens,
+                                                   uint32_t q_heads, size_t shared_tokens);
+
+/* gfxinfer_launch_gated_attention_decode_block for a batch over pages: token t of the i-th
+ * listed sequence (NULL: 0..count-1; one may be listed several times) attends to its first
+ * length + t + 1 positions (the block's own rows are appended, not yet committed).
+ * query fp16 [count][tokens][q_heads][hd] (16-byte aligned); gate fp32
+ * [count][tokens][q_heads][2 hd], its second half per head row used, or NULL for no gate;
+ * output fp16 [count][tokens][q_heads][hd]; tokens 1..32, q_heads a multiple of the cache's
+ * KV heads.
+ *
+ * shared_tokens: the first positions, at most the shortest length, that hold the same rows
+ * for every listed sequence (their fork point, or 0).  They are read once, through the first
+ * listed sequence's table, for the rows of all.  The result does not depend on it but for
+ * the order of fp32 additions.
+ *
+ * A position without a page is not seen; a row that sees nothing becomes zeros. */
+int32_t gfxinfer_launch_kv_pages_gated_attention(const gfxinfer_kv_pages* pages, uint32_t layer, const uint16_t* query,
+                                                 const float* gate, uint16_t* output, const uint32_t* sequences,
+                                                 uint32_t count, uint32_t tokens, uint32_t q_heads, size_t shared_tokens,
+                                                 float* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- rules on logits -------------------------------------------------------------------
  * No reference counterpart (the reference picks the plain argmax).  For row b and token v of
  * fp32 logits, with c = how often v occurs among the row's generated tokens and r = whether

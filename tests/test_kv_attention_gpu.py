@@ -1,0 +1,286 @@
+"""Paged attention with a shared prefix on the GPU against the definition in 64 bits.
+
+Tolerance.  u = 2^-24 is half a step of fp32.  A score is a sum of D products accumulated in fp32: off by at most
+D u |q|.|k| / sqrt(D), and scaling, the difference to the maximum and the exponential add a few u of the score and of the
+weight.  A weight is therefore off by e = 2 (D + 8) u max(|q|.|k|) / sqrt(D) + 2^-21 relatively (twice: against the maximum
+too; 2^-21 covers the exponential and the fp16 pair that carries a weight), numerator and denominator both.  A wave sums
+at most a quarter of the positions, in at most two additions each, and the merges add a few dozen more: (n / 2 + 64) u.
+The sum of both, times the weighted mean of |v| and the gate, is added to the half step of the fp16 result (2^-11
+relatively, 2^-25 below the normal numbers).
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+from gpu_util import dev, host, say
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+class Problem:
+    """Two layers of pages in no order; what no sequence sees is NaN: rows past the ends, free pages, layer 0."""
+
+    def __init__(self, rng, q_heads, kv_heads, d, page, lengths, tokens, shared, gate=True, slack=3, spread=1.0):
+        self.heads, self.page, self.lengths, self.tokens, self.shared = (q_heads, kv_heads, d), page, lengths, tokens, shared
+        n = len(lengths)
+        held = [-(-(x + tokens) // page) for x in lengths]
+        common = shared // page
+        pages = common + sum(h - common for h in held) + slack
+        order = rng.permutation(pages).tolist()
+        self.k, self.v = (np.full((2, pages, page, kv_heads, d), np.nan, np.float16) for _ in range(2))
+        self.table = np.full((n + 1, max(held) + 1), -1, np.int32)
+        self.references = np.zeros(pages, np.int32)
+        prefix = [rng.standard_normal((shared, kv_heads, d)).astype(np.float16) * spread for _ in range(2)]
+        self.rows = []
+        at = common
+        for i, h in enumerate(held):
+            mine = order[:common] + order[at:at + h - common]
+            at += h - common
+            self.table[i, :h] = mine
+            self.references[mine] += 1
+            own = [rng.standard_normal((lengths[i] + tokens - shared, kv_heads, d)).astype(np.float16) * spread for _ in range(2)]
+            kv = [np.concatenate([a, b]).astype(np.float16) for a, b in zip(prefix, own)]
+            self.rows.append(kv)
+            for pool, x in zip((self.k, self.v), kv):
+                for j in range(0, len(x), page):
+                    pool[1, mine[j // page], :len(x[j:j + page])] = x[j:j + page]
+        self.query = rng.standard_normal((n, tokens, q_heads, d)).astype(np.float16)
+        self.gate = (rng.standard_normal((n, tokens, q_heads, 2 * d)) * 2).astype(np.float32) if gate else None
+        if gate:
+            self.gate[..., :d] = np.nan                       # the query half of the projection is not read
+
+    def put(self, i, position, k=None, v=None):
+        """Overwrites rows of one position of one sequence, in its page and in the reference."""
+        for pool, rows, x in ((self.k, self.rows[i][0], k), (self.v, self.rows[i][1], v)):
+            if x is not None:
+                rows[position] = x
+                pool[1, self.table[i, position // self.page], position % self.page] = x
+
+    def run(self, gx, listed=None, shared=None, stream=None):
+        import torch
+        q_heads, kv_heads, d = self.heads
+        listed = list(range(len(self.lengths))) if listed is None else listed
+        shared = self.shared if shared is None else shared
+        keep = [dev(x) for x in (self.k, self.v, self.table, np.array(self.lengths + [0], np.int32), self.references)]
+        pages = gx.KvPages.of(*keep)
+        query = dev(self.query[listed])
+        gate = dev(self.gate[listed]) if self.gate is not None else None
+        out = torch.full((len(listed) + 1, self.tokens, q_heads, d), 7.0, dtype=torch.float16, device="cuda")
+        work = torch.full((gx.kv_pages_attention_workspace_bytes(pages, len(listed), self.tokens, q_heads, shared),), 0xff,
+                          dtype=torch.uint8, device="cuda")
+        gx.launch_kv_pages_gated_attention(pages, 1, query, gate, out, listed, self.tokens, q_heads, shared, work, stream=stream)
+        got = host(out)
+        assert np.all(got[-1] == 7.0)                         # rows behind the last sequence stay
+        return got[:-1]
+
+    def expect(self, i):
+        """(result, tolerance) of sequence i, [tokens, q_heads, d]."""
+        q_heads, kv_heads, d = self.heads
+        group = q_heads // kv_heads
+        k, v = (x.astype(np.float64) for x in self.rows[i])
+        want, tol = np.zeros((self.tokens, q_heads, d)), np.zeros((self.tokens, q_heads, d))
+        for t in range(self.tokens):
+            n = self.lengths[i] + t + 1
+            for h in range(q_heads):
+                q, kk, vv = self.query[i, t, h].astype(np.float64), k[:n, h // group], v[:n, h // group]
+                s = kk @ q / math.sqrt(d)
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                e = 2 * (d + 8) * U * (np.abs(kk) @ np.abs(q)).max() / math.sqrt(d) + 2.0 ** -21
+                g = 1 / (1 + np.exp(-self.gate[i, t, h, d:].astype(np.float64))) if self.gate is not None else 1.0
+                want[t, h] = w @ vv * g
+                tol[t, h] = (2 * e + (n / 2 + 64) * U) * (w @ np.abs(vv)) * g
+        return want, tol + np.maximum(np.abs(want) * 2.0 ** -11, 2.0 ** -25) * (1 + 2.0 ** -10)
+
+    def check(self, got, listed=None):
+        for at, i in enumerate(range(len(self.lengths)) if listed is None else listed):
+            want, tol = self.expect(i)
+            assert np.all(np.abs(got[at].astype(np.float64) - want) <= tol), (i, float(np.max(np.abs(got[at] - want) / tol)))
+
+
+A, B = (40, 8, 128), (24, 4, 256)
+
+
+@pytest.mark.parametrize("heads,page,lengths,tokens,shared", [
+    ((1, 1, 128), 16, [0], 1, 0),                             # one position: the token itself
+    ((1, 1, 256), 16, [0, 1, 2], 1, 0),
+    ((2, 1, 128), 16, [0, 15, 16, 17, 31, 32, 33], 1, 0),
+    ((6, 2, 128), 32, [16, 16, 40], 1, 16),                   # the prefix is all that some have
+    ((16, 1, 128), 16, [100, 130], 1, 96),                    # 16 rows a sequence: full tiles
+    ((17, 1, 128), 64, [100, 130], 1, 65),                    # 17: one row in the second tile
+    (A, 16, [509, 512, 530, 600], 1, 509),
+    (A, 64, [700] * 3 + [1500, 701], 5, 700),
+    (A, 128, [300, 290, 333], 32, 289),                       # a full block of 32 tokens, two tiles of rows and more
+    (A, 16, [77], 9, 0),
+    (A, 256, [2100] * 14, 1, 2048),
+    (B, 16, [509, 512, 530, 600], 1, 500),
+    (B, 32, [200, 300, 201], 5, 200),
+    (B, 64, [129, 257], 32, 100),
+    (B, 4096, [5000, 4990], 2, 4987),                         # pages longer than a split
+    ((8, 8, 128), 16, list(range(40, 73)), 1, 40),            # no grouping, 33 sequences
+    ((24, 3, 256), 16, list(range(1, 20)), 3, 0),
+])
+@pytest.mark.parametrize("gate", [True, False])
+def test_attention_equals_the_definition(device, gx, heads, page, lengths, tokens, shared, gate):
+    rng = np.random.default_rng(len(lengths) * 1000 + page + shared)
+    p = Problem(rng, *heads, page, lengths, tokens, shared, gate)
+    say("paged attention", heads, page, lengths[:6], tokens, shared, gate)
+    p.check(p.run(gx))
+
+
+@pytest.mark.parametrize("heads", [A, B])
+def test_prefix_length_only_changes_the_order_of_sums(device, gx, heads):
+    rng = np.random.default_rng(3)
+    p = Problem(rng, *heads, 32, [400, 431, 500], 2, 400)
+    say("prefix lengths", heads)
+    for shared in (0, 1, 31, 200, 399, 400):
+        p.check(p.run(gx, shared=shared))
+
+
+def test_listed_sequences_in_any_order_and_twice(device, gx):
+    rng = np.random.default_rng(4)
+    p = Problem(rng, *A, 16, [64, 80, 70, 99], 1, 64)
+    say("listed sequences")
+    for listed in ([3, 0], [2, 2, 1], [1]):
+        p.check(p.run(gx, listed=listed), listed)
+
+
+def test_large_scores_and_late_maxima(device, gx):
+    """Scores of some hundreds, growing along the context: the running maximum moves in every block."""
+    rng = np.random.default_rng(5)
+    p = Problem(rng, *A, 16, [300, 310], 1, 256, spread=4.0)
+    for i in range(2):
+        for at in range(256, p.lengths[i] + 1):
+            p.put(i, at, k=(p.rows[i][0][at] * np.float16(1 + (at - 256) / 32)))
+    say("large scores")
+    p.check(p.run(gx))
+
+
+def test_strange_values_stay_where_they_are_seen(device, gx):
+    """Infinities and NaN in positions of later tokens of a block do not reach earlier ones; visible ones do."""
+    rng = np.random.default_rng(6)
+    for heads in (A, B):
+        p = Problem(rng, *heads, 16, [40, 75], 4, 32)
+        kv_heads, d = heads[1], heads[2]
+        p.check(p.run(gx))
+        bad = rng.standard_normal((kv_heads, d)).astype(np.float16)
+        bad[0, 3], bad[1, 5], bad[2, 0] = np.inf, np.nan, -np.inf
+        p.put(0, 42, v=bad)                                   # token 2 of sequence 0 sees it first
+        p.put(1, 78, k=np.full((kv_heads, d), np.nan, np.float16))   # token 3 of sequence 1
+        say("strange values", heads)
+        got = p.run(gx)
+        group = heads[0] // kv_heads
+        touched = np.zeros(got.shape, bool)
+        for head, dim in ((0, 3), (1, 5), (2, 0)):
+            touched[0, 2:, head * group:(head + 1) * group, dim] = True
+        touched[1, 3] = True
+        assert np.array_equal(np.isfinite(got), ~touched)
+        assert np.all(got[0, 2:, :group, 3] == np.inf) and np.all(got[0, 2:, 2 * group:3 * group, 0] == -np.inf)
+        # The rows that do not see them: the block's products are added one by one there and by 32s otherwise, two orders
+        # of the same sum, each within the tolerance of the definition.
+        p.rows = [[np.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0) for x in rows] for rows in p.rows]
+        for i, first in ((0, 2), (1, 3)):
+            want, tol = p.expect(i)
+            assert np.all(np.abs(got[i, :first].astype(np.float64) - want[:first]) <= tol[:first])
+
+
+def test_nan_queries_give_nan_and_missing_pages_zeros(device, gx):
+    rng = np.random.default_rng(7)
+    p = Problem(rng, *A, 16, [40, 50], 1, 0)
+    p.query[0, 0, 7] = np.nan
+    say("nan query")
+    got = p.run(gx)
+    assert np.all(np.isnan(got[0, 0, 7])) and np.isfinite(np.delete(got[0, 0], 7, 0)).all() and np.isfinite(got[1]).all()
+    p.query[0, 0, 7] = 0
+    p.table[0] = -1                                           # no page at all: nothing is seen
+    p.table[1, 2] = 10000                                     # one page outside the pool: its positions are not seen
+    got = p.run(gx)
+    assert np.all(got[0] == 0)
+    p.rows[1] = [np.concatenate([x[:32], x[48:]]) for x in p.rows[1]]
+    p.lengths = [40, 34]
+    want, tol = p.expect(1)
+    assert np.all(np.abs(got[1] - want) <= tol)
+
+
+def test_a_prefix_longer_than_a_sequence_is_masked(device, gx):
+    """shared_tokens past a length: the rows of the shorter sequence stop at their own end."""
+    rng = np.random.default_rng(8)
+    p = Problem(rng, *A, 32, [320, 320], 1, 320)
+    p.lengths = [320, 100]
+    p.rows[1] = [x[:101] for x in p.rows[1]]
+    say("short sequence")
+    p.check(p.run(gx))
+    p.lengths = [100, 320]                                    # and where the first is the short one
+    p.rows = [[x[:101] for x in p.rows[0]], [np.concatenate([p.rows[0][i][:320], p.k[1, p.table[1, 10], :1] if i == 0 else p.v[1, p.table[1, 10], :1]]) for i in range(2)]]
+    p.check(p.run(gx))
+
+
+def test_long_contexts_and_many_splits(device, gx):
+    rng = np.random.default_rng(9)
+    p = Problem(rng, 10, 2, 128, 64, [20000, 20050], 1, 15000)
+    say("long context")
+    p.check(p.run(gx))
+
+
+def test_pools_past_32_bit_offsets(device, gx):
+    """Pages whose rows lie more than 2^32 bytes and 2^32 elements into a pool."""
+    import torch
+    q_heads, kv_heads, d, page = 8, 8, 128, 4096
+    layers, pages = 2, 520                                    # 2 x 520 x 4096 x 1024 halves: 8.7 GB a pool
+    k, v = (torch.zeros((layers, pages, page, kv_heads, d), dtype=torch.float16, device="cuda") for _ in range(2))
+    rng = np.random.default_rng(10)
+    n = 5000
+    rows = [rng.standard_normal((n + 1, kv_heads, d)).astype(np.float16) for _ in range(2)]
+    table = np.array([[519, 517]], np.int32)
+    lengths = dev(np.array([0], np.int32))
+    references = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    t = dev(table)
+    cache = gx.KvPages.of(k, v, t, lengths, references)
+    say("32-bit offsets")
+    gx.launch_kv_pages_append(cache, 1, dev(rows[0][None]), dev(rows[1][None].astype(np.float32)), [0], n + 1)
+    gx.launch_kv_pages_advance(cache, [0], n)
+    p = Problem(rng, q_heads, kv_heads, d, page, [n], 1, 0)
+    p.rows = [rows]
+    query, gate = dev(p.query), dev(p.gate)
+    out = torch.zeros((1, 1, q_heads, d), dtype=torch.float16, device="cuda")
+    work = torch.zeros(gx.kv_pages_attention_workspace_bytes(cache, 1, 1, q_heads, 0), dtype=torch.uint8, device="cuda")
+    gx.launch_kv_pages_gated_attention(cache, 1, query, gate, out, [0], 1, q_heads, 0, work)
+    p.check(host(out))
+    assert float(k[0].abs().max()) == 0.0
+
+
+def test_results_repeat_and_replay(device, gx):
+    """The same bits on every call, on another stream and from a graph replayed as lengths grow."""
+    import torch
+    rng = np.random.default_rng(11)
+    q_heads, kv_heads, d = B
+    p = Problem(rng, *B, 16, [100, 120, 97], 3, 96)
+    say("repeat")
+    first = p.run(gx)
+    p.check(first)
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert np.array_equal(p.run(gx, stream=other).view(np.uint16), first.view(np.uint16))
+    lengths = dev(np.array([96, 96, 96, 0], np.int32))
+    keep = [dev(x) for x in (p.k, p.v, p.table)]
+    cache = gx.KvPages.of(*keep, lengths, dev(p.references))
+    query, gate = dev(p.query), dev(p.gate)
+    out = torch.zeros((3, 3, q_heads, d), dtype=torch.float16, device="cuda")
+    work = torch.zeros(gx.kv_pages_attention_workspace_bytes(cache, 3, 3, q_heads, 96), dtype=torch.uint8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        gx.launch_kv_pages_gated_attention(cache, 1, query, gate, out, [0, 1, 2], 3, q_heads, 96, work)
+    goal = [100, 120, 97]
+    full = p.rows
+    for turn in range(4):
+        p.lengths = [96 + (g - 96) * turn // 3 for g in goal]
+        p.rows = [[x[:n + 3] for x in rows] for rows, n in zip(full, p.lengths)]
+        lengths.copy_(dev(np.array(p.lengths + [0], np.int32)))
+        graph.replay()
+        p.check(host(out))
+    assert np.array_equal(host(out).view(np.uint16), first.view(np.uint16))
