@@ -9,14 +9,21 @@
 // Each writes (maximum, sum, unnormalized output) and a second launch merges a row's items
 // and applies the gate.
 //
-// Inside an item the four waves take every fourth block of 32 positions and merge at the end:
-// a wave meets each K and V row once, for all the rows of the tile, and no barrier stands
-// in its loop.  Scores are computed transposed, S^T = K Q^T, so that a lane holds one
-// row's scores: the running maximum takes two lane exchanges, the sum none, and the
-// weights are already the B operand of O^T = V^T P^T when the positions of a block are
-// numbered as the score tiles leave them (k slot 8 b + e is position 4 b + e of the first
-// tile for e < 4 and 4 b + e - 4 of the second otherwise).  K comes from memory as the A
-// operand; V goes through LDS, whose transposing reads turn rows of V into columns.
+// Scores are computed transposed, S^T = K Q^T, so that a lane holds one row's scores: the
+// running maximum takes two lane exchanges, the sum none, and the weights are already the
+// B operand of O^T = V^T P^T when the positions of a block are numbered as the score tiles
+// leave them (k slot 8 b + e is position 4 b + e of the first tile for e < 4 and 4 b + e - 4
+// of the second otherwise).  V passes through LDS, whose transposing reads turn rows of V
+// into columns.
+//
+// Two ways to share an item among the waves of a workgroup:
+//  - few rows (attend_positions): the waves take turns at blocks of 32 positions and merge at
+//    the end.  K goes from memory straight into the A operand; no barrier stands in the loop.
+//  - many rows (attend_rows): each wave takes 16 of up to 128 rows, and a K / V row staged in
+//    LDS serves them all.
+// Both load into LDS directly, without registers.  By rows, a wave of head size 128 fits 128
+// registers and two workgroups a CU, and their four waves a SIMD fill each other's waits;
+// the two ways are two kernels, so that the other one's registers do not count.
 #include <algorithm>
 #include <cmath>
 
@@ -29,13 +36,19 @@ using h8 = _Float16 __attribute__((ext_vector_type(8)));
 using f4 = float __attribute__((ext_vector_type(4)));
 using u32x4 = unsigned __attribute__((ext_vector_type(4)));
 using s16x4 = short __attribute__((ext_vector_type(4)));
-using s16x8 = short __attribute__((ext_vector_type(8)));
 using lds_s16x4 = __attribute__((address_space(3))) s16x4;
+using lds_void = __attribute__((address_space(3))) void;
+using global_void = __attribute__((address_space(1))) void;
 
-constexpr unsigned kWaves = 4;
-constexpr unsigned kBlock = 32;           // positions of one step of a wave
-constexpr unsigned kMinBlocks = 2 * kWaves;  // blocks a split is worth at least
+constexpr unsigned kBlock = 32;  // positions of one step of a wave
 constexpr float kLog2E = 1.4426950408889634F;
+
+constexpr unsigned kWaves = 8;     // by rows: 128 rows
+constexpr unsigned kPosWaves = 4;  // by positions: small workgroups, of which more fill the GPU
+// Waves per SIMD a kernel is built for.
+constexpr unsigned resident(unsigned head_size, bool by_rows) { return head_size == 256 ? 2u : by_rows ? 4u : 3u; }
+// Blocks a split is worth at least.
+constexpr uint32_t kMinBlocks = 8;
 
 struct PagedAttnArgs {
   KvPages pages;
@@ -62,7 +75,7 @@ __device__ __forceinline__ uint32_t splits_used(uint32_t blocks, uint32_t splits
 }
 // Positions the batch's prefix covers: what the first sequence has of them.
 __device__ __forceinline__ uint32_t prefix_length(const PagedAttnArgs& a) {
-  return min(a.shared, a.pages.lengths[a.list.slot[0]]);
+  return min(a.shared, a.pages.lengths[listed_slot(a.list, 0)]);
 }
 // A sequence's own positions run from the tile of 16 that holds the prefix's end.
 __device__ __forceinline__ uint32_t own_blocks(uint32_t shared, uint32_t end) {
@@ -78,350 +91,634 @@ __device__ __forceinline__ void unspread(uint32_t id, uint32_t tiles, uint32_t& 
   range = eighth / tiles * 8 + id % 8;
 }
 
+// Over the four lanes (one per 16-lane row) that hold a row's scores.
 __device__ __forceinline__ float max_over_quarters(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  const unsigned u = __float_as_uint(v);
+  const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const unsigned w = __float_as_uint(fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1])));
+  const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 __device__ __forceinline__ float sum_over_quarters(float v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
 }
 
-template <unsigned D>
-constexpr unsigned kPitch = D + 16;  // halves per V row in LDS: rows of a transposing read fall on different banks
-
-template <unsigned D, unsigned NQ>
-constexpr std::size_t shared_bytes() {
-  const std::size_t values = kWaves * kBlock * kPitch<D> * 2;
-  const std::size_t merge = (kWaves - 1) * (D / 64) * NQ * 64 * 16 + kWaves * 16 * NQ * 8;
-  return values > merge ? values : merge;
+// Waits until at most Loads of the wave's loads from memory are on their way, and for all of
+// its LDS accesses.
+template <unsigned Loads>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(Loads < 64);
+  __builtin_amdgcn_s_waitcnt((Loads & 15u) | (Loads >> 4) << 14 | 7u << 4);
+  asm volatile("" ::: "memory");
 }
 
-// One work item: rows first .. first + 16 NQ - 1 (of `rows`; row = (i * tokens + t) * group + g
-// with i counted from `base`), KV head hk, positions [lo, hi) in blocks first_block ..
-// last_block - 1 from position `start`, pages of sequence `slot`, result into split `split`.
-template <unsigned D, unsigned NQ>
-__device__ __forceinline__ void attend(const PagedAttnArgs& a, uint32_t base, uint32_t first, uint32_t rows, uint32_t hk,
-                                       uint32_t slot, uint32_t start, uint32_t first_block, uint32_t last_block,
-                                       uint32_t lo, uint32_t hi, uint32_t split, char* smem) {
-  constexpr unsigned kSteps = D / 32;       // K-steps of the scores
-  constexpr unsigned kTiles = D / 16;       // output tiles of 16 dims
-  constexpr unsigned kLoads = kBlock * D / 8 / 64;  // 16-byte pieces of a block's V rows per lane
-  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned n = lane & 15u, kb = lane >> 4;
-  const uint32_t group = a.q_heads / a.kv_heads;
-  const KvPages& pg = a.pages;
-  const uint32_t in_page = (1u << pg.page_shift) - 1;
+// K and V rows in LDS have no padding (loads into LDS fill it lane after lane); instead the
+// 16-byte pieces of a row are permuted, by the address each lane loads from: piece c of K row
+// r lies in slot c ^ (r % 16), of V row r in slot c ^ 2 (r % 8).  The rows of a score operand
+// and of a transposing read then fall on different banks.
+__device__ __forceinline__ unsigned key_slot(unsigned piece, unsigned row) { return piece ^ (row & 15u); }
+__device__ __forceinline__ unsigned value_slot(unsigned piece, unsigned row) { return piece ^ 2 * (row & 7u); }
 
-  // The lane's row of each row tile: its query as B operand, and the positions it sees.
-  h8 q[NQ][kSteps];
-  uint32_t visible[NQ], out_row[NQ];
-  uint32_t least = 0xffffffffu;
+// The A operands of output tiles first .. first + 3 (dims 16 first ..) of 32 V rows at
+// `rows`, complete when it returns.  The compiler would let the reads wait for every load into
+// LDS that is on its way, since it cannot tell the places apart; the callers have waited for
+// these rows, so the reads are written out with their own wait.
+template <unsigned D>
+__device__ __forceinline__ void read_values(const _Float16* rows, unsigned lane, unsigned first, h8 (&v)[4]) {
+  const unsigned n = lane & 15u, row = 4 * (lane >> 4) + (n >> 2);
+  unsigned at[4];
 #pragma unroll
-  for (unsigned j = 0; j < NQ; ++j) {
-    const uint32_t row = first + 16 * j + n;
-    visible[j] = 0;
-    out_row[j] = 0xffffffffu;
+  for (unsigned u = 0; u < 4; ++u) {
+    const _Float16* p = rows + row * D + 8 * value_slot(2 * (first + u) + ((n & 3u) >> 1), row) + 4 * (n & 1u);
+    at[u] = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)(p)));
+  }
+  s16x4 a[8];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(a[4]), "=&v"(a[5]), "=&v"(a[6]), "=&v"(a[7])
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(16 * D * 2)
+      : "memory");
 #pragma unroll
-    for (unsigned s = 0; s < kSteps; ++s) q[j][s] = h8{};
+  for (unsigned u = 0; u < 4; ++u) {
+    v[u] = __builtin_bit_cast(h8, __builtin_shufflevector(a[2 * u], a[2 * u + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+
+// The lane's number, made anew: what is computed from it inside a loop is not kept in
+// registers around the loop, where 128 of them do not suffice.
+__device__ __forceinline__ unsigned fresh_lane() {
+  unsigned lane = threadIdx.x & 63u;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+// Sixteen rows of a wave: lane column n's row is the query q (B operand), sees the positions
+// below `visible`, and its result goes to row out_row (none: 0xffffffff).
+template <unsigned D>
+struct Rows {
+  h8 q[D / 32];
+  uint32_t visible, out_row;
+  uint32_t least;  // of visible over the rows
+  f4 o[D / 16];
+  float m, l;  // m in units of log2; l of the lane's own positions
+
+  // Rows first + n of `rows`; row = (i * tokens + t) * group + g, i counted from `base`.  Own:
+  // the rows are one sequence's, with hi - tokens committed positions.
+  template <bool Own>
+  __device__ __forceinline__ void load(const PagedAttnArgs& a, uint32_t base, uint32_t first, uint32_t rows, uint32_t hk,
+                                       uint32_t hi) {
+    const unsigned lane = threadIdx.x & 63u, kb = lane >> 4;
+    const uint32_t group = a.q_heads / a.kv_heads, row = first + (lane & 15u);
+    visible = 0;
+    out_row = 0xffffffffu;
+#pragma unroll
+    for (unsigned s = 0; s < D / 32; ++s) q[s] = h8{};
     if (row < rows) {
-      const uint32_t it = row / group, g = row - it * group, i = it / a.tokens, t = it - i * a.tokens;
-      out_row[j] = ((base + i) * a.tokens + t) * a.q_heads + hk * group + g;
-      visible[j] = min(pg.lengths[a.list.slot[base + i]] + t + 1, hi);
-      const __half* src = a.query + static_cast<std::size_t>(out_row[j]) * D + 8 * kb;
+      const uint32_t it = row / group, g = row - it * group, i = Own ? 0u : it / a.tokens, t = it - i * a.tokens;
+      out_row = ((base + i) * a.tokens + t) * a.q_heads + hk * group + g;
+      const __half* src = a.query + static_cast<std::size_t>(out_row) * D + 8 * kb;
 #pragma unroll
-      for (unsigned s = 0; s < kSteps; ++s) q[j][s] = *reinterpret_cast<const h8*>(src + 32 * s);
-      least = min(least, visible[j]);
+      for (unsigned s = 0; s < D / 32; ++s) q[s] = *reinterpret_cast<const h8*>(src + 32 * s);
+      visible = Own ? hi - a.tokens + t + 1 : min(a.pages.lengths[a.list.slot[base + i]] + t + 1, hi);
+    }
+    // Own: the first row sees least.  Prefix: every row sees all of it unless the caller's
+    // prefix is longer than a sequence, and then every block is treated as an edge.
+    if (Own) least = first < rows ? hi - a.tokens + first / group + 1 : 0xffffffffu;
+    else least = __all(row >= rows || visible == hi) ? hi : 0u;
+  }
+
+  // The queries have arrived here: a wait for them inside a loop would wait for the loop's
+  // own loads too.
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (unsigned s = 0; s < D / 32; ++s) asm volatile("" : "+v"(q[s]));
+  }
+
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.0F;
+#pragma unroll
+    for (unsigned d = 0; d < D / 16; ++d) o[d] = f4{0, 0, 0, 0};
+  }
+
+  // Whether an output is an infinity or NaN: weights are below 2^8, so only such values (or
+  // NaN scores) can make one.
+  __device__ __forceinline__ bool strange() const {
+    bool found = false;
+#pragma unroll
+    for (unsigned d = 0; d < D / 16; ++d) {
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) found |= !(fabsf(o[d][e]) < INFINITY);
+    }
+    return found;
+  }
+
+  // The weights of a block of 32 positions from `at`: s the scores (raw products), the weights
+  // afterwards.  An edge block holds positions that some row does not see (below lo, past its
+  // end, or in a tile of 16 whose page is missing: bit t of `missing`).
+  //
+  // The weights go out as an fp16 pair p = high + low, high cut off and low the rest: two
+  // products carry about 22 bits of p, so the output keeps the accuracy of an fp32 product.
+  __device__ __forceinline__ void weigh(f4 (&s)[2], unsigned lane, float scale, bool edge, uint32_t at, uint32_t lo,
+                                        unsigned missing, h8& high, h8& low) {
+    if (edge) {
+      const unsigned kb = lane >> 4;
+#pragma unroll
+      for (unsigned t = 0; t < 2; ++t) {
+#pragma unroll
+        for (unsigned r = 0; r < 4; ++r) {
+          const uint32_t position = at + 16 * t + 4 * kb + r;
+          if (position < lo || position >= visible || (missing >> t & 1u) != 0) s[t][r] = -INFINITY;
+        }
+      }
+    }
+    float best = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (unsigned r = 1; r < 4; ++r) best = fmaxf(fmaxf(best, s[0][r]), s[1][r]);
+    const float top = max_over_quarters(best) * scale;
+    // The stored maximum moves only when a row's grows by more than 8 (a factor of 256):
+    // weights stay below 2^8 and most blocks skip the rescaling.
+    if (__any(top > m + 8.0F)) {
+      const float next_m = fmaxf(m, top);
+      const float factor = next_m == -INFINITY ? 1.0F : __builtin_amdgcn_exp2f(m - next_m);
+      m = next_m;
+      l *= factor;
+#pragma unroll
+      for (unsigned d = 0; d < D / 16; ++d) o[d] *= factor;
+    }
+    const float floor = m == -INFINITY ? 0.0F : m;
+#pragma unroll
+    for (unsigned t = 0; t < 2; ++t) {
+#pragma unroll
+      for (unsigned r = 0; r < 4; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][r], scale, -floor));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][r + 1], scale, -floor));
+        s[t][r] = p0;
+        s[t][r + 1] = p1;
+        l += p0;
+        l += p1;
+        const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+        high[4 * t + r] = h[0];
+        high[4 * t + r + 1] = h[1];
+        const auto rest = __builtin_amdgcn_cvt_pkrtz(p0 - static_cast<float>(h[0]), p1 - static_cast<float>(h[1]));
+        low[4 * t + r] = rest[0];
+        low[4 * t + r + 1] = rest[1];
+      }
     }
   }
-#pragma unroll
-  for (unsigned d = 1; d < 16; d <<= 1) least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), d)));
-  least = __builtin_amdgcn_readfirstlane(least);
 
-  const std::size_t plane = static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift;
-  const __half* keys = pg.key + plane * pg.row + hk * D;
-  const __half* values = pg.value + plane * pg.row + hk * D;
-  _Float16* vs = reinterpret_cast<_Float16*>(smem) + wave * kBlock * kPitch<D>;
+  // Output tiles first .. first + 3.
+  __device__ __forceinline__ void add(const h8 (&v)[4], unsigned first, const h8& high, const h8& low) {
+#pragma unroll
+    for (unsigned u = 0; u < 4; ++u) o[first + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[u], low, o[first + u], 0, 0, 0);
+#pragma unroll
+    for (unsigned u = 0; u < 4; ++u) o[first + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[u], high, o[first + u], 0, 0, 0);
+  }
+
+  // In a careful pass the infinities and NaNs among the values of a block are zeros in LDS,
+  // since a row must not meet those of positions it does not see; here the rows that see them
+  // get their products, one by one from the pages.  s: the weights of the block.
+  __device__ __forceinline__ void add_strange(const f4 (&s)[2], const KvPages& pages, const __half* values, uint32_t slot,
+                                              uint32_t at, uint32_t lo, uint32_t hi) {
+    const unsigned lane = threadIdx.x & 63u, n = lane & 15u, kb = lane >> 4;
+#pragma unroll 1
+    for (unsigned p = 0; p < kBlock; ++p) {
+      const uint32_t position = at + p;
+      const int32_t page = position < lo || position >= hi ? -1 : table_page(pages, slot, position >> pages.page_shift);
+      if (page < 0) continue;
+      const __half* row = values + ((static_cast<std::size_t>(page) << pages.page_shift) +
+                                    (position & ((1u << pages.page_shift) - 1))) * pages.row;
+      const unsigned owner = ((p % 16) / 4) * 16 + n;
+      float w = 0.0F;
+#pragma unroll
+      for (unsigned e = 0; e < 8; ++e) {
+        const float x = __shfl(s[e / 4][e % 4], owner);
+        if (e == p / 16 * 4 + p % 4) w = x;
+      }
+#pragma unroll
+      for (unsigned d = 0; d < D / 16; ++d) {
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) {
+          const float x = __half2float(row[16 * d + 4 * kb + e]);
+          if (!(fabsf(x) < INFINITY) && position < visible) o[d][e] += w * x;
+        }
+      }
+    }
+    // Nothing is on its way when the ordinary blocks go on.
+    wait_loads<0>();
+  }
+
+  // The row sums, complete; only NaN scores make a NaN row, not an empty one.
+  __device__ __forceinline__ void finish() {
+    l = sum_over_quarters(l);
+    if (l != l && m == -INFINITY) m = 0.0F;
+  }
+};
+
+// Eight values in LDS: infinities and NaNs become zeros.  Whether there were any.
+__device__ __forceinline__ bool take_strange(u32x4* at) {
+  u32x4 v = *at;
+  bool strange = false;
+#pragma unroll
+  for (unsigned e = 0; e < 4; ++e) {
+    const bool low = (v[e] & 0x7c00u) == 0x7c00u, high = (v[e] & 0x7c000000u) == 0x7c000000u;
+    strange |= low || high;
+    v[e] &= (low ? 0xffff0000u : 0xffffffffu) & (high ? 0xffffu : 0xffffffffu);
+  }
+  if (strange) *at = v;
+  return strange;
+}
+
+// A sequence's table row, 64 columns at a time in the lanes of a wave: a block's page is a
+// lane read, not a load on the way to the block's addresses.
+struct PageWindow {
+  uint32_t first;
+  int32_t entry;
+  __device__ __forceinline__ void start(const KvPages& pages, uint32_t slot, uint32_t column) {
+    first = column;
+    entry = table_page(pages, slot, column + (threadIdx.x & 63u));
+  }
+  __device__ __forceinline__ int32_t find(const KvPages& pages, uint32_t slot, uint32_t column) {
+    if (column - first >= 64u) start(pages, slot, column);  // uniform: columns only grow
+    return __builtin_amdgcn_readlane(entry, column - first);
+  }
+};
+
+// The K or V rows of a KV head of the launch's layer.
+__device__ __forceinline__ const __half* head_rows(const PagedAttnArgs& a, const __half* pool, uint32_t hk, unsigned d) {
+  return pool + (static_cast<std::size_t>(a.layer) * a.pages.page_count << a.pages.page_shift) * a.pages.row + hk * d;
+}
+
+// One work item: rows first .. (see Rows::load), KV head hk, positions [lo, hi) in blocks
+// first_block .. last_block - 1 from position `start` (a multiple of 16), pages of sequence
+// `slot`, result into split `split`.
+struct Item {
+  uint32_t base, first, rows, hk, slot, start, first_block, last_block, lo, hi, split;
+  bool own;
+};
+
+// Bytes of LDS: V blocks of the waves, later their outputs, then maxima and sums.
+template <unsigned D>
+constexpr std::size_t positions_bytes() {
+  return kPosWaves * kBlock * D * 2 + kPosWaves * 16 * 8;
+}
+
+// Sixteen rows; the waves divide the positions.
+template <unsigned D>
+__device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const Item& w, char* smem) {
+  constexpr unsigned kSteps = D / 32, kTiles = D / 16;
+  constexpr unsigned kLoads = kBlock * D / 8 / 64;   // of a block's V rows, per lane
+  constexpr unsigned kLoadRows = 64 / (D / 8);       // rows one of them covers
+  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned n = lane & 15u, kb = lane >> 4;
+  const KvPages& pg = a.pages;
+  const uint32_t in_page = (1u << pg.page_shift) - 1;
+  PageWindow window;
+  window.start(pg, w.slot, (w.start + min(w.first_block + wave, w.last_block - 1) * kBlock) >> pg.page_shift);
+  Rows<D> rows;
+  if (w.own) rows.template load<true>(a, w.base, w.first, w.rows, w.hk, w.hi);
+  else rows.template load<false>(a, w.base, w.first, w.rows, w.hk, w.hi);
+  const __half* keys = head_rows(a, pg.key, w.hk, D);
+  const __half* values = head_rows(a, pg.value, w.hk, D);
+  _Float16* vs = reinterpret_cast<_Float16*>(smem) + wave * kBlock * D;
+
+  // Where the lane's piece of a tile's K rows, and of the V rows of a load, lies.
+  const uint32_t key_part = n * pg.row + 8 * kb;
+  constexpr unsigned kParts = 8 / kLoadRows;
+  uint32_t value_part[kParts];
+#pragma unroll
+  for (unsigned u = 0; u < kParts; ++u) {
+    const unsigned r = kLoadRows * u + lane / (D / 8);
+    value_part[u] = r * pg.row + 8 * value_slot(lane % (D / 8), r);
+  }
 
   h8 kr[2][kSteps];
-  u32x4 vr[kLoads];
   int32_t page[2];
   auto find_pages = [&](uint32_t at, int32_t (&out)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (unsigned t = 0; t < 2; ++t) {
-      out[t] = at + 16 * t < hi ? table_page(pg, slot, (at + 16 * t) >> pg.page_shift) : -1;
-      out[t] = __builtin_amdgcn_readfirstlane(out[t]);
-    }
+    for (unsigned t = 0; t < 2; ++t) out[t] = at + 16 * t < w.hi ? window.find(pg, w.slot, (at + 16 * t) >> pg.page_shift) : -1;
   };
   // Missing tiles load page 0 of the pool (always there); their scores and values are masked.
+  auto tile_row = [&](uint32_t at, unsigned t, const int32_t (&p)[2]) __attribute__((always_inline)) {
+    return (static_cast<std::size_t>(max(p[t], 0)) << pg.page_shift) + ((at + 16 * t) & in_page);
+  };
   auto load_k = [&](uint32_t at, const int32_t (&p)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (unsigned t = 0; t < 2; ++t) {
-      const std::size_t row = (static_cast<std::size_t>(max(p[t], 0)) << pg.page_shift) + ((at + 16 * t + n) & in_page);
-      const __half* src = keys + row * pg.row + 8 * kb;
+      const __half* src = keys + tile_row(at, t, p) * pg.row;  // uniform; the lane's part is 32 bits
 #pragma unroll
-      for (unsigned s = 0; s < kSteps; ++s) kr[t][s] = *reinterpret_cast<const h8*>(src + 32 * s);
+      for (unsigned s = 0; s < kSteps; ++s) kr[t][s] = *reinterpret_cast<const h8*>(src + key_part + 32 * s);
     }
   };
   auto load_v = [&](uint32_t at, const int32_t (&p)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (unsigned u = 0; u < kLoads; ++u) {
-      const unsigned piece = lane + 64 * u, r = piece / (D / 8), c = piece % (D / 8);
-      const std::size_t row = (static_cast<std::size_t>(max(p[u / (kLoads / 2)], 0)) << pg.page_shift) + ((at + r) & in_page);
-      vr[u] = *reinterpret_cast<const u32x4*>(values + row * pg.row + 8 * c);
+      const unsigned t = u / (kLoads / 2), r8 = kLoadRows * (u % (kLoads / 2)) & ~7u;
+      const __half* src = values + (tile_row(at, t, p) + r8) * pg.row;
+      __builtin_amdgcn_global_load_lds((global_void*)(src + value_part[u % kParts]), (lds_void*)(vs + kLoadRows * u * D), 16, 0, 0);
     }
   };
 
-  f4 o[NQ][kTiles];
-  float m[NQ], l[NQ];
-#pragma unroll
-  for (unsigned j = 0; j < NQ; ++j) {
-    m[j] = -INFINITY;
-    l[j] = 0.0F;
-#pragma unroll
-    for (unsigned d = 0; d < kTiles; ++d) o[j][d] = f4{0, 0, 0, 0};
-  }
-
-  uint32_t block = first_block + wave;
-  if (block < last_block) {
-    find_pages(start + block * kBlock, page);
-    load_k(start + block * kBlock, page);
-    load_v(start + block * kBlock, page);
-  }
-  for (; block < last_block; block += kWaves) {
-    const uint32_t at = start + block * kBlock, next = at + kWaves * kBlock;
-    const bool more = block + kWaves < last_block;
-    int32_t next_page[2] = {-1, -1};
-    if (more) find_pages(next, next_page);
-    const bool edge = at < lo || at + kBlock > least || page[0] < 0 || page[1] < 0;
-    // Scores of 32 positions, the lane's row in the columns.
-    f4 s[NQ][2];
-#pragma unroll
-    for (unsigned j = 0; j < NQ; ++j) {
-#pragma unroll
-      for (unsigned t = 0; t < 2; ++t) s[j][t] = f4{0, 0, 0, 0};
+  // A second, careful pass follows in the rare case that an output of the first is an
+  // infinity or NaN: values are then looked at before they are used.
+  for (bool careful = false;; careful = true) {
+    rows.clear();
+    if (careful) window.first = 0xffffffc0u;  // 64 before column 0
+    uint32_t block = w.first_block + wave;
+    if (block < w.last_block) {
+      find_pages(w.start + block * kBlock, page);
+      load_k(w.start + block * kBlock, page);
+      load_v(w.start + block * kBlock, page);
     }
-#pragma unroll
-    for (unsigned st = 0; st < kSteps; ++st) {
-#pragma unroll
-      for (unsigned t = 0; t < 2; ++t) {
-#pragma unroll
-        for (unsigned j = 0; j < NQ; ++j) s[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kr[t][st], q[j][st], s[j][t], 0, 0, 0);
-      }
-    }
-    if (more) load_k(next, next_page);
-    // Values into LDS as they lie in memory; rows no one sees become zeros (what a page
-    // holds past a sequence's end may be anything, and 0 * NaN would be NaN).
-    bool strange = false;  // an infinity or NaN among the values of an edge block
-#pragma unroll
-    for (unsigned u = 0; u < kLoads; ++u) {
-      const unsigned piece = lane + 64 * u, r = piece / (D / 8), c = piece % (D / 8);
-      if (edge) {
-        if (at + r < lo || at + r >= hi || page[u / (kLoads / 2)] < 0) vr[u] = u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (unsigned e = 0; e < 4; ++e) {
-          strange |= (vr[u][e] & 0x7c00u) == 0x7c00u || (vr[u][e] & 0x7c000000u) == 0x7c000000u;
-        }
-      }
-      *reinterpret_cast<u32x4*>(vs + r * kPitch<D> + 8 * c) = vr[u];
-    }
-    if (more) load_v(next, next_page);
-    // Running maximum.  The stored maximum moves only when a row's grows by more than 8
-    // (a factor of 256): weights stay below 2^8 and most blocks skip the rescaling.
-    bool grown = false;
-    float top[NQ];
-#pragma unroll
-    for (unsigned j = 0; j < NQ; ++j) {
-      float best = -INFINITY;
-#pragma unroll
-      for (unsigned t = 0; t < 2; ++t) {
-#pragma unroll
-        for (unsigned r = 0; r < 4; ++r) {
-          float x = s[j][t][r] * a.scale;
-          if (edge) {
-            const uint32_t position = at + 16 * t + 4 * kb + r;
-            if (position < lo || position >= visible[j] || page[t] < 0) x = -INFINITY;
-          }
-          s[j][t][r] = x;
-          best = fmaxf(best, x);
-        }
-      }
-      top[j] = max_over_quarters(best);
-      grown |= top[j] > m[j] + 8.0F;
-    }
-    if (__any(grown)) {
-#pragma unroll
-      for (unsigned j = 0; j < NQ; ++j) {
-        const float next_m = fmaxf(m[j], top[j]);
-        const float factor = next_m == -INFINITY ? 1.0F : __builtin_amdgcn_exp2f(m[j] - next_m);
-        m[j] = next_m;
-        l[j] *= factor;
-#pragma unroll
-        for (unsigned d = 0; d < kTiles; ++d) o[j][d] *= factor;
-      }
-    }
-    // Weights as an fp16 pair p = hi + lo: two products carry about 22 bits of p, so the
-    // output keeps the accuracy of an fp32 product.
-    h8 hi_p[NQ], lo_p[NQ];
-#pragma unroll
-    for (unsigned j = 0; j < NQ; ++j) {
-      const float floor = m[j] == -INFINITY ? 0.0F : m[j];
-#pragma unroll
-      for (unsigned t = 0; t < 2; ++t) {
-#pragma unroll
-        for (unsigned r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f(s[j][t][r] - floor);
-          s[j][t][r] = p;
-          l[j] += p;
-          const _Float16 h = static_cast<_Float16>(p);
-          hi_p[j][4 * t + r] = h;
-          lo_p[j][4 * t + r] = static_cast<_Float16>(p - static_cast<float>(h));
-        }
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (edge && __any(strange)) {
-      // A row must not meet the infinities and NaNs of positions it does not see: products
-      // one by one, in fp32, for the positions it does.
+    rows.settle();
 #pragma unroll 1
-      for (unsigned p = 0; p < kBlock; ++p) {
-        const unsigned t = p / 16, owner = ((p % 16) / 4) * 16 + n, r = p % 4;
+    for (; block < w.last_block; block += kPosWaves) {
+      const uint32_t at = w.start + block * kBlock;
+      const unsigned fresh = fresh_lane();
+      const bool edge = at < w.lo || at + kBlock > rows.least || page[0] < 0 || page[1] < 0;
+      const unsigned missing = (page[0] < 0 ? 1u : 0u) | (page[1] < 0 ? 2u : 0u);
+      f4 s[2];
 #pragma unroll
-        for (unsigned j = 0; j < NQ; ++j) {
-          float w = 0.0F;
+      for (unsigned t = 0; t < 2; ++t) {
+        s[t] = f4{0, 0, 0, 0};
 #pragma unroll
-          for (unsigned e = 0; e < 8; ++e) {
-            const float v = __shfl(s[j][e / 4][e % 4], owner);
-            if (e == 4 * t + r) w = v;
-          }
-          const bool seen = at + p >= lo && at + p < visible[j];
-#pragma unroll
-          for (unsigned d = 0; d < kTiles; ++d) {
-#pragma unroll
-            for (unsigned e = 0; e < 4; ++e) {
-              const float v = static_cast<float>(vs[p * kPitch<D> + 16 * d + 4 * kb + e]);
-              if (seen) o[j][d][e] += w * v;
-            }
-          }
-        }
+        for (unsigned st = 0; st < kSteps; ++st) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kr[t][st], rows.q[st], s[t], 0, 0, 0);
       }
-    } else {
-#pragma unroll
-      for (unsigned d = 0; d < kTiles; ++d) {
-        const _Float16* src = vs + (4 * kb + (n >> 2)) * kPitch<D> + 16 * d + 4 * (n & 3u);
-        const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src));
-        const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + 16 * kPitch<D>));
-        const h8 v = __builtin_bit_cast(h8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (unsigned j = 0; j < NQ; ++j) {
-          o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo_p[j], o[j][d], 0, 0, 0);
-          o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi_p[j], o[j][d], 0, 0, 0);
-        }
+      const bool more = block + kPosWaves < w.last_block;
+      if (more) {
+        find_pages(at + kPosWaves * kBlock, page);
+        load_k(at + kPosWaves * kBlock, page);
       }
+      h8 high, low;
+      rows.weigh(s, fresh, a.scale, edge, at, w.lo, missing, high, low);
+      // The V rows are there when only the next K rows are on their way.
+      if (more) wait_loads<2 * kSteps>();
+      else wait_loads<0>();
+      bool strange = false;
+      if (edge || careful) {
+        // V rows no one sees become zeros (what a page holds past a sequence's end may be
+        // anything, and 0 * NaN would be NaN).
+#pragma unroll
+        for (unsigned u = 0; u < kLoads; ++u) {
+          const unsigned t = u / (kLoads / 2), r = kLoadRows * u + fresh / (D / 8);
+          u32x4* piece = reinterpret_cast<u32x4*>(vs + kLoadRows * u * D) + fresh;
+          if (at + r < w.lo || at + r >= w.hi || (missing >> t & 1u) != 0) *piece = u32x4{0, 0, 0, 0};
+          if (careful) strange |= take_strange(piece);
+        }
+        wait_loads<63>();
+        if (__any(strange)) rows.add_strange(s, pg, values, w.slot, at, w.lo, w.hi);
+      }
+#pragma unroll
+      for (unsigned d = 0; d < kTiles; d += 4) {
+        h8 v[4];
+        read_values<D>(vs, fresh, d, v);
+        rows.add(v, d, high, low);
+      }
+      if (more) load_v(at + kPosWaves * kBlock, page);
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    page[0] = next_page[0];
-    page[1] = next_page[1];
+    if (careful || !__syncthreads_or(rows.strange())) break;
   }
 
-  // Merge the four waves: a common maximum per row, then each wave sums one quarter of
-  // the output dims (a lane holds the same row and dims in every wave).
+  // Merge the waves (a lane holds the same row and dims in every wave): all maxima and
+  // outputs through LDS, then each wave sums its share of the output tiles in wave order.
   __syncthreads();  // the V rows are no longer needed
-  f4* quarter = reinterpret_cast<f4*>(smem);                                              // [3][D / 64 * NQ][64]
-  float2* ml = reinterpret_cast<float2*>(smem + (kWaves - 1) * (D / 64) * NQ * 64 * 16);  // [4][16 NQ]
+  f4* outputs = reinterpret_cast<f4*>(smem);                                 // [waves][D / 16][64]
+  float2* ml = reinterpret_cast<float2*>(smem + kPosWaves * kTiles * 64 * 16);  // [waves][16]
+  rows.finish();
+  if (kb == 0) ml[wave * 16 + n] = float2{rows.m, rows.l};
 #pragma unroll
-  for (unsigned j = 0; j < NQ; ++j) {
-    l[j] = sum_over_quarters(l[j]);
-    if (l[j] != l[j] && m[j] == -INFINITY) m[j] = 0.0F;  // only NaN scores: the row is NaN, not empty
-    if (kb == 0) ml[wave * 16 * NQ + 16 * j + n] = float2{m[j], l[j]};
-  }
+  for (unsigned d = 0; d < kTiles; ++d) outputs[(wave * kTiles + d) * 64 + lane] = rows.o[d];
   __syncthreads();
-  float best[NQ], total[NQ];
+  float best = -INFINITY, total = 0.0F, factor[kPosWaves];
 #pragma unroll
-  for (unsigned j = 0; j < NQ; ++j) {
-    best[j] = -INFINITY;
-    total[j] = 0.0F;
+  for (unsigned v = 0; v < kPosWaves; ++v) best = fmaxf(best, ml[v * 16 + n].x);
 #pragma unroll
-    for (unsigned w = 0; w < kWaves; ++w) best[j] = fmaxf(best[j], ml[w * 16 * NQ + 16 * j + n].x);
-#pragma unroll
-    for (unsigned w = 0; w < kWaves; ++w) {
-      const float2 v = ml[w * 16 * NQ + 16 * j + n];
-      if (v.x != -INFINITY) total[j] += v.y * __builtin_amdgcn_exp2f(v.x - best[j]);
-    }
-    const float factor = m[j] == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(m[j] - best[j]);
-#pragma unroll
-    for (unsigned d = 0; d < kTiles; ++d) {
-      if (m[j] != -INFINITY) o[j][d] *= factor;
-    }
+  for (unsigned v = 0; v < kPosWaves; ++v) {
+    const float2 x = ml[v * 16 + n];
+    factor[v] = x.x == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(x.x - best);
+    if (x.x != -INFINITY) total += x.y * factor[v];
   }
-  const uint32_t splits = a.prefix_splits + a.own_splits;
-  constexpr unsigned kQuarter = D / 64;
+  if (rows.out_row == 0xffffffffu) return;
+  const std::size_t at = static_cast<std::size_t>(rows.out_row) * (a.prefix_splits + a.own_splits) + w.split;
 #pragma unroll
-  for (unsigned c = 0; c < kWaves; ++c) {
-    if (wave != c) {
-      const unsigned place = wave < c ? wave : wave - 1;
+  for (unsigned u = 0; u < kTiles / kPosWaves; ++u) {
+    const unsigned d = wave * (kTiles / kPosWaves) + u;
+    f4 sum = {0, 0, 0, 0};
 #pragma unroll
-      for (unsigned d = 0; d < kQuarter; ++d) {
-#pragma unroll
-        for (unsigned j = 0; j < NQ; ++j) quarter[(place * kQuarter * NQ + d * NQ + j) * 64 + lane] = o[j][c * kQuarter + d];
-      }
+    for (unsigned v = 0; v < kPosWaves; ++v) {
+      const f4 x = outputs[(v * kTiles + d) * 64 + lane];
+      if (factor[v] != 0.0F) sum += x * factor[v];
     }
-    __syncthreads();
-    if (wave == c) {
-#pragma unroll
-      for (unsigned j = 0; j < NQ; ++j) {
-        if (out_row[j] != 0xffffffffu) {
-          const std::size_t at = static_cast<std::size_t>(out_row[j]) * splits + split;
-#pragma unroll
-          for (unsigned d = 0; d < kQuarter; ++d) {
-            f4 v = o[j][c * kQuarter + d];
-#pragma unroll
-            for (unsigned w = 0; w < kWaves - 1; ++w) v += quarter[(w * kQuarter * NQ + d * NQ + j) * 64 + lane];
-            *reinterpret_cast<f4*>(a.partial_o + at * D + 16 * (c * kQuarter + d) + 4 * kb) = v;
-          }
-          if (c == 0 && kb == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{best[j], total[j]};
-        }
-      }
-    }
-    __syncthreads();
+    *reinterpret_cast<f4*>(a.partial_o + at * D + 16 * d + 4 * kb) = sum;
   }
+  if (wave == 0 && kb == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{best, total};
 }
 
-template <unsigned D, unsigned NQP, unsigned NQS>
-__global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(PagedAttnArgs a) {
-  constexpr std::size_t kBytes = std::max(shared_bytes<D, NQP>(), shared_bytes<D, NQS>());
-  __shared__ __align__(16) char smem[kBytes];
-  const uint32_t shared = prefix_length(a);
+// Positions of a tile of attend_rows (16 KB of K and of V), and the tiles its LDS ring
+// holds: two workgroups a CU at head size 128, one at 256.
+template <unsigned D>
+constexpr unsigned kTile = D == 128 ? 64u : 32u;
+template <unsigned D>
+constexpr unsigned kRing = D == 128 ? 2u : 4u;
+
+template <unsigned D>
+constexpr std::size_t rows_bytes() {
+  return kRing<D> * (kTile<D> * D * 2 * 2 + 4 * kWaves);
+}
+
+// A barrier that orders LDS accesses and leaves loads from memory into LDS on their way
+// (__syncthreads would wait for them).
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Up to 128 rows, 16 a wave; each K / V row is loaded into LDS once for all of them, tiles
+// ahead, with one barrier a tile.
+template <unsigned D>
+__device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& w, char* smem) {
+  constexpr unsigned R = kRing<D>, T = kTile<D>;
+  constexpr unsigned kLoads = T * D / 8 / (kWaves * 64);  // of K, and of V, per tile and lane
+  constexpr unsigned kLoadRows = 64 / (D / 8);            // rows a load of a wave covers
+  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const KvPages& pg = a.pages;
+  const uint32_t in_page = (1u << pg.page_shift) - 1;
+  const __half* keys = head_rows(a, pg.key, w.hk, D);
+  const __half* values = head_rows(a, pg.value, w.hk, D);
+  _Float16* kring = reinterpret_cast<_Float16*>(smem);            // [ring][tile][D]
+  _Float16* vring = kring + R * T * D;                            // [ring][tile][D]
+  uint32_t* marks = reinterpret_cast<uint32_t*>(vring + R * T * D);  // [ring][waves]
+  const uint32_t begin = w.start + w.first_block * kBlock, last = w.start + w.last_block * kBlock;
+  const uint32_t end = min(last, w.hi);
+
+  PageWindow window;
+  window.start(pg, w.slot, begin >> pg.page_shift);
+  bool lost = false;  // a page was missing
+  // Load u of a wave covers rows kLoadRows * (wave + 8 u) .. of the tile, all of one part of
+  // 16 positions.  Parts without a page load from page 0 (always there) and are dealt with
+  // in the careful pass; tiles past the item are not asked for.
+  auto part_page = [&](unsigned u, uint32_t at) __attribute__((always_inline)) {
+    const uint32_t part = at + (kLoadRows * (wave + kWaves * u) & ~15u);
+    return part < end ? window.find(pg, w.slot, part >> pg.page_shift) : 0;
+  };
+  auto load = [&](unsigned slot, uint32_t at) __attribute__((always_inline)) {
+#pragma unroll
+    for (unsigned u = 0; u < kLoads; ++u) {
+      const unsigned row0 = kLoadRows * (wave + kWaves * u), r = (row0 & 15u) + lane / (D / 8), p = lane % (D / 8);
+      const int32_t page = part_page(u, at);
+      lost |= page < 0;
+      const std::size_t base = ((static_cast<std::size_t>(max(page, 0)) << pg.page_shift) + ((at + (row0 & ~15u)) & in_page)) * pg.row;
+      __builtin_amdgcn_global_load_lds((global_void*)(keys + base + (r * pg.row + 8 * key_slot(p, r))),
+                                       (lds_void*)(kring + (slot * T + row0) * D), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_void*)(values + base + (r * pg.row + 8 * value_slot(p, r))),
+                                       (lds_void*)(vring + (slot * T + row0) * D), 16, 0, 0);
+    }
+  };
+  // The wave's own pieces of a tile, once they have arrived: V rows no one sees become zeros
+  // (see attend_positions); a careful pass also takes out infinities and NaNs, and notes them
+  // (bit 8) and the missing parts (bit t) for all waves.
+  auto repair = [&](unsigned slot, uint32_t at, bool careful) __attribute__((always_inline)) {
+    const unsigned lane = fresh_lane();
+    uint32_t mark = 0;
+    bool strange = false;
+#pragma unroll
+    for (unsigned u = 0; u < kLoads; ++u) {
+      const unsigned row0 = kLoadRows * (wave + kWaves * u), r = row0 + lane / (D / 8);
+      bool gone = at + r < w.lo || at + r >= w.hi;
+      if (careful && part_page(u, at) < 0) {
+        gone = true;
+        mark |= 1u << (row0 / 16);
+      }
+      u32x4* piece = reinterpret_cast<u32x4*>(vring + (slot * T + row0) * D) + lane;
+      if (gone) *piece = u32x4{0, 0, 0, 0};
+      if (careful) strange |= take_strange(piece);
+    }
+    if (__any(strange)) mark |= 0x100u;
+    if (careful && lane == 0) marks[slot * kWaves + wave] = mark;
+  };
+
+  Rows<D> rows;
+  const uint32_t first = w.first + wave * 16;
+  if (w.own) rows.template load<true>(a, w.base, first, w.rows, w.hk, w.hi);
+  else rows.template load<false>(a, w.base, first, w.rows, w.hk, w.hi);
+  const bool works = first < w.rows;
+  // A second, careful pass follows in the rare case that an output of the first is an
+  // infinity or NaN, or a page was missing: values and pages are then looked at.
+  for (bool careful = false;; careful = true) {
+    rows.clear();
+    if (careful) window.first = 0xffffffc0u;  // 64 before column 0
+#pragma unroll
+    for (unsigned i = 0; i + 1 < R; ++i) {
+      if (begin + i * T < last) load(i, begin + i * T);
+    }
+    rows.settle();
+    unsigned slot = 0;
+#pragma unroll 1
+    for (uint32_t at = begin; at < last; at += T) {
+      // This tile has arrived when only the loads of the R - 2 after it are on their way.
+      if (at + (R - 2) * T < last) wait_loads<(R - 2) * 2 * kLoads>();
+      else wait_loads<0>();
+      if (careful || at < w.lo || at + T > w.hi) {
+        repair(slot, at, careful);
+        wait_loads<63>();
+      }
+      lds_barrier();
+      // Every wave is past the tile before this one: its slot takes the next loads.
+      if (at + (R - 1) * T < last) load((slot + R - 1) % R, at + (R - 1) * T);
+      if (works) {
+        uint32_t mark = 0;
+        if (careful) {
+          for (unsigned v = 0; v < kWaves; ++v) mark |= marks[slot * kWaves + v];
+          mark = __builtin_amdgcn_readfirstlane(mark);
+        }
+#pragma unroll 1
+        for (unsigned b = 0; b < T / kBlock; ++b) {
+          const uint32_t from = at + b * kBlock;
+          if (from >= last) break;
+          const unsigned fresh = fresh_lane(), n = fresh & 15u, kb = fresh >> 4;
+          const _Float16* ks = kring + (slot * T + b * kBlock + n) * D;
+          const _Float16* vs = vring + (slot * T + b * kBlock) * D;
+          f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll
+          for (unsigned st = 0; st < D / 32; ++st) {
+#pragma unroll
+            for (unsigned t = 0; t < 2; ++t) {
+              const h8 k = *reinterpret_cast<const h8*>(ks + 16 * t * D + 8 * key_slot(4 * st + kb, n));
+              s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, rows.q[st], s[t], 0, 0, 0);
+            }
+          }
+          const uint32_t gone = mark >> (2 * b) & 3u;
+          const bool edge = from < w.lo || from + kBlock > rows.least || gone != 0;
+          h8 high, low;
+          rows.weigh(s, fresh, a.scale, edge, from, w.lo, gone, high, low);
+          if ((mark & 0x100u) != 0) rows.add_strange(s, pg, values, w.slot, from, w.lo, w.hi);
+#pragma unroll
+          for (unsigned d = 0; d < D / 16; d += 4) {
+            h8 v[4];
+            read_values<D>(vs, fresh, d, v);
+            rows.add(v, d, high, low);
+          }
+        }
+      }
+      slot = (slot + 1) % R;
+    }
+    if (careful || !__syncthreads_or((works && rows.strange()) || lost)) break;
+  }
+  if (!works) return;
+  rows.finish();
+  if (rows.out_row == 0xffffffffu) return;
+  const std::size_t to = static_cast<std::size_t>(rows.out_row) * (a.prefix_splits + a.own_splits) + w.split;
+#pragma unroll
+  for (unsigned d = 0; d < D / 16; ++d) *reinterpret_cast<f4*>(a.partial_o + to * D + 16 * d + 4 * (lane >> 4)) = rows.o[d];
+  if (lane < 16) *reinterpret_cast<float2*>(a.partial_ml + 2 * to) = float2{rows.m, rows.l};
+}
+
+__host__ __device__ constexpr uint32_t tile_rows(bool by_rows) { return by_rows ? 128u : 16u; }
+
+// Work items from number `first` on, all shared among the waves the same way: the prefix's
+// come before the sequences' own.
+template <unsigned D, bool ByRows>
+__global__ __launch_bounds__((ByRows ? kWaves : kPosWaves) * 64, resident(D, ByRows)) void paged_attention_kernel(PagedAttnArgs a, uint32_t first) {
+  __shared__ __align__(16) char smem[ByRows ? rows_bytes<D>() : positions_bytes<D>()];
+  const uint32_t shared = prefix_length(a), id = first + blockIdx.x;
   const uint32_t group = a.q_heads / a.kv_heads, count = a.list.count;
   uint32_t range, tile;
-  if (blockIdx.x < a.prefix_groups) {
-    unspread(blockIdx.x, a.prefix_tiles, range, tile);
+  Item item;
+  if (id < a.prefix_groups) {
+    unspread(id, a.prefix_tiles, range, tile);
     const uint32_t split = range / a.kv_heads, hk = range - split * a.kv_heads;
     const uint32_t blocks = (shared + kBlock - 1) / kBlock, per = split_length(blocks, a.prefix_splits);
     const uint32_t from = split * per;
     if (split >= a.prefix_splits || from >= blocks) return;
-    const uint32_t to = min(from + per, blocks);
-    attend<D, NQP>(a, 0, tile * 16 * NQP, count * a.tokens * group, hk, a.list.slot[0], 0, from, to, 0, shared, split, smem);
-    return;
+    item = Item{0, tile * tile_rows(ByRows), count * a.tokens * group, hk, listed_slot(a.list, 0), 0, from,
+                min(from + per, blocks), 0, shared, split, false};
+  } else {
+    unspread(id - a.prefix_groups, a.own_tiles, range, tile);
+    const uint32_t hk = range % a.kv_heads, is = range / a.kv_heads, split = is / count, i = is - split * count;
+    if (split >= a.own_splits) return;
+    const uint32_t slot = listed_slot(a.list, i), end = a.pages.lengths[slot] + a.tokens;
+    const uint32_t blocks = own_blocks(shared, end), per = split_length(blocks, a.own_splits), from = split * per;
+    if (from >= blocks) return;
+    item = Item{i, tile * tile_rows(ByRows), a.tokens * group, hk, slot, shared & ~15u, from,
+                min(from + per, blocks), shared, end, a.prefix_splits + split, true};
   }
-  unspread(blockIdx.x - a.prefix_groups, a.own_tiles, range, tile);
-  const uint32_t hk = range % a.kv_heads, is = range / a.kv_heads, split = is / count, i = is - split * count;
-  if (split >= a.own_splits) return;
-  const uint32_t slot = a.list.slot[i], end = a.pages.lengths[slot] + a.tokens;
-  const uint32_t blocks = own_blocks(shared, end), per = split_length(blocks, a.own_splits), from = split * per;
-  if (from >= blocks) return;
-  const uint32_t to = min(from + per, blocks);
-  attend<D, NQS>(a, i, tile * 16 * NQS, a.tokens * group, hk, slot, shared & ~15u, from, to, shared, end,
-                 a.prefix_splits + split, smem);
+  if constexpr (ByRows) attend_rows<D>(a, item, smem);
+  else attend_positions<D>(a, item, smem);
 }
 
 // Merges a row's items and applies the gate: one wave per (row, 128 dims), two dims a lane.
+// Lane s holds item s's maximum and sum, so its weight is computed once; the outputs are
+// loaded kBatch at a time ahead of their use.
 template <unsigned D>
 __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
-  constexpr unsigned kGroups = D / 128;
-  const uint32_t linear = blockIdx.x * 4u + (threadIdx.x >> 6);
+  constexpr unsigned kGroups = D / 128, kBatch = 8;
+  const uint32_t linear = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t rows = a.list.count * a.tokens * a.q_heads;
   if (linear >= rows * kGroups) return;
   const unsigned lane = threadIdx.x & 63u;
@@ -430,22 +727,42 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
   const unsigned d = 128 * part + 2 * lane;
   float2 g = {0.0F, 0.0F};
   if (a.gate != nullptr) g = *reinterpret_cast<const float2*>(a.gate + static_cast<std::size_t>(row) * 2 * D + D + d);
-  const uint32_t shared = prefix_length(a), end = a.pages.lengths[a.list.slot[i]] + a.tokens;
+  const uint32_t shared = prefix_length(a), end = a.pages.lengths[listed_slot(a.list, i)] + a.tokens;
   const uint32_t prefix = a.prefix_splits != 0 ? splits_used((shared + kBlock - 1) / kBlock, a.prefix_splits) : 0u;
-  const uint32_t own = splits_used(own_blocks(shared, end), a.own_splits);
+  const uint32_t items = prefix + splits_used(own_blocks(shared, end), a.own_splits);
+  const uint32_t skipped = a.prefix_splits - prefix;  // unused between the prefix's items and the own ones
   const std::size_t first = static_cast<std::size_t>(row) * (a.prefix_splits + a.own_splits);
-  float best = -INFINITY;
-  auto at = [&](uint32_t s) { return first + (s < prefix ? s : a.prefix_splits + (s - prefix)); };
-  for (uint32_t s = 0; s < prefix + own; ++s) best = fmaxf(best, a.partial_ml[2 * at(s)]);
-  float total = 0.0F, o0 = 0.0F, o1 = 0.0F;
-  for (uint32_t s = 0; s < prefix + own; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.partial_ml + 2 * at(s));
-    if (ml.x == -INFINITY) continue;
-    const float w = __builtin_amdgcn_exp2f(ml.x - best);
-    const float2 v = *reinterpret_cast<const float2*>(a.partial_o + at(s) * D + d);
-    total = fmaf(ml.y, w, total);
-    o0 = fmaf(v.x, w, o0);
-    o1 = fmaf(v.y, w, o1);
+  const float* ml = a.partial_ml + 2 * first;
+  const float* outputs = a.partial_o + first * D + d;
+  float best = -INFINITY, total = 0.0F, o0 = 0.0F, o1 = 0.0F;
+  for (uint32_t from = 0; from < items; from += 64) {
+    const uint32_t s = from + lane;
+    const float2 x = s < items ? *reinterpret_cast<const float2*>(ml + 2 * (s < prefix ? s : s + skipped)) : float2{-INFINITY, 0.0F};
+    const float next = fmaxf(best, wave_max(x.x));
+    if (next == -INFINITY) continue;
+    const float keep = best == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(best - next);
+    best = next;
+    const float w = x.x == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(x.x - best);
+    total = total * keep + wave_sum(w == 0.0F ? 0.0F : x.y * w);
+    o0 *= keep;
+    o1 *= keep;
+    const uint32_t here = min(64u, items - from);
+    for (uint32_t k0 = 0; k0 < here; k0 += kBatch) {
+      float2 v[kBatch];
+#pragma unroll
+      for (unsigned k = 0; k < kBatch; ++k) {
+        const uint32_t at = from + min(k0 + k, here - 1);
+        v[k] = *reinterpret_cast<const float2*>(outputs + static_cast<std::size_t>(at < prefix ? at : at + skipped) * D);
+      }
+#pragma unroll
+      for (unsigned k = 0; k < kBatch; ++k) {
+        const float wk = k0 + k < here ? lane_value(w, k0 + k < here ? k0 + k : 0) : 0.0F;
+        if (wk != 0.0F) {  // uniform; also past the last item
+          o0 = fmaf(v[k].x, wk, o0);
+          o1 = fmaf(v[k].y, wk, o1);
+        }
+      }
+    }
   }
   float y0 = 0.0F, y1 = 0.0F;
   if (best != -INFINITY) {
@@ -460,40 +777,36 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
   *reinterpret_cast<__half2*>(out) = __halves2half2(to_half(y0), to_half(y1));
 }
 
-// Row tiles per wave: as few as hold the rows, at most 4 (2 at head size 256, whose rows
-// take twice the registers).
-unsigned row_tiles(uint32_t rows, uint32_t head_size) {
-  const unsigned tiles = (rows + 15) / 16;
-  if (tiles <= 1) return 1;
-  return tiles == 2 || head_size == 256 ? 2 : 4;
-}
+// Whether the waves share an item's rows or its positions: 16-row items read the cache once
+// for every 16 rows, which three of them on one XCD's L2 still do faster than eight waves
+// with idle ones among them.
+bool by_rows(uint32_t rows) { return rows > 48; }
 
 struct Shape {
-  unsigned prefix_nq, own_nq;
+  bool prefix_rows, own_rows;
   uint32_t prefix_tiles, own_tiles, prefix_splits, own_splits;
   std::size_t rows;
 };
-
-// Workgroups that fill the GPU.
-constexpr uint32_t kWantedGroups = 2 * kComputeUnits;
 
 Shape shape_of(const KvPages& p, uint32_t kv_heads, uint32_t head_size, uint32_t count, uint32_t tokens, uint32_t q_heads,
                uint32_t shared) {
   Shape s{};
   const uint32_t group = q_heads / kv_heads;
   s.rows = static_cast<std::size_t>(count) * tokens * q_heads;
-  auto splits = [](uint32_t ranges, uint64_t positions) {
+  // Workgroups that fill the GPU, of at least kMinBlocks blocks each.
+  auto splits = [head_size](bool by_rows, uint32_t ranges, uint64_t positions) {
+    const uint32_t wanted = kComputeUnits * resident(head_size, by_rows) * 4 / (by_rows ? kWaves : kPosWaves);
     const uint64_t most = std::max<uint64_t>(1, (positions + kBlock - 1) / kBlock / kMinBlocks);
-    return static_cast<uint32_t>(std::min<uint64_t>(most, std::max(1u, kWantedGroups / ranges)));
+    return static_cast<uint32_t>(std::min<uint64_t>(most, std::max(1u, wanted / ranges)));
   };
   const uint32_t all = count * tokens * group, one = tokens * group;
-  s.prefix_nq = shared != 0 ? row_tiles(all, head_size) : 1;
-  s.own_nq = row_tiles(one, head_size);
-  s.prefix_tiles = (all + 16 * s.prefix_nq - 1) / (16 * s.prefix_nq);
-  s.own_tiles = (one + 16 * s.own_nq - 1) / (16 * s.own_nq);
-  s.prefix_splits = shared != 0 ? splits(s.prefix_tiles * kv_heads, shared) : 0;
+  s.prefix_rows = shared != 0 && by_rows(all);
+  s.own_rows = by_rows(one);
+  s.prefix_tiles = (all + tile_rows(s.prefix_rows) - 1) / tile_rows(s.prefix_rows);
+  s.own_tiles = (one + tile_rows(s.own_rows) - 1) / tile_rows(s.own_rows);
+  s.prefix_splits = shared != 0 ? splits(s.prefix_rows, s.prefix_tiles * kv_heads, shared) : 0;
   const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift;
-  s.own_splits = splits(s.own_tiles * kv_heads * count, capacity > shared ? capacity - shared : 1);
+  s.own_splits = splits(s.own_rows, s.own_tiles * kv_heads * count, capacity > shared ? capacity - shared : 1);
   return s;
 }
 
@@ -511,16 +824,13 @@ int32_t read_batch(const gfxinfer_kv_pages* pages, uint32_t count, uint32_t toke
   return GFXI_OK;
 }
 
-template <unsigned D, unsigned NQP, unsigned NQS>
-void launch(const PagedAttnArgs& a, dim3 grid, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_attention_kernel<D, NQP, NQS>), grid, dim3(kWaves * 64), 0, stream, a);
-}
-
-template <unsigned D, unsigned NQP>
-void launch_own(unsigned own, const PagedAttnArgs& a, dim3 grid, hipStream_t stream) {
-  if (own == 1) return launch<D, NQP, 1>(a, grid, stream);
-  if (own == 2) return launch<D, NQP, 2>(a, grid, stream);
-  if constexpr (D == 128) launch<D, NQP, 4>(a, grid, stream);
+// Items first .. first + count - 1.
+void launch_items(uint32_t head_size, bool by_rows, const PagedAttnArgs& a, uint32_t first, uint32_t count, hipStream_t stream) {
+  const dim3 grid(count), block((by_rows ? kWaves : kPosWaves) * 64);
+  if (head_size == 128 && by_rows) hipLaunchKernelGGL((paged_attention_kernel<128, true>), grid, block, 0, stream, a, first);
+  else if (head_size == 128) hipLaunchKernelGGL((paged_attention_kernel<128, false>), grid, block, 0, stream, a, first);
+  else if (by_rows) hipLaunchKernelGGL((paged_attention_kernel<256, true>), grid, block, 0, stream, a, first);
+  else hipLaunchKernelGGL((paged_attention_kernel<256, false>), grid, block, 0, stream, a, first);
 }
 
 }  // namespace
@@ -580,15 +890,13 @@ extern "C" int32_t gfxinfer_launch_kv_pages_gated_attention(const gfxinfer_kv_pa
     a.scale = kLog2E / std::sqrt(static_cast<float>(head_size));
     const uint64_t groups = a.prefix_groups + static_cast<uint64_t>(spread_groups(shape.own_splits * count * kv_heads, shape.own_tiles));
     if (groups > (1u << 23)) return fail(GFXI_INVALID_ARGUMENT, "paged attention over too many rows for one launch");
-    const dim3 grid(static_cast<unsigned>(groups));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (head_size == 128) {
-      if (shape.prefix_nq == 1) launch_own<128, 1>(shape.own_nq, a, grid, st);
-      else if (shape.prefix_nq == 2) launch_own<128, 2>(shape.own_nq, a, grid, st);
-      else launch_own<128, 4>(shape.own_nq, a, grid, st);
+    const uint32_t all = static_cast<uint32_t>(groups);
+    if (a.prefix_groups == 0 || shape.prefix_rows == shape.own_rows) {
+      launch_items(head_size, shape.own_rows, a, 0, all, st);
     } else {
-      if (shape.prefix_nq == 1) launch_own<256, 1>(shape.own_nq, a, grid, st);
-      else launch_own<256, 2>(shape.own_nq, a, grid, st);
+      launch_items(head_size, shape.prefix_rows, a, 0, a.prefix_groups, st);
+      launch_items(head_size, shape.own_rows, a, a.prefix_groups, all - a.prefix_groups, st);
     }
     if (const int32_t s = launch_status("paged attention launch failed"); s != GFXI_OK) return s;
     const dim3 combine(static_cast<unsigned>((shape.rows * (head_size / 128) + 3) / 4));

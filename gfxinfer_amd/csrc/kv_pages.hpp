@@ -15,7 +15,7 @@ constexpr uint32_t kMaxSequences = 65536;
 
 struct SequenceList {
   uint32_t count;
-  uint16_t slot[kMaxListed];
+  alignas(4) uint16_t slot[kMaxListed];
 };
 
 // gfxinfer_kv_pages with the sizes the kernels index by.
@@ -30,6 +30,13 @@ struct KvPages {
 
 __device__ __forceinline__ uint32_t pages_for(uint64_t tokens, uint32_t shift) {
   return static_cast<uint32_t>((tokens + (1u << shift) - 1) >> shift);
+}
+
+// The i-th listed slot (i the same in all lanes) through the scalar cache, which has no
+// 16-bit loads.
+__device__ __forceinline__ uint32_t listed_slot(const SequenceList& list, uint32_t i) {
+  const uint32_t pair = reinterpret_cast<const uint32_t*>(list.slot)[i / 2];
+  return i % 2 != 0 ? pair >> 16 : pair & 0xffffu;
 }
 
 // The page of a sequence's table entry, or -1: entries that name no page of the pool are
