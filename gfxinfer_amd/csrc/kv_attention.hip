@@ -46,7 +46,7 @@ constexpr float kLog2E = 1.4426950408889634F;
 constexpr unsigned kWaves = 8;     // by rows: 128 rows
 constexpr unsigned kPosWaves = 4;  // by positions: small workgroups, of which more fill the GPU
 // Waves per SIMD a kernel is built for.
-constexpr unsigned resident(unsigned head_size, bool by_rows) { return head_size == 256 ? 2u : by_rows ? 4u : 3u; }
+constexpr unsigned resident(unsigned head_size, bool by_rows) { return head_size == 256 ? (by_rows ? 2u : 1u) : by_rows ? 4u : 3u; }
 // Blocks a split is worth at least.
 constexpr uint32_t kMinBlocks = 8;
 
@@ -95,9 +95,9 @@ __device__ __forceinline__ void unspread(uint32_t id, uint32_t tiles, uint32_t& 
 __device__ __forceinline__ float max_over_quarters(float v) {
   const unsigned u = __float_as_uint(v);
   const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const unsigned w = __float_as_uint(fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1])));
+  const unsigned w = __float_as_uint(__builtin_elementwise_maximum(__uint_as_float(p[0]), __uint_as_float(p[1])));
   const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+  return __builtin_elementwise_maximum(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 __device__ __forceinline__ float sum_over_quarters(float v) {
   v += __shfl_xor(v, 16);
@@ -120,19 +120,45 @@ __device__ __forceinline__ void wait_loads() {
 __device__ __forceinline__ unsigned key_slot(unsigned piece, unsigned row) { return piece ^ (row & 15u); }
 __device__ __forceinline__ unsigned value_slot(unsigned piece, unsigned row) { return piece ^ 2 * (row & 7u); }
 
-// The A operands of output tiles first .. first + 3 (dims 16 first ..) of 32 V rows at
-// `rows`, complete when it returns.  The compiler would let the reads wait for every load into
-// LDS that is on its way, since it cannot tell the places apart; the callers have waited for
-// these rows, so the reads are written out with their own wait.
+// Where the lane's part of the first score operand of 16 K rows, and of the first output tile
+// of 16 V rows, lies in bytes from the rows.  Operand s is at the address ^ 64 s, output tile
+// d at the address ^ 32 d: the slots of a row are permuted by exclusive or, and rows start at
+// multiples of their size.
 template <unsigned D>
-__device__ __forceinline__ void read_values(const _Float16* rows, unsigned lane, unsigned first, h8 (&v)[4]) {
-  const unsigned n = lane & 15u, row = 4 * (lane >> 4) + (n >> 2);
-  unsigned at[4];
-#pragma unroll
-  for (unsigned u = 0; u < 4; ++u) {
-    const _Float16* p = rows + row * D + 8 * value_slot(2 * (first + u) + ((n & 3u) >> 1), row) + 4 * (n & 1u);
-    at[u] = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)(p)));
-  }
+__device__ __forceinline__ unsigned key_place() {
+  const unsigned lane = threadIdx.x & 63u, n = lane & 15u;
+  return n * (D * 2) + 16 * key_slot(lane >> 4, n);
+}
+template <unsigned D>
+__device__ __forceinline__ unsigned value_place() {
+  const unsigned lane = threadIdx.x & 63u, n = lane & 15u, row = 4 * (lane >> 4) + (n >> 2);
+  return row * (D * 2) + 16 * value_slot((n & 3u) >> 1, row) + 8 * (n & 1u);
+}
+__device__ __forceinline__ unsigned lds_address(const _Float16* p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)(p)));
+}
+
+// Reads from LDS that are complete when they return.  The compiler lets its own reads wait
+// for every load into LDS that is on its way, since it cannot tell the places apart; the
+// callers have waited for these rows, so the reads are written out with their own wait.
+//
+// Score operands first .. first + 3 of 32 K rows (k[0]: the first 16 rows).
+template <unsigned D>
+__device__ __forceinline__ void read_keys(unsigned place, unsigned first, h8 (&k)[2][4]) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %4, %8 offset:%12\n\t"
+      "ds_read_b128 %1, %9\n\tds_read_b128 %5, %9 offset:%12\n\t"
+      "ds_read_b128 %2, %10\n\tds_read_b128 %6, %10 offset:%12\n\t"
+      "ds_read_b128 %3, %11\n\tds_read_b128 %7, %11 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[0][2]), "=&v"(k[0][3]), "=&v"(k[1][0]), "=&v"(k[1][1]), "=&v"(k[1][2]), "=&v"(k[1][3])
+      : "v"(place ^ 64 * first), "v"(place ^ 64 * (first + 1)), "v"(place ^ 64 * (first + 2)), "v"(place ^ 64 * (first + 3)),
+        "n"(16 * D * 2)
+      : "memory");
+}
+// Output tiles first .. first + 3 of 32 V rows.
+template <unsigned D>
+__device__ __forceinline__ void read_values(unsigned place, unsigned first, h8 (&v)[4]) {
   s16x4 a[8];
   asm volatile(
       "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
@@ -141,7 +167,8 @@ __device__ __forceinline__ void read_values(const _Float16* rows, unsigned lane,
       "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(a[4]), "=&v"(a[5]), "=&v"(a[6]), "=&v"(a[7])
-      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(16 * D * 2)
+      : "v"(place ^ 32 * first), "v"(place ^ 32 * (first + 1)), "v"(place ^ 32 * (first + 2)), "v"(place ^ 32 * (first + 3)),
+        "n"(16 * D * 2)
       : "memory");
 #pragma unroll
   for (unsigned u = 0; u < 4; ++u) {
@@ -237,9 +264,10 @@ struct Rows {
         }
       }
     }
-    float best = fmaxf(s[0][0], s[1][0]);
+    // (A NaN score makes the maximum NaN and the row's result with it, as it has to.)
+    float best = __builtin_elementwise_maximum(s[0][0], s[1][0]);
 #pragma unroll
-    for (unsigned r = 1; r < 4; ++r) best = fmaxf(fmaxf(best, s[0][r]), s[1][r]);
+    for (unsigned r = 1; r < 4; ++r) best = __builtin_elementwise_maximum(__builtin_elementwise_maximum(best, s[0][r]), s[1][r]);
     const float top = max_over_quarters(best) * scale;
     // The stored maximum moves only when a row's grows by more than 8 (a factor of 256):
     // weights stay below 2^8 and most blocks skip the rescaling.
@@ -387,7 +415,8 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
   const __half* values = head_rows(a, pg.value, w.hk, D);
   _Float16* vs = reinterpret_cast<_Float16*>(smem) + wave * kBlock * D;
 
-  // Where the lane's piece of a tile's K rows, and of the V rows of a load, lies.
+  const unsigned value_at = lds_address(vs) + value_place<D>();
+  // Where the lane's piece of a tile's K rows, and of the V rows of a load, lies in memory.
   const uint32_t key_part = n * pg.row + 8 * kb;
   constexpr unsigned kParts = 8 / kLoadRows;
   uint32_t value_part[kParts];
@@ -463,7 +492,7 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
       if (edge || careful) {
         // V rows no one sees become zeros (what a page holds past a sequence's end may be
         // anything, and 0 * NaN would be NaN).
-#pragma unroll
+#pragma unroll 1
         for (unsigned u = 0; u < kLoads; ++u) {
           const unsigned t = u / (kLoads / 2), r = kLoadRows * u + fresh / (D / 8);
           u32x4* piece = reinterpret_cast<u32x4*>(vs + kLoadRows * u * D) + fresh;
@@ -476,7 +505,7 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
 #pragma unroll
       for (unsigned d = 0; d < kTiles; d += 4) {
         h8 v[4];
-        read_values<D>(vs, fresh, d, v);
+        read_values<D>(value_at, d, v);
         rows.add(v, d, high, low);
       }
       if (more) load_v(at + kPosWaves * kBlock, page);
@@ -554,6 +583,7 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
   _Float16* kring = reinterpret_cast<_Float16*>(smem);            // [ring][tile][D]
   _Float16* vring = kring + R * T * D;                            // [ring][tile][D]
   uint32_t* marks = reinterpret_cast<uint32_t*>(vring + R * T * D);  // [ring][waves]
+  const unsigned key_at = lds_address(kring) + key_place<D>(), value_at = lds_address(vring) + value_place<D>();
   const uint32_t begin = w.start + w.first_block * kBlock, last = w.start + w.last_block * kBlock;
   const uint32_t end = min(last, w.hi);
 
@@ -641,29 +671,31 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
         for (unsigned b = 0; b < T / kBlock; ++b) {
           const uint32_t from = at + b * kBlock;
           if (from >= last) break;
-          const unsigned fresh = fresh_lane(), n = fresh & 15u, kb = fresh >> 4;
-          const _Float16* ks = kring + (slot * T + b * kBlock + n) * D;
-          const _Float16* vs = vring + (slot * T + b * kBlock) * D;
+          const unsigned rows_at = (slot * T + b * kBlock) * D * 2, fresh = fresh_lane();
           f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
 #pragma unroll
-          for (unsigned st = 0; st < D / 32; ++st) {
+          for (unsigned st = 0; st < D / 32; st += 4) {
+            h8 k[2][4];
+            read_keys<D>(key_at + rows_at, st, k);
 #pragma unroll
-            for (unsigned t = 0; t < 2; ++t) {
-              const h8 k = *reinterpret_cast<const h8*>(ks + 16 * t * D + 8 * key_slot(4 * st + kb, n));
-              s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, rows.q[st], s[t], 0, 0, 0);
+            for (unsigned u = 0; u < 4; ++u) {
+#pragma unroll
+              for (unsigned t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][u], rows.q[st + u], s[t], 0, 0, 0);
             }
           }
           const uint32_t gone = mark >> (2 * b) & 3u;
           const bool edge = from < w.lo || from + kBlock > rows.least || gone != 0;
           h8 high, low;
+          __builtin_amdgcn_s_setprio(1);
           rows.weigh(s, fresh, a.scale, edge, from, w.lo, gone, high, low);
           if ((mark & 0x100u) != 0) rows.add_strange(s, pg, values, w.slot, from, w.lo, w.hi);
 #pragma unroll
           for (unsigned d = 0; d < D / 16; d += 4) {
             h8 v[4];
-            read_values<D>(vs, fresh, d, v);
+            read_values<D>(value_at + rows_at, d, v);
             rows.add(v, d, high, low);
           }
+          __builtin_amdgcn_s_setprio(0);
         }
       }
       slot = (slot + 1) % R;
@@ -685,7 +717,7 @@ __host__ __device__ constexpr uint32_t tile_rows(bool by_rows) { return by_rows 
 // come before the sequences' own.
 template <unsigned D, bool ByRows>
 __global__ __launch_bounds__((ByRows ? kWaves : kPosWaves) * 64, resident(D, ByRows)) void paged_attention_kernel(PagedAttnArgs a, uint32_t first) {
-  __shared__ __align__(16) char smem[ByRows ? rows_bytes<D>() : positions_bytes<D>()];
+  __shared__ __align__(1024) char smem[ByRows ? rows_bytes<D>() : positions_bytes<D>()];
   const uint32_t shared = prefix_length(a), id = first + blockIdx.x;
   const uint32_t group = a.q_heads / a.kv_heads, count = a.list.count;
   uint32_t range, tile;
