@@ -47,8 +47,8 @@ constexpr unsigned kWaves = 8;     // by rows: 128 rows
 constexpr unsigned kPosWaves = 4;  // by positions: small workgroups, of which more fill the GPU
 // Waves per SIMD a kernel is built for.
 constexpr unsigned resident(unsigned head_size, bool by_rows) { return head_size == 256 ? (by_rows ? 2u : 1u) : by_rows ? 4u : 3u; }
-// Blocks a split is worth at least.
-constexpr uint32_t kMinBlocks = 8;
+// Blocks a split of the prefix, and of a sequence's own positions, is worth at least.
+constexpr uint32_t kPrefixBlocks = 4, kOwnBlocks = 8;
 
 struct PagedAttnArgs {
   KvPages pages;
@@ -65,12 +65,13 @@ struct PagedAttnArgs {
   float scale;                          // log2(e) / sqrt(D)
 };
 
-// `blocks` blocks over at most `splits` splits: blocks per split, and the splits in use.
-__device__ __forceinline__ uint32_t split_length(uint32_t blocks, uint32_t splits) {
-  return max(kMinBlocks, (blocks + splits - 1) / splits);
+// `blocks` blocks over at most `splits` splits of at least `least`: blocks per split, and the
+// splits in use.
+__device__ __forceinline__ uint32_t split_length(uint32_t blocks, uint32_t splits, uint32_t least) {
+  return max(least, (blocks + splits - 1) / splits);
 }
-__device__ __forceinline__ uint32_t splits_used(uint32_t blocks, uint32_t splits) {
-  const uint32_t per = split_length(blocks, splits);
+__device__ __forceinline__ uint32_t splits_used(uint32_t blocks, uint32_t splits, uint32_t least) {
+  const uint32_t per = split_length(blocks, splits, least);
   return (blocks + per - 1) / per;
 }
 // Positions the batch's prefix covers: what the first sequence has of them.
@@ -725,7 +726,7 @@ __global__ __launch_bounds__((ByRows ? kWaves : kPosWaves) * 64, resident(D, ByR
   if (id < a.prefix_groups) {
     unspread(id, a.prefix_tiles, range, tile);
     const uint32_t split = range / a.kv_heads, hk = range - split * a.kv_heads;
-    const uint32_t blocks = (shared + kBlock - 1) / kBlock, per = split_length(blocks, a.prefix_splits);
+    const uint32_t blocks = (shared + kBlock - 1) / kBlock, per = split_length(blocks, a.prefix_splits, kPrefixBlocks);
     const uint32_t from = split * per;
     if (split >= a.prefix_splits || from >= blocks) return;
     item = Item{0, tile * tile_rows(ByRows), count * a.tokens * group, hk, listed_slot(a.list, 0), 0, from,
@@ -735,7 +736,7 @@ __global__ __launch_bounds__((ByRows ? kWaves : kPosWaves) * 64, resident(D, ByR
     const uint32_t hk = range % a.kv_heads, is = range / a.kv_heads, split = is / count, i = is - split * count;
     if (split >= a.own_splits) return;
     const uint32_t slot = listed_slot(a.list, i), end = a.pages.lengths[slot] + a.tokens;
-    const uint32_t blocks = own_blocks(shared, end), per = split_length(blocks, a.own_splits), from = split * per;
+    const uint32_t blocks = own_blocks(shared, end), per = split_length(blocks, a.own_splits, kOwnBlocks), from = split * per;
     if (from >= blocks) return;
     item = Item{i, tile * tile_rows(ByRows), a.tokens * group, hk, slot, shared & ~15u, from,
                 min(from + per, blocks), shared, end, a.prefix_splits + split, true};
@@ -760,8 +761,8 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
   float2 g = {0.0F, 0.0F};
   if (a.gate != nullptr) g = *reinterpret_cast<const float2*>(a.gate + static_cast<std::size_t>(row) * 2 * D + D + d);
   const uint32_t shared = prefix_length(a), end = a.pages.lengths[listed_slot(a.list, i)] + a.tokens;
-  const uint32_t prefix = a.prefix_splits != 0 ? splits_used((shared + kBlock - 1) / kBlock, a.prefix_splits) : 0u;
-  const uint32_t items = prefix + splits_used(own_blocks(shared, end), a.own_splits);
+  const uint32_t prefix = a.prefix_splits != 0 ? splits_used((shared + kBlock - 1) / kBlock, a.prefix_splits, kPrefixBlocks) : 0u;
+  const uint32_t items = prefix + splits_used(own_blocks(shared, end), a.own_splits, kOwnBlocks);
   const uint32_t skipped = a.prefix_splits - prefix;  // unused between the prefix's items and the own ones
   const std::size_t first = static_cast<std::size_t>(row) * (a.prefix_splits + a.own_splits);
   const float* ml = a.partial_ml + 2 * first;
@@ -825,20 +826,26 @@ Shape shape_of(const KvPages& p, uint32_t kv_heads, uint32_t head_size, uint32_t
   Shape s{};
   const uint32_t group = q_heads / kv_heads;
   s.rows = static_cast<std::size_t>(count) * tokens * q_heads;
-  // Workgroups that fill the GPU, of at least kMinBlocks blocks each.
-  auto splits = [head_size](bool by_rows, uint32_t ranges, uint64_t positions) {
-    const uint32_t wanted = kComputeUnits * resident(head_size, by_rows) * 4 / (by_rows ? kWaves : kPosWaves);
-    const uint64_t most = std::max<uint64_t>(1, (positions + kBlock - 1) / kBlock / kMinBlocks);
-    return static_cast<uint32_t>(std::min<uint64_t>(most, std::max(1u, wanted / ranges)));
-  };
   const uint32_t all = count * tokens * group, one = tokens * group;
   s.prefix_rows = shared != 0 && by_rows(all);
   s.own_rows = by_rows(one);
   s.prefix_tiles = (all + tile_rows(s.prefix_rows) - 1) / tile_rows(s.prefix_rows);
   s.own_tiles = (one + tile_rows(s.own_rows) - 1) / tile_rows(s.own_rows);
-  s.prefix_splits = shared != 0 ? splits(s.prefix_rows, s.prefix_tiles * kv_heads, shared) : 0;
-  const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift;
-  s.own_splits = splits(s.own_rows, s.own_tiles * kv_heads * count, capacity > shared ? capacity - shared : 1);
+  // Workgroups for every place on the GPU, but a prefix whose pieces would get shorter than
+  // 2 kPrefixBlocks by that only one for every CU (32 sequences on 4096 positions: 16 splits
+  // 23 us with their merge, 32 of them 25 us; 8 verify blocks on 2000 positions at head size
+  // 256: 7 splits 32 us, 15 of them 27 us).
+  auto fill = [head_size](bool by_rows, uint32_t ranges) {
+    return std::max(1u, kComputeUnits * resident(head_size, by_rows) * 4 / (by_rows ? kWaves : kPosWaves) / ranges);
+  };
+  const uint32_t blocks = (shared + kBlock - 1) / kBlock, ranges = s.prefix_tiles * kv_heads;
+  if (shared != 0) {
+    s.prefix_splits = std::max({1u, std::min(kComputeUnits / ranges, blocks / kPrefixBlocks),
+                                std::min(fill(s.prefix_rows, ranges), blocks / (2 * kPrefixBlocks))});
+  }
+  const uint64_t capacity = (static_cast<uint64_t>(p.stride) << p.page_shift) - shared;
+  s.own_splits = static_cast<uint32_t>(std::clamp<uint64_t>(capacity / (kBlock * kOwnBlocks), 1,
+                                                            fill(s.own_rows, s.own_tiles * kv_heads * count)));
   return s;
 }
 
