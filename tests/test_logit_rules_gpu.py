@@ -222,3 +222,26 @@ def test_rules_in_a_graph_on_another_stream(device, gx):
         gx.launch_logit_rules(logits, rules, eager, tokens, work, stream=side)
         torch.cuda.synchronize()
         assert np.array_equal(host(eager).view(np.uint32), got.view(np.uint32))
+
+
+@pytest.mark.parametrize("stride,shift", [(12288, 0), (12289, 0), (12288, 1), (12290, 2)])
+def test_unaligned_rows_and_large_batches(device, gx, stride, shift):
+    """Rows on 16-byte boundaries or off them, in a batch that takes the larger slices; what lies around a row stays."""
+    import torch
+    rng = np.random.default_rng(stride + shift)
+    batch, vocabulary = 400, 12285
+    a = _problem(rng, batch, vocabulary, 70, 9, 30)
+    logits = (rng.standard_normal((batch, vocabulary)) * 3).astype(np.float32)
+    flat = torch.full((batch * stride + 8,), -9.0, device="cuda")
+    out = torch.full((batch * stride + 8,), 123.0, device="cuda")
+    view, to = (t[shift:shift + batch * stride].view(batch, stride) for t in (flat, out))
+    view[:, :vocabulary] = dev(logits)
+    rules = gx.LogitRules.of(**{k: dev(v) for k, v in a.items()})
+    tokens = empty((batch,), np.uint32)
+    work = empty((gx.logit_rules_workspace_bytes(vocabulary, batch),), np.uint8)
+    say("unaligned rows", stride, shift)
+    gx.launch_logit_rules(view, rules, to, tokens, work, vocabulary)
+    got = host(to)
+    _check(got[:, :vocabulary], *_formula(logits, a))
+    assert np.all(got[:, vocabulary:] == 123.0) and np.all(host(out)[:shift] == 123.0) and np.all(host(out)[shift + batch * stride:] == 123.0)
+    assert np.array_equal(host(tokens), _argmax(got[:, :vocabulary]))
