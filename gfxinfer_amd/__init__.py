@@ -15,6 +15,7 @@ import ctypes
 import os
 import re
 import subprocess
+from array import array
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -375,10 +376,8 @@ def _bytes(workspace) -> int:
 
 
 def _host_ids(values):
-    """A host list of uint32 (None stays None); a ctypes array is passed as it is."""
-    if values is None or isinstance(values, ctypes.Array):
-        return values
-    return (U32 * len(values))(*values)
+    """A host list of uint32 in memory the caller keeps for the call (an array is passed as it is)."""
+    return values if isinstance(values, array) and values.itemsize == 4 else array("I", values)
 
 
 def kv_pages_workspace_bytes(pages) -> int:
@@ -391,40 +390,42 @@ def launch_kv_pages_reset(pages, stream=None):
 
 def launch_kv_pages_fork(pages, parent, children, stream=None):
     ids = _host_ids(children)
-    check(lib().gfxinfer_launch_kv_pages_fork(ctypes.byref(pages), parent, ids, len(ids), _stream(stream)))
+    check(lib().gfxinfer_launch_kv_pages_fork(ctypes.byref(pages), parent, ids.buffer_info()[0], len(ids), _stream(stream)))
 
 
 def launch_kv_pages_reserve(pages, sequences, tokens, status, workspace, stream=None):
     ids = _host_ids(sequences)
-    check(lib().gfxinfer_launch_kv_pages_reserve(ctypes.byref(pages), ids, len(ids), tokens, _p(status), _p(workspace),
+    check(lib().gfxinfer_launch_kv_pages_reserve(ctypes.byref(pages), ids.buffer_info()[0], len(ids), tokens, _p(status), _p(workspace),
                                                  _bytes(workspace), _stream(stream)))
 
 
 def launch_kv_pages_append(pages, layer, key, value, sequences, tokens, stream=None):
     ids = _host_ids(sequences)
-    check(lib().gfxinfer_launch_kv_pages_append(ctypes.byref(pages), layer, _p(key), _p(value), ids, len(ids), tokens,
+    check(lib().gfxinfer_launch_kv_pages_append(ctypes.byref(pages), layer, _p(key), _p(value), ids.buffer_info()[0], len(ids), tokens,
                                                 _stream(stream)))
 
 
 def launch_kv_pages_advance(pages, sequences, tokens, token_counts=None, stream=None):
     """token_counts: device uint32 per listed sequence, or None for `tokens` each."""
     ids = _host_ids(sequences)
-    check(lib().gfxinfer_launch_kv_pages_advance(ctypes.byref(pages), ids, len(ids), tokens, _p(token_counts),
+    check(lib().gfxinfer_launch_kv_pages_advance(ctypes.byref(pages), ids.buffer_info()[0], len(ids), tokens, _p(token_counts),
                                                  _stream(stream)))
 
 
 def launch_kv_pages_free(pages, sequences, keep_tokens=None, stream=None):
-    ids, keep = _host_ids(sequences), _host_ids(keep_tokens)
+    ids, keep = _host_ids(sequences), None if keep_tokens is None else _host_ids(keep_tokens)
     if keep is not None and len(keep) != len(ids):
         raise ValueError("one length to keep per sequence")
-    check(lib().gfxinfer_launch_kv_pages_free(ctypes.byref(pages), ids, keep, len(ids), _stream(stream)))
+    check(lib().gfxinfer_launch_kv_pages_free(ctypes.byref(pages), ids.buffer_info()[0],
+                                              None if keep is None else keep.buffer_info()[0], len(ids), _stream(stream)))
 
 
 def launch_kv_pages_copy(pages, sources, destinations, stream=None):
     a, b = _host_ids(sources), _host_ids(destinations)
     if len(a) != len(b):
         raise ValueError("as many destinations as sources")
-    check(lib().gfxinfer_launch_kv_pages_copy(ctypes.byref(pages), a, b, len(a), _stream(stream)))
+    check(lib().gfxinfer_launch_kv_pages_copy(ctypes.byref(pages), a.buffer_info()[0], b.buffer_info()[0], len(a),
+                                              _stream(stream)))
 
 
 def launch_kv_pages_compact(pages, live_pages, workspace, stream=None):
@@ -440,8 +441,8 @@ def launch_kv_pages_gated_attention(pages, layer, query, gate, output, sequences
                                     stream=None):
     """gate may be None."""
     ids = _host_ids(sequences)
-    check(lib().gfxinfer_launch_kv_pages_gated_attention(ctypes.byref(pages), layer, _p(query), _p(gate), _p(output), ids,
-                                                         len(ids), tokens, q_heads, shared_tokens, _p(workspace),
+    check(lib().gfxinfer_launch_kv_pages_gated_attention(ctypes.byref(pages), layer, _p(query), _p(gate), _p(output),
+                                                         ids.buffer_info()[0], len(ids), tokens, q_heads, shared_tokens, _p(workspace),
                                                          _bytes(workspace), _stream(stream)))
 
 

@@ -256,7 +256,7 @@ extern "C" int32_t gfxinfer_launch_logit_rules(const float* logits, size_t row_s
       return fail(GFXI_INVALID_ARGUMENT, "logit rule workspace is null, not 8-byte aligned or too small");
     }
     const uint32_t slices = slice_count(vocabulary_size, batch);
-    if (static_cast<uint64_t>(slices) * batch > (1u << 23)) {
+    if (static_cast<uint64_t>(slices) * batch >= (1u << 23)) {
       return fail(GFXI_INVALID_ARGUMENT, "logit rules over too many rows for one launch");
     }
     RulesArgs a{};

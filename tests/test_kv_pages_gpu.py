@@ -177,6 +177,23 @@ def test_listed_calls_at_their_limit(device, gx):
     c.check()
 
 
+def test_append_leaves_shared_pages_alone(device, gx):
+    """Rows for a page that another sequence holds are skipped until a reserve has made it private."""
+    c = Cache(gx, 1, 12, 16, 1, 128, 4, 4)
+    c.grow([0], 21)
+    c.fork(0, [1, 2])
+    c.free([1], [18])
+    say("append to shared pages")
+    c.append([0, 1, 2], 20)
+    c.check()
+    assert c.reserve([1], 2) == 0
+    c.append([0, 1, 2], 20)
+    c.check()
+    assert c.reserve([2, 0], 20) == 0
+    c.append([0, 1, 2], 20)
+    c.check()
+
+
 def test_copy_pages(device, gx):
     c = Cache(gx, 3, 12, 64, 2, 128, 2, 4)
     say("copy pages")
