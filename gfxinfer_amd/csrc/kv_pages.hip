@@ -336,9 +336,9 @@ __global__ __launch_bounds__(256) void append_kernel(KvPages p, SequenceList lis
   const uint64_t position = static_cast<uint64_t>(p.lengths[slot]) + t;
   if (position >> p.page_shift >= p.stride) return;
   const int32_t page = table_page(p, slot, static_cast<uint32_t>(position >> p.page_shift));
-  // Only the sequence's own pages are written: without a reserve since the last fork, two
+  // Shared pages are not written: without a reserve since the last fork, two
   // sequences would write the same rows, in no order.
-  if (page < 0 || p.references[page] != 1u) return;
+  if (page < 0 || p.references[page] > 1u) return;
   h16x8 v;
 #pragma unroll
   for (unsigned e = 0; e < 4; ++e) {

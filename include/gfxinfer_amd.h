@@ -651,9 +651,9 @@ int32_t gfxinfer_launch_kv_pages_reserve(const gfxinfer_kv_pages* pages, const u
 
 /* gfxinfer_launch_kv_append_block for pages: K (fp16) and V (fp32 -> fp16) rows
  * [count][tokens][kv_heads * head_size] (16-byte aligned) of one layer at positions length +
- * 0..tokens-1 of each listed sequence (distinct; NULL: 0..count-1).  Positions that are not on
- * a page of the sequence's own (reserve makes them so; fork undoes it) are skipped; lengths
- * stay as they are. */
+ * 0..tokens-1 of each listed sequence (distinct; NULL: 0..count-1).  Positions that are on no
+ * page, or on one that other sequences share (reserve makes them the sequence's own; fork
+ * undoes it), are skipped; lengths stay as they are. */
 int32_t gfxinfer_launch_kv_pages_append(const gfxinfer_kv_pages* pages, uint32_t layer, const uint16_t* key,
                                         const float* value, const uint32_t* sequences, uint32_t count,
                                         uint32_t tokens, void* stream);

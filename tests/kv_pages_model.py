@@ -73,7 +73,7 @@ class PagesModel:
         for i, s in enumerate(sequences):
             for t in range(key.shape[1]):
                 at = self.lengths[s] + t
-                if at // self.page < len(self.table[s]) and self.references[self.table[s][at // self.page]] == 1:
+                if at // self.page < len(self.table[s]) and self.references[self.table[s][at // self.page]] <= 1:
                     self.k[layer, self.table[s][at // self.page], at % self.page] = key[i, t]
                     self.v[layer, self.table[s][at // self.page], at % self.page] = value[i, t].astype(np.float16)
 
