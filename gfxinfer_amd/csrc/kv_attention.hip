@@ -16,14 +16,15 @@
 // of the second otherwise).  V passes through LDS, whose transposing reads turn rows of V
 // into columns.
 //
-// Two ways to share an item among the waves of a workgroup:
-//  - few rows (attend_positions): the waves take turns at blocks of 32 positions and merge at
-//    the end.  K goes from memory straight into the A operand; no barrier stands in the loop.
+// Two ways to share an item among the eight waves of a workgroup:
+//  - few rows (attend_positions): four waves take turns at blocks of 32 positions, each with its
+//    own K and V block in LDS and no barrier in the loop, and merge at the end.
 //  - many rows (attend_rows): each wave takes 16 of up to 128 rows, and a K / V row staged in
 //    LDS serves them all.
-// Both load into LDS directly, without registers.  By rows, a wave of head size 128 fits 128
-// registers and two workgroups a CU, and their four waves a SIMD fill each other's waits;
-// the two ways are two kernels, so that the other one's registers do not count.
+// Both load into LDS directly, without registers, and fill the same places on a CU, so one
+// launch holds the prefix's items and the sequences' own, whichever way each goes (two launches
+// of two kernels took 6 us more; 64 sequences, 32768 shared and 33..1024 own positions of
+// 8 x 128: 119 us against 130).
 #include <algorithm>
 #include <cmath>
 
@@ -43,12 +44,12 @@ using global_void = __attribute__((address_space(1))) void;
 constexpr unsigned kBlock = 32;  // positions of one step of a wave
 constexpr float kLog2E = 1.4426950408889634F;
 
-constexpr unsigned kWaves = 8;     // by rows: 128 rows
-constexpr unsigned kPosWaves = 4;  // by positions: small workgroups, of which more fill the GPU
-// Waves per SIMD a kernel is built for.
-constexpr unsigned resident(unsigned head_size, bool by_rows) { return head_size == 256 ? (by_rows ? 2u : 1u) : by_rows ? 4u : 3u; }
+constexpr unsigned kWaves = 8;     // of a workgroup; by rows: 128 rows
+constexpr unsigned kPosWaves = 4;  // of them, those that divide positions: a block of K and of V each in LDS
+// Workgroups a CU holds: 64 KB of LDS and 128 registers at head size 128, 128 KB and 256 at 256.
+constexpr unsigned resident(unsigned head_size) { return head_size == 256 ? 1u : 2u; }
 // Blocks a split of the prefix, and of a sequence's own positions, is worth at least.
-constexpr uint32_t kPrefixBlocks = 4, kOwnBlocks = 8;
+constexpr uint32_t kPrefixBlocks = 4, kOwnBlocks = 4;
 
 struct PagedAttnArgs {
   KvPages pages;
@@ -76,7 +77,7 @@ __device__ __forceinline__ uint32_t splits_used(uint32_t blocks, uint32_t splits
 }
 // Positions the batch's prefix covers: what the first sequence has of them.
 __device__ __forceinline__ uint32_t prefix_length(const PagedAttnArgs& a) {
-  return min(a.shared, a.pages.lengths[listed_slot(a.list, 0)]);
+  return min(a.shared, __builtin_amdgcn_readfirstlane(a.pages.lengths[listed_slot(a.list, 0)]));
 }
 // A sequence's own positions run from the tile of 16 that holds the prefix's end.
 __device__ __forceinline__ uint32_t own_blocks(uint32_t shared, uint32_t end) {
@@ -120,6 +121,21 @@ __device__ __forceinline__ void wait_loads() {
 // and of a transposing read then fall on different banks.
 __device__ __forceinline__ unsigned key_slot(unsigned piece, unsigned row) { return piece ^ (row & 15u); }
 __device__ __forceinline__ unsigned value_slot(unsigned piece, unsigned row) { return piece ^ 2 * (row & 7u); }
+
+// A load of a wave into LDS covers 512 / D rows: where the lane's piece lies in memory, in
+// elements from the first of them, if that is row 0 of a tile.  From row r on (a multiple of
+// the rows of a load) it is at this ^ 8 (r % 16) for K and ^ 16 (r % 8) for V: rows start at
+// multiples of D elements.
+template <unsigned D>
+__device__ __forceinline__ uint32_t key_piece(unsigned lane, uint32_t row_elements) {
+  const unsigned r = lane / (D / 8);
+  return r * row_elements + 8 * key_slot(lane % (D / 8), r);
+}
+template <unsigned D>
+__device__ __forceinline__ uint32_t value_piece(unsigned lane, uint32_t row_elements) {
+  const unsigned r = lane / (D / 8);
+  return r * row_elements + 8 * value_slot(lane % (D / 8), r);
+}
 
 // Where the lane's part of the first score operand of 16 K rows, and of the first output tile
 // of 16 V rows, lies in bytes from the rows.  Operand s is at the address ^ 64 s, output tile
@@ -185,6 +201,12 @@ __device__ __forceinline__ unsigned fresh_lane() {
   return lane;
 }
 
+// The same for a number that is equal in all lanes.
+__device__ __forceinline__ uint32_t fresh_number(uint32_t x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
 // Sixteen rows of a wave: lane column n's row is the query q (B operand), sees the positions
 // below `visible`, and its result goes to row out_row (none: 0xffffffff).
 template <unsigned D>
@@ -244,6 +266,21 @@ struct Rows {
       for (unsigned e = 0; e < 4; ++e) found |= !(fabsf(o[d][e]) < INFINITY);
     }
     return found;
+  }
+
+  // The raw products of the rows with a block of 32 positions (K rows in LDS, see read_keys).
+  __device__ __forceinline__ void score(unsigned place, f4 (&s)[2]) const {
+    s[0] = s[1] = f4{0, 0, 0, 0};
+#pragma unroll
+    for (unsigned st = 0; st < D / 32; st += 4) {
+      h8 k[2][4];
+      read_keys<D>(place, st, k);
+#pragma unroll
+      for (unsigned u = 0; u < 4; ++u) {
+#pragma unroll
+        for (unsigned t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][u], q[st + u], s[t], 0, 0, 0);
+      }
+    }
   }
 
   // The weights of a block of 32 positions from `at`: s the scores (raw products), the weights
@@ -391,20 +428,13 @@ struct Item {
   bool own;
 };
 
-// Bytes of LDS: V blocks of the waves, later their outputs, then maxima and sums.
-template <unsigned D>
-constexpr std::size_t positions_bytes() {
-  return kPosWaves * kBlock * D * 2 + kPosWaves * 16 * 8;
-}
-
 // Sixteen rows; the waves divide the positions.
 template <unsigned D>
 __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const Item& w, char* smem) {
-  constexpr unsigned kSteps = D / 32, kTiles = D / 16;
-  constexpr unsigned kLoads = kBlock * D / 8 / 64;   // of a block's V rows, per lane
+  constexpr unsigned kTiles = D / 16;
+  constexpr unsigned kLoads = kBlock * D / 8 / 64;   // of a block's K rows, and of its V rows, per lane
   constexpr unsigned kLoadRows = 64 / (D / 8);       // rows one of them covers
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned n = lane & 15u, kb = lane >> 4;
   const KvPages& pg = a.pages;
   const uint32_t in_page = (1u << pg.page_shift) - 1;
   PageWindow window;
@@ -414,20 +444,10 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
   else rows.template load<false>(a, w.base, w.first, w.rows, w.hk, w.hi);
   const __half* keys = head_rows(a, pg.key, w.hk, D);
   const __half* values = head_rows(a, pg.value, w.hk, D);
-  _Float16* vs = reinterpret_cast<_Float16*>(smem) + wave * kBlock * D;
+  _Float16* ks = reinterpret_cast<_Float16*>(smem) + wave * 2 * kBlock * D;
+  _Float16* vs = ks + kBlock * D;
+  const unsigned key_at = lds_address(ks) + key_place<D>(), value_at = lds_address(vs) + value_place<D>();
 
-  const unsigned value_at = lds_address(vs) + value_place<D>();
-  // Where the lane's piece of a tile's K rows, and of the V rows of a load, lies in memory.
-  const uint32_t key_part = n * pg.row + 8 * kb;
-  constexpr unsigned kParts = 8 / kLoadRows;
-  uint32_t value_part[kParts];
-#pragma unroll
-  for (unsigned u = 0; u < kParts; ++u) {
-    const unsigned r = kLoadRows * u + lane / (D / 8);
-    value_part[u] = r * pg.row + 8 * value_slot(lane % (D / 8), r);
-  }
-
-  h8 kr[2][kSteps];
   int32_t page[2];
   auto find_pages = [&](uint32_t at, int32_t (&out)[2]) __attribute__((always_inline)) {
 #pragma unroll
@@ -438,19 +458,21 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
     return (static_cast<std::size_t>(max(p[t], 0)) << pg.page_shift) + ((at + 16 * t) & in_page);
   };
   auto load_k = [&](uint32_t at, const int32_t (&p)[2]) __attribute__((always_inline)) {
+    const uint32_t key_part = key_piece<D>(fresh_lane(), pg.row);
 #pragma unroll
-    for (unsigned t = 0; t < 2; ++t) {
-      const __half* src = keys + tile_row(at, t, p) * pg.row;  // uniform; the lane's part is 32 bits
-#pragma unroll
-      for (unsigned s = 0; s < kSteps; ++s) kr[t][s] = *reinterpret_cast<const h8*>(src + key_part + 32 * s);
+    for (unsigned u = 0; u < kLoads; ++u) {
+      const unsigned t = u / (kLoads / 2), r = kLoadRows * (u % (kLoads / 2));
+      __builtin_amdgcn_global_load_lds((global_void*)(keys + (tile_row(at, t, p) + r) * pg.row + (key_part ^ 8 * r)),
+                                       (lds_void*)(ks + kLoadRows * u * D), 16, 0, 0);
     }
   };
   auto load_v = [&](uint32_t at, const int32_t (&p)[2]) __attribute__((always_inline)) {
+    const uint32_t value_part = value_piece<D>(fresh_lane(), pg.row);
 #pragma unroll
     for (unsigned u = 0; u < kLoads; ++u) {
-      const unsigned t = u / (kLoads / 2), r8 = kLoadRows * (u % (kLoads / 2)) & ~7u;
-      const __half* src = values + (tile_row(at, t, p) + r8) * pg.row;
-      __builtin_amdgcn_global_load_lds((global_void*)(src + value_part[u % kParts]), (lds_void*)(vs + kLoadRows * u * D), 16, 0, 0);
+      const unsigned t = u / (kLoads / 2), r = kLoadRows * (u % (kLoads / 2));
+      __builtin_amdgcn_global_load_lds((global_void*)(values + (tile_row(at, t, p) + r) * pg.row + (value_part ^ 16 * (r & 7u))),
+                                       (lds_void*)(vs + kLoadRows * u * D), 16, 0, 0);
     }
   };
 
@@ -459,7 +481,7 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
   for (bool careful = false;; careful = true) {
     rows.clear();
     if (careful) window.first = 0xffffffc0u;  // 64 before column 0
-    uint32_t block = w.first_block + wave;
+    uint32_t block = fresh_number(wave < kPosWaves ? w.first_block + wave : w.last_block);
     if (block < w.last_block) {
       find_pages(w.start + block * kBlock, page);
       load_k(w.start + block * kBlock, page);
@@ -472,13 +494,10 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
       const unsigned fresh = fresh_lane();
       const bool edge = at < w.lo || at + kBlock > rows.least || page[0] < 0 || page[1] < 0;
       const unsigned missing = (page[0] < 0 ? 1u : 0u) | (page[1] < 0 ? 2u : 0u);
+      // The K rows are there when only their V rows are on their way.
+      wait_loads<kLoads>();
       f4 s[2];
-#pragma unroll
-      for (unsigned t = 0; t < 2; ++t) {
-        s[t] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (unsigned st = 0; st < kSteps; ++st) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kr[t][st], rows.q[st], s[t], 0, 0, 0);
-      }
+      rows.score(key_at, s);
       const bool more = block + kPosWaves < w.last_block;
       if (more) {
         find_pages(at + kPosWaves * kBlock, page);
@@ -487,7 +506,7 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
       h8 high, low;
       rows.weigh(s, fresh, a.scale, edge, at, w.lo, missing, high, low);
       // The V rows are there when only the next K rows are on their way.
-      if (more) wait_loads<2 * kSteps>();
+      if (more) wait_loads<kLoads>();
       else wait_loads<0>();
       bool strange = false;
       if (edge || careful) {
@@ -516,13 +535,16 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
 
   // Merge the waves (a lane holds the same row and dims in every wave): all maxima and
   // outputs through LDS, then each wave sums its share of the output tiles in wave order.
-  __syncthreads();  // the V rows are no longer needed
+  __syncthreads();  // the K and V rows are no longer needed
+  const unsigned late = fresh_lane(), n = late & 15u, kb = late >> 4;
   f4* outputs = reinterpret_cast<f4*>(smem);                                 // [waves][D / 16][64]
   float2* ml = reinterpret_cast<float2*>(smem + kPosWaves * kTiles * 64 * 16);  // [waves][16]
   rows.finish();
-  if (kb == 0) ml[wave * 16 + n] = float2{rows.m, rows.l};
+  if (wave < kPosWaves) {
+    if (kb == 0) ml[wave * 16 + n] = float2{rows.m, rows.l};
 #pragma unroll
-  for (unsigned d = 0; d < kTiles; ++d) outputs[(wave * kTiles + d) * 64 + lane] = rows.o[d];
+    for (unsigned d = 0; d < kTiles; ++d) outputs[(wave * kTiles + d) * 64 + late] = rows.o[d];
+  }
   __syncthreads();
   float best = -INFINITY, total = 0.0F, factor[kPosWaves];
 #pragma unroll
@@ -536,12 +558,12 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
   if (rows.out_row == 0xffffffffu) return;
   const std::size_t at = static_cast<std::size_t>(rows.out_row) * (a.prefix_splits + a.own_splits) + w.split;
 #pragma unroll
-  for (unsigned u = 0; u < kTiles / kPosWaves; ++u) {
-    const unsigned d = wave * (kTiles / kPosWaves) + u;
+  for (unsigned u = 0; u < kTiles / kWaves; ++u) {
+    const unsigned d = wave * (kTiles / kWaves) + u;
     f4 sum = {0, 0, 0, 0};
 #pragma unroll
     for (unsigned v = 0; v < kPosWaves; ++v) {
-      const f4 x = outputs[(v * kTiles + d) * 64 + lane];
+      const f4 x = outputs[(v * kTiles + d) * 64 + late];
       if (factor[v] != 0.0F) sum += x * factor[v];
     }
     *reinterpret_cast<f4*>(a.partial_o + at * D + 16 * d + 4 * kb) = sum;
@@ -585,11 +607,11 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
   _Float16* vring = kring + R * T * D;                            // [ring][tile][D]
   uint32_t* marks = reinterpret_cast<uint32_t*>(vring + R * T * D);  // [ring][waves]
   const unsigned key_at = lds_address(kring) + key_place<D>(), value_at = lds_address(vring) + value_place<D>();
-  const uint32_t begin = w.start + w.first_block * kBlock, last = w.start + w.last_block * kBlock;
+  const uint32_t last = w.start + w.last_block * kBlock;
   const uint32_t end = min(last, w.hi);
 
   PageWindow window;
-  window.start(pg, w.slot, begin >> pg.page_shift);
+  window.start(pg, w.slot, (w.start + w.first_block * kBlock) >> pg.page_shift);
   bool lost = false;  // a page was missing
   // Load u of a wave covers rows kLoadRows * (wave + 8 u) .. of the tile, all of one part of
   // 16 positions.  Parts without a page load from page 0 (always there) and are dealt with
@@ -599,15 +621,17 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
     return part < end ? window.find(pg, w.slot, part >> pg.page_shift) : 0;
   };
   auto load = [&](unsigned slot, uint32_t at) __attribute__((always_inline)) {
+    const unsigned fresh = D == 128 ? fresh_lane() : lane;
+    const uint32_t key_part = key_piece<D>(fresh, pg.row), value_part = value_piece<D>(fresh, pg.row);
 #pragma unroll
     for (unsigned u = 0; u < kLoads; ++u) {
-      const unsigned row0 = kLoadRows * (wave + kWaves * u), r = (row0 & 15u) + lane / (D / 8), p = lane % (D / 8);
+      const unsigned row0 = kLoadRows * (wave + kWaves * u);
       const int32_t page = part_page(u, at);
       lost |= page < 0;
-      const std::size_t base = ((static_cast<std::size_t>(max(page, 0)) << pg.page_shift) + ((at + (row0 & ~15u)) & in_page)) * pg.row;
-      __builtin_amdgcn_global_load_lds((global_void*)(keys + base + (r * pg.row + 8 * key_slot(p, r))),
+      const std::size_t base = ((static_cast<std::size_t>(max(page, 0)) << pg.page_shift) + ((at + row0) & in_page)) * pg.row;
+      __builtin_amdgcn_global_load_lds((global_void*)(keys + base + (key_part ^ 8 * (row0 & 15u))),
                                        (lds_void*)(kring + (slot * T + row0) * D), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((global_void*)(values + base + (r * pg.row + 8 * value_slot(p, r))),
+      __builtin_amdgcn_global_load_lds((global_void*)(values + base + (value_part ^ 16 * (row0 & 7u))),
                                        (lds_void*)(vring + (slot * T + row0) * D), 16, 0, 0);
     }
   };
@@ -644,6 +668,7 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
   for (bool careful = false;; careful = true) {
     rows.clear();
     if (careful) window.first = 0xffffffc0u;  // 64 before column 0
+    const uint32_t begin = fresh_number(w.start + w.first_block * kBlock);
 #pragma unroll
     for (unsigned i = 0; i + 1 < R; ++i) {
       if (begin + i * T < last) load(i, begin + i * T);
@@ -673,17 +698,8 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
           const uint32_t from = at + b * kBlock;
           if (from >= last) break;
           const unsigned rows_at = (slot * T + b * kBlock) * D * 2, fresh = fresh_lane();
-          f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
-#pragma unroll
-          for (unsigned st = 0; st < D / 32; st += 4) {
-            h8 k[2][4];
-            read_keys<D>(key_at + rows_at, st, k);
-#pragma unroll
-            for (unsigned u = 0; u < 4; ++u) {
-#pragma unroll
-              for (unsigned t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][u], rows.q[st + u], s[t], 0, 0, 0);
-            }
-          }
+          f4 s[2];
+          rows.score(key_at + rows_at, s);
           const uint32_t gone = mark >> (2 * b) & 3u;
           const bool edge = from < w.lo || from + kBlock > rows.least || gone != 0;
           h8 high, low;
@@ -712,37 +728,57 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
   if (lane < 16) *reinterpret_cast<float2*>(a.partial_ml + 2 * to) = float2{rows.m, rows.l};
 }
 
-__host__ __device__ constexpr uint32_t tile_rows(bool by_rows) { return by_rows ? 128u : 16u; }
+// Whether the waves share an item's rows or its positions.  By positions, every 16 rows read
+// the range again, but four waves work where one or two of eight would.  Microseconds of a call
+// by rows and by positions: 8 heads of 128, 25 rows on a prefix of 2000 12.3 and 11.7, of 16000
+// both 24.3, 50 rows 13.8 and 12.8, 26.4 and 27.1; 8 sequences of 3900 own positions, 5 rows 27.9
+// and 27.1, 20 rows 30.0 and 31.6, 40 rows 32 and 45.  4 heads of 256, 30 rows on 2000 16.9 and
+// 15.1, on 16000 32.6 and 29.0, 60 rows 19.6 and 17.5, 35.4 and 35.6; 8 sequences of 3900, 6 rows
+// 33.1 and 28.6, 24 rows 35.4 and 33.0, 48 rows 39 and 51.
+__host__ __device__ constexpr bool by_rows(uint32_t rows, uint32_t head_size, bool own) {
+  return rows > (own && head_size == 128 ? 16u : 32u);
+}
+// Tiles of rows: of 16, or as few of up to 128 as hold them, evenly filled (10 x 16 rows as 5 + 5,
+// not 8 + 2: 160 rows on 16000 positions 42 -> 40 us, on 4 x 256 61 -> 58 us).
+__host__ __device__ constexpr uint32_t row_tiles(uint32_t rows, uint32_t head_size, bool own) {
+  return by_rows(rows, head_size, own) ? (rows + 16 * kWaves - 1) / (16 * kWaves) : (rows + 15) / 16;
+}
+__host__ __device__ constexpr uint32_t tile_rows(uint32_t rows, uint32_t tiles) { return ((rows + 15) / 16 + tiles - 1) / tiles * 16; }
 
-// Work items from number `first` on, all shared among the waves the same way: the prefix's
-// come before the sequences' own.
-template <unsigned D, bool ByRows>
-__global__ __launch_bounds__((ByRows ? kWaves : kPosWaves) * 64, resident(D, ByRows)) void paged_attention_kernel(PagedAttnArgs a, uint32_t first) {
-  __shared__ __align__(1024) char smem[ByRows ? rows_bytes<D>() : positions_bytes<D>()];
-  const uint32_t shared = prefix_length(a), id = first + blockIdx.x;
+// Work items: the prefix's come before the sequences' own.
+template <unsigned D>
+__global__ __launch_bounds__(kWaves * 64, resident(D) * kWaves / 4) void paged_attention_kernel(PagedAttnArgs a) {
+  __shared__ __align__(1024) char smem[rows_bytes<D>()];
+  const uint32_t shared = prefix_length(a), id = blockIdx.x;
   const uint32_t group = a.q_heads / a.kv_heads, count = a.list.count;
   uint32_t range, tile;
   Item item;
+  bool few;
   if (id < a.prefix_groups) {
     unspread(id, a.prefix_tiles, range, tile);
     const uint32_t split = range / a.kv_heads, hk = range - split * a.kv_heads;
     const uint32_t blocks = (shared + kBlock - 1) / kBlock, per = split_length(blocks, a.prefix_splits, kPrefixBlocks);
     const uint32_t from = split * per;
     if (split >= a.prefix_splits || from >= blocks) return;
-    item = Item{0, tile * tile_rows(ByRows), count * a.tokens * group, hk, listed_slot(a.list, 0), 0, from,
+    const uint32_t rows = count * a.tokens * group, per_tile = tile_rows(rows, a.prefix_tiles);
+    few = !by_rows(rows, D, false);
+    item = Item{0, tile * per_tile, min(rows, (tile + 1) * per_tile), hk, listed_slot(a.list, 0), 0, from,
                 min(from + per, blocks), 0, shared, split, false};
   } else {
     unspread(id - a.prefix_groups, a.own_tiles, range, tile);
     const uint32_t hk = range % a.kv_heads, is = range / a.kv_heads, split = is / count, i = is - split * count;
     if (split >= a.own_splits) return;
-    const uint32_t slot = listed_slot(a.list, i), end = a.pages.lengths[slot] + a.tokens;
+    const uint32_t slot = listed_slot(a.list, i), end = __builtin_amdgcn_readfirstlane(a.pages.lengths[slot]) + a.tokens;
     const uint32_t blocks = own_blocks(shared, end), per = split_length(blocks, a.own_splits, kOwnBlocks), from = split * per;
     if (from >= blocks) return;
-    item = Item{i, tile * tile_rows(ByRows), a.tokens * group, hk, slot, shared & ~15u, from,
+    const uint32_t rows = a.tokens * group, per_tile = tile_rows(rows, a.own_tiles);
+    // (One tile's positions are shared more quickly by rows: nothing is merged.)
+    few = !by_rows(rows, D, true) && (blocks - from) * kBlock > kTile<D>;
+    item = Item{i, tile * per_tile, min(rows, (tile + 1) * per_tile), hk, slot, shared & ~15u, from,
                 min(from + per, blocks), shared, end, a.prefix_splits + split, true};
   }
-  if constexpr (ByRows) attend_rows<D>(a, item, smem);
-  else attend_positions<D>(a, item, smem);
+  if (few) attend_positions<D>(a, item, smem);
+  else attend_rows<D>(a, item, smem);
 }
 
 // Merges a row's items and applies the gate: one wave per (row, 128 dims), two dims a lane.
@@ -810,13 +846,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
   *reinterpret_cast<__half2*>(out) = __halves2half2(to_half(y0), to_half(y1));
 }
 
-// Whether the waves share an item's rows or its positions: 16-row items read the cache once
-// for every 16 rows, which three of them on one XCD's L2 still do faster than eight waves
-// with idle ones among them.
-bool by_rows(uint32_t rows) { return rows > 48; }
-
 struct Shape {
-  bool prefix_rows, own_rows;
   uint32_t prefix_tiles, own_tiles, prefix_splits, own_splits;
   std::size_t rows;
 };
@@ -827,25 +857,23 @@ Shape shape_of(const KvPages& p, uint32_t kv_heads, uint32_t head_size, uint32_t
   const uint32_t group = q_heads / kv_heads;
   s.rows = static_cast<std::size_t>(count) * tokens * q_heads;
   const uint32_t all = count * tokens * group, one = tokens * group;
-  s.prefix_rows = shared != 0 && by_rows(all);
-  s.own_rows = by_rows(one);
-  s.prefix_tiles = (all + tile_rows(s.prefix_rows) - 1) / tile_rows(s.prefix_rows);
-  s.own_tiles = (one + tile_rows(s.own_rows) - 1) / tile_rows(s.own_rows);
+  s.prefix_tiles = row_tiles(all, head_size, false);
+  s.own_tiles = row_tiles(one, head_size, true);
   // Workgroups for every place on the GPU, but a prefix whose pieces would get shorter than
   // 2 kPrefixBlocks by that only one for every CU (32 sequences on 4096 positions: 16 splits
   // 23 us with their merge, 32 of them 25 us; 8 verify blocks on 2000 positions at head size
   // 256: 7 splits 32 us, 15 of them 27 us).
-  auto fill = [head_size](bool by_rows, uint32_t ranges) {
-    return std::max(1u, kComputeUnits * resident(head_size, by_rows) * 4 / (by_rows ? kWaves : kPosWaves) / ranges);
+  auto fill = [head_size](uint32_t ranges, uint32_t tiles) {
+    return std::max(1u, 8 * (kComputeUnits / 8 * resident(head_size) / tiles) / ranges);
   };
   const uint32_t blocks = (shared + kBlock - 1) / kBlock, ranges = s.prefix_tiles * kv_heads;
   if (shared != 0) {
     s.prefix_splits = std::max({1u, std::min(kComputeUnits / ranges, blocks / kPrefixBlocks),
-                                std::min(fill(s.prefix_rows, ranges), blocks / (2 * kPrefixBlocks))});
+                                std::min(fill(kv_heads, s.prefix_tiles), blocks / (2 * kPrefixBlocks))});
   }
   const uint64_t capacity = (static_cast<uint64_t>(p.stride) << p.page_shift) - shared;
   s.own_splits = static_cast<uint32_t>(std::clamp<uint64_t>(capacity / (kBlock * kOwnBlocks), 1,
-                                                            fill(s.own_rows, s.own_tiles * kv_heads * count)));
+                                                            fill(kv_heads * count, s.own_tiles)));
   return s;
 }
 
@@ -861,15 +889,6 @@ int32_t read_batch(const gfxinfer_kv_pages* pages, uint32_t count, uint32_t toke
                                        "multiple of the KV heads, a shared prefix within the table)");
   }
   return GFXI_OK;
-}
-
-// Items first .. first + count - 1.
-void launch_items(uint32_t head_size, bool by_rows, const PagedAttnArgs& a, uint32_t first, uint32_t count, hipStream_t stream) {
-  const dim3 grid(count), block((by_rows ? kWaves : kPosWaves) * 64);
-  if (head_size == 128 && by_rows) hipLaunchKernelGGL((paged_attention_kernel<128, true>), grid, block, 0, stream, a, first);
-  else if (head_size == 128) hipLaunchKernelGGL((paged_attention_kernel<128, false>), grid, block, 0, stream, a, first);
-  else if (by_rows) hipLaunchKernelGGL((paged_attention_kernel<256, true>), grid, block, 0, stream, a, first);
-  else hipLaunchKernelGGL((paged_attention_kernel<256, false>), grid, block, 0, stream, a, first);
 }
 
 }  // namespace
@@ -931,12 +950,9 @@ extern "C" int32_t gfxinfer_launch_kv_pages_gated_attention(const gfxinfer_kv_pa
     if (groups > (1u << 23)) return fail(GFXI_INVALID_ARGUMENT, "paged attention over too many rows for one launch");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const uint32_t all = static_cast<uint32_t>(groups);
-    if (a.prefix_groups == 0 || shape.prefix_rows == shape.own_rows) {
-      launch_items(head_size, shape.own_rows, a, 0, all, st);
-    } else {
-      launch_items(head_size, shape.prefix_rows, a, 0, a.prefix_groups, st);
-      launch_items(head_size, shape.own_rows, a, a.prefix_groups, all - a.prefix_groups, st);
-    }
+    const dim3 block(kWaves * 64);
+    if (head_size == 128) hipLaunchKernelGGL(paged_attention_kernel<128>, dim3(all), block, 0, st, a);
+    else hipLaunchKernelGGL(paged_attention_kernel<256>, dim3(all), block, 0, st, a);
     if (const int32_t s = launch_status("paged attention launch failed"); s != GFXI_OK) return s;
     const dim3 combine(static_cast<unsigned>((shape.rows * (head_size / 128) + 3) / 4));
     if (head_size == 128) hipLaunchKernelGGL(paged_combine_kernel<128>, combine, dim3(256), 0, st, a);
