@@ -66,10 +66,17 @@ struct PagedAttnArgs {
   float scale;                          // log2(e) / sqrt(D)
 };
 
-// `blocks` blocks over at most `splits` splits of at least `least`: blocks per split, and the
-// splits in use.
+// Positions of a tile of attend_rows (16 KB of K and of V at head size 128, 32 KB at 256), and the
+// tiles its LDS ring holds.  A wave takes a tile's positions as one step: with 32 a step, more
+// maxima and longer waits, 64 sequences on 32768 positions took 118 us, not 115, and at head size
+// 256 32 rows of one sequence on 16000 57 us, not 54.
+constexpr unsigned kTile = 64, kRing = 2;
+
+// `blocks` blocks over at most `splits` splits of at least `least`: blocks per split (whole
+// tiles), and the splits in use.
 __device__ __forceinline__ uint32_t split_length(uint32_t blocks, uint32_t splits, uint32_t least) {
-  return max(least, (blocks + splits - 1) / splits);
+  constexpr uint32_t kUnit = kTile / kBlock;
+  return max(least, ((blocks + splits - 1) / splits + kUnit - 1) / kUnit * kUnit);
 }
 __device__ __forceinline__ uint32_t splits_used(uint32_t blocks, uint32_t splits, uint32_t least) {
   const uint32_t per = split_length(blocks, splits, least);
@@ -269,32 +276,33 @@ struct Rows {
   }
 
   // The raw products of the rows with a block of 32 positions (K rows in LDS, see read_keys).
-  __device__ __forceinline__ void score(unsigned place, f4 (&s)[2]) const {
-    s[0] = s[1] = f4{0, 0, 0, 0};
+  __device__ __forceinline__ void score(unsigned place, f4& s0, f4& s1) const {
+    s0 = s1 = f4{0, 0, 0, 0};
 #pragma unroll
     for (unsigned st = 0; st < D / 32; st += 4) {
       h8 k[2][4];
       read_keys<D>(place, st, k);
 #pragma unroll
       for (unsigned u = 0; u < 4; ++u) {
-#pragma unroll
-        for (unsigned t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][u], q[st + u], s[t], 0, 0, 0);
+        s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][u], q[st + u], s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][u], q[st + u], s1, 0, 0, 0);
       }
     }
   }
 
-  // The weights of a block of 32 positions from `at`: s the scores (raw products), the weights
+  // The weights of T tiles of 16 positions from `at`: s the scores (raw products), the weights
   // afterwards.  An edge block holds positions that some row does not see (below lo, past its
   // end, or in a tile of 16 whose page is missing: bit t of `missing`).
   //
   // The weights go out as an fp16 pair p = high + low, high cut off and low the rest: two
   // products carry about 22 bits of p, so the output keeps the accuracy of an fp32 product.
-  __device__ __forceinline__ void weigh(f4 (&s)[2], unsigned lane, float scale, bool edge, uint32_t at, uint32_t lo,
-                                        unsigned missing, h8& high, h8& low) {
+  template <unsigned T>
+  __device__ __forceinline__ void weigh(f4 (&s)[T], unsigned lane, float scale, bool edge, uint32_t at, uint32_t lo,
+                                        unsigned missing, h8 (&high)[T / 2], h8 (&low)[T / 2]) {
     if (edge) {
       const unsigned kb = lane >> 4;
 #pragma unroll
-      for (unsigned t = 0; t < 2; ++t) {
+      for (unsigned t = 0; t < T; ++t) {
 #pragma unroll
         for (unsigned r = 0; r < 4; ++r) {
           const uint32_t position = at + 16 * t + 4 * kb + r;
@@ -303,9 +311,9 @@ struct Rows {
       }
     }
     // (A NaN score makes the maximum NaN and the row's result with it, as it has to.)
-    float best = __builtin_elementwise_maximum(s[0][0], s[1][0]);
+    float best = s[0][0];
 #pragma unroll
-    for (unsigned r = 1; r < 4; ++r) best = __builtin_elementwise_maximum(__builtin_elementwise_maximum(best, s[0][r]), s[1][r]);
+    for (unsigned r = 1; r < 4 * T; ++r) best = __builtin_elementwise_maximum(best, s[r / 4][r % 4]);
     const float top = max_over_quarters(best) * scale;
     // The stored maximum moves only when a row's grows by more than 8 (a factor of 256):
     // weights stay below 2^8 and most blocks skip the rescaling.
@@ -319,7 +327,7 @@ struct Rows {
     }
     const float floor = m == -INFINITY ? 0.0F : m;
 #pragma unroll
-    for (unsigned t = 0; t < 2; ++t) {
+    for (unsigned t = 0; t < T; ++t) {
 #pragma unroll
       for (unsigned r = 0; r < 4; r += 2) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][r], scale, -floor));
@@ -329,11 +337,11 @@ struct Rows {
         l += p0;
         l += p1;
         const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-        high[4 * t + r] = h[0];
-        high[4 * t + r + 1] = h[1];
+        high[t / 2][t % 2 * 4 + r] = h[0];
+        high[t / 2][t % 2 * 4 + r + 1] = h[1];
         const auto rest = __builtin_amdgcn_cvt_pkrtz(p0 - static_cast<float>(h[0]), p1 - static_cast<float>(h[1]));
-        low[4 * t + r] = rest[0];
-        low[4 * t + r + 1] = rest[1];
+        low[t / 2][t % 2 * 4 + r] = rest[0];
+        low[t / 2][t % 2 * 4 + r + 1] = rest[1];
       }
     }
   }
@@ -349,11 +357,12 @@ struct Rows {
   // In a careful pass the infinities and NaNs among the values of a block are zeros in LDS,
   // since a row must not meet those of positions it does not see; here the rows that see them
   // get their products, one by one from the pages.  s: the weights of the block.
-  __device__ __forceinline__ void add_strange(const f4 (&s)[2], const KvPages& pages, const __half* values, uint32_t slot,
+  template <unsigned T>
+  __device__ __forceinline__ void add_strange(const f4 (&s)[T], const KvPages& pages, const __half* values, uint32_t slot,
                                               uint32_t at, uint32_t lo, uint32_t hi) {
     const unsigned lane = threadIdx.x & 63u, n = lane & 15u, kb = lane >> 4;
 #pragma unroll 1
-    for (unsigned p = 0; p < kBlock; ++p) {
+    for (unsigned p = 0; p < 16 * T; ++p) {
       const uint32_t position = at + p;
       const int32_t page = position < lo || position >= hi ? -1 : table_page(pages, slot, position >> pages.page_shift);
       if (page < 0) continue;
@@ -362,7 +371,7 @@ struct Rows {
       const unsigned owner = ((p % 16) / 4) * 16 + n;
       float w = 0.0F;
 #pragma unroll
-      for (unsigned e = 0; e < 8; ++e) {
+      for (unsigned e = 0; e < 4 * T; ++e) {
         const float x = __shfl(s[e / 4][e % 4], owner);
         if (e == p / 16 * 4 + p % 4) w = x;
       }
@@ -497,13 +506,13 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
       // The K rows are there when only their V rows are on their way.
       wait_loads<kLoads>();
       f4 s[2];
-      rows.score(key_at, s);
+      rows.score(key_at, s[0], s[1]);
       const bool more = block + kPosWaves < w.last_block;
       if (more) {
         find_pages(at + kPosWaves * kBlock, page);
         load_k(at + kPosWaves * kBlock, page);
       }
-      h8 high, low;
+      h8 high[1], low[1];
       rows.weigh(s, fresh, a.scale, edge, at, w.lo, missing, high, low);
       // The V rows are there when only the next K rows are on their way.
       if (more) wait_loads<kLoads>();
@@ -526,7 +535,7 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
       for (unsigned d = 0; d < kTiles; d += 4) {
         h8 v[4];
         read_values<D>(value_at, d, v);
-        rows.add(v, d, high, low);
+        rows.add(v, d, high[0], low[0]);
       }
       if (more) load_v(at + kPosWaves * kBlock, page);
     }
@@ -571,16 +580,9 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
   if (wave == 0 && kb == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{best, total};
 }
 
-// Positions of a tile of attend_rows (16 KB of K and of V), and the tiles its LDS ring
-// holds: two workgroups a CU at head size 128, one at 256.
-template <unsigned D>
-constexpr unsigned kTile = D == 128 ? 64u : 32u;
-template <unsigned D>
-constexpr unsigned kRing = D == 128 ? 2u : 4u;
-
 template <unsigned D>
 constexpr std::size_t rows_bytes() {
-  return kRing<D> * (kTile<D> * D * 2 * 2 + 4 * kWaves);
+  return kRing * (kTile * D * 2 * 2 + 4 * kWaves);
 }
 
 // A barrier that orders LDS accesses and leaves loads from memory into LDS on their way
@@ -595,7 +597,7 @@ __device__ __forceinline__ void lds_barrier() {
 // ahead, with one barrier a tile.
 template <unsigned D>
 __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& w, char* smem) {
-  constexpr unsigned R = kRing<D>, T = kTile<D>;
+  constexpr unsigned R = kRing, T = kTile;
   constexpr unsigned kLoads = T * D / 8 / (kWaves * 64);  // of K, and of V, per tile and lane
   constexpr unsigned kLoadRows = 64 / (D / 8);            // rows a load of a wave covers
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -693,27 +695,25 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
           for (unsigned v = 0; v < kWaves; ++v) mark |= marks[slot * kWaves + v];
           mark = __builtin_amdgcn_readfirstlane(mark);
         }
-#pragma unroll 1
+        const unsigned rows_at = slot * T * D * 2, fresh = fresh_lane();
+        f4 s[T / 16];
+#pragma unroll
+        for (unsigned b = 0; b < T / kBlock; ++b) rows.score(key_at + rows_at + b * kBlock * D * 2, s[2 * b], s[2 * b + 1]);
+        const bool edge = at < w.lo || at + T > rows.least || (mark & 0xffu) != 0;
+        h8 high[T / kBlock], low[T / kBlock];
+        __builtin_amdgcn_s_setprio(1);
+        rows.weigh(s, fresh, a.scale, edge, at, w.lo, mark, high, low);
+        if ((mark & 0x100u) != 0) rows.add_strange(s, pg, values, w.slot, at, w.lo, w.hi);
+#pragma unroll
         for (unsigned b = 0; b < T / kBlock; ++b) {
-          const uint32_t from = at + b * kBlock;
-          if (from >= last) break;
-          const unsigned rows_at = (slot * T + b * kBlock) * D * 2, fresh = fresh_lane();
-          f4 s[2];
-          rows.score(key_at + rows_at, s);
-          const uint32_t gone = mark >> (2 * b) & 3u;
-          const bool edge = from < w.lo || from + kBlock > rows.least || gone != 0;
-          h8 high, low;
-          __builtin_amdgcn_s_setprio(1);
-          rows.weigh(s, fresh, a.scale, edge, from, w.lo, gone, high, low);
-          if ((mark & 0x100u) != 0) rows.add_strange(s, pg, values, w.slot, from, w.lo, w.hi);
 #pragma unroll
           for (unsigned d = 0; d < D / 16; d += 4) {
             h8 v[4];
-            read_values<D>(value_at + rows_at, d, v);
-            rows.add(v, d, high, low);
+            read_values<D>(value_at + rows_at + b * kBlock * D * 2, d, v);
+            rows.add(v, d, high[b], low[b]);
           }
-          __builtin_amdgcn_s_setprio(0);
         }
+        __builtin_amdgcn_s_setprio(0);
       }
       slot = (slot + 1) % R;
     }
@@ -773,7 +773,7 @@ __global__ __launch_bounds__(kWaves * 64, resident(D) * kWaves / 4) void paged_a
     if (from >= blocks) return;
     const uint32_t rows = a.tokens * group, per_tile = tile_rows(rows, a.own_tiles);
     // (One tile's positions are shared more quickly by rows: nothing is merged.)
-    few = !by_rows(rows, D, true) && (blocks - from) * kBlock > kTile<D>;
+    few = !by_rows(rows, D, true) && (blocks - from) * kBlock > kTile;
     item = Item{i, tile * per_tile, min(rows, (tile + 1) * per_tile), hk, slot, shared & ~15u, from,
                 min(from + per, blocks), shared, end, a.prefix_splits + split, true};
   }
