@@ -23,8 +23,13 @@
 //    LDS serves them all.
 // Both load into LDS directly, without registers, and fill the same places on a CU, so one
 // launch holds the prefix's items and the sequences' own, whichever way each goes (two launches
-// of two kernels took 6 us more; 64 sequences, 32768 shared and 33..1024 own positions of
-// 8 x 128: 119 us against 130).
+// of two kernels took 6 us more).
+//
+// What bounds it: with few rows the reads of the cache (64 sequences of 100..900 own positions,
+// 8 x 128: 134 MB in 33 us, 4.1 TB/s); with many the waves' own instructions, of which a tile of
+// 64 positions x 16 rows takes 48 matrix products (768 cycles of a SIMD) and about 180 others
+// (900 cycles): 64 sequences on 32768 shared positions, 320 rows of a KV head, 90 us and 480
+// TFLOP/s, 720 with the second product of the weights' low halves.
 #include <algorithm>
 #include <cmath>
 
@@ -48,7 +53,10 @@ constexpr unsigned kWaves = 8;     // of a workgroup; by rows: 128 rows
 constexpr unsigned kPosWaves = 4;  // of them, those that divide positions: a block of K and of V each in LDS
 // Workgroups a CU holds: 64 KB of LDS and 128 registers at head size 128, 128 KB and 256 at 256.
 constexpr unsigned resident(unsigned head_size) { return head_size == 256 ? 1u : 2u; }
-// Blocks a split of the prefix, and of a sequence's own positions, is worth at least.
+// Blocks a split of the prefix, and of a sequence's own positions, is worth at least.  With 8 of
+// the prefix, 8 verify blocks on 2000 positions at head size 256 take 31 us, not 27 (with 2, 32
+// sequences on 4000 35 us, not 27); with 8 of its own, one sequence of 4000 15.0 us, not 13.1
+// (with 2, 14.1).
 constexpr uint32_t kPrefixBlocks = 4, kOwnBlocks = 4;
 
 struct PagedAttnArgs {
@@ -82,9 +90,13 @@ __device__ __forceinline__ uint32_t splits_used(uint32_t blocks, uint32_t splits
   const uint32_t per = split_length(blocks, splits, least);
   return (blocks + per - 1) / per;
 }
+// Committed positions of a slot; a damaged length does not lead far past the table.
+__device__ __forceinline__ uint32_t committed(const KvPages& p, uint32_t slot) {
+  return min(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(p.lengths[slot])), p.stride << p.page_shift);
+}
 // Positions the batch's prefix covers: what the first sequence has of them.
 __device__ __forceinline__ uint32_t prefix_length(const PagedAttnArgs& a) {
-  return min(a.shared, __builtin_amdgcn_readfirstlane(a.pages.lengths[listed_slot(a.list, 0)]));
+  return min(a.shared, committed(a.pages, listed_slot(a.list, 0)));
 }
 // A sequence's own positions run from the tile of 16 that holds the prefix's end.
 __device__ __forceinline__ uint32_t own_blocks(uint32_t shared, uint32_t end) {
@@ -768,12 +780,11 @@ __global__ __launch_bounds__(kWaves * 64, resident(D) * kWaves / 4) void paged_a
     unspread(id - a.prefix_groups, a.own_tiles, range, tile);
     const uint32_t hk = range % a.kv_heads, is = range / a.kv_heads, split = is / count, i = is - split * count;
     if (split >= a.own_splits) return;
-    const uint32_t slot = listed_slot(a.list, i), end = __builtin_amdgcn_readfirstlane(a.pages.lengths[slot]) + a.tokens;
+    const uint32_t slot = listed_slot(a.list, i), end = committed(a.pages, slot) + a.tokens;
     const uint32_t blocks = own_blocks(shared, end), per = split_length(blocks, a.own_splits, kOwnBlocks), from = split * per;
     if (from >= blocks) return;
     const uint32_t rows = a.tokens * group, per_tile = tile_rows(rows, a.own_tiles);
-    // (One tile's positions are shared more quickly by rows: nothing is merged.)
-    few = !by_rows(rows, D, true) && (blocks - from) * kBlock > kTile;
+    few = !by_rows(rows, D, true);
     item = Item{i, tile * per_tile, min(rows, (tile + 1) * per_tile), hk, slot, shared & ~15u, from,
                 min(from + per, blocks), shared, end, a.prefix_splits + split, true};
   }
@@ -796,7 +807,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
   const unsigned d = 128 * part + 2 * lane;
   float2 g = {0.0F, 0.0F};
   if (a.gate != nullptr) g = *reinterpret_cast<const float2*>(a.gate + static_cast<std::size_t>(row) * 2 * D + D + d);
-  const uint32_t shared = prefix_length(a), end = a.pages.lengths[listed_slot(a.list, i)] + a.tokens;
+  const uint32_t shared = prefix_length(a), end = committed(a.pages, listed_slot(a.list, i)) + a.tokens;
   const uint32_t prefix = a.prefix_splits != 0 ? splits_used((shared + kBlock - 1) / kBlock, a.prefix_splits, kPrefixBlocks) : 0u;
   const uint32_t items = prefix + splits_used(own_blocks(shared, end), a.own_splits, kOwnBlocks);
   const uint32_t skipped = a.prefix_splits - prefix;  // unused between the prefix's items and the own ones
@@ -859,21 +870,26 @@ Shape shape_of(const KvPages& p, uint32_t kv_heads, uint32_t head_size, uint32_t
   const uint32_t all = count * tokens * group, one = tokens * group;
   s.prefix_tiles = row_tiles(all, head_size, false);
   s.own_tiles = row_tiles(one, head_size, true);
-  // Workgroups for every place on the GPU, but a prefix whose pieces would get shorter than
-  // 2 kPrefixBlocks by that only one for every CU (32 sequences on 4096 positions: 16 splits
-  // 23 us with their merge, 32 of them 25 us; 8 verify blocks on 2000 positions at head size
-  // 256: 7 splits 32 us, 15 of them 27 us).
-  auto fill = [head_size](uint32_t ranges, uint32_t tiles) {
-    return std::max(1u, 8 * (kComputeUnits / 8 * resident(head_size) / tiles) / ranges);
-  };
-  const uint32_t blocks = (shared + kBlock - 1) / kBlock, ranges = s.prefix_tiles * kv_heads;
+  // Workgroups for the places of an XCD, all row tiles of a range on one (see spread_groups).
+  auto splits = [](uint32_t workgroups, uint32_t tiles, uint32_t ranges) { return std::max(1u, workgroups / 8 / tiles * 8 / ranges); };
+  // The prefix: a workgroup for every CU, of four blocks or more.  At head size 128 a CU holds a
+  // second one, which is left to the own positions until the pieces pass 48 blocks (64 sequences
+  // with few own positions: on 8192 with one a CU 38 us, with two 41; on 16384 59 and 58, on
+  // 32768 105 and 97, on 65536 194 and 170; on 32768 with 100..900 own positions 119 and 122).
+  // At 256 there is no second place, so the own positions have up to a quarter of the GPU left
+  // (none: 10 sequences on 16000 35.5 us, not 29.7, 32 rows of one 53.7 us, not 45.6; up to half:
+  // 25 sequences 57.5 us, not 49.1).
+  const uint32_t blocks = (shared + kBlock - 1) / kBlock;
   if (shared != 0) {
-    s.prefix_splits = std::max({1u, std::min(kComputeUnits / ranges, blocks / kPrefixBlocks),
-                                std::min(fill(kv_heads, s.prefix_tiles), blocks / (2 * kPrefixBlocks))});
+    const uint32_t left = head_size == 256 ? std::min(count * kv_heads * s.own_tiles, kComputeUnits / 4) : 0u;
+    uint32_t most = splits(kComputeUnits - left, s.prefix_tiles, kv_heads);
+    if (blocks / most > 48) most = splits(kComputeUnits * resident(head_size) - left, s.prefix_tiles, kv_heads);
+    s.prefix_splits = std::max(1u, std::min(most, blocks / kPrefixBlocks));
   }
+  // Own positions: a workgroup for every place, if all sequences fill their tables.
   const uint64_t capacity = (static_cast<uint64_t>(p.stride) << p.page_shift) - shared;
   s.own_splits = static_cast<uint32_t>(std::clamp<uint64_t>(capacity / (kBlock * kOwnBlocks), 1,
-                                                            fill(kv_heads * count, s.own_tiles)));
+                                                            splits(kComputeUnits * resident(head_size), s.own_tiles, kv_heads * count)));
   return s;
 }
 
