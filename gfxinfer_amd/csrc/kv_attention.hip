@@ -794,7 +794,9 @@ __global__ __launch_bounds__(kWaves * 64, resident(D) * kWaves / 4) void paged_a
 
 // Merges a row's items and applies the gate: one wave per (row, 128 dims), two dims a lane.
 // Lane s holds item s's maximum and sum, so its weight is computed once; the outputs are
-// loaded kBatch at a time ahead of their use.
+// loaded kBatch at a time ahead of their use (issued before the maxima are known, or 16 at a
+// time, they were no faster: the registers leave fewer waves).  Bound by its chain of lengths,
+// maxima and outputs: 1280 rows of up to 18 items 5.4 us, 2560 of 22 8.2 us.
 template <unsigned D>
 __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
   constexpr unsigned kGroups = D / 128, kBatch = 8;

@@ -192,6 +192,8 @@ __global__ __launch_bounds__(kThreads) void logit_rules_kernel(RulesArgs a) {
   }
 }
 
+// The largest of a row's slice keys: a second launch, one load chain (2.6 us for 75 keys a row,
+// 4.6 us for 38 keys of 256 rows).
 __global__ __launch_bounds__(kThreads) void rule_tokens_kernel(const unsigned long long* __restrict__ keys,
                                                                uint32_t slices, uint32_t* __restrict__ tokens) {
   __shared__ unsigned long long partial[kThreads / 64];

@@ -627,7 +627,8 @@ typedef struct gfxinfer_kv_pages {
 } gfxinfer_kv_pages;
 
 /* Bytes of device workspace (16-byte aligned) that reserve and compact need; 0 for an
- * invalid description.  Its contents need not be kept between calls. */
+ * invalid description.  Its contents need not be kept between calls; calls that may run at once
+ * need one each. */
 size_t gfxinfer_kv_pages_workspace_bytes(const gfxinfer_kv_pages* pages);
 
 /* Every page free, every sequence empty (the pools are left as they are). */
@@ -682,7 +683,8 @@ int32_t gfxinfer_launch_kv_pages_compact(const gfxinfer_kv_pages* pages, uint32_
                                          size_t workspace_bytes, void* stream);
 
 /* Bytes of device workspace (16-byte aligned) of gfxinfer_launch_kv_pages_gated_attention; 0
- * for invalid arguments. */
+ * for invalid arguments.  Its contents need not be kept between calls; calls that may run at
+ * once need one each. */
 size_t gfxinfer_kv_pages_attention_workspace_bytes(const gfxinfer_kv_pages* pages, uint32_t count, uint32_t tokens,
                                                    uint32_t q_heads, size_t shared_tokens);
 
@@ -737,7 +739,8 @@ typedef struct gfxinfer_logit_rules {
   uint32_t allowed_stride;         /* at least vocabulary_size / 32, rounded up */
 } gfxinfer_logit_rules;
 
-/* Bytes of device workspace (8-byte aligned) the greedy pick needs; 0 for invalid sizes. */
+/* Bytes of device workspace (8-byte aligned) the greedy pick needs; 0 for invalid sizes.
+ * Calls that may run at once need one each. */
 size_t gfxinfer_logit_rules_workspace_bytes(size_t vocabulary_size, uint32_t batch);
 
 /* Applies the rules to logits [batch][row_stride], of which the first vocabulary_size of a
