@@ -253,7 +253,7 @@ struct Rows {
       const __half* src = a.query + static_cast<std::size_t>(out_row) * D + 8 * kb;
 #pragma unroll
       for (unsigned s = 0; s < D / 32; ++s) q[s] = *reinterpret_cast<const h8*>(src + 32 * s);
-      visible = Own ? hi - a.tokens + t + 1 : min(a.pages.lengths[a.list.slot[base + i]] + t + 1, hi);
+      visible = Own ? hi - a.tokens + t + 1 : min(min(a.pages.lengths[a.list.slot[base + i]], hi) + t + 1, hi);
     }
     // Own: the first row sees least.  Prefix: every row sees all of it unless the caller's
     // prefix is longer than a sequence, and then every block is treated as an edge.
@@ -532,9 +532,10 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
       bool strange = false;
       if (edge || careful) {
         // V rows no one sees become zeros (what a page holds past a sequence's end may be
-        // anything, and 0 * NaN would be NaN).
+        // anything, and 0 * NaN would be NaN); nearly always those from the end on.
+        const bool end_only = !careful && missing == 0 && at >= w.lo;
 #pragma unroll 1
-        for (unsigned u = 0; u < kLoads; ++u) {
+        for (unsigned u = end_only ? (w.hi - at) / kLoadRows : 0; u < kLoads; ++u) {
           const unsigned t = u / (kLoads / 2), r = kLoadRows * u + fresh / (D / 8);
           u32x4* piece = reinterpret_cast<u32x4*>(vs + kLoadRows * u * D) + fresh;
           if (at + r < w.lo || at + r >= w.hi || (missing >> t & 1u) != 0) *piece = u32x4{0, 0, 0, 0};
@@ -886,7 +887,7 @@ Shape shape_of(const KvPages& p, uint32_t kv_heads, uint32_t head_size, uint32_t
     const uint32_t left = head_size == 256 ? std::min(count * kv_heads * s.own_tiles, kComputeUnits / 4) : 0u;
     uint32_t most = splits(kComputeUnits - left, s.prefix_tiles, kv_heads);
     if (blocks / most > 48) most = splits(kComputeUnits * resident(head_size) - left, s.prefix_tiles, kv_heads);
-    s.prefix_splits = std::max(1u, std::min(most, blocks / kPrefixBlocks));
+    s.prefix_splits = std::max(1u, std::min(most, (blocks + kPrefixBlocks - 1) / kPrefixBlocks));
   }
   // Own positions: a workgroup for every place, if all sequences fill their tables.
   const uint64_t capacity = (static_cast<uint64_t>(p.stride) << p.page_shift) - shared;

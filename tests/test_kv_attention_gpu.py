@@ -284,3 +284,32 @@ def test_results_repeat_and_replay(device, gx):
         graph.replay()
         p.check(host(out))
     assert np.array_equal(host(out).view(np.uint16), first.view(np.uint16))
+
+
+ROWS = [(A, 2, 4), (A, 3, 7), (A, 1, 17), (B, 5, 6), (B, 3, 11), (B, 1, 32), (B, 9, 15)]
+
+
+@pytest.mark.parametrize("own", [1, 33, 64, 65, 128, 130])
+@pytest.mark.parametrize("heads,count,tokens", ROWS)
+def test_row_counts_at_the_edges_of_tiles(device, gx, heads, count, tokens, own):
+    """Row counts around 16, 32 and 128 of a KV head, ends around the blocks and tiles of positions."""
+    rng = np.random.default_rng(count * 100 + tokens + own)
+    shared = [0, 63, 129, 256][(count + own) % 4]
+    lengths = [max(shared, shared + own - tokens + 3 * i) for i in range(count)]
+    p = Problem(rng, *heads, 16, lengths, tokens, shared)
+    say("edges", heads, count, tokens, shared, own)
+    p.check(p.run(gx))
+
+
+@pytest.mark.parametrize("heads,tokens", [(A, 1), (A, 7), (B, 1), (B, 7)])
+def test_a_damaged_length_stays_its_own_fault(device, gx, heads, tokens):
+    """A length past the table leads to missing pages, not past the table; the other sequences keep their results."""
+    rng = np.random.default_rng(tokens)
+    p = Problem(rng, *heads, 32, [100, 90, 131], tokens, 64)
+    p.lengths[1] = -1                                         # 2^32 - 1
+    say("damaged length", heads, tokens)
+    got = p.run(gx)
+    p.lengths[1] = 90
+    for i in (0, 2):
+        want, tol = p.expect(i)
+        assert np.all(np.abs(got[i].astype(np.float64) - want) <= tol)
