@@ -372,8 +372,9 @@ class KvPages(ctypes.Structure):
         sequences, stride = page_table.shape
         if (tuple(value_pages.shape) != tuple(key_pages.shape) or tuple(lengths.shape) != (sequences,)
                 or tuple(references.shape) != (pages,) or not all(t.is_contiguous() for t in tensors)
-                or any(t.element_size() != size for t, size in zip(tensors, (2, 2, 4, 4, 4)))):
-            raise ValueError("K/V pages: pools of one shape in 16 bits, 32-bit state, all contiguous")
+                or any(t.element_size() != size for t, size in zip(tensors, (2, 2, 4, 4, 4)))
+                or any(str(t.dtype) == "torch.bfloat16" for t in tensors)):
+            raise ValueError("K/V pages: fp16 pools of one shape, 32-bit state, all contiguous")
         self = cls(*(_p(t) for t in tensors), layers, pages, page_tokens, kv_heads, head_size, sequences, stride)
         self.tensors = tensors
         return self
@@ -385,7 +386,7 @@ def _bytes(workspace) -> int:
 
 def _host_ids(values):
     """A host list of uint32 in memory the caller keeps for the call (an array is passed as it is)."""
-    return values if isinstance(values, array) and values.itemsize == 4 else array("I", values)
+    return values if isinstance(values, array) and values.typecode == "I" else array("I", values)
 
 
 def kv_pages_workspace_bytes(pages) -> int:
@@ -469,6 +470,7 @@ class LogitRules(ctypes.Structure):
         bias_values [batch, entries], allowed [masks, words], the others [batch]."""
         self = cls()
         wide = ("history", "bias_tokens", "bias_values", "allowed")
+        real = ("repetition", "presence", "frequency", "bias_values")
         for name, t in tensors.items():
             if name not in dict(cls._fields_[:12]):
                 raise TypeError(f"no logit rule is called {name}")
@@ -476,6 +478,8 @@ class LogitRules(ctypes.Structure):
                 continue
             if not t.is_contiguous() or t.element_size() != 4 or t.dim() != (2 if name in wide else 1):
                 raise ValueError(f"logit rules: {name} is a contiguous 32-bit {'matrix' if name in wide else 'vector'}")
+            if t.is_floating_point() != (name in real):
+                raise ValueError(f"logit rules: {name} holds {'fp32 numbers' if name in real else '32-bit integers'}")
             setattr(self, name, _p(t))
         shape = lambda name: tuple(tensors[name].shape) if tensors.get(name) is not None else (0, 0)  # noqa: E731
         if shape("bias_tokens") != shape("bias_values"):
@@ -500,10 +504,13 @@ def launch_logit_rules(logits, rules, output, tokens, workspace, vocabulary=None
     batch, columns = logits.shape
     if rules.batch not in (None, batch):
         raise ValueError("logit rules: made for another number of rows")
+    vocabulary = columns if vocabulary is None else vocabulary
     for t in (logits,) if output is None else (logits, output):
-        if t.stride(1) != 1 or t.element_size() != 4 or t.shape[0] != batch:
-            raise ValueError("logit rules: logits are fp32 [batch, columns] with dense rows")
-    check(lib().gfxinfer_launch_logit_rules(_p(logits), logits.stride(0), columns if vocabulary is None else vocabulary, batch,
+        if t.stride(1) != 1 or t.element_size() != 4 or t.shape[0] != batch or t.shape[1] < vocabulary:
+            raise ValueError("logit rules: logits are fp32 [batch, columns] with dense rows that hold the vocabulary")
+    if tokens is not None and (tokens.numel() < batch or tokens.element_size() != 4 or not tokens.is_contiguous()):
+        raise ValueError("logit rules: tokens is a contiguous 32-bit vector with an entry per row")
+    check(lib().gfxinfer_launch_logit_rules(_p(logits), logits.stride(0), vocabulary, batch,
                                             ctypes.byref(rules), _p(output), 0 if output is None else output.stride(0),
                                             _p(tokens), _p(workspace), _bytes(workspace), _stream(stream)))
 

@@ -119,3 +119,21 @@ def test_descriptions_from_tensors_check_shapes(gx):
                 (k, k, table.long(), lengths, references)):
         with pytest.raises(ValueError):
             gx.KvPages.of(*bad)
+
+
+def test_pages_are_not_bfloat16_and_lists_are_whole_numbers(gx):
+    import array
+
+    import torch
+    pool = torch.zeros((1, 4, 16, 2, 128), dtype=torch.bfloat16)
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError):
+        gx.KvPages.of(pool, pool, i(3, 4), i(3), i(4))
+    pages = gx.KvPages.of(pool.half(), pool.half(), i(3, 4), i(3), i(4))
+    for bad in (array.array("f", [1.0]), [1.5]):
+        with pytest.raises(TypeError):
+            gx.launch_kv_pages_fork(pages, 0, bad, stream=0)
+    with pytest.raises(OverflowError):
+        gx.launch_kv_pages_fork(pages, 0, [-1], stream=0)
+    with pytest.raises(gx.GfxinferError):
+        gx.launch_kv_pages_fork(pages, 0, array.array("I", [9]), stream=0)

@@ -79,3 +79,18 @@ def test_rules_from_tensors_check_shapes(gx):
                            (f(4, 70), f(3, 70))):
         with pytest.raises(ValueError):
             gx.launch_logit_rules(logits, rules, output, i(4), i(100), stream=0)
+
+
+def test_rules_from_tensors_check_types_and_room(gx):
+    import torch
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    f = lambda *s: torch.zeros(s)  # noqa: E731
+    for bad in (dict(presence=i(2)), dict(repetition=i(2)), dict(history=f(2, 9)), dict(bias_counts=f(2)), dict(allowed=f(2, 3)),
+                dict(bias_tokens=i(2, 3), bias_values=i(2, 3))):
+        with pytest.raises(ValueError):
+            gx.LogitRules.of(**bad)
+    rules = gx.LogitRules.of(presence=f(4))
+    for output, tokens, vocabulary in ((None, i(3), 70), (None, i(8)[::2], 70), (None, i(4).long(), 70), (None, i(4), 71),
+                                       (f(4, 60), i(4), 70)):
+        with pytest.raises(ValueError):
+            gx.launch_logit_rules(f(4, 70), rules, output, tokens, i(100), vocabulary, stream=0)
