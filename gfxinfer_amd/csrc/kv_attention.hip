@@ -26,10 +26,12 @@
 // of two kernels took 6 us more).
 //
 // What bounds it: with few rows the reads of the cache (64 sequences of 100..900 own positions,
-// 8 x 128: 134 MB in 33 us, 4.1 TB/s); with many the waves' own instructions, of which a tile of
-// 64 positions x 16 rows takes 48 matrix products (768 cycles of a SIMD) and about 180 others
-// (900 cycles): 64 sequences on 32768 shared positions, 320 rows of a KV head, 90 us and 480
-// TFLOP/s, 720 with the second product of the weights' low halves.
+// 8 x 128: 134 MB in 33 us, 4.1 TB/s).  With many, three things that overlap only in part, since
+// the waves of a workgroup reach them together: 64 sequences on 32768 shared positions (320 rows
+// of a KV head, 480 TFLOP/s, 720 with the second product of the weights) take 91 us, of which
+// the matrix units of the fullest SIMDs are busy 45 %, their vector units 53 % and the LDS reads
+// take about as much; in copies that leave one out they take 79 us without the second product,
+// 81 us without the softmax and 90 us with an eighth of the reads of V.
 #include <algorithm>
 #include <cmath>
 
@@ -714,7 +716,6 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
         for (unsigned b = 0; b < T / kBlock; ++b) rows.score(key_at + rows_at + b * kBlock * D * 2, s[2 * b], s[2 * b + 1]);
         const bool edge = at < w.lo || at + T > rows.least || (mark & 0xffu) != 0;
         h8 high[T / kBlock], low[T / kBlock];
-        __builtin_amdgcn_s_setprio(1);
         rows.weigh(s, fresh, a.scale, edge, at, w.lo, mark, high, low);
         if ((mark & 0x100u) != 0) rows.add_strange(s, pg, values, w.slot, at, w.lo, w.hi);
 #pragma unroll
@@ -726,7 +727,6 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
             rows.add(v, d, high[b], low[b]);
           }
         }
-        __builtin_amdgcn_s_setprio(0);
       }
       slot = (slot + 1) % R;
     }
