@@ -44,11 +44,10 @@ using h8 = _Float16 __attribute__((ext_vector_type(8)));
 using f4 = float __attribute__((ext_vector_type(4)));
 using u32x4 = unsigned __attribute__((ext_vector_type(4)));
 using s16x4 = short __attribute__((ext_vector_type(4)));
-using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 using lds_void = __attribute__((address_space(3))) void;
 using global_void = __attribute__((address_space(1))) void;
 
-constexpr unsigned kBlock = 32;  // positions of one step of a wave
+constexpr unsigned kBlock = 32;  // positions: a step of a wave by positions, half of one by rows
 constexpr float kLog2E = 1.4426950408889634F;
 
 constexpr unsigned kWaves = 8;     // of a workgroup; by rows: 128 rows
