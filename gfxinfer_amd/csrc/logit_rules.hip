@@ -35,7 +35,9 @@ constexpr uint32_t kMaxHistory = (1u << 19) - 1;
 constexpr uint32_t kMaxBias = (1u << 12) - 1;
 
 constexpr unsigned kThreads = 256;
-constexpr unsigned kHistoryLoads = 8;  // history tokens a lane has on their way at once
+// History tokens a lane has on their way at once (256 rows x 151936 with 2000-token histories:
+// 8 of them 73.7 us, 4 of them 77 us in more rounds, 16 of them 90 us with fewer waves).
+constexpr unsigned kHistoryLoads = 8;
 
 struct RulesArgs {
   gfxinfer_logit_rules rules;
