@@ -42,6 +42,8 @@ namespace {
 
 using h8 = _Float16 __attribute__((ext_vector_type(8)));
 using f4 = float __attribute__((ext_vector_type(4)));
+using h2 = _Float16 __attribute__((ext_vector_type(2)));
+using f2 = float __attribute__((ext_vector_type(2)));
 using u32x4 = unsigned __attribute__((ext_vector_type(4)));
 using s16x4 = short __attribute__((ext_vector_type(4)));
 using lds_void = __attribute__((address_space(3))) void;
@@ -49,6 +51,17 @@ using global_void = __attribute__((address_space(1))) void;
 
 constexpr unsigned kBlock = 32;  // positions: a step of a wave by positions, half of one by rows
 constexpr float kLog2E = 1.4426950408889634F;
+
+// A row's weights are 2^(score - m + kLift), scores in units of log2.  The stored maximum m follows
+// the maxima of the blocks of positions, downwards too, once one leaves [m - kFall, m + kRise], but
+// stays within kSpan of its highest value so that the sums fit fp32.  The largest weight of every
+// block so lies between 2^3 and 2^15, near the top of fp16, and 2^-25, half of fp16's last place, is
+// at least 2^28 below it.  (At most 2^8, cut off at 2^-24 and never raised again, the weights beside
+// a score 16 nats above 600 others lost 16 % of their sum.)
+constexpr float kLift = 11.0F, kRise = 4.0F, kFall = 8.0F, kSpan = 32.0F;
+// In a block that moves m, weights below 2^kSmall are multiplied on their own, times kSmallScale:
+// down to 2^-49, 41 nats below m.
+constexpr float kSmall = -9.0F, kSmallScale = 0x1p24F;
 
 constexpr unsigned kWaves = 8;     // of a workgroup; by rows: 128 rows
 constexpr unsigned kPosWaves = 4;  // of them, those that divide positions: a block of K and of V each in LDS
@@ -122,8 +135,11 @@ __device__ __forceinline__ float max_over_quarters(float v) {
   return __builtin_elementwise_maximum(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 __device__ __forceinline__ float sum_over_quarters(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  const unsigned u = __float_as_uint(v);
+  const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const unsigned w = __float_as_uint(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
 // Waits until at most Loads of the wave's loads from memory are on their way, and for all of
@@ -216,8 +232,8 @@ __device__ __forceinline__ void read_values(unsigned place, unsigned first, h8 (
 // The lane's number, made anew: what is computed from it inside a loop is not kept in
 // registers around the loop, where 128 of them do not suffice.
 __device__ __forceinline__ unsigned fresh_lane() {
-  unsigned lane = threadIdx.x & 63u;
-  asm volatile("" : "+v"(lane));
+  unsigned lane;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
   return lane;
 }
 
@@ -228,24 +244,27 @@ __device__ __forceinline__ uint32_t fresh_number(uint32_t x) {
 }
 
 // Sixteen rows of a wave: lane column n's row is the query q (B operand), sees the positions
-// below `visible`, and its result goes to row out_row (none: 0xffffffff).
+// below `visible`.
 template <unsigned D>
 struct Rows {
   h8 q[D / 32];
-  uint32_t visible, out_row;
+  uint32_t visible;
   uint32_t least;  // of visible over the rows
   f4 o[D / 16];
   float m, l;  // m in units of log2; l of the lane's own positions
+  float peak;  // the highest m so far
 
   // Rows first + n of `rows`; row = (i * tokens + t) * group + g, i counted from `base`.  Own:
-  // the rows are one sequence's, with hi - tokens committed positions.
+  // the rows are one sequence's, with hi - tokens committed positions.  The rows of the output
+  // (none: 0xffffffff) wait in LDS at out_rows: kept in a register they cost a spill, whose store
+  // the first loads then wait for (200 sequences of 250..500 positions: 81 us, not 75).
   template <bool Own>
   __device__ __forceinline__ void load(const PagedAttnArgs& a, uint32_t base, uint32_t first, uint32_t rows, uint32_t hk,
-                                       uint32_t hi) {
+                                       uint32_t hi, uint32_t* out_rows) {
     const unsigned lane = threadIdx.x & 63u, kb = lane >> 4;
     const uint32_t group = a.q_heads / a.kv_heads, row = first + (lane & 15u);
+    uint32_t out_row = 0xffffffffu;
     visible = 0;
-    out_row = 0xffffffffu;
 #pragma unroll
     for (unsigned s = 0; s < D / 32; ++s) q[s] = h8{};
     if (row < rows) {
@@ -260,6 +279,7 @@ struct Rows {
     // prefix is longer than a sequence, and then every block is treated as an edge.
     if (Own) least = first < rows ? hi - a.tokens + first / group + 1 : 0xffffffffu;
     else least = __all(row >= rows || visible == hi) ? hi : 0u;
+    if (lane < 16u) out_rows[lane] = out_row;
   }
 
   // The queries have arrived here: a wait for them inside a loop would wait for the loop's
@@ -270,7 +290,7 @@ struct Rows {
   }
 
   __device__ __forceinline__ void clear() {
-    m = -INFINITY;
+    m = peak = -INFINITY;
     l = 0.0F;
 #pragma unroll
     for (unsigned d = 0; d < D / 16; ++d) o[d] = f4{0, 0, 0, 0};
@@ -303,15 +323,63 @@ struct Rows {
     }
   }
 
+  // p = high + low, both rounded to nearest: off by 2^-23 p, or by 2^-25 if that is more.
+  static __device__ __forceinline__ void halves(float p0, float p1, h8& high, h8& low, unsigned at) {
+    const h2 h = __builtin_convertvector((f2{p0, p1}), h2);
+    const h2 rest = __builtin_convertvector((f2{p0 - static_cast<float>(h[0]), p1 - static_cast<float>(h[1])}), h2);
+#pragma unroll
+    for (unsigned e = 0; e < 2; ++e) {
+      high[at + e] = h[e];
+      low[at + e] = rest[e];
+    }
+  }
+
+  // Takes the small weights out of the scores s of a block and adds their products.  The outputs
+  // are scaled for that and back: powers of two, so nothing is rounded, and no registers.
+  template <unsigned T>
+  __device__ __forceinline__ void add_small(f4 (&s)[T], float scale, unsigned value_at, bool moved) {
+#pragma unroll
+    for (unsigned d = 0; d < D / 16; ++d) o[d] *= kSmallScale;
+#pragma unroll
+    for (unsigned b = 0; b < T / 2; ++b) {
+      h8 high, low;
+#pragma unroll
+      for (unsigned e = 0; e < 8; e += 2) {
+        float p[2];
+#pragma unroll
+        for (unsigned u = 0; u < 2; ++u) {
+          const float x = fmaf(s[2 * b + e / 4][e % 4 + u], scale, kLift - m);
+          const bool here = moved && x < kSmall;
+          p[u] = here ? __builtin_amdgcn_exp2f(x) : 0.0F;
+          if (here) s[2 * b + e / 4][e % 4 + u] = -INFINITY;
+          l += p[u];
+          p[u] *= kSmallScale;
+        }
+        halves(p[0], p[1], high, low, e);
+      }
+#pragma unroll
+      for (unsigned d = 0; d < D / 16; d += 4) {
+        h8 v[4];
+        read_values<D>(value_at + b * kBlock * D * 2, d, v);
+        add(v, d, high, low);
+      }
+    }
+#pragma unroll
+    for (unsigned d = 0; d < D / 16; ++d) o[d] *= 1.0F / kSmallScale;
+  }
+
   // The weights of T tiles of 16 positions from `at`: s the scores (raw products), the weights
   // afterwards.  An edge block holds positions that some row does not see (below lo, past its
   // end, or in a tile of 16 whose page is missing: bit t of `missing`).
   //
-  // The weights go out as an fp16 pair p = high + low, high cut off and low the rest: two
-  // products carry about 22 bits of p, so the output keeps the accuracy of an fp32 product.
-  template <unsigned T>
+  // The weights go out as fp16 pairs, which keeps the accuracy of an fp32 product unless one score
+  // lies far above the others of its block and the others carry the output (its value is near
+  // zero): then, with `split`, add_small takes the others.  ready() returns when the block's V rows
+  // are in LDS at value_at, zeros where no row sees them.
+  template <unsigned T, typename Ready>
   __device__ __forceinline__ void weigh(f4 (&s)[T], unsigned lane, float scale, bool edge, uint32_t at, uint32_t lo,
-                                        unsigned missing, h8 (&high)[T / 2], h8 (&low)[T / 2]) {
+                                        unsigned missing, bool split, unsigned value_at, Ready ready, h8 (&high)[T / 2],
+                                        h8 (&low)[T / 2]) {
     if (edge) {
       const unsigned kb = lane >> 4;
 #pragma unroll
@@ -328,17 +396,35 @@ struct Rows {
 #pragma unroll
     for (unsigned r = 1; r < 4 * T; ++r) best = __builtin_elementwise_maximum(best, s[r / 4][r % 4]);
     const float top = max_over_quarters(best) * scale;
-    // The stored maximum moves only when a row's grows by more than 8 (a factor of 256):
-    // weights stay below 2^8 and most blocks skip the rescaling.
-    if (__any(top > m + 8.0F)) {
-      const float next_m = fmaxf(m, top);
-      const float factor = next_m == -INFINITY ? 1.0F : __builtin_amdgcn_exp2f(m - next_m);
+    // Most blocks skip this.  m moves only for the rows that need it, so that a row's result does
+    // not depend on the scores of the others.
+    if (__any(fabsf(top - (m - 0.5F * (kFall - kRise))) > 0.5F * (kFall + kRise))) {
+      const float target = fmaxf(top, peak - kSpan);
+      const float next_m = top > m + kRise ? top : top != -INFINITY && target < m - kFall ? target : m;
+      const float factor = next_m == m ? 1.0F : __builtin_amdgcn_exp2f(m - next_m);
       m = next_m;
+      peak = fmaxf(peak, m);
       l *= factor;
 #pragma unroll
       for (unsigned d = 0; d < D / 16; ++d) o[d] *= factor;
+      float least_score = s[0][0];
+#pragma unroll
+      for (unsigned e = 1; e < 4 * T; ++e) least_score = __builtin_elementwise_minimum(least_score, s[e / 4][e % 4]);
+      if (edge) {  // of the positions that are seen
+        least_score = INFINITY;
+#pragma unroll
+        for (unsigned e = 0; e < 4 * T; ++e) {
+          const float x = s[e / 4][e % 4];
+          least_score = __builtin_elementwise_minimum(least_score, x == -INFINITY ? INFINITY : x);
+        }
+      }
+      const bool moved = factor != 1.0F;
+      if (__builtin_expect(split && __any(moved && fmaf(least_score, scale, kLift - m) < kSmall), 0)) {
+        ready();
+        add_small(s, scale, value_at, moved);
+      }
     }
-    const float floor = m == -INFINITY ? 0.0F : m;
+    const float floor = m == -INFINITY ? 0.0F : m - kLift;
 #pragma unroll
     for (unsigned t = 0; t < T; ++t) {
 #pragma unroll
@@ -349,12 +435,7 @@ struct Rows {
         s[t][r + 1] = p1;
         l += p0;
         l += p1;
-        const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-        high[t / 2][t % 2 * 4 + r] = h[0];
-        high[t / 2][t % 2 * 4 + r + 1] = h[1];
-        const auto rest = __builtin_amdgcn_cvt_pkrtz(p0 - static_cast<float>(h[0]), p1 - static_cast<float>(h[1]));
-        low[t / 2][t % 2 * 4 + r] = rest[0];
-        low[t / 2][t % 2 * 4 + r + 1] = rest[1];
+        halves(p0, p1, high[t / 2], low[t / 2], t % 2 * 4 + r);
       }
     }
   }
@@ -450,20 +531,40 @@ struct Item {
   bool own;
 };
 
+// Whether x holds in any lane of the workgroup.  flags: a word per wave, used once.
+__device__ __forceinline__ bool in_any_wave(bool x, unsigned wave, uint32_t* flags) {
+  const bool mine = __any(x);
+  if (fresh_lane() == 0) flags[wave] = mine ? 1u : 0u;
+  __syncthreads();
+  uint32_t found = 0;
+#pragma unroll
+  for (unsigned v = 0; v < kWaves; ++v) found |= flags[v];
+  return __builtin_amdgcn_readfirstlane(found) != 0;
+}
+
+// Tiles of K and V rows and their marks (attend_rows); the output rows of 16 rows a wave and the
+// waves' flags follow.
+template <unsigned D>
+constexpr std::size_t rows_bytes() {
+  return kRing * (kTile * D * 2 * 2 + 4 * kWaves);
+}
+
 // Sixteen rows; the waves divide the positions.
 template <unsigned D>
 __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const Item& w, char* smem) {
   constexpr unsigned kTiles = D / 16;
   constexpr unsigned kLoads = kBlock * D / 8 / 64;   // of a block's K rows, and of its V rows, per lane
   constexpr unsigned kLoadRows = 64 / (D / 8);       // rows one of them covers
-  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const KvPages& pg = a.pages;
   const uint32_t in_page = (1u << pg.page_shift) - 1;
   PageWindow window;
   window.start(pg, w.slot, (w.start + min(w.first_block + wave, w.last_block - 1) * kBlock) >> pg.page_shift);
+  uint32_t* flags = reinterpret_cast<uint32_t*>(smem + rows_bytes<D>());
+  uint32_t* out_rows = flags + kWaves + 16 * wave;
   Rows<D> rows;
-  if (w.own) rows.template load<true>(a, w.base, w.first, w.rows, w.hk, w.hi);
-  else rows.template load<false>(a, w.base, w.first, w.rows, w.hk, w.hi);
+  if (w.own) rows.template load<true>(a, w.base, w.first, w.rows, w.hk, w.hi, out_rows);
+  else rows.template load<false>(a, w.base, w.first, w.rows, w.hk, w.hi, out_rows);
   const __half* keys = head_rows(a, pg.key, w.hk, D);
   const __half* values = head_rows(a, pg.value, w.hk, D);
   _Float16* ks = reinterpret_cast<_Float16*>(smem) + wave * 2 * kBlock * D;
@@ -525,25 +626,39 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
         find_pages(at + kPosWaves * kBlock, page);
         load_k(at + kPosWaves * kBlock, page);
       }
-      h8 high[1], low[1];
-      rows.weigh(s, fresh, a.scale, edge, at, w.lo, missing, high, low);
       // The V rows are there when only the next K rows are on their way.
-      if (more) wait_loads<kLoads>();
-      else wait_loads<0>();
-      bool strange = false;
-      if (edge || careful) {
-        // V rows no one sees become zeros (what a page holds past a sequence's end may be
-        // anything, and 0 * NaN would be NaN); nearly always those from the end on.
-        const bool end_only = !careful && missing == 0 && at >= w.lo;
+      auto values_arrive = [&]() __attribute__((always_inline)) {
+        if (more) wait_loads<kLoads>();
+        else wait_loads<0>();
+      };
+      // V rows no one sees become zeros (what a page holds past a sequence's end may be anything,
+      // and 0 * NaN would be NaN); nearly always those from the end on.
+      auto clear_unseen = [&]() __attribute__((always_inline)) {
+        const unsigned fresh = fresh_lane();
 #pragma unroll 1
-        for (unsigned u = end_only ? (w.hi - at) / kLoadRows : 0; u < kLoads; ++u) {
+        for (unsigned u = missing == 0 && at >= w.lo ? (w.hi - at) / kLoadRows : 0; u < kLoads; ++u) {
           const unsigned t = u / (kLoads / 2), r = kLoadRows * u + fresh / (D / 8);
           u32x4* piece = reinterpret_cast<u32x4*>(vs + kLoadRows * u * D) + fresh;
           if (at + r < w.lo || at + r >= w.hi || (missing >> t & 1u) != 0) *piece = u32x4{0, 0, 0, 0};
-          if (careful) strange |= take_strange(piece);
         }
         wait_loads<63>();
-        if (__any(strange)) rows.add_strange(s, pg, values, w.slot, at, w.lo, w.hi);
+      };
+      auto ready = [&]() __attribute__((always_inline)) {
+        values_arrive();
+        if (edge) clear_unseen();
+      };
+      h8 high[1], low[1];
+      rows.weigh(s, fresh, a.scale, edge, at, w.lo, missing, !careful, value_at, ready, high, low);
+      values_arrive();
+      if (edge || careful) {
+        if (edge) clear_unseen();
+        if (careful) {
+          bool strange = false;
+#pragma unroll 1
+          for (unsigned u = 0; u < kLoads; ++u) strange |= take_strange(reinterpret_cast<u32x4*>(vs + kLoadRows * u * D) + fresh_lane());
+          wait_loads<63>();
+          if (__any(strange)) rows.add_strange(s, pg, values, w.slot, at, w.lo, w.hi);
+        }
       }
 #pragma unroll
       for (unsigned d = 0; d < kTiles; d += 4) {
@@ -553,7 +668,7 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
       }
       if (more) load_v(at + kPosWaves * kBlock, page);
     }
-    if (careful || !__syncthreads_or(rows.strange())) break;
+    if (careful || !in_any_wave(rows.strange(), wave, flags)) break;
   }
 
   // Merge the waves (a lane holds the same row and dims in every wave): all maxima and
@@ -578,8 +693,9 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
     factor[v] = x.x == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(x.x - best);
     if (x.x != -INFINITY) total += x.y * factor[v];
   }
-  if (rows.out_row == 0xffffffffu) return;
-  const std::size_t at = static_cast<std::size_t>(rows.out_row) * (a.prefix_splits + a.own_splits) + w.split;
+  const uint32_t out_row = out_rows[n];
+  if (out_row == 0xffffffffu) return;
+  const std::size_t at = static_cast<std::size_t>(out_row) * (a.prefix_splits + a.own_splits) + w.split;
 #pragma unroll
   for (unsigned u = 0; u < kTiles / kWaves; ++u) {
     const unsigned d = wave * (kTiles / kWaves) + u;
@@ -592,11 +708,6 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
     *reinterpret_cast<f4*>(a.partial_o + at * D + 16 * d + 4 * kb) = sum;
   }
   if (wave == 0 && kb == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{best, total};
-}
-
-template <unsigned D>
-constexpr std::size_t rows_bytes() {
-  return kRing * (kTile * D * 2 * 2 + 4 * kWaves);
 }
 
 // A barrier that orders LDS accesses and leaves loads from memory into LDS on their way
@@ -675,9 +786,11 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
   };
 
   Rows<D> rows;
+  uint32_t* flags = reinterpret_cast<uint32_t*>(smem + rows_bytes<D>());
+  uint32_t* out_rows = flags + kWaves + 16 * wave;
   const uint32_t first = w.first + wave * 16;
-  if (w.own) rows.template load<true>(a, w.base, first, w.rows, w.hk, w.hi);
-  else rows.template load<false>(a, w.base, first, w.rows, w.hk, w.hi);
+  if (w.own) rows.template load<true>(a, w.base, first, w.rows, w.hk, w.hi, out_rows);
+  else rows.template load<false>(a, w.base, first, w.rows, w.hk, w.hi, out_rows);
   const bool works = first < w.rows;
   // A second, careful pass follows in the rare case that an output of the first is an
   // infinity or NaN, or a page was missing: values and pages are then looked at.
@@ -715,7 +828,7 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
         for (unsigned b = 0; b < T / kBlock; ++b) rows.score(key_at + rows_at + b * kBlock * D * 2, s[2 * b], s[2 * b + 1]);
         const bool edge = at < w.lo || at + T > rows.least || (mark & 0xffu) != 0;
         h8 high[T / kBlock], low[T / kBlock];
-        rows.weigh(s, fresh, a.scale, edge, at, w.lo, mark, high, low);
+        rows.weigh(s, fresh, a.scale, edge, at, w.lo, mark, !careful, value_at + rows_at, [] {}, high, low);
         if ((mark & 0x100u) != 0) rows.add_strange(s, pg, values, w.slot, at, w.lo, w.hi);
 #pragma unroll
         for (unsigned b = 0; b < T / kBlock; ++b) {
@@ -729,15 +842,17 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
       }
       slot = (slot + 1) % R;
     }
-    if (careful || !__syncthreads_or((works && rows.strange()) || lost)) break;
+    if (careful || !in_any_wave((works && rows.strange()) || lost, wave, flags)) break;
   }
   if (!works) return;
   rows.finish();
-  if (rows.out_row == 0xffffffffu) return;
-  const std::size_t to = static_cast<std::size_t>(rows.out_row) * (a.prefix_splits + a.own_splits) + w.split;
+  const unsigned late = fresh_lane();
+  const uint32_t out_row = out_rows[late & 15u];
+  if (out_row == 0xffffffffu) return;
+  const std::size_t to = static_cast<std::size_t>(out_row) * (a.prefix_splits + a.own_splits) + w.split;
 #pragma unroll
-  for (unsigned d = 0; d < D / 16; ++d) *reinterpret_cast<f4*>(a.partial_o + to * D + 16 * d + 4 * (lane >> 4)) = rows.o[d];
-  if (lane < 16) *reinterpret_cast<float2*>(a.partial_ml + 2 * to) = float2{rows.m, rows.l};
+  for (unsigned d = 0; d < D / 16; ++d) *reinterpret_cast<f4*>(a.partial_o + to * D + 16 * d + 4 * (late >> 4)) = rows.o[d];
+  if (late < 16) *reinterpret_cast<float2*>(a.partial_ml + 2 * to) = float2{rows.m, rows.l};
 }
 
 // Whether the waves share an item's rows or its positions.  By positions, every 16 rows read
@@ -760,7 +875,7 @@ __host__ __device__ constexpr uint32_t tile_rows(uint32_t rows, uint32_t tiles) 
 // Work items: the prefix's come before the sequences' own.
 template <unsigned D>
 __global__ __launch_bounds__(kWaves * 64, resident(D) * kWaves / 4) void paged_attention_kernel(PagedAttnArgs a) {
-  __shared__ __align__(1024) char smem[rows_bytes<D>()];
+  __shared__ __align__(1024) char smem[rows_bytes<D>() + 4 * 17 * kWaves];
   const uint32_t shared = prefix_length(a), id = blockIdx.x;
   const uint32_t group = a.q_heads / a.kv_heads, count = a.list.count;
   uint32_t range, tile;

@@ -313,3 +313,47 @@ def test_a_damaged_length_stays_its_own_fault(device, gx, heads, tokens):
     for i in (0, 2):
         want, tol = p.expect(i)
         assert np.all(np.abs(got[i].astype(np.float64) - want) <= tol)
+
+
+def _with_a_peak(rng, heads, page, lengths, tokens, shared, at, above):
+    """Every row's score at position `at` lies `above` nats over the mean of its others, whose own scores spread by one; the
+    value there is zero and all others are positive, large enough that the result is a normal fp16 number.  Nothing but the
+    small weights carries the result, and no loss among them is made up for by another."""
+    p = Problem(rng, *heads, page, lengths, tokens, shared)
+    d = heads[2]
+    p.query[..., 0] = 8
+    size = min(2.0 ** 14, max(1.0, np.exp(above) * 2.0 ** -20))
+    values = [(rng.uniform(0.5, 1.5, x[1].shape) * size).astype(np.float16) for x in p.rows]
+    for i, rows in enumerate(p.rows):
+        rows[0][..., 0] = 0
+        rows[0][at] = 0
+        rows[0][at, :, 0] = above * math.sqrt(d) / 8
+        values[i][:shared] = values[0][:shared]
+        rows[1][...] = values[i]
+        rows[1][at] = 0
+        for j in range(0, len(rows[0]), page):
+            for pool, x in zip((p.k, p.v), rows):
+                pool[1, p.table[i, j // page], :len(x[j:j + page])] = x[j:j + page]
+    return p
+
+
+@pytest.mark.parametrize("above", [10, 12, 14, 16, 20, 25])
+@pytest.mark.parametrize("heads,page,lengths,tokens,shared,at", [
+    ((64, 64, 128), 64, [600] * 8, 1, 0, 5),                  # one item a sequence, by positions
+    ((64, 64, 128), 64, [600] * 8, 1, 0, 333),
+    ((64, 64, 128), 64, [600] * 8, 32, 0, 5),                 # one item a sequence, by rows
+    ((64, 64, 128), 64, [600] * 8, 32, 0, 333),
+    ((64, 64, 256), 64, [600] * 8, 1, 0, 5),
+    ((128, 64, 256), 64, [600] * 8, 17, 0, 333),
+    (A, 16, [2100, 2060, 2200], 1, 2048, 3),                  # many items, the peak in the prefix
+    (A, 16, [2100, 2060, 2200], 3, 2048, 1000),
+    (B, 32, [2100, 2060, 2200], 3, 2048, 3),
+    (A, 16, [40, 33], 1, 0, 39),                              # the peak is the last position of the only block
+])
+def test_small_weights_beside_a_peak_are_kept(device, gx, heads, page, lengths, tokens, shared, at, above):
+    at = min(at, min(lengths))
+    p = _with_a_peak(np.random.default_rng(at + tokens), heads, page, lengths, tokens, shared, at, above)
+    say("peak", heads, lengths[:3], tokens, shared, at, above)
+    got = p.run(gx)
+    some = [0, len(lengths) - 1]
+    p.check(got[some], some)
