@@ -52,6 +52,13 @@ using global_void = __attribute__((address_space(1))) void;
 constexpr unsigned kBlock = 32;  // positions: a step of a wave by positions, half of one by rows
 constexpr float kLog2E = 1.4426950408889634F;
 
+// The factor between sums with maxima `from` and `to`, from <= to nearly always.  Never zero, so
+// that a NaN or an infinity of either reaches the result however far its scores lie below the
+// others (2^-126 of a finite sum is nothing beside theirs).
+__device__ __forceinline__ float rescale_factor(float from, float to) {
+  return fmaxf(__builtin_amdgcn_exp2f(from - to), 0x1p-126F);
+}
+
 // A row's weights are 2^(score - m + kLift), scores in units of log2.  The stored maximum m follows
 // the maxima of the blocks of positions, downwards too, once one leaves [m - kFall, m + kRise], but
 // stays within kSpan of its highest value so that the sums fit fp32.  The largest weight of every
@@ -296,8 +303,8 @@ struct Rows {
     for (unsigned d = 0; d < D / 16; ++d) o[d] = f4{0, 0, 0, 0};
   }
 
-  // Whether an output is an infinity or NaN: weights are below 2^8, so only such values (or
-  // NaN scores) can make one.
+  // Whether an output is an infinity or NaN: weights reach 2^15, 2^47 after m fell, so only such
+  // values (or NaN scores) can make one.
   __device__ __forceinline__ bool strange() const {
     bool found = false;
 #pragma unroll
@@ -374,11 +381,11 @@ struct Rows {
   //
   // The weights go out as fp16 pairs, which keeps the accuracy of an fp32 product unless one score
   // lies far above the others of its block and the others carry the output (its value is near
-  // zero): then, with `split`, add_small takes the others.  ready() returns when the block's V rows
+  // zero): then add_small takes the others.  ready() returns when the block's V rows
   // are in LDS at value_at, zeros where no row sees them.
   template <unsigned T, typename Ready>
   __device__ __forceinline__ void weigh(f4 (&s)[T], unsigned lane, float scale, bool edge, uint32_t at, uint32_t lo,
-                                        unsigned missing, bool split, unsigned value_at, Ready ready, h8 (&high)[T / 2],
+                                        unsigned missing, unsigned value_at, Ready ready, h8 (&high)[T / 2],
                                         h8 (&low)[T / 2]) {
     if (edge) {
       const unsigned kb = lane >> 4;
@@ -401,7 +408,7 @@ struct Rows {
     if (__any(fabsf(top - (m - 0.5F * (kFall - kRise))) > 0.5F * (kFall + kRise))) {
       const float target = fmaxf(top, peak - kSpan);
       const float next_m = top > m + kRise ? top : top != -INFINITY && target < m - kFall ? target : m;
-      const float factor = next_m == m ? 1.0F : __builtin_amdgcn_exp2f(m - next_m);
+      const float factor = next_m == m ? 1.0F : rescale_factor(m, next_m);
       m = next_m;
       peak = fmaxf(peak, m);
       l *= factor;
@@ -419,7 +426,7 @@ struct Rows {
         }
       }
       const bool moved = factor != 1.0F;
-      if (__builtin_expect(split && __any(moved && fmaf(least_score, scale, kLift - m) < kSmall), 0)) {
+      if (__builtin_expect(__any(moved && fmaf(least_score, scale, kLift - m) < kSmall), 0)) {
         ready();
         add_small(s, scale, value_at, moved);
       }
@@ -448,33 +455,25 @@ struct Rows {
     for (unsigned u = 0; u < 4; ++u) o[first + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[u], high, o[first + u], 0, 0, 0);
   }
 
-  // In a careful pass the infinities and NaNs among the values of a block are zeros in LDS,
-  // since a row must not meet those of positions it does not see; here the rows that see them
-  // get their products, one by one from the pages.  s: the weights of the block.
-  template <unsigned T>
-  __device__ __forceinline__ void add_strange(const f4 (&s)[T], const KvPages& pages, const __half* values, uint32_t slot,
+  // In a careful pass the infinities and NaNs among the values of `count` positions are zeros in
+  // LDS, since a row must not meet those of positions it does not see; here the rows that see them
+  // get them, one by one from the pages, whatever the weight: no weight is exactly zero.
+  __device__ __forceinline__ void add_strange(unsigned count, const KvPages& pages, const __half* values, uint32_t slot,
                                               uint32_t at, uint32_t lo, uint32_t hi) {
-    const unsigned lane = threadIdx.x & 63u, n = lane & 15u, kb = lane >> 4;
+    const unsigned kb = fresh_lane() >> 4;
 #pragma unroll 1
-    for (unsigned p = 0; p < 16 * T; ++p) {
+    for (unsigned p = 0; p < count; ++p) {
       const uint32_t position = at + p;
       const int32_t page = position < lo || position >= hi ? -1 : table_page(pages, slot, position >> pages.page_shift);
       if (page < 0) continue;
       const __half* row = values + ((static_cast<std::size_t>(page) << pages.page_shift) +
                                     (position & ((1u << pages.page_shift) - 1))) * pages.row;
-      const unsigned owner = ((p % 16) / 4) * 16 + n;
-      float w = 0.0F;
-#pragma unroll
-      for (unsigned e = 0; e < 4 * T; ++e) {
-        const float x = __shfl(s[e / 4][e % 4], owner);
-        if (e == p / 16 * 4 + p % 4) w = x;
-      }
 #pragma unroll
       for (unsigned d = 0; d < D / 16; ++d) {
 #pragma unroll
         for (unsigned e = 0; e < 4; ++e) {
           const float x = __half2float(row[16 * d + 4 * kb + e]);
-          if (!(fabsf(x) < INFINITY) && position < visible) o[d][e] += w * x;
+          if (!(fabsf(x) < INFINITY) && position < visible) o[d][e] += x;
         }
       }
     }
@@ -482,10 +481,11 @@ struct Rows {
     wait_loads<0>();
   }
 
-  // The row sums, complete; only NaN scores make a NaN row, not an empty one.
-  __device__ __forceinline__ void finish() {
+  // The row sums, complete.  Only NaN scores, and strange values at scores of -infinity, make a NaN
+  // row rather than an empty one.
+  __device__ __forceinline__ void finish(bool careful) {
     l = sum_over_quarters(l);
-    if (l != l && m == -INFINITY) m = 0.0F;
+    if (m == -INFINITY && (l != l || (careful && strange()))) m = 0.0F;
   }
 };
 
@@ -601,7 +601,8 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
 
   // A second, careful pass follows in the rare case that an output of the first is an
   // infinity or NaN: values are then looked at before they are used.
-  for (bool careful = false;; careful = true) {
+  bool careful = false;
+  for (;; careful = true) {
     rows.clear();
     if (careful) window.first = 0xffffffc0u;  // 64 before column 0
     uint32_t block = fresh_number(wave < kPosWaves ? w.first_block + wave : w.last_block);
@@ -626,40 +627,30 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
         find_pages(at + kPosWaves * kBlock, page);
         load_k(at + kPosWaves * kBlock, page);
       }
-      // The V rows are there when only the next K rows are on their way.
-      auto values_arrive = [&]() __attribute__((always_inline)) {
+      // The V rows are there when only the next K rows are on their way.  Rows no one sees become
+      // zeros (what a page holds past a sequence's end may be anything, and 0 * NaN would be NaN);
+      // nearly always those from the end on.
+      bool strange = false;
+      auto ready = [&]() __attribute__((always_inline)) {
         if (more) wait_loads<kLoads>();
         else wait_loads<0>();
-      };
-      // V rows no one sees become zeros (what a page holds past a sequence's end may be anything,
-      // and 0 * NaN would be NaN); nearly always those from the end on.
-      auto clear_unseen = [&]() __attribute__((always_inline)) {
-        const unsigned fresh = fresh_lane();
+        if (edge || careful) {
+          const unsigned fresh = fresh_lane();
+          const bool end_only = !careful && missing == 0 && at >= w.lo;
 #pragma unroll 1
-        for (unsigned u = missing == 0 && at >= w.lo ? (w.hi - at) / kLoadRows : 0; u < kLoads; ++u) {
-          const unsigned t = u / (kLoads / 2), r = kLoadRows * u + fresh / (D / 8);
-          u32x4* piece = reinterpret_cast<u32x4*>(vs + kLoadRows * u * D) + fresh;
-          if (at + r < w.lo || at + r >= w.hi || (missing >> t & 1u) != 0) *piece = u32x4{0, 0, 0, 0};
+          for (unsigned u = end_only ? (w.hi - at) / kLoadRows : 0; u < kLoads; ++u) {
+            const unsigned t = u / (kLoads / 2), r = kLoadRows * u + fresh / (D / 8);
+            u32x4* piece = reinterpret_cast<u32x4*>(vs + kLoadRows * u * D) + fresh;
+            if (at + r < w.lo || at + r >= w.hi || (missing >> t & 1u) != 0) *piece = u32x4{0, 0, 0, 0};
+            if (careful) strange |= take_strange(piece);
+          }
+          wait_loads<63>();
         }
-        wait_loads<63>();
-      };
-      auto ready = [&]() __attribute__((always_inline)) {
-        values_arrive();
-        if (edge) clear_unseen();
       };
       h8 high[1], low[1];
-      rows.weigh(s, fresh, a.scale, edge, at, w.lo, missing, !careful, value_at, ready, high, low);
-      values_arrive();
-      if (edge || careful) {
-        if (edge) clear_unseen();
-        if (careful) {
-          bool strange = false;
-#pragma unroll 1
-          for (unsigned u = 0; u < kLoads; ++u) strange |= take_strange(reinterpret_cast<u32x4*>(vs + kLoadRows * u * D) + fresh_lane());
-          wait_loads<63>();
-          if (__any(strange)) rows.add_strange(s, pg, values, w.slot, at, w.lo, w.hi);
-        }
-      }
+      rows.weigh(s, fresh, a.scale, edge, at, w.lo, missing, value_at, ready, high, low);
+      ready();
+      if (careful && __any(strange)) rows.add_strange(kBlock, pg, values, w.slot, at, w.lo, w.hi);
 #pragma unroll
       for (unsigned d = 0; d < kTiles; d += 4) {
         h8 v[4];
@@ -677,7 +668,7 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
   const unsigned late = fresh_lane(), n = late & 15u, kb = late >> 4;
   f4* outputs = reinterpret_cast<f4*>(smem);                                 // [waves][D / 16][64]
   float2* ml = reinterpret_cast<float2*>(smem + kPosWaves * kTiles * 64 * 16);  // [waves][16]
-  rows.finish();
+  rows.finish(careful);
   if (wave < kPosWaves) {
     if (kb == 0) ml[wave * 16 + n] = float2{rows.m, rows.l};
 #pragma unroll
@@ -690,7 +681,7 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
 #pragma unroll
   for (unsigned v = 0; v < kPosWaves; ++v) {
     const float2 x = ml[v * 16 + n];
-    factor[v] = x.x == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(x.x - best);
+    factor[v] = x.x == -INFINITY ? 0.0F : rescale_factor(x.x, best);
     if (x.x != -INFINITY) total += x.y * factor[v];
   }
   const uint32_t out_row = out_rows[n];
@@ -794,7 +785,8 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
   const bool works = first < w.rows;
   // A second, careful pass follows in the rare case that an output of the first is an
   // infinity or NaN, or a page was missing: values and pages are then looked at.
-  for (bool careful = false;; careful = true) {
+  bool careful = false;
+  for (;; careful = true) {
     rows.clear();
     if (careful) window.first = 0xffffffc0u;  // 64 before column 0
     const uint32_t begin = fresh_number(w.start + w.first_block * kBlock);
@@ -828,8 +820,8 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
         for (unsigned b = 0; b < T / kBlock; ++b) rows.score(key_at + rows_at + b * kBlock * D * 2, s[2 * b], s[2 * b + 1]);
         const bool edge = at < w.lo || at + T > rows.least || (mark & 0xffu) != 0;
         h8 high[T / kBlock], low[T / kBlock];
-        rows.weigh(s, fresh, a.scale, edge, at, w.lo, mark, !careful, value_at + rows_at, [] {}, high, low);
-        if ((mark & 0x100u) != 0) rows.add_strange(s, pg, values, w.slot, at, w.lo, w.hi);
+        rows.weigh(s, fresh, a.scale, edge, at, w.lo, mark, value_at + rows_at, [] {}, high, low);
+        if ((mark & 0x100u) != 0) rows.add_strange(T, pg, values, w.slot, at, w.lo, w.hi);
 #pragma unroll
         for (unsigned b = 0; b < T / kBlock; ++b) {
 #pragma unroll
@@ -845,7 +837,7 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
     if (careful || !in_any_wave((works && rows.strange()) || lost, wave, flags)) break;
   }
   if (!works) return;
-  rows.finish();
+  rows.finish(careful);
   const unsigned late = fresh_lane();
   const uint32_t out_row = out_rows[late & 15u];
   if (out_row == 0xffffffffu) return;
@@ -937,9 +929,9 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
     const float2 x = s < items ? *reinterpret_cast<const float2*>(ml + 2 * (s < prefix ? s : s + skipped)) : float2{-INFINITY, 0.0F};
     const float next = fmaxf(best, wave_max(x.x));
     if (next == -INFINITY) continue;
-    const float keep = best == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(best - next);
+    const float keep = best == -INFINITY ? 0.0F : rescale_factor(best, next);
     best = next;
-    const float w = x.x == -INFINITY ? 0.0F : __builtin_amdgcn_exp2f(x.x - best);
+    const float w = x.x == -INFINITY ? 0.0F : rescale_factor(x.x, best);
     total = total * keep + wave_sum(w == 0.0F ? 0.0F : x.y * w);
     o0 *= keep;
     o1 *= keep;

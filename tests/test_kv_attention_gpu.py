@@ -357,3 +357,43 @@ def test_small_weights_beside_a_peak_are_kept(device, gx, heads, page, lengths, 
     got = p.run(gx)
     some = [0, len(lengths) - 1]
     p.check(got[some], some)
+
+
+@pytest.mark.parametrize("heads,lengths,tokens,shared,at,bad", [
+    (A, [40, 45], 1, 0, 7, 30),                               # peak and strange position in one block
+    (A, [40, 45], 1, 0, 30, 7),
+    (A, [700, 650], 1, 0, 3, 600),                            # in blocks of different waves, in different items
+    (A, [700, 650], 1, 0, 600, 3),
+    (A, [700, 650], 7, 0, 3, 100),                            # by rows
+    (A, [700, 650], 7, 0, 640, 3),
+    (A, [2300, 2300], 1, 2048, 5, 2100),                      # the prefix and own positions
+    (B, [700, 650], 1, 0, 3, 600),
+    (B, [700, 650], 7, 0, 3, 600),
+    (B, [2300, 2300], 9, 2048, 5, 2100),
+])
+def test_strange_positions_far_below_the_peak(device, gx, heads, lengths, tokens, shared, at, bad):
+    """Scores 120 nats below a row's largest (2^-173 of its weight): a NaN key and strange values still reach the row."""
+    q_heads, kv_heads, d = heads
+    group = q_heads // kv_heads
+    say("far below", heads, lengths, tokens, shared, at, bad)
+    p = _with_a_peak(np.random.default_rng(bad), heads, 16, lengths, tokens, shared, at, 120)
+    p.put(0, bad, k=np.full((kv_heads, d), np.nan, np.float16))
+    got = p.run(gx)
+    assert np.isnan(got[0]).all()
+    p.check(got[1:], [1])
+    p = _with_a_peak(np.random.default_rng(bad), heads, 16, lengths, tokens, shared, at, 120)
+    good = p.rows[0][1][bad].copy()
+    value = good.copy()
+    value[0, 3], value[1, 5], value[2, d - 1] = np.inf, -np.inf, np.nan
+    p.put(0, bad, v=value)
+    got = p.run(gx)
+    assert np.all(got[0, :, :group, 3] == np.inf) and np.all(got[0, :, group:2 * group, 5] == -np.inf)
+    assert np.isnan(got[0, :, 2 * group:3 * group, d - 1]).all()
+    touched = np.zeros(got.shape[1:], bool)
+    for head, dim in ((0, 3), (1, 5), (2, d - 1)):
+        touched[:, head * group:(head + 1) * group, dim] = True
+    p.put(0, bad, v=good)
+    for i in range(2):
+        want, tol = p.expect(i)
+        fine = ~touched if i == 0 else np.ones_like(touched)
+        assert np.all(np.abs(got[i].astype(np.float64) - want)[fine] <= tol[fine])
