@@ -397,3 +397,34 @@ def test_strange_positions_far_below_the_peak(device, gx, heads, lengths, tokens
         want, tol = p.expect(i)
         fine = ~touched if i == 0 else np.ones_like(touched)
         assert np.all(np.abs(got[i].astype(np.float64) - want)[fine] <= tol[fine])
+
+
+@pytest.mark.parametrize("page,hole", [(16, 0), (16, 4), (16, 5), (16, 6), (16, 7), (16, 11), (32, 2), (32, 3), (64, 1), (16, -1)])
+@pytest.mark.parametrize("shared", [0, 150])
+@pytest.mark.parametrize("heads,tokens", [(A, 1), (A, 7), (B, 1), (B, 9)])
+def test_positions_of_missing_pages_are_not_seen(device, gx, heads, tokens, shared, page, hole):
+    """A page missing in any 16-position part of a tile, in the prefix or in own positions (and the last page, which holds
+    the block's own rows), by positions and by rows; the other sequences do not see it if it is not in the prefix."""
+    rng = np.random.default_rng(100 * page + hole + tokens)
+    p = Problem(rng, *heads, page, [200, 190, 233], tokens, shared)
+    say("missing page", heads, tokens, shared, page, hole)
+    held = -(-(p.lengths[0] + tokens) // page)
+    hole = hole % held
+    p.table[0, hole] = [-1, 100000][hole % 2]
+    got = p.run(gx)
+    gone = np.zeros(p.lengths[0] + tokens, bool)
+    gone[hole * page:(hole + 1) * page] = True
+    for i in range(3):
+        rows, length = p.rows[i], p.lengths[i]
+        for t in range(tokens):
+            n = length + t + 1
+            keep = np.ones(n, bool)
+            if i == 0:
+                keep = ~gone[:n]
+            else:                                             # the prefix is read through the first sequence's table
+                keep[:shared] = ~gone[:shared]
+            p.rows[i] = [x[:n][keep] for x in rows]
+            p.lengths[i] = int(keep.sum()) - 1 - t
+            want, tol = p.expect(i)
+            assert np.all(np.abs(got[i, t].astype(np.float64) - want[t]) <= tol[t]), (i, t)
+        p.rows[i], p.lengths[i] = rows, length
