@@ -215,7 +215,10 @@ def lib() -> ctypes.CDLL:
         # first lets this library bind to that same HIP runtime; loading
         # /opt/rocm's copy first would put two HIP runtimes in one process.
         try:
-            import torch  # noqa: F401
+            import torch
+            global _current_device, _raw_stream, _half, _real, _word
+            _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+            _half, _real, _word = (torch.float16, torch.int16, torch.uint16), (torch.float32,), (torch.int32, torch.uint32)
         except ImportError:
             pass
         L = ctypes.CDLL(LIBRARY)
@@ -252,6 +255,54 @@ def _p(x) -> int | None:
     if hasattr(x, "data_ptr"):
         return x.data_ptr()
     return x.ctypes.data
+
+
+# This thread's device and its current stream there, and the element types of checked operands (fp16 numbers also as their
+# bits); set by lib().
+_current_device = _raw_stream = None
+_half = _real = _word = ()
+
+
+def _device_of(tensors, what):
+    """The device all tensors are on: its number, -1 for memory that no GPU reaches.  Pinned host memory goes with any (None)."""
+    found = {t.get_device() for t in tensors if t.is_cuda or not t.is_pinned()}
+    if len(found) > 1:
+        raise ValueError(f"{what}: tensors of different devices")
+    return found.pop() if found else None
+
+
+def _operand(x, types, size, device, what):
+    """Address of an operand of `size` bytes: a contiguous tensor of one of the types in memory of that device (None: of any),
+    or an address, which is the caller's to know.  0.16 us more than taking the address (0.3 of an append's 4.5 us)."""
+    try:
+        if x.get_device() == device and x.dtype in types and x.nbytes >= size and x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:
+        if x is None or isinstance(x, int):
+            return x
+        raise ValueError(f"{what}: a tensor or an address") from None
+    if x.dtype not in types or x.nbytes < size or not x.is_contiguous():
+        raise ValueError(f"{what}: a contiguous tensor of {size} bytes or more, {' / '.join(str(t)[6:] for t in types)}")
+    if not (x.is_pinned() if not x.is_cuda else device is None):
+        raise ValueError(f"{what} is not in the memory of the GPU that the call runs on")
+    return x.data_ptr()
+
+
+def _scratch(workspace, device):
+    """Address and bytes of a workspace, which may be of any type."""
+    if workspace is None:
+        return None, 0
+    return _operand(workspace, (workspace.dtype,), 0, device, "workspace"), workspace.nbytes
+
+
+def _launch_stream(device, stream):
+    """The stream's handle, if a launch there reaches the memory of that device (None: not known)."""
+    if device is not None:
+        if stream is None and device == _current_device():
+            return _raw_stream(device)
+        if stream is None or device < 0:
+            raise GfxinferError(INVALID_ARGUMENT, "the tensors of the call are not in the memory of the current device")
+    return _stream(stream)
 
 
 _current_stream = None
@@ -362,6 +413,7 @@ class KvPages(ctypes.Structure):
     _fields_ = [("key_pages", P), ("value_pages", P), ("page_table", P), ("lengths", P), ("references", P),
                 ("layers", U32), ("page_count", U32), ("page_tokens", U32), ("kv_heads", U32), ("head_size", U32),
                 ("sequences", U32), ("table_stride", U32)]
+    device = None  # of tensors given to `of`
 
     @classmethod
     def of(cls, key_pages, value_pages, page_table, lengths, references):
@@ -373,15 +425,11 @@ class KvPages(ctypes.Structure):
         if (tuple(value_pages.shape) != tuple(key_pages.shape) or tuple(lengths.shape) != (sequences,)
                 or tuple(references.shape) != (pages,) or not all(t.is_contiguous() for t in tensors)
                 or any(t.element_size() != size for t, size in zip(tensors, (2, 2, 4, 4, 4)))
-                or any(str(t.dtype) == "torch.bfloat16" for t in tensors)):
-            raise ValueError("K/V pages: fp16 pools of one shape, 32-bit state, all contiguous")
+                or any(str(t.dtype) == "torch.bfloat16" for t in tensors) or any(t.is_floating_point() for t in tensors[2:])):
+            raise ValueError("K/V pages: fp16 pools of one shape, 32-bit integer state, all contiguous")
         self = cls(*(_p(t) for t in tensors), layers, pages, page_tokens, kv_heads, head_size, sequences, stride)
-        self.tensors = tensors
+        self.tensors, self.device = tensors, _device_of(tensors, "K/V pages")
         return self
-
-
-def _bytes(workspace) -> int:
-    return 0 if workspace is None else workspace.numel() * workspace.element_size()
 
 
 def _host_ids(values):
@@ -394,39 +442,48 @@ def kv_pages_workspace_bytes(pages) -> int:
 
 
 def launch_kv_pages_reset(pages, stream=None):
-    check(lib().gfxinfer_launch_kv_pages_reset(ctypes.byref(pages), _stream(stream)))
+    check(lib().gfxinfer_launch_kv_pages_reset(ctypes.byref(pages), _launch_stream(pages.device, stream)))
 
 
 def launch_kv_pages_fork(pages, parent, children, stream=None):
-    ids = _host_ids(children)
-    check(lib().gfxinfer_launch_kv_pages_fork(ctypes.byref(pages), parent, ids.buffer_info()[0], len(ids), _stream(stream)))
+    L, ids = lib(), _host_ids(children)
+    at, count = ids.buffer_info()
+    check(L.gfxinfer_launch_kv_pages_fork(ctypes.byref(pages), parent, at, count, _launch_stream(pages.device, stream)))
 
 
 def launch_kv_pages_reserve(pages, sequences, tokens, status, workspace, stream=None):
-    ids = _host_ids(sequences)
-    check(lib().gfxinfer_launch_kv_pages_reserve(ctypes.byref(pages), ids.buffer_info()[0], len(ids), tokens, _p(status), _p(workspace),
-                                                 _bytes(workspace), _stream(stream)))
+    """status: a device int32."""
+    L, ids, device = lib(), _host_ids(sequences), pages.device
+    at, count = ids.buffer_info()
+    check(L.gfxinfer_launch_kv_pages_reserve(ctypes.byref(pages), at, count, tokens, _operand(status, _word, 4, device, "status"),
+                                             *_scratch(workspace, device), _launch_stream(device, stream)))
 
 
 def launch_kv_pages_append(pages, layer, key, value, sequences, tokens, stream=None):
-    ids = _host_ids(sequences)
-    check(lib().gfxinfer_launch_kv_pages_append(ctypes.byref(pages), layer, _p(key), _p(value), ids.buffer_info()[0], len(ids), tokens,
-                                                _stream(stream)))
+    """key fp16, value fp32: [len(sequences), tokens, kv_heads * head_size]."""
+    L, ids, device = lib(), _host_ids(sequences), pages.device
+    at, count = ids.buffer_info()
+    size = 2 * count * tokens * pages.kv_heads * pages.head_size
+    check(L.gfxinfer_launch_kv_pages_append(ctypes.byref(pages), layer, _operand(key, _half, size, device, "key"),
+                                            _operand(value, _real, 2 * size, device, "value"), at, count, tokens,
+                                            _launch_stream(device, stream)))
 
 
 def launch_kv_pages_advance(pages, sequences, tokens, token_counts=None, stream=None):
-    """token_counts: device uint32 per listed sequence, or None for `tokens` each."""
-    ids = _host_ids(sequences)
-    check(lib().gfxinfer_launch_kv_pages_advance(ctypes.byref(pages), ids.buffer_info()[0], len(ids), tokens, _p(token_counts),
-                                                 _stream(stream)))
+    """token_counts: device 32-bit integers, one per listed sequence, or None for `tokens` each."""
+    L, ids, device = lib(), _host_ids(sequences), pages.device
+    at, count = ids.buffer_info()
+    counts = None if token_counts is None else _operand(token_counts, _word, 4 * count, device, "token_counts")
+    check(L.gfxinfer_launch_kv_pages_advance(ctypes.byref(pages), at, count, tokens, counts, _launch_stream(device, stream)))
 
 
 def launch_kv_pages_free(pages, sequences, keep_tokens=None, stream=None):
-    ids, keep = _host_ids(sequences), None if keep_tokens is None else _host_ids(keep_tokens)
+    L, ids, keep = lib(), _host_ids(sequences), None if keep_tokens is None else _host_ids(keep_tokens)
     if keep is not None and len(keep) != len(ids):
         raise ValueError("one length to keep per sequence")
-    check(lib().gfxinfer_launch_kv_pages_free(ctypes.byref(pages), ids.buffer_info()[0],
-                                              None if keep is None else keep.buffer_info()[0], len(ids), _stream(stream)))
+    at, count = ids.buffer_info()
+    check(L.gfxinfer_launch_kv_pages_free(ctypes.byref(pages), at, None if keep is None else keep.buffer_info()[0], count,
+                                          _launch_stream(pages.device, stream)))
 
 
 def launch_kv_pages_copy(pages, sources, destinations, stream=None):
@@ -434,12 +491,14 @@ def launch_kv_pages_copy(pages, sources, destinations, stream=None):
     if len(a) != len(b):
         raise ValueError("as many destinations as sources")
     check(lib().gfxinfer_launch_kv_pages_copy(ctypes.byref(pages), a.buffer_info()[0], b.buffer_info()[0], len(a),
-                                              _stream(stream)))
+                                              _launch_stream(pages.device, stream)))
 
 
 def launch_kv_pages_compact(pages, live_pages, workspace, stream=None):
-    check(lib().gfxinfer_launch_kv_pages_compact(ctypes.byref(pages), _p(live_pages), _p(workspace), _bytes(workspace),
-                                                 _stream(stream)))
+    """live_pages: a device int32, or None."""
+    L, device = lib(), pages.device
+    check(L.gfxinfer_launch_kv_pages_compact(ctypes.byref(pages), _operand(live_pages, _word, 4, device, "live_pages"),
+                                             *_scratch(workspace, device), _launch_stream(device, stream)))
 
 
 def kv_pages_attention_workspace_bytes(pages, count, tokens, q_heads, shared_tokens) -> int:
@@ -448,11 +507,14 @@ def kv_pages_attention_workspace_bytes(pages, count, tokens, q_heads, shared_tok
 
 def launch_kv_pages_gated_attention(pages, layer, query, gate, output, sequences, tokens, q_heads, shared_tokens, workspace,
                                     stream=None):
-    """gate may be None."""
-    ids = _host_ids(sequences)
-    check(lib().gfxinfer_launch_kv_pages_gated_attention(ctypes.byref(pages), layer, _p(query), _p(gate), _p(output),
-                                                         ids.buffer_info()[0], len(ids), tokens, q_heads, shared_tokens, _p(workspace),
-                                                         _bytes(workspace), _stream(stream)))
+    """query and output fp16 [len(sequences), tokens, q_heads, head_size]; gate fp32 with rows of 2 head_size, or None."""
+    L, ids, device = lib(), _host_ids(sequences), pages.device
+    at, count = ids.buffer_info()
+    size = 2 * count * tokens * q_heads * pages.head_size
+    check(L.gfxinfer_launch_kv_pages_gated_attention(ctypes.byref(pages), layer, _operand(query, _half, size, device, "query"),
+                                                     None if gate is None else _operand(gate, _real, 4 * size, device, "gate"),
+                                                     _operand(output, _half, size, device, "output"), at, count, tokens, q_heads,
+                                                     shared_tokens, *_scratch(workspace, device), _launch_stream(device, stream)))
 
 
 # ---- rules on logits -------------------------------------------------------------
@@ -463,6 +525,7 @@ class LogitRules(ctypes.Structure):
                                  "frequency", "bias_tokens", "bias_values", "bias_counts", "allowed", "allowed_rows")]
     _fields_ += [(n, U32) for n in ("history_row_count", "history_stride", "bias_stride", "allowed_row_count",
                                     "allowed_stride")]
+    device = None  # of tensors given to `of`
 
     @classmethod
     def of(cls, **tensors):
@@ -491,7 +554,7 @@ class LogitRules(ctypes.Structure):
         if len(vectors) > 1:
             raise ValueError("logit rules: one entry per row of the logits")
         self.batch = next(iter(vectors), None)
-        self.tensors = tensors
+        self.tensors, self.device = tensors, _device_of([t for t in tensors.values() if t is not None], "logit rules")
         return self
 
 
@@ -504,15 +567,21 @@ def launch_logit_rules(logits, rules, output, tokens, workspace, vocabulary=None
     batch, columns = logits.shape
     if rules.batch not in (None, batch):
         raise ValueError("logit rules: made for another number of rows")
+    L, device = lib(), logits.get_device()
+    if device < 0 and logits.is_pinned():
+        device = rules.device
+    if rules.device is not None and rules.device != device:
+        raise ValueError("logit rules: tensors of another device than the logits")
     vocabulary = columns if vocabulary is None else vocabulary
     for t in (logits,) if output is None else (logits, output):
-        if t.stride(1) != 1 or t.element_size() != 4 or t.shape[0] != batch or t.shape[1] < vocabulary:
+        if t.stride(1) != 1 or t.dtype not in _real or t.shape[0] != batch or t.shape[1] < vocabulary:
             raise ValueError("logit rules: logits are fp32 [batch, columns] with dense rows that hold the vocabulary")
-    if tokens is not None and (tokens.numel() < batch or tokens.element_size() != 4 or not tokens.is_contiguous()):
-        raise ValueError("logit rules: tokens is a contiguous 32-bit vector with an entry per row")
-    check(lib().gfxinfer_launch_logit_rules(_p(logits), logits.stride(0), vocabulary, batch,
-                                            ctypes.byref(rules), _p(output), 0 if output is None else output.stride(0),
-                                            _p(tokens), _p(workspace), _bytes(workspace), _stream(stream)))
+    if output is not None and output.get_device() != device and not (device is None if output.is_cuda else output.is_pinned()):
+        raise ValueError("logit rules: logits and output are on different devices")
+    picked = None if tokens is None else _operand(tokens, _word, 4 * batch, device, "logit rules: tokens")
+    check(L.gfxinfer_launch_logit_rules(logits.data_ptr(), logits.stride(0), vocabulary, batch, ctypes.byref(rules), _p(output),
+                                        0 if output is None else output.stride(0), picked, *_scratch(workspace, device),
+                                        _launch_stream(device, stream)))
 
 
 # ---- host-side layout (numpy) -------------------------------------------------

@@ -137,3 +137,82 @@ def test_pages_are_not_bfloat16_and_lists_are_whole_numbers(gx):
         gx.launch_kv_pages_fork(pages, 0, [-1], stream=0)
     with pytest.raises(gx.GfxinferError):
         gx.launch_kv_pages_fork(pages, 0, array.array("I", [9]), stream=0)
+
+
+def _tensor_calls(gx, pages, **change):
+    """Every wrapper that takes tensors beside the description: addresses (not looked at) but for what `change` gives."""
+    a = dict.fromkeys(("key", "value", "status", "token_counts", "live", "query", "gate", "output"), 4096)
+    a.update(work=None)
+    a.update(change)
+    return {
+        "append": lambda: gx.launch_kv_pages_append(pages, 0, a["key"], a["value"], [0, 1], 3, stream=0),
+        "reserve": lambda: gx.launch_kv_pages_reserve(pages, [0, 1], 3, a["status"], a["work"], stream=0),
+        "advance": lambda: gx.launch_kv_pages_advance(pages, [0, 1], 3, a["token_counts"], stream=0),
+        "compact": lambda: gx.launch_kv_pages_compact(pages, a["live"], a["work"], stream=0),
+        "attention": lambda: gx.launch_kv_pages_gated_attention(pages, 0, a["query"], a["gate"], a["output"], [0, 1], 3, 4, 0,
+                                                                a["work"], stream=0),
+    }
+
+
+@pytest.fixture()
+def tensor_pages(gx):
+    import torch
+    k = torch.zeros(2, 8, 16, 2, 128, dtype=torch.float16)
+    return gx.KvPages.of(k, k, *(torch.zeros(s, dtype=torch.int32) for s in ((4, 3), (4,), (8,))))
+
+
+def _bad_tensors():
+    import torch
+    z = torch.zeros
+    h, w = torch.float16, torch.int32
+    return [
+        ("append", dict(key=z(2, 3, 256)), "key"), ("append", dict(key=z(2, 3, 256, dtype=torch.bfloat16)), "key"),
+        ("append", dict(key=z(2, 3, 255, dtype=h)), "key"), ("append", dict(key=z(256, 3, 2, dtype=h).permute(2, 1, 0)), "key"),
+        ("append", dict(key=np.zeros((2, 3, 256), np.float16)), "key"), ("append", dict(value=z(2, 3, 256, dtype=h)), "value"),
+        ("append", dict(value=z(2, 2, 256)), "value"), ("append", dict(value=z(2, 3, 256).double()), "value"),
+        ("reserve", dict(status=z(1, dtype=torch.int64)), "status"), ("reserve", dict(status=z(0, dtype=w)), "status"),
+        ("reserve", dict(work=z(4096, 2, dtype=w)[:, 0]), "workspace"),
+        ("advance", dict(token_counts=z(2, dtype=torch.int64)), "token_counts"), ("advance", dict(token_counts=z(2)), "token_counts"),
+        ("advance", dict(token_counts=z(1, dtype=w)), "token_counts"), ("advance", dict(token_counts=z(4, dtype=w)[::2]), "token_counts"),
+        ("compact", dict(live=z(1)), "live_pages"), ("compact", dict(live=z(0, dtype=w)), "live_pages"),
+        ("attention", dict(query=z(2, 3, 4, 128)), "query"), ("attention", dict(query=z(2, 2, 4, 128, dtype=h)), "query"),
+        ("attention", dict(query=z(2, 4, 3, 128, dtype=h).transpose(1, 2)), "query"),
+        ("attention", dict(gate=z(2, 3, 4, 256, dtype=h)), "gate"), ("attention", dict(gate=z(2, 3, 4, 128)), "gate"),
+        ("attention", dict(output=z(2, 3, 4, 128)), "output"), ("attention", dict(output=z(2, 3, 3, 128, dtype=h)), "output"),
+        ("attention", dict(work=z(1, dtype=w).expand(4096)), "workspace"),
+    ]
+
+
+@pytest.mark.parametrize("at", range(25))
+def test_operands_of_other_types_or_sizes_are_refused(gx, tensor_pages, at):
+    """Before the library is called: what a kernel would read or write past the end of, or take for other numbers."""
+    name, change, word = _bad_tensors()[at]
+    tensor_pages.device = None                                # of no device, as a description from addresses
+    with pytest.raises(ValueError, match=word):
+        _tensor_calls(gx, tensor_pages, **change)[name]()
+
+
+def test_host_memory_is_refused(gx, tensor_pages):
+    """Good tensors that no GPU reaches, and a cache in such memory."""
+    import torch
+    assert len(_bad_tensors()) == 25
+    assert tensor_pages.device == -1
+    tensor_pages.device = None
+    z, h, w = torch.zeros, torch.float16, torch.int32
+    for name, change in (("append", dict(key=z(2, 3, 256, dtype=h))), ("append", dict(value=z(2, 3, 256))),
+                         ("reserve", dict(status=z(1, dtype=w))), ("reserve", dict(work=z(4096, dtype=w))),
+                         ("advance", dict(token_counts=z(2, dtype=w))), ("compact", dict(live=z(1, dtype=w))),
+                         ("compact", dict(work=z(4096))), ("attention", dict(query=z(2, 3, 4, 128, dtype=h))),
+                         ("attention", dict(gate=z(2, 3, 4, 256))), ("attention", dict(output=z(2, 3, 4, 128, dtype=h))),
+                         ("attention", dict(work=z(4096)))):
+        with pytest.raises(ValueError, match="memory"):
+            _tensor_calls(gx, tensor_pages, **change)[name]()
+    tensor_pages.device = -1
+    calls = [lambda: gx.launch_kv_pages_reset(tensor_pages, stream=0), lambda: gx.launch_kv_pages_fork(tensor_pages, 0, [1], stream=0),
+             lambda: gx.launch_kv_pages_free(tensor_pages, [1], stream=0), lambda: gx.launch_kv_pages_copy(tensor_pages, [1], [2], stream=0)]
+    for call in calls + list(_tensor_calls(gx, tensor_pages).values()):
+        with pytest.raises(gx.GfxinferError, match="memory"):
+            call()
+    pools = tensor_pages.tensors
+    with pytest.raises(ValueError):
+        gx.KvPages.of(pools[0], pools[1], torch.zeros(4, 3), pools[3], pools[4])

@@ -275,3 +275,21 @@ def test_graph_replays_and_other_stream(device, gx):
         graph.replay()
         model_step()
         c.check()
+
+
+def test_operands_in_host_memory(device, gx):
+    """Pinned memory is read and written like the GPU's; other host memory is refused before anything is launched."""
+    import torch
+    c = Cache(gx, 1, 8, 16, 1, 128, 2, 4)
+    say("host memory")
+    c.status = torch.full((1,), 9, dtype=torch.int32, pin_memory=True)
+    gx.launch_kv_pages_reserve(c.pages, [0], 5, c.status, c.work)
+    torch.cuda.synchronize()
+    assert int(c.status[0]) == c.model.reserve([0], 5) == 0
+    key, value = torch.zeros(1, 5, 1, 128, dtype=torch.float16), torch.zeros(1, 5, 1, 128)
+    for k, v in ((key, value.cuda()), (key.cuda(), value)):
+        with pytest.raises(ValueError, match="memory"):
+            gx.launch_kv_pages_append(c.pages, 0, k, v, [0], 5)
+    with pytest.raises(ValueError, match="key"):
+        gx.launch_kv_pages_append(c.pages, 0, key.cuda(), value.cuda(), [0, 1], 5)
+    c.check()

@@ -94,3 +94,16 @@ def test_rules_from_tensors_check_types_and_room(gx):
                                        (f(4, 60), i(4), 70)):
         with pytest.raises(ValueError):
             gx.launch_logit_rules(f(4, 70), rules, output, tokens, i(100), vocabulary, stream=0)
+
+
+def test_integer_logits_and_host_memory_are_refused(gx):
+    import torch
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    f = lambda *s: torch.zeros(s)  # noqa: E731
+    rules = gx.LogitRules.of(presence=f(4))
+    assert rules.device == -1
+    for logits, output in ((i(4, 70), None), (f(4, 70), i(4, 70))):
+        with pytest.raises(ValueError):
+            gx.launch_logit_rules(logits, rules, output, i(4), i(100), stream=0)
+    with pytest.raises(gx.GfxinferError, match="memory"):
+        gx.launch_logit_rules(f(4, 70), rules, f(4, 70), i(4), i(100), stream=0)
