@@ -636,16 +636,19 @@ int32_t gfxinfer_launch_kv_pages_reset(const gfxinfer_kv_pages* pages, void* str
 
 /* children[0..count) (host, distinct, none of them the parent) give back what they hold and
  * become copies of the parent's committed tokens: same pages, same length.  No K/V row
- * moves; rows the parent appended past its length stay the parent's. */
+ * moves.  Rows the parent appended past its length are not passed on, and the page of a
+ * partly filled tail is no longer the parent's alone: the next reserve that names the parent
+ * may give it a copy of that page with its committed rows only.  Commit such rows (advance)
+ * before that reserve, or append them again after it. */
 int32_t gfxinfer_launch_kv_pages_fork(const gfxinfer_kv_pages* pages, uint32_t parent, const uint32_t* children,
                                       uint32_t count, void* stream);
 
 /* Makes room for `tokens` (1..2^24) more tokens of each listed sequence (distinct; NULL:
  * 0..count-1): new pages for positions the sequence has no page for, and a private copy of
- * a partly filled last page that other sequences hold too (its committed rows, all layers;
- * where all holders are in the list the last of them keeps the page).  Pages are taken
- * lowest first, sequence by sequence in list order, a copy before new pages.  *status
- * (device) = 0, or 1 when the pool or a table row is too small: then nothing changed. */
+ * a partly filled last page that other sequences hold too (its committed rows, all layers,
+ * and none past them; where all holders are in the list the last of them keeps the page).
+ * Pages are taken lowest first, sequence by sequence in list order, a copy before new pages.
+ * *status (device) = 0, or 1 when the pool or a table row is too small: then nothing changed. */
 int32_t gfxinfer_launch_kv_pages_reserve(const gfxinfer_kv_pages* pages, const uint32_t* sequences, uint32_t count,
                                          uint32_t tokens, int32_t* status, void* workspace, size_t workspace_bytes,
                                          void* stream);

@@ -293,3 +293,35 @@ def test_operands_in_host_memory(device, gx):
     with pytest.raises(ValueError, match="key"):
         gx.launch_kv_pages_append(c.pages, 0, key.cuda(), value.cuda(), [0, 1], 5)
     c.check()
+
+
+@pytest.mark.parametrize("order", [[0, 1], [1, 0], [0], [1]])
+@pytest.mark.parametrize("commit", [True, False])
+def test_rows_appended_before_a_fork(device, gx, commit, order):
+    """A parent's rows past its length: committed before the next reserve they are kept whoever copies the tail page; if not,
+    the parent's copy holds the committed rows, and the appended ones are appended again."""
+    c = Cache(gx, 2, 12, 16, 1, 128, 3, 4)
+    c.grow([0], 20)
+    assert c.reserve([0], 5) == 0
+    c.append([0], 5)
+    appended = [c.model.rows(layer, 0, 25) for layer in range(2)]
+    say("rows before a fork", commit, order)
+    c.fork(0, [1])
+    c.check()
+    if commit:
+        c.advance([0], 5)
+    assert c.reserve(order, 4) == 0
+    c.check()
+    if not commit:
+        assert c.reserve([0], 5) == 0
+        for layer, (k, v) in enumerate(appended):
+            rows = [x[None, 20:] for x in (k.astype(np.float16), v.astype(np.float32))]
+            gx.launch_kv_pages_append(c.pages, layer, *(dev(x) for x in rows), [0], 5)
+            c.model.append(layer, *rows, [0])
+        c.advance([0], 5)
+    c.check()
+    for layer, (k, v) in enumerate(appended):
+        got = c.model.rows(layer, 0, 25)
+        assert np.array_equal(got[0], k) and np.array_equal(got[1], v)
+    c.grow([1], 9)
+    c.check()
