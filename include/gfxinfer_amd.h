@@ -648,7 +648,8 @@ int32_t gfxinfer_launch_kv_pages_fork(const gfxinfer_kv_pages* pages, uint32_t p
  * a partly filled last page that other sequences hold too (its committed rows, all layers,
  * and none past them; where all holders are in the list the last of them keeps the page).
  * Pages are taken lowest first, sequence by sequence in list order, a copy before new pages.
- * *status (device) = 0, or 1 when the pool or a table row is too small: then nothing changed. */
+ * *status (device) = 0, or 1 when the pool or a table row is too small: then nothing changed,
+ * append skips the positions that got no page, and the step must not be advanced. */
 int32_t gfxinfer_launch_kv_pages_reserve(const gfxinfer_kv_pages* pages, const uint32_t* sequences, uint32_t count,
                                          uint32_t tokens, int32_t* status, void* workspace, size_t workspace_bytes,
                                          void* stream);
@@ -664,12 +665,15 @@ int32_t gfxinfer_launch_kv_pages_append(const gfxinfer_kv_pages* pages, uint32_t
 
 /* Commits appended tokens: length += tokens, or += min(token_counts[i], tokens) for the
  * i-th listed sequence when token_counts (device, the accepted tokens of a verify block) is
- * not NULL.  A length never passes table_stride * page_tokens. */
+ * not NULL.  A length never passes table_stride * page_tokens, but it may pass the pages: a
+ * recorded step whose reserve can fail takes its counts from the status (0 where it is 1), or
+ * positions are committed that were never written. */
 int32_t gfxinfer_launch_kv_pages_advance(const gfxinfer_kv_pages* pages, const uint32_t* sequences, uint32_t count,
                                          uint32_t tokens, const uint32_t* token_counts, void* stream);
 
 /* Cuts each listed sequence (distinct; NULL: 0..count-1) to its first keep_tokens[i] tokens
- * (host; NULL: none) and gives back the pages past them. */
+ * (host; NULL: none; its length if it is shorter) and gives back the pages past them, pages
+ * reserved past its length among them. */
 int32_t gfxinfer_launch_kv_pages_free(const gfxinfer_kv_pages* pages, const uint32_t* sequences,
                                       const uint32_t* keep_tokens, uint32_t count, void* stream);
 

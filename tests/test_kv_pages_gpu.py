@@ -325,3 +325,30 @@ def test_rows_appended_before_a_fork(device, gx, commit, order):
         assert np.array_equal(got[0], k) and np.array_equal(got[1], v)
     c.grow([1], 9)
     c.check()
+
+
+def test_a_recorded_step_whose_reserve_fails(device, gx):
+    """Counts taken from the status: replays after the pool is full change nothing, and the step goes on once pages are free."""
+    import torch
+    c = Cache(gx, 1, 5, 16, 1, 128, 3, 5, seed=4)
+    c.grow([0, 1], 20)                                        # four of five pages
+    key, value = dev(c.rng.standard_normal((2, 10, 1, 128)).astype(np.float16)), dev(c.rng.standard_normal((2, 10, 1, 128)).astype(np.float32))
+    counts = torch.zeros(2, dtype=torch.int32, device="cuda")
+    c.status.zero_()
+    say("recorded step")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        gx.launch_kv_pages_reserve(c.pages, [0, 1], 10, c.status, c.work)
+        gx.launch_kv_pages_append(c.pages, 0, key, value, [0, 1], 10)
+        counts.copy_((c.status == 0).to(torch.int32).mul(10).expand(2))
+        gx.launch_kv_pages_advance(c.pages, [0, 1], 10, counts)
+    for want in (0, 1, 1, 0, 1):                              # 20 -> 30 inside the pages; then two pages, one left
+        if want == 0 and c.model.lengths[0] == 30:
+            c.free([1], [10])
+        graph.replay()
+        assert int(c.status[0]) == want == c.model.reserve([0, 1], 10)
+        c.model.append(0, host(key), host(value), [0, 1])
+        if want == 0:
+            c.model.advance([0, 1], 10)
+        c.check()
