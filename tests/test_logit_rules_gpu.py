@@ -245,3 +245,48 @@ def test_unaligned_rows_and_large_batches(device, gx, stride, shift):
     _check(got[:, :vocabulary], *_formula(logits, a))
     assert np.all(got[:, vocabulary:] == 123.0) and np.all(host(out)[:shift] == 123.0) and np.all(host(out)[shift + batch * stride:] == 123.0)
     assert np.array_equal(host(tokens), _argmax(got[:, :vocabulary]))
+
+
+def _formula_fp32(logits, a):
+    """The rules in fp32, one rounding an operation, in the order the header gives them."""
+    out = logits.copy()
+    batch, vocabulary = out.shape
+    one = np.float32
+    with np.errstate(all="ignore"):
+        for b in range(batch):
+            x = out[b]
+            row = int(a["history_rows"][b]) if "history_rows" in a else b
+            if "history" in a and 0 <= row < len(a["history"]):
+                tokens = a["history"][row][:a["history_lengths"][b]].astype(np.int64)
+                prompt = int(a["prompt_lengths"][b]) if "prompt_lengths" in a else 0
+                seen, count = (np.bincount(t[t < vocabulary], minlength=vocabulary) for t in (tokens, tokens[prompt:]))
+                factor, f, p = (one(a[k][b]) if k in a else one(d) for k, d in (("repetition", 1), ("frequency", 0), ("presence", 0)))
+                x = np.where(seen > 0, np.where(x > 0, x / factor, x * factor), x)
+                x = np.where(count > 0, (x - f * count.astype(np.float32)) - p, x)
+            if "bias_tokens" in a:
+                n = int(a["bias_counts"][b]) if "bias_counts" in a else a["bias_tokens"].shape[1]
+                x = x.copy()
+                for t, v in {int(t): v for t, v in zip(a["bias_tokens"][b][:n], a["bias_values"][b][:n]) if t < vocabulary}.items():
+                    x[t] += v
+            row = int(a["allowed_rows"][b]) if "allowed_rows" in a else b
+            if "allowed" in a and 0 <= row < len(a["allowed"]):
+                index = np.arange(vocabulary)
+                x = np.where((a["allowed"][row][index // 32] >> (index % 32).astype(np.uint32)) & 1, x, one(-np.inf))
+            assert x.dtype == np.float32
+            out[b] = x
+    return out
+
+
+@pytest.mark.parametrize("batch,vocabulary,history,bias,masks", [
+    (1, 1, 5, 2, 0), (3, 33, 40, 7, 2), (5, 5003, 700, 300, 3), (33, 4096, 2000, 17, 8), (2, 151936, 9000, 4095, 1), (256, 9001, 300, 30, 0)])
+def test_each_operation_is_rounded_once(device, gx, batch, vocabulary, history, bias, masks):
+    """The same bits as fp32 operations in the stated order, over small and large magnitudes."""
+    rng = np.random.default_rng(vocabulary * 3 + batch)
+    logits = (rng.standard_normal((batch, vocabulary)) * 2.0 ** rng.integers(-40, 20, (batch, vocabulary))).astype(np.float32)
+    logits[rng.random(logits.shape) < 0.01] = 0
+    a = _problem(rng, batch, vocabulary, history, bias, masks)
+    say("rules in fp32", batch, vocabulary, history, bias, masks)
+    out, tokens = _run(gx, logits, a, vocabulary)
+    want = _formula_fp32(logits, a)
+    assert np.array_equal(out.view(np.uint32), want.view(np.uint32))
+    assert np.array_equal(tokens, _argmax(want))
