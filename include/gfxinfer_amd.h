@@ -708,6 +708,12 @@ size_t gfxinfer_kv_pages_attention_workspace_bytes(const gfxinfer_kv_pages* page
  * listed sequence's table, for the rows of all.  The result does not depend on it but for
  * the order of fp32 additions.
  *
+ * That order depends on the shape of the call (count, tokens, q_heads, shared_tokens,
+ * table_stride) and on the row's own length, never on what other sequences hold.  A block of
+ * several tokens therefore does not repeat the bits of single-token calls, as
+ * gfxinfer_launch_gated_attention_decode_block does: a greedy pick can differ where two logits
+ * are that close.
+ *
  * A position without a page is not seen; a row that sees nothing becomes zeros. */
 int32_t gfxinfer_launch_kv_pages_gated_attention(const gfxinfer_kv_pages* pages, uint32_t layer, const uint16_t* query,
                                                  const float* gate, uint16_t* output, const uint32_t* sequences,

@@ -428,3 +428,27 @@ def test_positions_of_missing_pages_are_not_seen(device, gx, heads, tokens, shar
             want, tol = p.expect(i)
             assert np.all(np.abs(got[i, t].astype(np.float64) - want[t]) <= tol[t]), (i, t)
         p.rows[i], p.lengths[i] = rows, length
+
+
+@pytest.mark.parametrize("heads,tokens", [(A, 1), (A, 7), (B, 1), (B, 9)])
+def test_a_sequence_keeps_its_bits_whatever_the_others_hold(device, gx, heads, tokens):
+    """Other sequences' queries, own rows (peaks, infinities and NaN among them) and lengths do not change a result's bits."""
+    rng = np.random.default_rng(tokens)
+    q_heads, kv_heads, d = heads
+    lengths = [700, 650, 800, 655]
+    p = Problem(rng, *heads, 16, lengths, tokens, 600)
+    say("bits", heads, tokens)
+    first = p.run(gx)
+    p.check(first)
+    for i in (0, 3):
+        p.query[i] = rng.standard_normal(p.query[i].shape) * 30
+        for at in range(600, lengths[i] + tokens):
+            k, v = (rng.standard_normal((kv_heads, d)).astype(np.float16) * np.float16(s) for s in (8, 100))
+            p.put(i, at, k=k, v=v)
+    p.put(3, 610, v=np.full((kv_heads, d), np.inf, np.float16))
+    p.put(0, 620, k=np.full((kv_heads, d), np.nan, np.float16))
+    p.lengths[3] = 640
+    got = p.run(gx)
+    assert not np.array_equal(got[0], first[0])
+    for i in (1, 2):
+        assert np.array_equal(got[i].view(np.uint16), first[i].view(np.uint16)), i
