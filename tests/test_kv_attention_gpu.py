@@ -447,6 +447,7 @@ def test_a_sequence_keeps_its_bits_whatever_the_others_hold(device, gx, heads, t
             p.put(i, at, k=k, v=v)
     p.put(3, 610, v=np.full((kv_heads, d), np.inf, np.float16))
     p.put(0, 620, k=np.full((kv_heads, d), np.nan, np.float16))
+    p.query[3, 0, 1] = np.nan
     p.lengths[3] = 640
     got = p.run(gx)
     assert not np.array_equal(got[0], first[0])
