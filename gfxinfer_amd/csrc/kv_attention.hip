@@ -62,13 +62,16 @@ __device__ __forceinline__ float rescale_factor(float from, float to) {
 // A row's weights are 2^(score - m + kLift), scores in units of log2.  The stored maximum m follows
 // the maxima of the blocks of positions, downwards too, once one leaves [m - kFall, m + kRise], but
 // stays within kSpan of its highest value so that the sums fit fp32.  The largest weight of every
-// block so lies between 2^3 and 2^15, near the top of fp16, and 2^-25, half of fp16's last place, is
-// at least 2^28 below it.  (At most 2^8, cut off at 2^-24 and never raised again, the weights beside
-// a score 16 nats above 600 others lost 16 % of their sum.)
-constexpr float kLift = 11.0F, kRise = 4.0F, kFall = 8.0F, kSpan = 32.0F;
-// In a block that moves m, weights below 2^kSmall are multiplied on their own, times kSmallScale:
-// down to 2^-49, 41 nats below m.
-constexpr float kSmall = -9.0F, kSmallScale = 0x1p24F;
+// block so lies between 2^-1 and 2^15, near the top of fp16, and 2^-25, half of fp16's last place,
+// is at least 2^24 below it.  (At most 2^8, cut off at 2^-24 and never raised again, the weights
+// beside a score 16 nats above 600 others lost 16 % of their sum.)
+constexpr float kLift = 11.0F, kRise = 4.0F, kFall = 12.0F, kSpan = 32.0F;
+// In a block that moves m, weights below 2^kSmall are multiplied on their own, times kSmallScale
+// (down to 2^-49, 41 nats below m), if no weight of the row lies between 2^kBetween and the peak's:
+// one that does carries more of the output than the others lose.  Scores that spread by 6 nats have
+// one in nearly every block (64 sequences on 32768: 130 us, 168 without this condition, 118 where
+// scores spread by 1).
+constexpr float kSmall = -9.0F, kBetween = -4.0F, kPeak = 8.0F, kSmallScale = 0x1p24F;
 
 constexpr unsigned kWaves = 8;     // of a workgroup; by rows: 128 rows
 constexpr unsigned kPosWaves = 4;  // of them, those that divide positions: a block of K and of V each in LDS
@@ -251,27 +254,25 @@ __device__ __forceinline__ uint32_t fresh_number(uint32_t x) {
 }
 
 // Sixteen rows of a wave: lane column n's row is the query q (B operand), sees the positions
-// below `visible`.
+// below `visible`, and its result goes to row out_row (none: 0xffffffff).
 template <unsigned D>
 struct Rows {
   h8 q[D / 32];
-  uint32_t visible;
+  uint32_t visible, out_row;
   uint32_t least;  // of visible over the rows
   f4 o[D / 16];
   float m, l;  // m in units of log2; l of the lane's own positions
   float peak;  // the highest m so far
 
   // Rows first + n of `rows`; row = (i * tokens + t) * group + g, i counted from `base`.  Own:
-  // the rows are one sequence's, with hi - tokens committed positions.  The rows of the output
-  // (none: 0xffffffff) wait in LDS at out_rows: kept in a register they cost a spill, whose store
-  // the first loads then wait for (200 sequences of 250..500 positions: 81 us, not 75).
+  // the rows are one sequence's, with hi - tokens committed positions.
   template <bool Own>
   __device__ __forceinline__ void load(const PagedAttnArgs& a, uint32_t base, uint32_t first, uint32_t rows, uint32_t hk,
-                                       uint32_t hi, uint32_t* out_rows) {
+                                       uint32_t hi) {
     const unsigned lane = threadIdx.x & 63u, kb = lane >> 4;
     const uint32_t group = a.q_heads / a.kv_heads, row = first + (lane & 15u);
-    uint32_t out_row = 0xffffffffu;
     visible = 0;
+    out_row = 0xffffffffu;
 #pragma unroll
     for (unsigned s = 0; s < D / 32; ++s) q[s] = h8{};
     if (row < rows) {
@@ -286,7 +287,6 @@ struct Rows {
     // prefix is longer than a sequence, and then every block is treated as an edge.
     if (Own) least = first < rows ? hi - a.tokens + first / group + 1 : 0xffffffffu;
     else least = __all(row >= rows || visible == hi) ? hi : 0u;
-    if (lane < 16u) out_rows[lane] = out_row;
   }
 
   // The queries have arrived here: a wait for them inside a loop would wait for the loop's
@@ -341,10 +341,11 @@ struct Rows {
     }
   }
 
-  // Takes the small weights out of the scores s of a block and adds their products.  The outputs
-  // are scaled for that and back: powers of two, so nothing is rounded, and no registers.
+  // Takes the small weights of rows with a peak alone out of the scores s of a block and adds their
+  // products.  The outputs are scaled for that and back: powers of two, so nothing is rounded, and
+  // no registers.
   template <unsigned T>
-  __device__ __forceinline__ void add_small(f4 (&s)[T], float scale, unsigned value_at, bool moved) {
+  __device__ __forceinline__ void add_small(f4 (&s)[T], float scale, unsigned value_at, bool alone) {
 #pragma unroll
     for (unsigned d = 0; d < D / 16; ++d) o[d] *= kSmallScale;
 #pragma unroll
@@ -356,7 +357,7 @@ struct Rows {
 #pragma unroll
         for (unsigned u = 0; u < 2; ++u) {
           const float x = fmaf(s[2 * b + e / 4][e % 4 + u], scale, kLift - m);
-          const bool here = moved && x < kSmall;
+          const bool here = alone && x < kSmall;
           p[u] = here ? __builtin_amdgcn_exp2f(x) : 0.0F;
           if (here) s[2 * b + e / 4][e % 4 + u] = -INFINITY;
           l += p[u];
@@ -379,9 +380,9 @@ struct Rows {
   // afterwards.  An edge block holds positions that some row does not see (below lo, past its
   // end, or in a tile of 16 whose page is missing: bit t of `missing`).
   //
-  // The weights go out as fp16 pairs, which keeps the accuracy of an fp32 product unless one score
-  // lies far above the others of its block and the others carry the output (its value is near
-  // zero): then add_small takes the others.  ready() returns when the block's V rows
+  // The weights go out as fp16 pairs, which keeps the accuracy of an fp32 product unless a peak
+  // lies far above the others of its block and the others carry the output (the peak's value is
+  // near zero): then add_small takes the others.  ready() returns when the block's V rows
   // are in LDS at value_at, zeros where no row sees them.
   template <unsigned T, typename Ready>
   __device__ __forceinline__ void weigh(f4 (&s)[T], unsigned lane, float scale, bool edge, uint32_t at, uint32_t lo,
@@ -425,10 +426,22 @@ struct Rows {
           least_score = __builtin_elementwise_minimum(least_score, x == -INFINITY ? INFINITY : x);
         }
       }
-      const bool moved = factor != 1.0F;
-      if (__builtin_expect(__any(moved && fmaf(least_score, scale, kLift - m) < kSmall), 0)) {
-        ready();
-        add_small(s, scale, value_at, moved);
+      const bool small = factor != 1.0F && fmaf(least_score, scale, kLift - m) < kSmall;
+      if (__builtin_expect(__any(small), 0)) {
+        bool between = false;
+#pragma unroll
+        for (unsigned e = 0; e < 4 * T; ++e) {
+          const float x = fmaf(s[e / 4][e % 4], scale, kLift - m);
+          between |= x >= kBetween && x < kPeak;
+        }
+        uint64_t rows = __ballot(between);
+        rows |= rows >> 32 | rows << 32;  // a row's four lanes
+        rows |= rows >> 16 | rows << 48;
+        const bool alone = factor != 1.0F && (rows >> lane & 1u) == 0;
+        if (__any(alone && small)) {
+          ready();
+          add_small(s, scale, value_at, alone);
+        }
       }
     }
     const float floor = m == -INFINITY ? 0.0F : m - kLift;
@@ -531,7 +544,9 @@ struct Item {
   bool own;
 };
 
-// Whether x holds in any lane of the workgroup.  flags: a word per wave, used once.
+// Whether x holds in any lane of the workgroup.  flags: a word per wave, used once.  (__syncthreads_or
+// keeps the thread's number in a register for it: spilled before the loop, its store is one that
+// the first loads wait for; 200 sequences of 250..500 positions took 81 us, not 75.)
 __device__ __forceinline__ bool in_any_wave(bool x, unsigned wave, uint32_t* flags) {
   const bool mine = __any(x);
   if (fresh_lane() == 0) flags[wave] = mine ? 1u : 0u;
@@ -542,8 +557,7 @@ __device__ __forceinline__ bool in_any_wave(bool x, unsigned wave, uint32_t* fla
   return __builtin_amdgcn_readfirstlane(found) != 0;
 }
 
-// Tiles of K and V rows and their marks (attend_rows); the output rows of 16 rows a wave and the
-// waves' flags follow.
+// Tiles of K and V rows and their marks (attend_rows); the waves' flags follow.
 template <unsigned D>
 constexpr std::size_t rows_bytes() {
   return kRing * (kTile * D * 2 * 2 + 4 * kWaves);
@@ -561,10 +575,9 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
   PageWindow window;
   window.start(pg, w.slot, (w.start + min(w.first_block + wave, w.last_block - 1) * kBlock) >> pg.page_shift);
   uint32_t* flags = reinterpret_cast<uint32_t*>(smem + rows_bytes<D>());
-  uint32_t* out_rows = flags + kWaves + 16 * wave;
   Rows<D> rows;
-  if (w.own) rows.template load<true>(a, w.base, w.first, w.rows, w.hk, w.hi, out_rows);
-  else rows.template load<false>(a, w.base, w.first, w.rows, w.hk, w.hi, out_rows);
+  if (w.own) rows.template load<true>(a, w.base, w.first, w.rows, w.hk, w.hi);
+  else rows.template load<false>(a, w.base, w.first, w.rows, w.hk, w.hi);
   const __half* keys = head_rows(a, pg.key, w.hk, D);
   const __half* values = head_rows(a, pg.value, w.hk, D);
   _Float16* ks = reinterpret_cast<_Float16*>(smem) + wave * 2 * kBlock * D;
@@ -684,9 +697,8 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
     factor[v] = x.x == -INFINITY ? 0.0F : rescale_factor(x.x, best);
     if (x.x != -INFINITY) total += x.y * factor[v];
   }
-  const uint32_t out_row = out_rows[n];
-  if (out_row == 0xffffffffu) return;
-  const std::size_t at = static_cast<std::size_t>(out_row) * (a.prefix_splits + a.own_splits) + w.split;
+  if (rows.out_row == 0xffffffffu) return;
+  const std::size_t at = static_cast<std::size_t>(rows.out_row) * (a.prefix_splits + a.own_splits) + w.split;
 #pragma unroll
   for (unsigned u = 0; u < kTiles / kWaves; ++u) {
     const unsigned d = wave * (kTiles / kWaves) + u;
@@ -778,10 +790,9 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
 
   Rows<D> rows;
   uint32_t* flags = reinterpret_cast<uint32_t*>(smem + rows_bytes<D>());
-  uint32_t* out_rows = flags + kWaves + 16 * wave;
   const uint32_t first = w.first + wave * 16;
-  if (w.own) rows.template load<true>(a, w.base, first, w.rows, w.hk, w.hi, out_rows);
-  else rows.template load<false>(a, w.base, first, w.rows, w.hk, w.hi, out_rows);
+  if (w.own) rows.template load<true>(a, w.base, first, w.rows, w.hk, w.hi);
+  else rows.template load<false>(a, w.base, first, w.rows, w.hk, w.hi);
   const bool works = first < w.rows;
   // A second, careful pass follows in the rare case that an output of the first is an
   // infinity or NaN, or a page was missing: values and pages are then looked at.
@@ -839,9 +850,8 @@ __device__ __forceinline__ void attend_rows(const PagedAttnArgs& a, const Item& 
   if (!works) return;
   rows.finish(careful);
   const unsigned late = fresh_lane();
-  const uint32_t out_row = out_rows[late & 15u];
-  if (out_row == 0xffffffffu) return;
-  const std::size_t to = static_cast<std::size_t>(out_row) * (a.prefix_splits + a.own_splits) + w.split;
+  if (rows.out_row == 0xffffffffu) return;
+  const std::size_t to = static_cast<std::size_t>(rows.out_row) * (a.prefix_splits + a.own_splits) + w.split;
 #pragma unroll
   for (unsigned d = 0; d < D / 16; ++d) *reinterpret_cast<f4*>(a.partial_o + to * D + 16 * d + 4 * (late >> 4)) = rows.o[d];
   if (late < 16) *reinterpret_cast<float2*>(a.partial_ml + 2 * to) = float2{rows.m, rows.l};
@@ -867,7 +877,7 @@ __host__ __device__ constexpr uint32_t tile_rows(uint32_t rows, uint32_t tiles) 
 // Work items: the prefix's come before the sequences' own.
 template <unsigned D>
 __global__ __launch_bounds__(kWaves * 64, resident(D) * kWaves / 4) void paged_attention_kernel(PagedAttnArgs a) {
-  __shared__ __align__(1024) char smem[rows_bytes<D>() + 4 * 17 * kWaves];
+  __shared__ __align__(1024) char smem[rows_bytes<D>() + 4 * kWaves];
   const uint32_t shared = prefix_length(a), id = blockIdx.x;
   const uint32_t group = a.q_heads / a.kv_heads, count = a.list.count;
   uint32_t range, tile;
