@@ -453,3 +453,38 @@ def test_a_sequence_keeps_its_bits_whatever_the_others_hold(device, gx, heads, t
     assert not np.array_equal(got[0], first[0])
     for i in (1, 2):
         assert np.array_equal(got[i].view(np.uint16), first[i].view(np.uint16)), i
+
+
+@pytest.mark.parametrize("shape", ["falling", "rising", "waves", "steps", "wide", "two peaks"])
+@pytest.mark.parametrize("heads,lengths,tokens,shared", [
+    ((64, 64, 128), [600] * 8, 1, 0), ((64, 64, 128), [600] * 8, 20, 0), ((128, 64, 256), [600] * 4, 17, 0),
+    (A, [2100, 2060, 2200], 1, 2048), (B, [2100, 2060, 2200], 3, 2048)])
+def test_maxima_that_move_both_ways(device, gx, heads, lengths, tokens, shared, shape):
+    """Scores that drift by up to 60 nats along the context, so that a row's stored maximum moves again and again, up, down and
+    to the end of its span; values as much larger as scores are lower, as far as fp16 goes."""
+    rng = np.random.default_rng(tokens + shared)
+    d = heads[2]
+    p = Problem(rng, *heads, 16, lengths, tokens, shared)
+    p.query[..., 0] = 8
+    drift = {"falling": lambda x: -60 * x, "rising": lambda x: 60 * x, "waves": lambda x: 15 * np.sin(40 * x),
+             "steps": lambda x: -20 * np.floor(3 * x), "wide": lambda x: 8 * rng.standard_normal(x.shape),
+             "two peaks": lambda x: 24.0 * (x == x[3]) + 12.0 * (x == x[len(x) // 2])}[shape]
+    for i, rows in enumerate(p.rows):
+        n = len(rows[0])
+        if i == 0 or not shared:
+            high = drift(np.arange(n) / n)
+        else:
+            high = np.concatenate([first[:shared], drift(np.arange(n) / n)[shared:]])
+        first = high if i == 0 else first
+        rows[0][..., 0] = (high * math.sqrt(d) / 8)[:, None]
+        gain = np.minimum(np.exp(high.max() - high), 2.0 ** 13)
+        rows[1][...] = np.clip(rows[1].astype(np.float64) * gain[:, None, None], -60000, 60000)
+        if shared and i:
+            rows[1][:shared] = p.rows[0][1][:shared]
+        for j in range(0, n, 16):
+            for pool, x in zip((p.k, p.v), rows):
+                pool[1, p.table[i, j // 16], :len(x[j:j + 16])] = x[j:j + 16]
+    say("moving maxima", shape, heads, tokens, shared)
+    got = p.run(gx)
+    some = [0, len(lengths) - 1]
+    p.check(got[some], some)
