@@ -35,30 +35,12 @@
 #include <algorithm>
 #include <cmath>
 
-#include "kv_pages.hpp"
+#include "kv_attention.hpp"
 
 namespace gfx950 {
 namespace {
 
-using h8 = _Float16 __attribute__((ext_vector_type(8)));
-using f4 = float __attribute__((ext_vector_type(4)));
-using h2 = _Float16 __attribute__((ext_vector_type(2)));
-using f2 = float __attribute__((ext_vector_type(2)));
-using u32x4 = unsigned __attribute__((ext_vector_type(4)));
-using s16x4 = short __attribute__((ext_vector_type(4)));
-using lds_void = __attribute__((address_space(3))) void;
-using global_void = __attribute__((address_space(1))) void;
-
 constexpr unsigned kBlock = 32;  // positions: a step of a wave by positions, half of one by rows
-constexpr float kLog2E = 1.4426950408889634F;
-
-// The factor between sums with maxima `from` and `to`, from <= to nearly always.  Never zero, so
-// that a NaN or an infinity of either reaches the result however far its scores lie below the
-// others (2^-126 of a finite sum is nothing beside theirs).
-__device__ __forceinline__ float rescale_factor(float from, float to) {
-  return fmaxf(__builtin_amdgcn_exp2f(from - to), 0x1p-126F);
-}
-
 // A row's weights are 2^(score - m + kLift), scores in units of log2.  The stored maximum m follows
 // the maxima of the blocks of positions, downwards too, once one leaves [m - kFall, m + kRise], but
 // stays within kSpan of its highest value so that the sums fit fp32.  The largest weight of every
@@ -114,10 +96,6 @@ __device__ __forceinline__ uint32_t splits_used(uint32_t blocks, uint32_t splits
   const uint32_t per = split_length(blocks, splits, least);
   return (blocks + per - 1) / per;
 }
-// Committed positions of a slot; a damaged length does not lead far past the table.
-__device__ __forceinline__ uint32_t committed(const KvPages& p, uint32_t slot) {
-  return min(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(p.lengths[slot])), p.stride << p.page_shift);
-}
 // Positions the batch's prefix covers: what the first sequence has of them.
 __device__ __forceinline__ uint32_t prefix_length(const PagedAttnArgs& a) {
   return min(a.shared, committed(a.pages, listed_slot(a.list, 0)));
@@ -152,22 +130,6 @@ __device__ __forceinline__ float sum_over_quarters(float v) {
   return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
-// Waits until at most Loads of the wave's loads from memory are on their way, and for all of
-// its LDS accesses.
-template <unsigned Loads>
-__device__ __forceinline__ void wait_loads() {
-  static_assert(Loads < 64);
-  __builtin_amdgcn_s_waitcnt((Loads & 15u) | (Loads >> 4) << 14 | 7u << 4);
-  asm volatile("" ::: "memory");
-}
-
-// K and V rows in LDS have no padding (loads into LDS fill it lane after lane); instead the
-// 16-byte pieces of a row are permuted, by the address each lane loads from: piece c of K row
-// r lies in slot c ^ (r % 16), of V row r in slot c ^ 2 (r % 8).  The rows of a score operand
-// and of a transposing read then fall on different banks.
-__device__ __forceinline__ unsigned key_slot(unsigned piece, unsigned row) { return piece ^ (row & 15u); }
-__device__ __forceinline__ unsigned value_slot(unsigned piece, unsigned row) { return piece ^ 2 * (row & 7u); }
-
 // A load of a wave into LDS covers 512 / D rows: where the lane's piece lies in memory, in
 // elements from the first of them, if that is row 0 of a tile.  From row r on (a multiple of
 // the rows of a load) it is at this ^ 8 (r % 16) for K and ^ 16 (r % 8) for V: rows start at
@@ -197,10 +159,6 @@ __device__ __forceinline__ unsigned value_place() {
   const unsigned lane = threadIdx.x & 63u, n = lane & 15u, row = 4 * (lane >> 4) + (n >> 2);
   return row * (D * 2) + 16 * value_slot((n & 3u) >> 1, row) + 8 * (n & 1u);
 }
-__device__ __forceinline__ unsigned lds_address(const _Float16* p) {
-  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)(p)));
-}
-
 // Reads from LDS that are complete when they return.  The compiler lets its own reads wait
 // for every load into LDS that is on its way, since it cannot tell the places apart; the
 // callers have waited for these rows, so the reads are written out with their own wait.
@@ -237,20 +195,6 @@ __device__ __forceinline__ void read_values(unsigned place, unsigned first, h8 (
   for (unsigned u = 0; u < 4; ++u) {
     v[u] = __builtin_bit_cast(h8, __builtin_shufflevector(a[2 * u], a[2 * u + 1], 0, 1, 2, 3, 4, 5, 6, 7));
   }
-}
-
-// The lane's number, made anew: what is computed from it inside a loop is not kept in
-// registers around the loop, where 128 of them do not suffice.
-__device__ __forceinline__ unsigned fresh_lane() {
-  unsigned lane;
-  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
-  return lane;
-}
-
-// The same for a number that is equal in all lanes.
-__device__ __forceinline__ uint32_t fresh_number(uint32_t x) {
-  asm volatile("" : "+s"(x));
-  return x;
 }
 
 // Sixteen rows of a wave: lane column n's row is the query q (B operand), sees the positions
@@ -502,35 +446,6 @@ struct Rows {
   }
 };
 
-// Eight values in LDS: infinities and NaNs become zeros.  Whether there were any.
-__device__ __forceinline__ bool take_strange(u32x4* at) {
-  u32x4 v = *at;
-  bool strange = false;
-#pragma unroll
-  for (unsigned e = 0; e < 4; ++e) {
-    const bool low = (v[e] & 0x7c00u) == 0x7c00u, high = (v[e] & 0x7c000000u) == 0x7c000000u;
-    strange |= low || high;
-    v[e] &= (low ? 0xffff0000u : 0xffffffffu) & (high ? 0xffffu : 0xffffffffu);
-  }
-  if (strange) *at = v;
-  return strange;
-}
-
-// A sequence's table row, 64 columns at a time in the lanes of a wave: a block's page is a
-// lane read, not a load on the way to the block's addresses.
-struct PageWindow {
-  uint32_t first;
-  int32_t entry;
-  __device__ __forceinline__ void start(const KvPages& pages, uint32_t slot, uint32_t column) {
-    first = column;
-    entry = table_page(pages, slot, column + (threadIdx.x & 63u));
-  }
-  __device__ __forceinline__ int32_t find(const KvPages& pages, uint32_t slot, uint32_t column) {
-    if (column - first >= 64u) start(pages, slot, column);  // uniform: columns only grow
-    return __builtin_amdgcn_readlane(entry, column - first);
-  }
-};
-
 // The K or V rows of a KV head of the launch's layer.
 __device__ __forceinline__ const __half* head_rows(const PagedAttnArgs& a, const __half* pool, uint32_t hk, unsigned d) {
   return pool + (static_cast<std::size_t>(a.layer) * a.pages.page_count << a.pages.page_shift) * a.pages.row + hk * d;
@@ -711,14 +626,6 @@ __device__ __forceinline__ void attend_positions(const PagedAttnArgs& a, const I
     *reinterpret_cast<f4*>(a.partial_o + at * D + 16 * d + 4 * kb) = sum;
   }
   if (wave == 0 && kb == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{best, total};
-}
-
-// A barrier that orders LDS accesses and leaves loads from memory into LDS on their way
-// (__syncthreads would wait for them).
-__device__ __forceinline__ void lds_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
 }
 
 // Up to 128 rows, 16 a wave; each K / V row is loaded into LDS once for all of them, tiles
