@@ -29,6 +29,7 @@ HEADERS = [os.path.join(ROOT, "include", "gfxinfer_amd.h"),
 OK, INVALID_ARGUMENT, IO_ERROR, CORRUPT_ARTIFACT, UNSUPPORTED, HIP_ERROR, OUT_OF_MEMORY, INTERNAL = range(8)
 # include/gfxinfer/artifact.h:26-33
 W2G128, W3G128, W4G128 = 1, 2, 3
+TYPE_F16, TYPE_F32, TYPE_BF16 = 0, 1, 2  # GFXI_F16, GFXI_F32, GFXI_BF16
 ERROR_NAMES = {0: "ok", 1: "invalid_argument", 2: "io_error", 3: "corrupt_artifact",
                4: "unsupported", 5: "hip_error", 6: "out_of_memory", 7: "internal"}
 
@@ -144,6 +145,16 @@ SIGNATURES: dict[str, tuple] = {
     "gfxinfer_launch_kv_pages_compact": (I32, [P, P, P, SZ, P]),
     "gfxinfer_kv_pages_attention_workspace_bytes": (SZ, [P, U32, U32, U32, SZ]),
     "gfxinfer_launch_kv_pages_gated_attention": (I32, [P, U32, P, P, P, P, U32, U32, U32, SZ, P, SZ, P]),
+    "gfxinfer_kv_pages_chunk_attention_workspace_bytes": (SZ, [P, P, U32, U32]),
+    "gfxinfer_launch_kv_pages_chunk_attention": (I32, [P, U32, P, P, P, P, P, P, U32, U32, P, SZ, P]),
+    "gfxinfer_launch_kv_weights_begin": (I32, [P, P, P, P, U32, P]),
+    "gfxinfer_kv_weights_workspace_bytes": (SZ, [P, P, U32, U32]),
+    "gfxinfer_launch_kv_weights_add": (I32, [P, P, U32, P, P, P, P, U32, U32, P, SZ, P]),
+    "gfxinfer_kv_pages_evict_workspace_bytes": (SZ, [P, U32, U32]),
+    "gfxinfer_launch_kv_pages_evict": (I32, [P, P, P, U32, U32, U32, U32, P, P, SZ, P]),
+    "gfxinfer_launch_quantize_rows_i8": (I32, [P, I32, SZ, SZ, SZ, P, P, P]),
+    "gfxinfer_w8a8_gemm_workspace_bytes": (SZ, [SZ, SZ, SZ]),
+    "gfxinfer_launch_w8a8_gemm": (I32, [P, P, P, P, P, I32, SZ, SZ, SZ, P, SZ, P]),
     "gfxinfer_logit_rules_workspace_bytes": (SZ, [SZ, U32]),
     "gfxinfer_launch_logit_rules": (I32, [P, SZ, SZ, U32, P, P, SZ, P, P, SZ, P]),
     # include/gfxinfer_runtime.h
@@ -515,6 +526,129 @@ def launch_kv_pages_gated_attention(pages, layer, query, gate, output, sequences
                                                      None if gate is None else _operand(gate, _real, 4 * size, device, "gate"),
                                                      _operand(output, _half, size, device, "output"), at, count, tokens, q_heads,
                                                      shared_tokens, *_scratch(workspace, device), _launch_stream(device, stream)))
+
+
+# ---- prompts in chunks, in a cache that stays within a budget --------------------
+
+class KvWeights(ctypes.Structure):
+    """gfxinfer_kv_weights.  `of` describes tensors beside the pages and keeps them alive."""
+    _fields_ = [("weight", P), ("position", P), ("dropped", P)]
+    device = None
+
+    @classmethod
+    def of(cls, pages, weight, position, dropped):
+        """weight fp32 and position int32 [sequences, table columns * page_tokens]; dropped int32 [sequences]."""
+        tensors, shape = (weight, position, dropped), (pages.sequences, pages.table_stride * pages.page_tokens)
+        if (tuple(weight.shape) != shape or tuple(position.shape) != shape or tuple(dropped.shape) != shape[:1]
+                or not all(t.is_contiguous() and t.element_size() == 4 for t in tensors) or not weight.is_floating_point()
+                or any(t.is_floating_point() for t in tensors[1:])):
+            raise ValueError("K/V weights: contiguous fp32 weight and int32 position for every row of the table, int32 dropped")
+        self = cls(*(_p(t) for t in tensors))
+        self.tensors, self.device = tensors, _device_of(tensors, "K/V weights")
+        if pages.device is not None and self.device not in (None, pages.device):
+            raise ValueError("K/V weights: tensors of another device than the pages")
+        return self
+
+
+def _chunk_lists(sequences, tokens):
+    """Host lists of a chunk call, their addresses, the number of sequences and of rows."""
+    ids, counts = _host_ids(sequences), _host_ids(tokens)
+    if len(ids) != len(counts):
+        raise ValueError("one number of tokens per sequence")
+    at, count = ids.buffer_info()
+    return ids, counts, at, counts.buffer_info()[0], count, sum(counts)
+
+
+def kv_pages_chunk_attention_workspace_bytes(pages, tokens, q_heads) -> int:
+    counts = _host_ids(tokens)
+    return int(lib().gfxinfer_kv_pages_chunk_attention_workspace_bytes(ctypes.byref(pages), *counts.buffer_info(), q_heads))
+
+
+def launch_kv_pages_chunk_attention(pages, layer, query, gate, output, log_sums, sequences, tokens, q_heads, workspace, stream=None):
+    """tokens: host list, new tokens of each sequence.  query and output fp16 [rows, q_heads, head_size], gate fp32 with rows
+    of 2 head_size or None, log_sums fp32 [rows, q_heads] or None; rows = sum(tokens)."""
+    L, device = lib(), pages.device
+    _ids, _counts, at, tokens_at, count, rows = _chunk_lists(sequences, tokens)
+    size = 2 * rows * q_heads * pages.head_size
+    check(L.gfxinfer_launch_kv_pages_chunk_attention(
+        ctypes.byref(pages), layer, _operand(query, _half, size, device, "query"),
+        None if gate is None else _operand(gate, _real, 4 * size, device, "gate"), _operand(output, _half, size, device, "output"),
+        None if log_sums is None else _operand(log_sums, _real, 4 * rows * q_heads, device, "log_sums"), at, tokens_at, count,
+        q_heads, *_scratch(workspace, device), _launch_stream(device, stream)))
+
+
+def launch_kv_weights_begin(pages, weights, sequences, tokens, stream=None):
+    L = lib()
+    _ids, _counts, at, tokens_at, count, _ = _chunk_lists(sequences, tokens)
+    check(L.gfxinfer_launch_kv_weights_begin(ctypes.byref(pages), ctypes.byref(weights), at, tokens_at, count,
+                                             _launch_stream(pages.device, stream)))
+
+
+def kv_weights_workspace_bytes(pages, tokens, q_heads) -> int:
+    counts = _host_ids(tokens)
+    return int(lib().gfxinfer_kv_weights_workspace_bytes(ctypes.byref(pages), *counts.buffer_info(), q_heads))
+
+
+def launch_kv_weights_add(pages, weights, layer, query, log_sums, sequences, tokens, q_heads, workspace, stream=None):
+    """query and log_sums as of launch_kv_pages_chunk_attention."""
+    L, device = lib(), pages.device
+    _ids, _counts, at, tokens_at, count, rows = _chunk_lists(sequences, tokens)
+    check(L.gfxinfer_launch_kv_weights_add(
+        ctypes.byref(pages), ctypes.byref(weights), layer, _operand(query, _half, 2 * rows * q_heads * pages.head_size, device, "query"),
+        _operand(log_sums, _real, 4 * rows * q_heads, device, "log_sums"), at, tokens_at, count, q_heads,
+        *_scratch(workspace, device), _launch_stream(device, stream)))
+
+
+def kv_pages_evict_workspace_bytes(pages, count, budget) -> int:
+    return int(lib().gfxinfer_kv_pages_evict_workspace_bytes(ctypes.byref(pages), count, budget))
+
+
+def launch_kv_pages_evict(pages, weights, sequences, budget, first, recent, status, workspace, stream=None):
+    """status: a device int32."""
+    L, ids, device = lib(), _host_ids(sequences), pages.device
+    at, count = ids.buffer_info()
+    check(L.gfxinfer_launch_kv_pages_evict(ctypes.byref(pages), ctypes.byref(weights), at, count, budget, first, recent,
+                                           _operand(status, _word, 4, device, "status"), *_scratch(workspace, device),
+                                           _launch_stream(device, stream)))
+
+
+# ---- products in 8-bit integers, any number of tokens ----------------------------
+
+def _types():
+    import torch
+    return {torch.float16: TYPE_F16, torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16}
+
+
+def launch_quantize_rows_i8(x, codes, scales, stream=None):
+    """x [rows, columns], fp16, fp32 or bf16 with dense rows; codes int8 [rows, columns]; scales fp32 [rows]."""
+    import torch
+    rows, columns = x.shape
+    L, device, kind = lib(), x.get_device(), _types().get(x.dtype)
+    if kind is None or x.stride(1) != 1 or not x.is_cuda:
+        raise ValueError("row quantizer: x is fp16, fp32 or bf16 [rows, columns] on a GPU, with dense rows")
+    check(L.gfxinfer_launch_quantize_rows_i8(
+        x.data_ptr(), kind, rows, columns, x.stride(0) if rows > 1 else -(-columns // 8) * 8,
+        _operand(codes, (torch.int8,), rows * columns, device, "codes"), _operand(scales, _real, 4 * rows, device, "scales"),
+        _launch_stream(device, stream)))
+
+
+def w8a8_gemm_workspace_bytes(rows, columns, tokens) -> int:
+    return int(lib().gfxinfer_w8a8_gemm_workspace_bytes(rows, columns, tokens))
+
+
+def launch_w8a8_gemm(weights, weight_scales, codes, scales, output, workspace, stream=None):
+    """weights int8 [rows, columns], weight_scales fp32 [rows], codes int8 [tokens, columns], scales fp32 [tokens], output fp32
+    or fp16 [tokens, rows]; workspace may be None where w8a8_gemm_workspace_bytes is 0."""
+    import torch
+    (rows, columns), tokens, L = weights.shape, codes.shape[0], lib()
+    device, kind = weights.get_device(), _types().get(output.dtype)
+    if not weights.is_cuda or tuple(codes.shape) != (tokens, columns) or tuple(output.shape) != (tokens, rows) or kind in (None, TYPE_BF16):
+        raise ValueError("8-bit product: weights [rows, columns] on a GPU, codes [tokens, columns], output fp32 or fp16 [tokens, rows]")
+    check(L.gfxinfer_launch_w8a8_gemm(
+        _operand(weights, (torch.int8,), rows * columns, device, "weights"), _operand(weight_scales, _real, 4 * rows, device, "weight_scales"),
+        _operand(codes, (torch.int8,), tokens * columns, device, "codes"), _operand(scales, _real, 4 * tokens, device, "scales"),
+        _operand(output, (output.dtype,), tokens * rows * output.element_size(), device, "output"), kind, rows, columns, tokens,
+        *_scratch(workspace, device), _launch_stream(device, stream)))
 
 
 # ---- rules on logits -------------------------------------------------------------

@@ -1,0 +1,682 @@
+// Gated GQA attention of ragged chunks of new tokens over the pages of a K/V cache.
+//
+// Row (t, g) of a listed sequence and a KV head, new token t at query head g of the head's
+// group, attends to the first length + t + 1 positions:
+//     o = softmax(q . K / sqrt(D)) . V * sigmoid(gate),   L = log(sum exp(q . K / sqrt(D)))
+// The rows of a sequence and KV head are one tall matrix, in tiles of 128: a workgroup takes a
+// tile and a range of positions, each of its four waves 32 of the rows, and a K / V row staged
+// in LDS serves all of them.
+//
+// Scores are computed transposed, S^T = K Q^T (v_mfma_f32_32x32x16_f16), so that a lane holds
+// half of one row's scores, the running maximum takes one lane exchange, and the weights are
+// already the B operand of O^T = V^T P^T when the positions of a step are numbered as the score
+// tiles leave them (k slot 8 h + e is position 4 h + e % 4 + 8 (e / 4), h the lane's half).  V
+// passes through LDS, whose transposing reads turn rows of V into columns.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "kv_attention.hpp"
+#include "kv_weights.hpp"
+
+namespace gfx950 {
+namespace {
+
+using f16v = float __attribute__((ext_vector_type(16)));
+using h4 = _Float16 __attribute__((ext_vector_type(4)));
+using lds_s16x4 = __attribute__((address_space(3))) s16x4;
+
+constexpr unsigned kWaves = 4, kRowsOfWave = 32, kRows = kWaves * kRowsOfWave;
+constexpr float kLn2 = 0.6931471805599453F;
+
+// Positions of a tile: 16 KB of K and of V either way, two of each in LDS, so that a CU holds two
+// workgroups.
+template <unsigned D>
+constexpr unsigned kTile = 8192 / D;
+
+// A row's weights are 2^(score - m + kLift) in fp16, scores in units of log2.  m is a maximum of
+// the row so far that moves up once it is passed by kRise, so weights stay below 2^15.  Against
+// the row's largest, weights down to 2^-25 keep fp16's 11 bits and those below 2^-36 are not
+// counted: the one rounding of the weights is half the size of the output's own.
+constexpr float kLift = 11.0F, kRise = 4.0F;
+
+struct ChunkAttnArgs {
+  KvPages pages;
+  ChunkList list;
+  uint32_t first_tile[kMaxChunks + 1];  // of the listed sequences' row tiles
+  const __half* query;   // [rows][q_heads][D]
+  const float* gate;     // [rows][q_heads][2 D] or null
+  __half* output;        // [rows][q_heads][D]
+  float* log_sums;       // [rows][q_heads] or null
+  float* partial_o;      // [rows][q_heads][splits][D], where positions are divided
+  float* partial_ml;     // [rows][q_heads][splits][2]
+  uint32_t layer, q_heads, kv_heads, group, splits;
+  float scale;           // log2(e) / sqrt(D)
+};
+
+// The listed sequence a row tile belongs to: one round of loads of the list instead of a search.
+__device__ __forceinline__ uint32_t sequence_of(const uint32_t* first, uint32_t count, uint32_t x) {
+  if (count == 1) return 0;
+  const unsigned lane = threadIdx.x & 63u;
+  uint32_t found = 0;
+  for (uint32_t from = 0; from < count; from += 64) {
+    found += static_cast<uint32_t>(__popcll(__ballot(from + lane < count && first[min(from + lane, kMaxChunks)] <= x)));
+  }
+  return __builtin_amdgcn_readfirstlane(found) - 1;
+}
+
+// Tiles of positions a range holds at least, and how a row tile's positions are divided.
+constexpr uint32_t kLeastTiles = 4;
+__device__ __forceinline__ uint32_t tiles_per_split(uint32_t tiles, uint32_t splits) {
+  return max(kLeastTiles, (tiles + splits - 1) / splits);
+}
+
+__device__ __forceinline__ float max_over_halves(float v) {
+  const unsigned u = __float_as_uint(v);
+  const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float sum_over_halves(float v) {
+  const unsigned u = __float_as_uint(v);
+  const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// One item: row tile `tile` of listed sequence i at KV head hk, positions [from, to) tiles.
+template <unsigned D>
+__global__ __launch_bounds__(kWaves * 64, 2) void chunk_attention_kernel(ChunkAttnArgs a) {
+  constexpr unsigned T = kTile<D>, kSub = T / 32, kSteps = T / 16;
+  constexpr unsigned kLoadRows = 512 / D;                   // rows a load of a wave covers
+  constexpr unsigned kLoads = T / kLoadRows / kWaves;       // of K, and of V, per tile and wave
+  __shared__ __align__(1024) _Float16 k0[T * D];
+  __shared__ __align__(1024) _Float16 k1[T * D];
+  __shared__ __align__(1024) _Float16 v0[T * D];
+  __shared__ __align__(1024) _Float16 v1[T * D];
+  __shared__ uint32_t marks[2][kWaves];
+  __shared__ uint32_t again[kWaves];
+  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned n = lane & 31u, h = lane >> 5;
+  const KvPages& pg = a.pages;
+
+  // KV heads vary fastest: with eight of them each XCD reads one.  Late tokens, which see most, first.
+  const uint32_t hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
+  const uint32_t split = rest % a.splits, all_tiles = a.first_tile[kMaxChunks];
+  const uint32_t row_tile = all_tiles - 1 - rest / a.splits;
+  const uint32_t i = sequence_of(a.first_tile, a.list.count, row_tile);
+  const uint32_t slot = listed_slot(a.list, i), first_row = a.list.first[i], tokens = a.list.first[i + 1] - first_row;
+  const uint32_t length = committed(pg, slot), rows = tokens * a.group;
+  const uint32_t tile_row = (row_tile - a.first_tile[i]) * kRows;
+  // The tile's last row sees this many positions; what lies behind the sequence's end is not read.
+  const uint32_t last_row = min(rows, tile_row + kRows) - 1;
+  const uint32_t end = length + tokens, hi = length + last_row / a.group + 1;
+  const uint32_t tiles = (hi + T - 1) / T, per = tiles_per_split(tiles, a.splits);
+  const uint32_t from = split * per, to = min(from + per, tiles);
+  if (from >= tiles) return;
+
+  const uint32_t row = tile_row + wave * kRowsOfWave + n;
+  const bool works = tile_row + wave * kRowsOfWave < rows;   // the wave has a row
+  const uint32_t t = row / a.group, g = row - t * a.group;
+  const std::size_t out_row = (static_cast<std::size_t>(first_row) + t) * a.q_heads + hk * a.group + g;
+  const uint32_t visible = row < rows ? length + t + 1 : 0;
+  const uint32_t least = row < rows ? length + (tile_row + wave * kRowsOfWave) / a.group + 1 : 0;   // of the wave's rows
+  const uint32_t least_visible = __builtin_amdgcn_readfirstlane(least);
+  h8 q[D / 16];
+#pragma unroll
+  for (unsigned s = 0; s < D / 16; ++s) {
+    q[s] = h8{};
+    if (row < rows) q[s] = *reinterpret_cast<const h8*>(a.query + out_row * D + 16 * s + 8 * h);
+  }
+
+  const std::size_t layer_row = (static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) * pg.row + hk * D;
+  const __half* keys = pg.key + layer_row;
+  const __half* values = pg.value + layer_row;
+  const uint32_t in_page = (1u << pg.page_shift) - 1;
+  PageWindow window;
+  // The pages of a tile's parts of 16 positions; parts past the end load from page 0 of the pool
+  // (always there), as missing ones do.
+  int32_t page[T / 16];
+  auto find_pages = [&](uint32_t at) __attribute__((always_inline)) {
+    uint32_t missing = 0;
+#pragma unroll
+    for (unsigned p = 0; p < T / 16; ++p) {
+      page[p] = at + 16 * p < end ? window.find(pg, slot, (at + 16 * p) >> pg.page_shift) : -1;
+      if (page[p] < 0) missing |= 1u << p;
+    }
+    return missing;
+  };
+  auto load = [&](_Float16* ks, _Float16* vs, uint32_t at) __attribute__((always_inline)) {
+    const unsigned r = lane / (D / 8);
+#pragma unroll
+    for (unsigned u = 0; u < kLoads; ++u) {
+      // All rows of a load are of one part; parts go to the waves in turn.
+      const unsigned row0 = kLoadRows * (wave + kWaves * u);
+      int32_t p = page[0];
+#pragma unroll
+      for (unsigned e = 1; e < T / 16; ++e) p = row0 / 16 == e ? page[e] : p;
+      const std::size_t base = ((static_cast<std::size_t>(max(p, 0)) << pg.page_shift) + ((at + row0) & in_page) + r) * pg.row;
+      const unsigned key_piece = key_slot(lane % (D / 8), row0 + r), value_piece = value_slot(lane % (D / 8), row0 + r);
+      __builtin_amdgcn_global_load_lds((global_void*)(keys + base + 8 * key_piece), (lds_void*)(ks + row0 * D), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_void*)(values + base + 8 * value_piece), (lds_void*)(vs + row0 * D), 16, 0, 0);
+    }
+  };
+
+  f16v o[D / 32];
+  float m, l;
+  bool careful = false;
+  // What a page holds past a sequence's end, and what a missing one would, may be anything, and 0 * NaN
+  // is NaN: the wave's own V rows of such positions become zeros.  A careful pass also takes out
+  // infinities and NaNs, and marks the tile.
+  auto repair = [&](_Float16* vs, uint32_t at, uint32_t missing, unsigned b) __attribute__((always_inline)) {
+    bool strange = false;
+#pragma unroll
+    for (unsigned u = 0; u < kLoads; ++u) {
+      const unsigned row0 = kLoadRows * (wave + kWaves * u);
+      u32x4* piece = reinterpret_cast<u32x4*>(vs + row0 * D) + lane;
+      if (at + row0 + lane / (D / 8) >= end || (missing >> row0 / 16 & 1u) != 0) *piece = u32x4{0, 0, 0, 0};
+      if (careful) strange |= take_strange(piece);
+    }
+    if (careful) {
+      const bool any = __any(strange);
+      if (lane == 0) marks[b][wave] = any ? 1u : 0u;
+    }
+  };
+  // The rows that see an infinity or NaN among the values get it, whatever the weight: no weight is
+  // exactly zero.
+  auto add_strange = [&](uint32_t at) {
+#pragma unroll 1
+    for (unsigned p = 0; p < T; ++p) {
+      const uint32_t position = at + p;
+      const int32_t pp = position < end ? table_page(pg, slot, position >> pg.page_shift) : -1;
+      if (pp < 0) continue;
+      const __half* x = values + ((static_cast<std::size_t>(pp) << pg.page_shift) + (position & in_page)) * pg.row;
+#pragma unroll
+      for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+        for (unsigned r = 0; r < 16; ++r) {
+          const float y = __half2float(x[32 * d + 8 * (r / 4) + 4 * h + r % 4]);
+          if (!(fabsf(y) < INFINITY) && position < visible) o[d][r] += y;
+        }
+      }
+    }
+    wait_loads<0>();
+  };
+  auto attend = [&](const _Float16* ks, const _Float16* vs, uint32_t at, uint32_t missing, unsigned b) __attribute__((always_inline)) {
+    f16v s[kSub];
+#pragma unroll
+    for (unsigned u = 0; u < kSub; ++u) {
+      s[u] = f16v{};
+#pragma unroll
+      for (unsigned st = 0; st < D / 16; ++st) {
+        const h8 k = *reinterpret_cast<const h8*>(ks + (32 * u + n) * D + 8 * key_slot(2 * st + h, n));
+        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[st], s[u], 0, 0, 0);
+      }
+    }
+    if (at + T > least_visible || missing != 0) {
+#pragma unroll
+      for (unsigned u = 0; u < kSub; ++u) {
+#pragma unroll
+        for (unsigned r = 0; r < 16; ++r) {
+          const unsigned p = 32 * u + 8 * (r / 4) + 4 * h + r % 4;
+          if (at + p >= visible || (missing >> p / 16 & 1u) != 0) s[u][r] = -INFINITY;
+        }
+      }
+    }
+    // (A NaN score makes the maximum NaN and the row's result with it, as it has to.)
+    float best = s[0][0];
+#pragma unroll
+    for (unsigned e = 1; e < 16 * kSub; ++e) best = __builtin_elementwise_maximum(best, s[e / 16][e % 16]);
+    const float top = max_over_halves(best) * a.scale;
+    if (__any(!(top <= m + kRise))) {
+      const float next = top <= m + kRise ? m : top;
+      // From nothing to something: there is nothing to scale yet.
+      const float factor = next == m || m == -INFINITY ? 1.0F : rescale_factor(m, next);
+      m = next;
+      l *= factor;
+#pragma unroll
+      for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+        for (unsigned r = 0; r < 16; ++r) o[d][r] *= factor;
+      }
+    }
+    const float floor = m == -INFINITY ? 0.0F : m - kLift;
+    h8 p[kSteps];
+#pragma unroll
+    for (unsigned j = 0; j < kSteps; ++j) {
+#pragma unroll
+      for (unsigned e = 0; e < 8; ++e) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[j / 2][8 * (j % 2) + e], a.scale, -floor));
+        l += w;
+        p[j][e] = static_cast<_Float16>(w);
+      }
+    }
+    if (careful) {
+      uint32_t mark = 0;
+      for (unsigned w = 0; w < kWaves; ++w) mark |= marks[b][w];
+      if (__builtin_amdgcn_readfirstlane(mark) != 0) add_strange(at);
+    }
+    const unsigned group16 = lane >> 4, i16 = lane & 15u;
+    const unsigned vrow = 4 * (group16 >> 1) + (i16 >> 2), vpiece = 2 * (group16 & 1u) + ((i16 & 3u) >> 1);
+#pragma unroll
+    for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+      for (unsigned j = 0; j < kSteps; ++j) {
+        s16x4 x[2];
+#pragma unroll
+        for (unsigned e = 0; e < 2; ++e) {
+          const unsigned r = 16 * j + 8 * e + vrow;
+          const _Float16* at_value = vs + r * D + 8 * value_slot(4 * d + vpiece, r) + 4 * (i16 & 1u);
+          x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(const_cast<_Float16*>(at_value)));
+        }
+        const h8 v = __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[j], o[d], 0, 0, 0);
+      }
+    }
+  };
+
+  for (;; careful = true) {
+    m = -INFINITY;
+    l = 0.0F;
+#pragma unroll
+    for (unsigned d = 0; d < D / 32; ++d) o[d] = f16v{};
+    window.start(pg, slot, (from * T) >> pg.page_shift);
+    uint32_t missing0 = find_pages(from * T), missing1 = 0;
+    load(k0, v0, from * T);
+#pragma unroll 1
+    for (uint32_t x = from; x < to; x += 2) {
+      wait_loads<0>();
+      if (careful || missing0 != 0 || (x + 1) * T > end) {
+        repair(v0, x * T, missing0, 0);
+        wait_loads<63>();
+      }
+      __syncthreads();
+      if (x + 1 < to) {
+        missing1 = find_pages((x + 1) * T);
+        load(k1, v1, (x + 1) * T);
+      }
+      if (works) attend(k0, v0, x * T, missing0, 0);
+      if (x + 1 < to) {
+        wait_loads<0>();
+        if (careful || missing1 != 0 || (x + 2) * T > end) {
+          repair(v1, (x + 1) * T, missing1, 1);
+          wait_loads<63>();
+        }
+        __syncthreads();
+        if (x + 2 < to) {
+          missing0 = find_pages((x + 2) * T);
+          load(k0, v0, (x + 2) * T);
+        }
+        if (works) attend(k1, v1, (x + 1) * T, missing1, 1);
+      }
+    }
+    // Whether an output is an infinity or NaN: finite values at weights below 2^15 make none.
+    bool strange = false;
+#pragma unroll
+    for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+      for (unsigned r = 0; r < 16; ++r) strange |= !(fabsf(o[d][r]) < INFINITY);
+    }
+    const bool mine = works && __any(strange);
+    if (lane == 0) again[wave] = mine ? 1u : 0u;
+    __syncthreads();
+    uint32_t found = 0;
+    for (unsigned w = 0; w < kWaves; ++w) found |= again[w];
+    if (careful || __builtin_amdgcn_readfirstlane(found) == 0) {
+      l = sum_over_halves(l);
+      // Only NaN scores, and strange values at scores of -infinity, make a NaN row rather than an empty one.
+      if ((m == -INFINITY && (l != l || (careful && strange))) || m != m) m = 0.0F;
+      break;
+    }
+    __syncthreads();
+  }
+  if (row >= rows) return;
+  if (a.splits > 1) {
+    const std::size_t at = out_row * a.splits + split;
+#pragma unroll
+    for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+      for (unsigned r = 0; r < 16; r += 4) {
+        *reinterpret_cast<f4*>(a.partial_o + at * D + 32 * d + 2 * r + 4 * h) = f4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+      }
+    }
+    if (h == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{m, l};
+    return;
+  }
+  const bool empty = m == -INFINITY;
+  const float inverse = empty ? 0.0F : 1.0F / l;
+#pragma unroll
+  for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+    for (unsigned r = 0; r < 16; r += 4) {
+      const unsigned at = 32 * d + 2 * r + 4 * h;
+      f4 y;
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) y[e] = empty ? 0.0F : o[d][r + e] * inverse;
+      if (a.gate != nullptr) {
+        const f4 gate = *reinterpret_cast<const f4*>(a.gate + out_row * 2 * D + D + at);
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) y[e] *= 1.0F / (1.0F + expf(-gate[e]));
+      }
+      h4 out;
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) out[e] = static_cast<_Float16>(y[e]);
+      *reinterpret_cast<h4*>(a.output + out_row * D + at) = out;
+    }
+  }
+  if (a.log_sums != nullptr && h == 0) a.log_sums[out_row] = empty ? -INFINITY : (m - kLift) * kLn2 + logf(l);
+}
+
+// Merges a row's ranges of positions and applies the gate: a wave per row and query head, D / 64
+// dims a lane.
+template <unsigned D>
+__global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkAttnArgs a) {
+  constexpr unsigned J = D / 64;
+  const unsigned lane = threadIdx.x & 63u;
+  const uint32_t rows = a.list.first[kMaxChunks] * a.q_heads;
+  const uint32_t linear = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
+  if (linear >= rows) return;
+  const uint32_t row = linear / a.q_heads, i = sequence_of(a.list.first, a.list.count, row);
+  const uint32_t slot = listed_slot(a.list, i), tokens = a.list.first[i + 1] - a.list.first[i];
+  const uint32_t length = committed(a.pages, slot), t = row - a.list.first[i];
+  const uint32_t tile_row = (t * a.group + linear % a.q_heads % a.group) / kRows * kRows;
+  const uint32_t hi = length + (min(tokens * a.group, tile_row + kRows) - 1) / a.group + 1;
+  const uint32_t tiles = (hi + kTile<D> - 1) / kTile<D>, per = tiles_per_split(tiles, a.splits);
+  const uint32_t used = (tiles + per - 1) / per;
+  const std::size_t base = static_cast<std::size_t>(linear) * a.splits;
+  float best = -INFINITY;
+  for (uint32_t s = 0; s < used; ++s) best = fmaxf(best, a.partial_ml[2 * (base + s)]);
+  float total = 0.0F, y[J] = {};
+  for (uint32_t s = 0; s < used; ++s) {
+    const float2 x = *reinterpret_cast<const float2*>(a.partial_ml + 2 * (base + s));
+    if (x.x == -INFINITY) continue;
+    const float w = rescale_factor(x.x, best);
+    total += x.y * w;
+#pragma unroll
+    for (unsigned j = 0; j < J; ++j) y[j] = fmaf(a.partial_o[(base + s) * D + J * lane + j], w, y[j]);
+  }
+  const bool empty = best == -INFINITY;
+#pragma unroll
+  for (unsigned j = 0; j < J; ++j) {
+    y[j] = empty ? 0.0F : y[j] / total;
+    if (a.gate != nullptr) y[j] *= 1.0F / (1.0F + expf(-a.gate[static_cast<std::size_t>(linear) * 2 * D + D + J * lane + j]));
+    a.output[static_cast<std::size_t>(linear) * D + J * lane + j] = to_half(y[j]);
+  }
+  if (a.log_sums != nullptr && lane == 0) a.log_sums[linear] = empty ? -INFINITY : (best - kLift) * kLn2 + logf(total);
+}
+
+// ---- the weight that each position receives ---------------------------------------------
+
+struct WeightArgs {
+  KvPages pages;
+  KvWeights weights;
+  ChunkList list;
+  const __half* query;
+  const float* log_sums;
+  float* partial;  // [count][kv_heads * parts][capacity]
+  uint32_t layer, q_heads, kv_heads, group, parts;
+  uint32_t columns;  // workgroups along the positions
+  float scale;
+};
+
+constexpr unsigned kWeightPositions = 128;  // of a workgroup: 32 a wave
+constexpr unsigned kWeightRows = 32;        // rows staged at a time
+
+// A wave holds 32 positions of K as the A operand; the rows of a KV head pass through LDS, 32
+// at a time, and each score's exponential is added to the lane's sum of its position.
+template <unsigned D>
+__global__ __launch_bounds__(256) void weight_kernel(WeightArgs a) {
+  __shared__ __align__(1024) _Float16 rows0[kWeightRows * D];
+  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned n = lane & 31u, h = lane >> 5;
+  const KvPages& pg = a.pages;
+  const uint32_t hk = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads % a.parts;
+  const uint32_t column = blockIdx.x / a.kv_heads / a.parts, i = blockIdx.y;
+  const uint32_t slot = listed_slot(a.list, i), first_row = a.list.first[i], tokens = a.list.first[i + 1] - first_row;
+  const uint32_t length = committed(pg, slot), end = min(length + tokens, pg.stride << pg.page_shift);
+  const uint32_t rows = tokens * a.group, all = (rows + kWeightRows - 1) / kWeightRows;
+  const uint32_t per = (all + a.parts - 1) / a.parts, from = part * per, to = min(from + per, all);
+  const uint32_t in_page = (1u << pg.page_shift) - 1;
+  const __half* keys = pg.key + (static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) * pg.row + hk * D;
+  const std::size_t plane = (static_cast<std::size_t>(i) * a.kv_heads + hk) * a.parts + part;
+  float* sums = a.partial + plane * (static_cast<std::size_t>(pg.stride) << pg.page_shift);
+  for (uint32_t at = column * kWeightPositions; at < end; at += a.columns * kWeightPositions) {
+    const uint32_t mine = at + 32 * wave, position = mine + n;
+    const int32_t page = position < end ? table_page(pg, slot, position >> pg.page_shift) : -1;
+    const __half* source = keys + ((static_cast<std::size_t>(max(page, 0)) << pg.page_shift) + (page < 0 ? 0 : position & in_page)) * pg.row;
+    h8 k[D / 16];
+#pragma unroll
+    for (unsigned s = 0; s < D / 16; ++s) k[s] = *reinterpret_cast<const h8*>(source + 16 * s + 8 * h);
+    float sum[16] = {};
+    for (uint32_t x = from; x < to; ++x) {
+      const uint32_t row0 = x * kWeightRows;
+      // Rows before the tile's first position see nothing of it.
+      if (length + min(rows, row0 + kWeightRows) / a.group + 1 <= at) continue;
+      __syncthreads();
+#pragma unroll
+      for (unsigned u = threadIdx.x; u < kWeightRows * D / 8; u += 256) {
+        const uint32_t r = u / (D / 8), c = u % (D / 8), row = min(row0 + r, rows - 1), t = row / a.group;
+        const std::size_t out_row = (static_cast<std::size_t>(first_row) + t) * a.q_heads + hk * a.group + (row - t * a.group);
+        *reinterpret_cast<u32x4*>(rows0 + r * D + 8 * key_slot(c, r)) = *reinterpret_cast<const u32x4*>(a.query + out_row * D + 8 * c);
+      }
+      __syncthreads();
+      const uint32_t row = row0 + n, t = row / a.group;
+      float level = INFINITY;
+      uint32_t visible = 0;
+      if (row < rows) {
+        level = a.log_sums[(static_cast<std::size_t>(first_row) + t) * a.q_heads + hk * a.group + (row - t * a.group)] * kLog2E;
+        visible = level > -INFINITY ? length + t + 1 : 0;   // a row that sees nothing, or a NaN
+      }
+      f16v s = f16v{};
+#pragma unroll
+      for (unsigned st = 0; st < D / 16; ++st) {
+        const h8 q = *reinterpret_cast<const h8*>(rows0 + n * D + 8 * key_slot(2 * st + h, n));
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[st], q, s, 0, 0, 0);
+      }
+#pragma unroll
+      for (unsigned r = 0; r < 16; ++r) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale, -level));
+        sum[r] += mine + 8 * (r / 4) + 4 * h + r % 4 < visible ? w : 0.0F;
+      }
+    }
+    // A position's sum lies over the 32 lanes of a half.
+#pragma unroll
+    for (unsigned r = 0; r < 16; ++r) {
+#pragma unroll
+      for (unsigned d = 1; d < 32; d <<= 1) sum[r] += __shfl_xor(sum[r], d);
+    }
+#pragma unroll
+    for (unsigned r = 0; r < 16; ++r) {
+      const uint32_t p = mine + 8 * (r / 4) + 4 * h + r % 4;
+      if (n == r && p < end) sums[p] = sum[r];
+    }
+  }
+}
+
+// Adds the planes of the KV heads and row parts, in their order, to what the positions have.
+__global__ __launch_bounds__(256) void weight_join_kernel(WeightArgs a) {
+  const KvPages& pg = a.pages;
+  const uint32_t i = blockIdx.y, slot = listed_slot(a.list, i), tokens = a.list.first[i + 1] - a.list.first[i];
+  const uint32_t capacity = pg.stride << pg.page_shift, end = min(committed(pg, slot) + tokens, capacity);
+  if (tokens == 0) return;
+  const uint32_t planes = a.kv_heads * a.parts;
+  for (uint32_t p = blockIdx.x * 256 + threadIdx.x; p < end; p += gridDim.x * 256) {
+    if (table_page(pg, slot, p >> pg.page_shift) < 0) continue;
+    const float* at = a.partial + static_cast<std::size_t>(i) * planes * capacity + p;
+    float sum = 0.0F;
+    for (uint32_t x = 0; x < planes; ++x) sum += at[static_cast<std::size_t>(x) * capacity];
+    a.weights.weight[static_cast<std::size_t>(slot) * capacity + p] += sum;
+  }
+}
+
+// ---- host side ---------------------------------------------------------------------------
+
+int32_t read_heads(const gfxinfer_kv_pages* pages, uint32_t q_heads) {
+  if (q_heads == 0 || q_heads > 1024 || q_heads % pages->kv_heads != 0) {
+    return fail(GFXI_INVALID_ARGUMENT, "query heads are 1..1024 and a multiple of the cache's KV heads");
+  }
+  return GFXI_OK;
+}
+
+struct ChunkShape {
+  uint32_t tiles, splits;
+};
+
+ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads, uint32_t head_size,
+                       uint32_t* first_tile) {
+  ChunkShape s{};
+  const uint32_t group = q_heads / kv_heads;
+  for (uint32_t i = 0; i < list.count; ++i) {
+    first_tile[i] = s.tiles;
+    const uint64_t rows = static_cast<uint64_t>(list.first[i + 1] - list.first[i]) * group;
+    s.tiles += static_cast<uint32_t>((rows + kRows - 1) / kRows);
+  }
+  for (uint32_t i = list.count; i <= kMaxChunks; ++i) first_tile[i] = s.tiles;
+  const uint32_t tile = head_size == 128 ? kTile<128> : kTile<256>;
+  const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift;
+  const uint64_t places = 2 * kComputeUnits, items = static_cast<uint64_t>(s.tiles) * kv_heads;
+  const uint64_t most = std::max<uint64_t>(1, capacity / (tile * kLeastTiles));
+  s.splits = static_cast<uint32_t>(std::clamp<uint64_t>((places + items - 1) / items, 1, most));
+  return s;
+}
+
+std::size_t chunk_bytes(const ChunkShape& s, const ChunkList& list, uint32_t q_heads, uint32_t head_size) {
+  return s.splits == 1 ? 0 : static_cast<std::size_t>(list.first[kMaxChunks]) * q_heads * s.splits * (head_size + 2) * sizeof(float);
+}
+
+uint32_t weight_parts(const KvPages& p, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads, uint32_t& columns) {
+  const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift;
+  columns = static_cast<uint32_t>(std::min<uint64_t>((capacity + kWeightPositions - 1) / kWeightPositions, 1024));
+  uint32_t most = 0;
+  for (uint32_t i = 0; i < list.count; ++i) most = std::max(most, list.first[i + 1] - list.first[i]);
+  const uint64_t blocks = (static_cast<uint64_t>(most) * (q_heads / kv_heads) + kWeightRows - 1) / kWeightRows;
+  const uint64_t items = static_cast<uint64_t>(columns) * kv_heads * list.count;
+  return static_cast<uint32_t>(std::clamp<uint64_t>(4 * kComputeUnits / items, 1, std::max<uint64_t>(1, blocks / 4)));
+}
+
+std::size_t weight_bytes(const KvPages& p, const ChunkList& list, uint32_t kv_heads, uint32_t parts) {
+  return static_cast<std::size_t>(list.count) * kv_heads * parts * (static_cast<std::size_t>(p.stride) << p.page_shift) * sizeof(float);
+}
+
+}  // namespace
+}  // namespace gfx950
+
+using namespace gfx950;
+
+extern "C" size_t gfxinfer_kv_pages_chunk_attention_workspace_bytes(const gfxinfer_kv_pages* pages, const uint32_t* tokens,
+                                                                    uint32_t count, uint32_t q_heads) {
+  size_t bytes = 0;
+  guarded([&] {
+    ChunkAttnArgs a{};
+    if (const int32_t s = read_pages(pages, a.pages); s != GFXI_OK) return s;
+    if (const int32_t s = read_heads(pages, q_heads); s != GFXI_OK) return s;
+    // The slots do not matter here: every entry names the first one.
+    const std::vector<uint32_t> any(std::min(count, kMaxChunks + 1), 0u);
+    if (const int32_t s = read_chunks(a.pages, any.data(), tokens, count, false, a.list); s != GFXI_OK) return s;
+    const ChunkShape shape = chunk_shape(a.pages, a.list, q_heads, pages->kv_heads, pages->head_size, a.first_tile);
+    bytes = chunk_bytes(shape, a.list, q_heads, pages->head_size);
+    return GFXI_OK;
+  });
+  return bytes;
+}
+
+extern "C" int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pages* pages, uint32_t layer, const uint16_t* query,
+                                                            const float* gate, uint16_t* output, float* log_sums,
+                                                            const uint32_t* sequences, const uint32_t* tokens, uint32_t count,
+                                                            uint32_t q_heads, float* workspace, size_t workspace_bytes,
+                                                            void* stream) {
+  return guarded([&] {
+    ChunkAttnArgs a{};
+    if (const int32_t s = read_pages(pages, a.pages); s != GFXI_OK) return s;
+    if (const int32_t s = read_heads(pages, q_heads); s != GFXI_OK) return s;
+    if (const int32_t s = read_chunks(a.pages, sequences, tokens, count, false, a.list); s != GFXI_OK) return s;
+    if (layer >= a.pages.layers || query == nullptr || output == nullptr || !aligned16(query) || !aligned16(gate) ||
+        (reinterpret_cast<uintptr_t>(output) & 7u) != 0 || (reinterpret_cast<uintptr_t>(log_sums) & 3u) != 0) {
+      return fail(GFXI_INVALID_ARGUMENT, "chunk attention needs a layer of the cache and aligned rows (query and gate 16 bytes, "
+                                         "output 8)");
+    }
+    const uint32_t head_size = pages->head_size, kv_heads = pages->kv_heads;
+    const ChunkShape shape = chunk_shape(a.pages, a.list, q_heads, kv_heads, head_size, a.first_tile);
+    const std::size_t need = chunk_bytes(shape, a.list, q_heads, head_size);
+    if (need != 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need)) {
+      return fail(GFXI_INVALID_ARGUMENT, "chunk attention workspace is null, not 16-byte aligned or too small");
+    }
+    const std::size_t rows = static_cast<std::size_t>(a.list.first[kMaxChunks]) * q_heads;
+    a.query = reinterpret_cast<const __half*>(query);
+    a.gate = gate;
+    a.output = reinterpret_cast<__half*>(output);
+    a.log_sums = log_sums;
+    a.partial_o = workspace;
+    a.partial_ml = workspace == nullptr ? nullptr : workspace + rows * shape.splits * head_size;
+    a.layer = layer;
+    a.q_heads = q_heads;
+    a.kv_heads = kv_heads;
+    a.group = q_heads / kv_heads;
+    a.splits = shape.splits;
+    a.scale = kLog2E / std::sqrt(static_cast<float>(head_size));
+    const uint64_t items = static_cast<uint64_t>(shape.tiles) * shape.splits * kv_heads;
+    if (items > (1u << 30)) return fail(GFXI_INVALID_ARGUMENT, "chunk attention over too many rows for one launch");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const dim3 grid(static_cast<unsigned>(items)), block(kWaves * 64);
+    if (head_size == 128) hipLaunchKernelGGL(chunk_attention_kernel<128>, grid, block, 0, st, a);
+    else hipLaunchKernelGGL(chunk_attention_kernel<256>, grid, block, 0, st, a);
+    if (const int32_t s = launch_status("chunk attention launch failed"); s != GFXI_OK || shape.splits == 1) return s;
+    const dim3 combine(static_cast<unsigned>((rows + 3) / 4));
+    if (head_size == 128) hipLaunchKernelGGL(chunk_combine_kernel<128>, combine, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(chunk_combine_kernel<256>, combine, dim3(256), 0, st, a);
+    return launch_status("chunk attention combine launch failed");
+  });
+}
+
+extern "C" size_t gfxinfer_kv_weights_workspace_bytes(const gfxinfer_kv_pages* pages, const uint32_t* tokens, uint32_t count,
+                                                      uint32_t q_heads) {
+  size_t bytes = 0;
+  guarded([&] {
+    KvPages p;
+    ChunkList list;
+    if (const int32_t s = read_pages(pages, p); s != GFXI_OK) return s;
+    if (const int32_t s = read_heads(pages, q_heads); s != GFXI_OK) return s;
+    const std::vector<uint32_t> any(std::min(count, kMaxChunks + 1), 0u);
+    if (const int32_t s = read_chunks(p, any.data(), tokens, count, false, list); s != GFXI_OK) return s;
+    uint32_t columns;
+    bytes = weight_bytes(p, list, pages->kv_heads, weight_parts(p, list, q_heads, pages->kv_heads, columns));
+    return GFXI_OK;
+  });
+  return bytes;
+}
+
+extern "C" int32_t gfxinfer_launch_kv_weights_add(const gfxinfer_kv_pages* pages, const gfxinfer_kv_weights* weights,
+                                                  uint32_t layer, const uint16_t* query, const float* log_sums,
+                                                  const uint32_t* sequences, const uint32_t* tokens, uint32_t count,
+                                                  uint32_t q_heads, void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    WeightArgs a{};
+    if (const int32_t s = read_pages(pages, a.pages); s != GFXI_OK) return s;
+    if (const int32_t s = read_weights(weights, a.weights); s != GFXI_OK) return s;
+    if (const int32_t s = read_heads(pages, q_heads); s != GFXI_OK) return s;
+    if (const int32_t s = read_chunks(a.pages, sequences, tokens, count, true, a.list); s != GFXI_OK) return s;
+    if (layer >= a.pages.layers || query == nullptr || log_sums == nullptr || !aligned16(query) ||
+        (reinterpret_cast<uintptr_t>(log_sums) & 3u) != 0) {
+      return fail(GFXI_INVALID_ARGUMENT, "weights need a layer of the cache, 16-byte aligned queries and their log sums");
+    }
+    a.kv_heads = pages->kv_heads;
+    a.parts = weight_parts(a.pages, a.list, q_heads, a.kv_heads, a.columns);
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < weight_bytes(a.pages, a.list, a.kv_heads, a.parts)) {
+      return fail(GFXI_INVALID_ARGUMENT, "K/V weights workspace is null, not 16-byte aligned or too small");
+    }
+    a.query = reinterpret_cast<const __half*>(query);
+    a.log_sums = log_sums;
+    a.partial = static_cast<float*>(workspace);
+    a.layer = layer;
+    a.q_heads = q_heads;
+    a.group = q_heads / a.kv_heads;
+    a.scale = kLog2E / std::sqrt(static_cast<float>(pages->head_size));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const dim3 grid(a.columns * a.kv_heads * a.parts, count);
+    if (pages->head_size == 128) hipLaunchKernelGGL(weight_kernel<128>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(weight_kernel<256>, grid, dim3(256), 0, st, a);
+    if (const int32_t s = launch_status("K/V weights launch failed"); s != GFXI_OK) return s;
+    const uint64_t capacity = static_cast<uint64_t>(a.pages.stride) << a.pages.page_shift;
+    hipLaunchKernelGGL(weight_join_kernel, dim3(static_cast<unsigned>(std::min<uint64_t>((capacity + 255) / 256, 1024)), count),
+                       dim3(256), 0, st, a);
+    return launch_status("K/V weights join launch failed");
+  });
+}

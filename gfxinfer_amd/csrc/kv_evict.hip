@@ -1,0 +1,466 @@
+// A K/V cache within a budget: what each cached row has been worth, and the eviction of the
+// rows that were worth least.
+//
+// Attention does not depend on the order of a sequence's committed rows, so nothing is shifted:
+// the kept rows past the budget move into the holes that dropped rows leave before it, at most
+// as many rows as are dropped.  Sources lie past the budget and targets before it, so the
+// moves of a call are independent.  The rows' positions in the text move beside them.
+//
+// Three launches: a workgroup per sequence chooses (select_kernel), one workgroup gives out
+// pages for private copies (grant_kernel), and a grid that fills the GPU moves rows and
+// commits (move_kernel).
+#include <algorithm>
+#include <string>
+
+#include "kv_weights.hpp"
+
+namespace gfx950 {
+namespace {
+
+using u32x4 = unsigned __attribute__((ext_vector_type(4)));
+
+constexpr unsigned kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
+
+// The workspace: a header per sequence, then its moves and its copies, then the bits of kept
+// rows.  All offsets by the host's sizes alone.
+struct EvictHeader {
+  uint32_t moves;    // rows to move (0: the sequence stays as it is)
+  uint32_t copies;   // pages to copy
+  uint32_t length;   // before; 0: nothing to do
+  uint32_t failed;   // of the first header: the call fails
+};
+struct RowMove {
+  int32_t page;          // of the source, -1: none
+  uint32_t row, target;  // row in its page; the target's row of the sequence
+  uint32_t source;       // row of the sequence
+};
+struct PageCopy {
+  uint32_t column;
+  int32_t from, to;
+  uint32_t unused;
+};
+
+struct EvictArgs {
+  KvPages pages;
+  KvWeights weights;
+  SequenceList list;
+  EvictHeader* headers;   // [count]
+  RowMove* moves;         // [count][most_moves]
+  PageCopy* copies;       // [count][most_copies]
+  uint32_t* kept;         // [count][kept_words]: bit r % 32 of word r / 32, rows before the budget
+  uint32_t most_moves, most_copies, kept_words;
+  uint32_t budget, first, recent;
+  int32_t* status;
+};
+
+__device__ __forceinline__ uint32_t capacity_of(const KvPages& p) { return p.stride << p.page_shift; }
+
+// Order of weights as unsigned numbers; NaN above all, the zeros equal.
+__device__ __forceinline__ uint32_t order_of(float w) {
+  if (w != w) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(w + 0.0F);
+  return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ uint32_t scan_waves(uint32_t v, uint32_t* partial, uint32_t& total) {
+  const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  uint32_t sum = v;
+#pragma unroll
+  for (unsigned d = 1; d < 64; d <<= 1) {
+    const uint32_t o = __shfl_up(sum, d);
+    if (lane >= d) sum += o;
+  }
+  if (lane == 63u) partial[wave] = sum;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (unsigned w = 0; w < kSelectWaves; ++w) {
+    const uint32_t part = partial[w];
+    if (w < wave) before += part;
+    total += part;
+  }
+  __syncthreads();
+  return before + sum - v;
+}
+
+// Chooses the rows of one sequence: the number of rows that stay for their position, then the
+// key of the last row that fits (a radix select over 8 bits a pass, largest first), then in row
+// order which rows stay, and the lists of holes and movers.
+__global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictArgs a) {
+  __shared__ uint32_t histogram[256];
+  __shared__ uint32_t partial[kSelectWaves];
+  __shared__ uint32_t chosen[3];  // digit, how many of it are wanted
+  const unsigned tid = threadIdx.x, lane = tid & 63u;
+  const KvPages& pg = a.pages;
+  const uint32_t i = blockIdx.x, slot = listed_slot(a.list, i);
+  const uint32_t capacity = capacity_of(pg), n = min(pg.lengths[slot], capacity);
+  if (n <= a.budget) {
+    if (tid == 0) a.headers[i] = EvictHeader{0, 0, 0, 0};
+    return;
+  }
+  const std::size_t base = static_cast<std::size_t>(slot) * capacity;
+  const float* weight = a.weights.weight + base;
+  const int32_t* position = a.weights.position + base;
+  const int64_t last = static_cast<int64_t>(n) + a.weights.dropped[slot] - a.recent;  // positions from here on stay
+  auto fixed = [&](uint32_t row) __attribute__((always_inline)) {
+    const int32_t p = position[row];
+    return p < static_cast<int64_t>(a.first) || p >= last;
+  };
+  uint32_t mine = 0;
+  for (uint32_t row = tid; row < n; row += kSelectThreads) mine += fixed(row) ? 1u : 0u;
+  uint32_t protected_rows;
+  scan_waves(mine, partial, protected_rows);
+  // At most first + recent <= budget where positions are distinct, as begin makes them.
+  const uint32_t room = a.budget - min(protected_rows, a.budget);
+  const bool crowded = protected_rows > a.budget;  // damaged positions: then none is protected
+  uint32_t wanted = crowded ? a.budget : room, prefix = 0;
+  bool none = wanted == 0;
+  for (int shift = 24; shift >= 0 && !none; shift -= 8) {
+    if (tid < 256) histogram[tid] = 0;
+    __syncthreads();
+    const uint32_t high = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+    for (uint32_t row = tid; row < n; row += kSelectThreads) {
+      const uint32_t key = order_of(weight[row]);
+      if ((key & high) == prefix && (crowded || !fixed(row))) atomicAdd(&histogram[key >> shift & 255u], 1u);
+    }
+    __syncthreads();
+    // The digit in which the wanted-th largest lies: the first wave sums from the top.
+    if (tid < 64) {
+      uint32_t four[4], sum = 0;
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) {
+        four[e] = histogram[255u - (4 * lane + e)];
+        sum += four[e];
+      }
+      uint32_t upto = sum;
+#pragma unroll
+      for (unsigned d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+      }
+      uint32_t before = upto - sum;
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) {
+        if (before < wanted && wanted <= before + four[e]) {
+          chosen[0] = 255u - (4 * lane + e);
+          chosen[1] = wanted - before;
+        }
+        before += four[e];
+      }
+    }
+    __syncthreads();
+    prefix |= chosen[0] << shift;
+    wanted = chosen[1];
+    __syncthreads();
+  }
+  // Rows above the key stay, and the first `wanted` of those at it.
+  const uint32_t key_at = prefix;
+  uint32_t* kept_bits = a.kept + static_cast<std::size_t>(i) * a.kept_words;
+  RowMove* moves = a.moves + static_cast<std::size_t>(i) * a.most_moves;
+  uint32_t ties = 0, holes = 0, movers = 0;
+  for (uint32_t from = 0; from < n; from += kSelectThreads) {
+    const uint32_t row = from + tid;
+    bool stays = false, tie = false;
+    if (row < n) {
+      const bool stands = !crowded && fixed(row);
+      const uint32_t key = order_of(weight[row]);
+      stays = stands || (!none && key > key_at);
+      tie = !stands && !none && key == key_at;
+    }
+    uint32_t total;
+    const uint32_t rank = ties + scan_waves(tie ? 1u : 0u, partial, total);
+    ties += total;
+    stays |= tie && rank < wanted;
+    const bool hole = row < a.budget && !stays, mover = row >= a.budget && row < n && stays;
+    const uint64_t bits = __ballot(stays && row < a.budget);
+    if (lane == 0 && row / 32 < a.kept_words) kept_bits[row / 32] = static_cast<uint32_t>(bits);
+    if (lane == 32 && row / 32 < a.kept_words) kept_bits[row / 32] = static_cast<uint32_t>(bits >> 32);
+    // Holes in the low half, movers in the high half: at most 1024 each.
+    const uint32_t both = scan_waves((hole ? 1u : 0u) | (mover ? 1u : 0u) << 16, partial, total);
+    if (hole) {
+      const uint32_t at = holes + (both & 0xffffu);
+      if (at < a.most_moves) moves[at].target = row;
+    }
+    if (mover) {
+      const uint32_t at = movers + (both >> 16);
+      if (at < a.most_moves) {
+        moves[at].page = table_page(pg, slot, row >> pg.page_shift);
+        moves[at].row = row & ((1u << pg.page_shift) - 1);
+        moves[at].source = row;
+      }
+    }
+    holes += total & 0xffffu;
+    movers += total >> 16;
+  }
+  __threadfence_block();
+  __syncthreads();
+  // Pages with a hole that other sequences hold too.
+  PageCopy* copies = a.copies + static_cast<std::size_t>(i) * a.most_copies;
+  const uint32_t columns = pages_for(a.budget, pg.page_shift), page_tokens = 1u << pg.page_shift;
+  uint32_t found = 0;
+  for (uint32_t from = 0; from < columns; from += kSelectThreads) {
+    const uint32_t column = from + tid;
+    int32_t page = -1;
+    bool copy = false;
+    if (column < columns) {
+      page = table_page(pg, slot, column);
+      if (page >= 0 && pg.references[page] > 1) {
+        // A row of the page before the budget whose bit is off.
+        const uint32_t begin = column << pg.page_shift, end = min(begin + page_tokens, a.budget);
+        for (uint32_t r = begin; r < end; r += 32) {  // begin is a multiple of 16
+          const uint32_t word = kept_bits[r / 32], low = r % 32, count = min(end - r, 32u - low);
+          const uint32_t wanted_bits = (count == 32 ? 0xffffffffu : (1u << count) - 1u) << low;
+          copy |= (word & wanted_bits) != wanted_bits;
+          if (low != 0) r -= low;
+        }
+      }
+    }
+    uint32_t total;
+    const uint32_t at = found + scan_waves(copy ? 1u : 0u, partial, total);
+    if (copy) copies[at] = PageCopy{column, page, -1, 0};
+    found += total;
+  }
+  if (tid == 0) a.headers[i] = EvictHeader{min(holes, movers), found, n, 0};
+}
+
+// One workgroup gives every copy a free page, lowest first, sequence by sequence, or fails the
+// call as a whole; then it renames the pages.
+__global__ __launch_bounds__(kSelectThreads) void grant_kernel(EvictArgs a) {
+  __shared__ uint32_t partial[kSelectWaves];
+  __shared__ uint32_t start[kMaxListed + 1];
+  const unsigned tid = threadIdx.x;
+  const KvPages& pg = a.pages;
+  uint32_t total;
+  const uint32_t before = scan_waves(tid < a.list.count ? a.headers[tid].copies : 0u, partial, total);
+  if (tid < a.list.count) start[tid] = before;
+  if (tid == 0) start[a.list.count] = total;
+  __syncthreads();
+  if (total == 0) {
+    if (tid == 0) *a.status = 0;
+    return;
+  }
+  // Twice over the counts: is there enough, then who gets what.
+  uint32_t available = 0;
+  for (uint32_t from = 0; from < pg.page_count && available < total; from += kSelectThreads) {
+    uint32_t found;
+    scan_waves(from + tid < pg.page_count && pg.references[from + tid] == 0 ? 1u : 0u, partial, found);
+    available += found;
+  }
+  if (tid == 0) {
+    *a.status = available < total ? 1 : 0;
+    if (available < total) a.headers[0].failed = 1;
+  }
+  if (available < total) return;
+  uint32_t given = 0;
+  for (uint32_t from = 0; from < pg.page_count && given < total; from += kSelectThreads) {
+    const uint32_t page = from + tid;
+    const bool free = page < pg.page_count && pg.references[page] == 0;
+    uint32_t found;
+    const uint32_t rank = given + scan_waves(free ? 1u : 0u, partial, found);
+    if (free && rank < total) {
+      uint32_t low = 0, high = a.list.count;  // the last sequence whose start is <= rank
+      while (high - low > 1) {
+        const uint32_t mid = (low + high) / 2;
+        if (start[mid] <= rank) low = mid;
+        else high = mid;
+      }
+      PageCopy& copy = a.copies[static_cast<std::size_t>(low) * a.most_copies + rank - start[low]];
+      copy.to = static_cast<int32_t>(page);
+      pg.references[page] = 1;
+      pg.table[static_cast<std::size_t>(listed_slot(a.list, low)) * pg.stride + copy.column] = static_cast<int32_t>(page);
+    }
+    given += found;
+  }
+  // The holders' shares of the old pages, once no page is looked for any more: one that all of
+  // them leave is free for the next call, not for this one.
+  __syncthreads();
+  for (uint32_t i = 0; i < a.list.count; ++i) {
+    for (uint32_t c = tid; c < start[i + 1] - start[i]; c += kSelectThreads) {
+      atomicSub(&pg.references[a.copies[static_cast<std::size_t>(i) * a.most_copies + c].from], 1u);
+    }
+  }
+}
+
+constexpr unsigned kMoveThreads = 256, kMoveWorkgroups = 2048;
+
+// Moves rows of all layers, K and V, a wave a row and plane at a time; then commits.  Sources
+// were looked up before pages were renamed, targets are looked up now.
+__global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a) {
+  const KvPages& pg = a.pages;
+  if (a.headers[0].failed != 0) return;
+  const uint32_t s = blockIdx.y, slot = listed_slot(a.list, s);
+  const EvictHeader header = a.headers[s];
+  if (header.length == 0) return;
+  const unsigned lane = threadIdx.x & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (kMoveThreads / 64) + (threadIdx.x >> 6));
+  const uint32_t waves = gridDim.x * (kMoveThreads / 64);
+  const uint32_t page_tokens = 1u << pg.page_shift, units = pg.row / 8, planes = 2 * pg.layers;
+  const RowMove* moves = a.moves + static_cast<std::size_t>(s) * a.most_moves;
+  const PageCopy* copies = a.copies + static_cast<std::size_t>(s) * a.most_copies;
+  const uint32_t* kept = a.kept + static_cast<std::size_t>(s) * a.kept_words;
+  const uint64_t rows = header.moves + static_cast<uint64_t>(header.copies) * page_tokens;
+  auto copy_row = [&](uint32_t plane, int32_t from, uint32_t from_row, int32_t to, uint32_t to_row) __attribute__((always_inline)) {
+    u32x4* pool = reinterpret_cast<u32x4*>(plane < pg.layers ? pg.key : pg.value);
+    const std::size_t layer = static_cast<std::size_t>(plane < pg.layers ? plane : plane - pg.layers) * pg.page_count;
+    const u32x4* source = pool + (((layer + from) << pg.page_shift) + from_row) * units;
+    u32x4* target = pool + (((layer + to) << pg.page_shift) + to_row) * units;
+    for (uint32_t u = lane; u < units; u += 64) target[u] = source[u];
+  };
+  for (uint64_t item = wave; item < rows * planes; item += waves) {
+    const uint32_t plane = static_cast<uint32_t>(item % planes);
+    const uint64_t row = item / planes;
+    if (row < header.moves) {
+      const RowMove m = moves[row];
+      const int32_t to = table_page(pg, slot, m.target >> pg.page_shift);
+      if (m.page >= 0 && to >= 0) copy_row(plane, m.page, m.row, to, m.target & (page_tokens - 1));
+    } else {
+      const uint32_t at = static_cast<uint32_t>(row - header.moves);
+      const PageCopy c = copies[at >> pg.page_shift];
+      const uint32_t r = at & (page_tokens - 1), j = (c.column << pg.page_shift) + r;
+      if (j < a.budget && (kept[j / 32] >> j % 32 & 1u) != 0) copy_row(plane, c.from, r, c.to, r);
+    }
+  }
+  // The commit: no part of this launch reads what it writes.
+  const uint32_t thread = blockIdx.x * kMoveThreads + threadIdx.x, threads = gridDim.x * kMoveThreads;
+  const std::size_t base = static_cast<std::size_t>(slot) * capacity_of(pg);
+  for (uint32_t m = thread; m < header.moves; m += threads) {
+    const RowMove move = moves[m];
+    a.weights.weight[base + move.target] = a.weights.weight[base + move.source];
+    a.weights.position[base + move.target] = a.weights.position[base + move.source];
+  }
+  for (uint32_t column = pages_for(a.budget, pg.page_shift) + thread; column < pg.stride; column += threads) {
+    const int32_t page = table_page(pg, slot, column);
+    if (page >= 0) atomicSub(&pg.references[page], 1u);
+    pg.table[static_cast<std::size_t>(slot) * pg.stride + column] = -1;
+  }
+  if (thread == 0) {
+    a.weights.dropped[slot] += header.length - a.budget;
+    pg.lengths[slot] = a.budget;
+  }
+}
+
+__global__ __launch_bounds__(256) void begin_kernel(KvPages p, KvWeights w, ChunkList list) {
+  const uint32_t i = blockIdx.y, slot = listed_slot(list, i), tokens = list.first[i + 1] - list.first[i];
+  const uint32_t t = blockIdx.x * 256 + threadIdx.x, capacity = capacity_of(p), length = min(p.lengths[slot], capacity);
+  // Every workgroup of an empty sequence takes 0, whether the first one has written it or not.
+  const uint32_t dropped = length == 0 ? 0u : w.dropped[slot];
+  if (t == 0 && length == 0) w.dropped[slot] = 0;
+  if (t >= tokens || t >= capacity - length) return;
+  const std::size_t at = static_cast<std::size_t>(slot) * capacity + length + t;
+  w.weight[at] = 0.0F;
+  w.position[at] = static_cast<int32_t>(length + t + dropped);
+}
+
+// Most rows that a sequence can lose and move, pages it can copy, and words of its bits.
+struct EvictSizes {
+  std::size_t moves, copies, words, bytes;
+};
+EvictSizes evict_sizes(const KvPages& p, uint32_t count, uint32_t budget) {
+  const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift;
+  EvictSizes s{};
+  s.moves = budget < capacity ? std::min<uint64_t>(budget, capacity - budget) : 0;
+  s.copies = std::min<uint64_t>(p.stride, (budget + (1ull << p.page_shift) - 1) >> p.page_shift);
+  s.words = (std::min<uint64_t>(budget, capacity) + 127) / 128 * 4;
+  s.bytes = count * (sizeof(EvictHeader) + s.moves * sizeof(RowMove) + s.copies * sizeof(PageCopy) + s.words * 4);
+  return s;
+}
+
+}  // namespace
+
+int32_t read_chunks(const KvPages& pages, const uint32_t* sequences, const uint32_t* tokens, uint32_t count, bool distinct,
+                    ChunkList& out) {
+  if (tokens == nullptr || count == 0 || count > kMaxChunks || (sequences == nullptr && count > pages.sequences)) {
+    return fail(GFXI_INVALID_ARGUMENT, "a chunk call names 1.." + std::to_string(kMaxChunks) + " sequences of the cache and their tokens");
+  }
+  SequenceList list;
+  if (const int32_t s = read_sequences(pages, sequences, count, distinct, list); s != GFXI_OK) return s;
+  out = ChunkList{};
+  out.count = count;
+  uint64_t rows = 0;
+  for (uint32_t i = 0; i < count; ++i) {
+    out.slot[i] = list.slot[i];
+    out.first[i] = static_cast<uint32_t>(rows);
+    rows += tokens[i];
+    if (rows > kMaxRows) return fail(GFXI_INVALID_ARGUMENT, "a chunk call has at most 2^20 rows");
+  }
+  if (rows == 0) return fail(GFXI_INVALID_ARGUMENT, "a chunk call has at least one token");
+  for (uint32_t i = count; i <= kMaxChunks; ++i) out.first[i] = static_cast<uint32_t>(rows);
+  return GFXI_OK;
+}
+
+int32_t read_weights(const gfxinfer_kv_weights* weights, KvWeights& out) {
+  if (weights == nullptr || weights->weight == nullptr || weights->position == nullptr || weights->dropped == nullptr) {
+    return fail(GFXI_INVALID_ARGUMENT, "K/V weights: weight, position and dropped must be set");
+  }
+  out = KvWeights{weights->weight, weights->position, weights->dropped};
+  return GFXI_OK;
+}
+
+}  // namespace gfx950
+
+using namespace gfx950;
+
+extern "C" int32_t gfxinfer_launch_kv_weights_begin(const gfxinfer_kv_pages* pages, const gfxinfer_kv_weights* weights,
+                                                    const uint32_t* sequences, const uint32_t* tokens, uint32_t count,
+                                                    void* stream) {
+  return guarded([&] {
+    KvPages p;
+    KvWeights w;
+    ChunkList list;
+    if (const int32_t s = read_pages(pages, p); s != GFXI_OK) return s;
+    if (const int32_t s = read_weights(weights, w); s != GFXI_OK) return s;
+    if (const int32_t s = read_chunks(p, sequences, tokens, count, true, list); s != GFXI_OK) return s;
+    const uint32_t most = *std::max_element(tokens, tokens + count);
+    hipLaunchKernelGGL(begin_kernel, dim3((most + 255) / 256, count), dim3(256), 0, static_cast<hipStream_t>(stream), p, w, list);
+    return launch_status("K/V weights launch failed");
+  });
+}
+
+extern "C" size_t gfxinfer_kv_pages_evict_workspace_bytes(const gfxinfer_kv_pages* pages, uint32_t count, uint32_t budget) {
+  size_t bytes = 0;
+  guarded([&] {
+    KvPages p;
+    const int32_t s = read_pages(pages, p);
+    if (s == GFXI_OK && count != 0 && count <= kMaxListed && budget != 0) bytes = evict_sizes(p, count, budget).bytes;
+    return s;
+  });
+  return bytes;
+}
+
+extern "C" int32_t gfxinfer_launch_kv_pages_evict(const gfxinfer_kv_pages* pages, const gfxinfer_kv_weights* weights,
+                                                  const uint32_t* sequences, uint32_t count, uint32_t budget, uint32_t first,
+                                                  uint32_t recent, int32_t* status, void* workspace, size_t workspace_bytes,
+                                                  void* stream) {
+  return guarded([&] {
+    EvictArgs a{};
+    if (const int32_t s = read_pages(pages, a.pages); s != GFXI_OK) return s;
+    if (const int32_t s = read_weights(weights, a.weights); s != GFXI_OK) return s;
+    if (const int32_t s = read_sequences(a.pages, sequences, count, true, a.list); s != GFXI_OK) return s;
+    if (budget == 0 || static_cast<uint64_t>(first) + recent > budget || status == nullptr) {
+      return fail(GFXI_INVALID_ARGUMENT, "eviction needs a budget of at least first + recent rows and 1, and a status word");
+    }
+    const EvictSizes sizes = evict_sizes(a.pages, count, budget);
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < sizes.bytes) {
+      return fail(GFXI_INVALID_ARGUMENT, "eviction workspace is null, not 16-byte aligned or too small");
+    }
+    a.headers = static_cast<EvictHeader*>(workspace);
+    a.moves = reinterpret_cast<RowMove*>(a.headers + count);
+    a.copies = reinterpret_cast<PageCopy*>(a.moves + count * sizes.moves);
+    a.kept = reinterpret_cast<uint32_t*>(a.copies + count * sizes.copies);
+    a.most_moves = static_cast<uint32_t>(sizes.moves);
+    a.most_copies = static_cast<uint32_t>(sizes.copies);
+    a.kept_words = static_cast<uint32_t>(sizes.words);
+    a.budget = budget;
+    a.first = first;
+    a.recent = recent;
+    a.status = status;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(select_kernel, dim3(count), dim3(kSelectThreads), 0, st, a);
+    if (const int32_t s = launch_status("K/V eviction launch failed"); s != GFXI_OK) return s;
+    hipLaunchKernelGGL(grant_kernel, dim3(1), dim3(kSelectThreads), 0, st, a);
+    if (const int32_t s = launch_status("K/V eviction launch failed"); s != GFXI_OK) return s;
+    hipLaunchKernelGGL(move_kernel, dim3(std::max(1u, kMoveWorkgroups / count), count), dim3(kMoveThreads), 0, st, a);
+    return launch_status("K/V eviction launch failed");
+  });
+}

@@ -40,6 +40,11 @@ extern "C" {
 #define GFXI_W3G128 2
 #define GFXI_W4G128 3
 
+/* Element types of calls that take several. */
+#define GFXI_F16 0
+#define GFXI_F32 1
+#define GFXI_BF16 2
+
 /* Thread-local text of the last failing call (status.h:22-36 message()). */
 const char* gfxinfer_last_error(void);
 
@@ -719,6 +724,109 @@ int32_t gfxinfer_launch_kv_pages_gated_attention(const gfxinfer_kv_pages* pages,
                                                  const float* gate, uint16_t* output, const uint32_t* sequences,
                                                  uint32_t count, uint32_t tokens, uint32_t q_heads, size_t shared_tokens,
                                                  float* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- prompts in chunks, in a cache that stays within a budget ----------------------------
+ * No reference counterpart (the reference feeds a prompt token by token and its cache only
+ * grows).  A step of a server that feeds prompts beside sequences that decode:
+ *     reserve, begin; per layer: append, chunk_attention, weights_add; advance, evict
+ * Every listed sequence brings its own number of new tokens (host list; 0 is allowed, a call
+ * has at least one), and their rows are packed: sequence by sequence in list order, token by
+ * token.  A call lists at most 256 sequences and has at most 2^20 rows. */
+
+/* Bytes of device workspace (16-byte aligned) of gfxinfer_launch_kv_pages_chunk_attention; 0
+ * where it needs none and for invalid arguments.  Calls that may run at once need one each. */
+size_t gfxinfer_kv_pages_chunk_attention_workspace_bytes(const gfxinfer_kv_pages* pages, const uint32_t* tokens,
+                                                         uint32_t count, uint32_t q_heads);
+
+/* gfxinfer_launch_kv_pages_gated_attention for chunks: token t of the i-th listed sequence
+ * (NULL: 0..count-1; one may be listed several times) attends to its first length + t + 1
+ * positions (the chunk's own rows are appended, not yet committed).  query fp16
+ * [rows][q_heads][hd] (16-byte aligned); gate fp32 [rows][q_heads][2 hd], its second half per
+ * head row used, or NULL for no gate; output fp16 [rows][q_heads][hd]; log_sums fp32
+ * [rows][q_heads], or NULL: the natural logarithm of the sum of exp(score) of a row, -inf for
+ * a row that sees nothing (its output is zeros).  A position without a page is not seen.
+ * The order of fp32 additions depends on the shape of the call (token counts, q_heads,
+ * table_stride) and on the row's own position. */
+int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pages* pages, uint32_t layer, const uint16_t* query,
+                                                 const float* gate, uint16_t* output, float* log_sums,
+                                                 const uint32_t* sequences, const uint32_t* tokens, uint32_t count,
+                                                 uint32_t q_heads, float* workspace, size_t workspace_bytes, void* stream);
+
+/* What each cached row of a sequence has been worth so far, beside the pages: caller's
+ * device memory, rows of capacity = table_stride * page_tokens entries. */
+typedef struct gfxinfer_kv_weights {
+  float* weight;      /* [sequences][capacity]: attention weight the row has received, all layers and heads */
+  int32_t* position;  /* [sequences][capacity]: the row's position in the text (rows move when others are evicted) */
+  uint32_t* dropped;  /* [sequences]: rows evicted so far; length + dropped is the next token's position */
+} gfxinfer_kv_weights;
+
+/* The next tokens[i] rows of each listed sequence (distinct; NULL: 0..count-1) begin without
+ * weight, at the positions length + dropped + 0..tokens[i]-1; a sequence of length 0 begins
+ * with dropped = 0.  Rows past the capacity are passed over.  A sequence forked from another
+ * takes over its parent's weight, position and dropped by copies that the caller makes. */
+int32_t gfxinfer_launch_kv_weights_begin(const gfxinfer_kv_pages* pages, const gfxinfer_kv_weights* weights,
+                                         const uint32_t* sequences, const uint32_t* tokens, uint32_t count, void* stream);
+
+/* Bytes of device workspace (16-byte aligned) of gfxinfer_launch_kv_weights_add; 0 for invalid
+ * arguments.  Calls that may run at once need one each. */
+size_t gfxinfer_kv_weights_workspace_bytes(const gfxinfer_kv_pages* pages, const uint32_t* tokens, uint32_t count,
+                                           uint32_t q_heads);
+
+/* weight[s][j] += sum of exp(score - log_sum) over the chunk's tokens and query heads that see
+ * position j, for each listed sequence (distinct) and one layer; query, log_sums and tokens as
+ * given to and by gfxinfer_launch_kv_pages_chunk_attention.  Rows whose log_sum is -inf or NaN
+ * add nothing; positions without a page are left as they are.  No atomics: the sums' order
+ * depends on the shape of the call alone. */
+int32_t gfxinfer_launch_kv_weights_add(const gfxinfer_kv_pages* pages, const gfxinfer_kv_weights* weights, uint32_t layer,
+                                       const uint16_t* query, const float* log_sums, const uint32_t* sequences,
+                                       const uint32_t* tokens, uint32_t count, uint32_t q_heads, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace (16-byte aligned) of gfxinfer_launch_kv_pages_evict; 0 for invalid
+ * arguments.  Calls that may run at once need one each. */
+size_t gfxinfer_kv_pages_evict_workspace_bytes(const gfxinfer_kv_pages* pages, uint32_t count, uint32_t budget);
+
+/* Cuts each listed sequence (distinct; NULL: 0..count-1) longer than `budget` tokens to its
+ * `budget` worthiest rows: those at the text positions below `first` and at the last `recent`
+ * ones stay, then the rows of greatest weight (NaN counts as the greatest; of equal ones the
+ * lower row).  first + recent <= budget, budget >= 1.  Kept rows past the budget move, in order, to the
+ * places of dropped rows before it, in order: all layers, K and V, weight and position.  A
+ * page that other sequences hold too is not written: where a row of it is dropped, the
+ * sequence gets a copy (pages lowest first, sequence by sequence in list order).  Pages past
+ * the budget are given back, pages reserved past the length among them; length = budget,
+ * dropped grows by the rows dropped.  Shorter sequences stay as they are.
+ * *status (device) = 0, or 1 when the pool has too few free pages for the copies (pages given
+ * back by this call do not count): then nothing changed. */
+int32_t gfxinfer_launch_kv_pages_evict(const gfxinfer_kv_pages* pages, const gfxinfer_kv_weights* weights,
+                                       const uint32_t* sequences, uint32_t count, uint32_t budget, uint32_t first,
+                                       uint32_t recent, int32_t* status, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+
+/* ---- products in 8-bit integers, any number of tokens ---------------------------------------
+ * No reference counterpart (its products take at most 32 tokens and group scales).  A scale
+ * per token and one per output channel:
+ *     y[t][n] = (sum over k of codes[t][k] * weights[n][k]) * (scales[t] * weight_scales[n])
+ * The integer sum is exact at every shape. */
+
+/* Rows [rows][columns] at a pitch of row_stride elements (8 | row_stride, rows 16-byte
+ * aligned) of GFXI_F16, GFXI_F32 or GFXI_BF16 to codes int8 [rows][columns] and scales fp32
+ * [rows]: scale = max |x| / 127 (at least 2^-126), code = the integer nearest x / scale, ties
+ * to even, within -127..127.  For tokens, and once for a matrix's output channels.  A row with
+ * an infinity or a NaN gets zero codes and a NaN scale.  1..2^24 rows; columns a multiple of
+ * 16 below 2^17. */
+int32_t gfxinfer_launch_quantize_rows_i8(const void* input, int32_t input_type, size_t rows, size_t columns,
+                                         size_t row_stride, int8_t* codes, float* scales, void* stream);
+
+/* Bytes of device workspace (16-byte aligned) of gfxinfer_launch_w8a8_gemm; 0 where it needs
+ * none and for invalid sizes.  Calls that may run at once need one each. */
+size_t gfxinfer_w8a8_gemm_workspace_bytes(size_t rows, size_t columns, size_t tokens);
+
+/* weights int8 [rows][columns], weight_scales fp32 [rows], codes int8 [tokens][columns], scales
+ * fp32 [tokens] -> output [tokens][rows], GFXI_F32 or GFXI_F16 (rounded once from fp32).  Codes
+ * and output 16-byte aligned; columns a multiple of 16 below 2^17, rows and tokens 1..2^24. */
+int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float* weight_scales, const int8_t* codes,
+                                  const float* scales, void* output, int32_t output_type, size_t rows, size_t columns,
+                                  size_t tokens, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- rules on logits -------------------------------------------------------------------
  * No reference counterpart (the reference picks the plain argmax).  For row b and token v of
