@@ -3,17 +3,22 @@
 // Row (t, g) of a listed sequence and a KV head, new token t at query head g of the head's
 // group, attends to the first length + t + 1 positions:
 //     o = softmax(q . K / sqrt(D)) . V * sigmoid(gate),   L = log(sum exp(q . K / sqrt(D)))
-// The rows of a sequence and KV head are one tall matrix, in tiles of 128: a workgroup takes a
-// tile and a range of positions, each of its four waves 32 of the rows, and a K / V row staged
-// in LDS serves all of them.
+// The rows of a sequence and KV head are one tall matrix: a workgroup takes a tile of its rows
+// and a range of positions, each of its four waves 32 or 64 of the rows, and a K / V row staged in
+// LDS serves all of them.
 //
 // Scores are computed transposed, S^T = K Q^T (v_mfma_f32_32x32x16_f16), so that a lane holds
 // half of one row's scores, the running maximum takes one lane exchange, and the weights are
 // already the B operand of O^T = V^T P^T when the positions of a step are numbered as the score
 // tiles leave them (k slot 8 h + e is position 4 h + e % 4 + 8 (e / 4), h the lane's half).  V
 // passes through LDS, whose transposing reads turn rows of V into columns.
+//
+// The scores of a tile of positions are computed beside the exponentials of the tile before it:
+// the exponentials alone take a wave's vector unit nearly as long as both products take the
+// matrix unit.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "kv_attention.hpp"
@@ -26,13 +31,14 @@ using f16v = float __attribute__((ext_vector_type(16)));
 using h4 = _Float16 __attribute__((ext_vector_type(4)));
 using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 
-constexpr unsigned kWaves = 4, kRowsOfWave = 32, kRows = kWaves * kRowsOfWave;
+constexpr unsigned kWaves = 4;
 constexpr float kLn2 = 0.6931471805599453F;
 
-// Positions of a tile: 16 KB of K and of V either way, two of each in LDS, so that a CU holds two
-// workgroups.
-template <unsigned D>
-constexpr unsigned kTile = 8192 / D;
+// A row tile: G groups of 32 rows a wave.  Positions of a step, and workgroups a CU holds.
+constexpr unsigned rows_of(unsigned g) { return kWaves * 32 * g; }
+constexpr unsigned kTile = 64;
+template <unsigned D, unsigned G>
+constexpr unsigned kResident = D == 128 && G == 1 ? 2 : 1;
 
 // A row's weights are 2^(score - m + kLift) in fp16, scores in units of log2.  m is a maximum of
 // the row so far that moves up once it is passed by kRise, so weights stay below 2^15.  Against
@@ -50,7 +56,7 @@ struct ChunkAttnArgs {
   float* log_sums;       // [rows][q_heads] or null
   float* partial_o;      // [rows][q_heads][splits][D], where positions are divided
   float* partial_ml;     // [rows][q_heads][splits][2]
-  uint32_t layer, q_heads, kv_heads, group, splits;
+  uint32_t layer, q_heads, kv_heads, group, splits, tile_rows;
   float scale;           // log2(e) / sqrt(D)
 };
 
@@ -82,10 +88,16 @@ __device__ __forceinline__ float sum_over_halves(float v) {
   return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
-// One item: row tile `tile` of listed sequence i at KV head hk, positions [from, to) tiles.
-template <unsigned D>
-__global__ __launch_bounds__(kWaves * 64, 2) void chunk_attention_kernel(ChunkAttnArgs a) {
-  constexpr unsigned T = kTile<D>, kSub = T / 32, kSteps = T / 16;
+// Sixteen-position parts of a tile: their pages, -1 where there is none.
+struct TilePages {
+  int32_t page[kTile / 16];
+  uint32_t missing;
+};
+
+// One item: a row tile of a listed sequence at KV head hk, tiles [from, to) of positions.
+template <unsigned D, unsigned G>
+__global__ __launch_bounds__(kWaves * 64, (kResident<D, G>)) void chunk_attention_kernel(ChunkAttnArgs a) {
+  constexpr unsigned T = kTile, kSub = T / 32, kSteps = T / 16, kRows = rows_of(G);
   constexpr unsigned kLoadRows = 512 / D;                   // rows a load of a wave covers
   constexpr unsigned kLoads = T / kLoadRows / kWaves;       // of K, and of V, per tile and wave
   __shared__ __align__(1024) _Float16 k0[T * D];
@@ -113,18 +125,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void chunk_attention_kernel(ChunkAt
   const uint32_t from = split * per, to = min(from + per, tiles);
   if (from >= tiles) return;
 
-  const uint32_t row = tile_row + wave * kRowsOfWave + n;
-  const bool works = tile_row + wave * kRowsOfWave < rows;   // the wave has a row
-  const uint32_t t = row / a.group, g = row - t * a.group;
-  const std::size_t out_row = (static_cast<std::size_t>(first_row) + t) * a.q_heads + hk * a.group + g;
-  const uint32_t visible = row < rows ? length + t + 1 : 0;
-  const uint32_t least = row < rows ? length + (tile_row + wave * kRowsOfWave) / a.group + 1 : 0;   // of the wave's rows
-  const uint32_t least_visible = __builtin_amdgcn_readfirstlane(least);
-  h8 q[D / 16];
+  const uint32_t wave_row = tile_row + wave * 32 * G;
+  const bool works = wave_row < rows;                        // the wave has a row
+  const uint32_t least_visible = length + wave_row / a.group + 1;
+  uint32_t visible[G], out_row[G];                           // out_row: [rows][q_heads], below 2^30
+  h8 q[G][D / 16];
 #pragma unroll
-  for (unsigned s = 0; s < D / 16; ++s) {
-    q[s] = h8{};
-    if (row < rows) q[s] = *reinterpret_cast<const h8*>(a.query + out_row * D + 16 * s + 8 * h);
+  for (unsigned g = 0; g < G; ++g) {
+    const uint32_t row = wave_row + 32 * g + n, t = row / a.group;
+    const bool there = row < rows;
+    visible[g] = there ? length + t + 1 : 0;
+    out_row[g] = there ? (first_row + t) * a.q_heads + hk * a.group + (row - t * a.group) : 0xffffffffu;
+#pragma unroll
+    for (unsigned s = 0; s < D / 16; ++s) {
+      q[g][s] = h8{};
+      if (there) q[g][s] = *reinterpret_cast<const h8*>(a.query + static_cast<std::size_t>(out_row[g]) * D + 16 * s + 8 * h);
+    }
   }
 
   const std::size_t layer_row = (static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) * pg.row + hk * D;
@@ -132,237 +148,296 @@ __global__ __launch_bounds__(kWaves * 64, 2) void chunk_attention_kernel(ChunkAt
   const __half* values = pg.value + layer_row;
   const uint32_t in_page = (1u << pg.page_shift) - 1;
   PageWindow window;
-  // The pages of a tile's parts of 16 positions; parts past the end load from page 0 of the pool
-  // (always there), as missing ones do.
-  int32_t page[T / 16];
-  auto find_pages = [&](uint32_t at) __attribute__((always_inline)) {
-    uint32_t missing = 0;
+  auto find_pages = [&](uint32_t x) __attribute__((always_inline)) {
+    TilePages p;
+    p.missing = 0;
 #pragma unroll
-    for (unsigned p = 0; p < T / 16; ++p) {
-      page[p] = at + 16 * p < end ? window.find(pg, slot, (at + 16 * p) >> pg.page_shift) : -1;
-      if (page[p] < 0) missing |= 1u << p;
+    for (unsigned e = 0; e < T / 16; ++e) {
+      const uint32_t at = x * T + 16 * e;
+      p.page[e] = at < end ? window.find(pg, slot, at >> pg.page_shift) : -1;
+      if (p.page[e] < 0) p.missing |= 1u << e;
     }
-    return missing;
+    return p;
   };
-  auto load = [&](_Float16* ks, _Float16* vs, uint32_t at) __attribute__((always_inline)) {
-    const unsigned r = lane / (D / 8);
+  // Where the lane's piece of a load lies in memory, in elements from the first of the load's rows:
+  // this ^ 8 (row0 % 16) for K, ^ 16 (row0 % 8) for V.
+  const uint32_t load_row = lane / (D / 8);
+  const uint32_t key_part = load_row * pg.row + 8 * key_slot(lane % (D / 8), load_row);
+  const uint32_t value_part = load_row * pg.row + 8 * value_slot(lane % (D / 8), load_row);
+  // Rows of a tile into LDS.  All rows of a load are of one part; parts without a page load from page 0 of
+  // the pool (always there), and so do those past the end.
+  auto load = [&](_Float16* to_lds, const __half* pool, uint32_t part, unsigned swizzle, uint32_t x, const TilePages& p) __attribute__((always_inline)) {
 #pragma unroll
     for (unsigned u = 0; u < kLoads; ++u) {
-      // All rows of a load are of one part; parts go to the waves in turn.
-      const unsigned row0 = kLoadRows * (wave + kWaves * u);
-      int32_t p = page[0];
-#pragma unroll
-      for (unsigned e = 1; e < T / 16; ++e) p = row0 / 16 == e ? page[e] : p;
-      const std::size_t base = ((static_cast<std::size_t>(max(p, 0)) << pg.page_shift) + ((at + row0) & in_page) + r) * pg.row;
-      const unsigned key_piece = key_slot(lane % (D / 8), row0 + r), value_piece = value_slot(lane % (D / 8), row0 + r);
-      __builtin_amdgcn_global_load_lds((global_void*)(keys + base + 8 * key_piece), (lds_void*)(ks + row0 * D), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((global_void*)(values + base + 8 * value_piece), (lds_void*)(vs + row0 * D), 16, 0, 0);
+      const unsigned row0 = kLoadRows * (wave + kWaves * u), e = kLoadRows * kWaves * u / 16;
+      const std::size_t base = ((static_cast<std::size_t>(max(p.page[e], 0)) << pg.page_shift) + ((x * T + row0) & in_page)) * pg.row;
+      __builtin_amdgcn_global_load_lds((global_void*)(pool + base + (part ^ 8 * (swizzle == 0 ? row0 & 15u : 2 * (row0 & 7u)))),
+                                       (lds_void*)(to_lds + row0 * D), 16, 0, 0);
     }
   };
 
-  f16v o[D / 32];
-  float m, l;
-  bool careful = false;
+  // Where the lane's part of the first score operand of 32 K rows, and of the first output tile of
+  // 16 V rows, lies in bytes.  Operand s is at the place ^ 32 s, output tile d at the place ^ 64 d:
+  // the slots of a row are permuted by exclusive or, and rows start at multiples of their size.
+  const unsigned i16 = lane & 15u, vrow = 4 * h + (i16 >> 2);
+  const unsigned key_place = n * (2 * D) + 16 * key_slot(h, n);
+  const unsigned value_place = vrow * (2 * D) + 16 * value_slot(2 * (lane >> 4 & 1u) + ((i16 & 3u) >> 1), vrow) + 8 * (i16 & 1u);
+
+  f16v o[G][D / 32], s[G][kSub], s_next[G][kSub];
+  float m[G], l[G];
   // What a page holds past a sequence's end, and what a missing one would, may be anything, and 0 * NaN
   // is NaN: the wave's own V rows of such positions become zeros.  A careful pass also takes out
   // infinities and NaNs, and marks the tile.
-  auto repair = [&](_Float16* vs, uint32_t at, uint32_t missing, unsigned b) __attribute__((always_inline)) {
+  auto repair = [&](_Float16* vs, uint32_t x, uint32_t missing, bool careful) __attribute__((always_inline)) {
     bool strange = false;
-#pragma unroll
+#pragma unroll 1
     for (unsigned u = 0; u < kLoads; ++u) {
       const unsigned row0 = kLoadRows * (wave + kWaves * u);
       u32x4* piece = reinterpret_cast<u32x4*>(vs + row0 * D) + lane;
-      if (at + row0 + lane / (D / 8) >= end || (missing >> row0 / 16 & 1u) != 0) *piece = u32x4{0, 0, 0, 0};
+      if (x * T + row0 + load_row >= end || (missing >> row0 / 16 & 1u) != 0) *piece = u32x4{0, 0, 0, 0};
       if (careful) strange |= take_strange(piece);
     }
     if (careful) {
       const bool any = __any(strange);
-      if (lane == 0) marks[b][wave] = any ? 1u : 0u;
+      if (lane == 0) marks[x & 1u][wave] = any ? 1u : 0u;
     }
+    wait_loads<63>();
   };
   // The rows that see an infinity or NaN among the values get it, whatever the weight: no weight is
   // exactly zero.
-  auto add_strange = [&](uint32_t at) {
+  auto add_strange = [&](uint32_t x) {
 #pragma unroll 1
     for (unsigned p = 0; p < T; ++p) {
-      const uint32_t position = at + p;
-      const int32_t pp = position < end ? table_page(pg, slot, position >> pg.page_shift) : -1;
-      if (pp < 0) continue;
-      const __half* x = values + ((static_cast<std::size_t>(pp) << pg.page_shift) + (position & in_page)) * pg.row;
+      const uint32_t position = x * T + p;
+      const int32_t page = position < end ? table_page(pg, slot, position >> pg.page_shift) : -1;
+      if (page < 0) continue;
+      const __half* v = values + ((static_cast<std::size_t>(page) << pg.page_shift) + (position & in_page)) * pg.row;
 #pragma unroll
       for (unsigned d = 0; d < D / 32; ++d) {
 #pragma unroll
         for (unsigned r = 0; r < 16; ++r) {
-          const float y = __half2float(x[32 * d + 8 * (r / 4) + 4 * h + r % 4]);
-          if (!(fabsf(y) < INFINITY) && position < visible) o[d][r] += y;
+          const float y = __half2float(v[32 * d + 8 * (r / 4) + 4 * h + r % 4]);
+#pragma unroll
+          for (unsigned g = 0; g < G; ++g) {
+            if (!(fabsf(y) < INFINITY) && position < visible[g]) o[g][d][r] += y;
+          }
         }
       }
     }
     wait_loads<0>();
   };
-  auto attend = [&](const _Float16* ks, const _Float16* vs, uint32_t at, uint32_t missing, unsigned b) __attribute__((always_inline)) {
-    f16v s[kSub];
+  // Raw products of the rows with a tile of K rows.
+  auto score = [&](const _Float16* ks, f16v (&out)[G][kSub]) __attribute__((always_inline)) {
+    const char* kb = reinterpret_cast<const char*>(ks);
 #pragma unroll
-    for (unsigned u = 0; u < kSub; ++u) {
-      s[u] = f16v{};
+    for (unsigned g = 0; g < G; ++g) {
 #pragma unroll
-      for (unsigned st = 0; st < D / 16; ++st) {
-        const h8 k = *reinterpret_cast<const h8*>(ks + (32 * u + n) * D + 8 * key_slot(2 * st + h, n));
-        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[st], s[u], 0, 0, 0);
-      }
+      for (unsigned u = 0; u < kSub; ++u) out[g][u] = f16v{};
     }
-    if (at + T > least_visible || missing != 0) {
+#pragma unroll
+    for (unsigned st = 0; st < D / 16; ++st) {
 #pragma unroll
       for (unsigned u = 0; u < kSub; ++u) {
+        const h8 k = *reinterpret_cast<const h8*>(kb + (key_place ^ 32 * st) + u * 64 * D);
 #pragma unroll
-        for (unsigned r = 0; r < 16; ++r) {
-          const unsigned p = 32 * u + 8 * (r / 4) + 4 * h + r % 4;
-          if (at + p >= visible || (missing >> p / 16 & 1u) != 0) s[u][r] = -INFINITY;
+        for (unsigned g = 0; g < G; ++g) out[g][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[g][st], out[g][u], 0, 0, 0);
+      }
+    }
+  };
+  // Scores of a tile are ready: hides what a row does not see, and moves the maxima.
+  auto settle = [&](f16v (&sc)[G][kSub], uint32_t x, uint32_t missing) __attribute__((always_inline)) {
+    if (x * T + T > least_visible || missing != 0) {
+#pragma unroll
+      for (unsigned g = 0; g < G; ++g) {
+#pragma unroll
+        for (unsigned u = 0; u < kSub; ++u) {
+#pragma unroll
+          for (unsigned r = 0; r < 16; ++r) {
+            const unsigned p = 32 * u + 8 * (r / 4) + 4 * h + r % 4;
+            if (x * T + p >= visible[g] || (missing >> (2 * u + r / 8) & 1u) != 0) sc[g][u][r] = -INFINITY;
+          }
         }
       }
     }
     // (A NaN score makes the maximum NaN and the row's result with it, as it has to.)
-    float best = s[0][0];
+    float top[G];
+    bool rises = false;
 #pragma unroll
-    for (unsigned e = 1; e < 16 * kSub; ++e) best = __builtin_elementwise_maximum(best, s[e / 16][e % 16]);
-    const float top = max_over_halves(best) * a.scale;
-    if (__any(!(top <= m + kRise))) {
-      const float next = top <= m + kRise ? m : top;
-      // From nothing to something: there is nothing to scale yet.
-      const float factor = next == m || m == -INFINITY ? 1.0F : rescale_factor(m, next);
-      m = next;
-      l *= factor;
+    for (unsigned g = 0; g < G; ++g) {
+      float best = sc[g][0][0];
 #pragma unroll
-      for (unsigned d = 0; d < D / 32; ++d) {
-#pragma unroll
-        for (unsigned r = 0; r < 16; ++r) o[d][r] *= factor;
-      }
+      for (unsigned e = 1; e < 16 * kSub; ++e) best = __builtin_elementwise_maximum(best, sc[g][e / 16][e % 16]);
+      top[g] = max_over_halves(best) * a.scale;
+      rises |= !(top[g] <= m[g] + kRise);
     }
-    const float floor = m == -INFINITY ? 0.0F : m - kLift;
-    h8 p[kSteps];
+    if (__any(rises)) {
 #pragma unroll
-    for (unsigned j = 0; j < kSteps; ++j) {
+      for (unsigned g = 0; g < G; ++g) {
+        const float next = top[g] <= m[g] + kRise ? m[g] : top[g];
+        // From nothing to something: there is nothing to scale yet.
+        const float factor = next == m[g] || m[g] == -INFINITY ? 1.0F : rescale_factor(m[g], next);
+        m[g] = next;
+        l[g] *= factor;
 #pragma unroll
-      for (unsigned e = 0; e < 8; ++e) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(s[j / 2][8 * (j % 2) + e], a.scale, -floor));
-        l += w;
-        p[j][e] = static_cast<_Float16>(w);
-      }
-    }
-    if (careful) {
-      uint32_t mark = 0;
-      for (unsigned w = 0; w < kWaves; ++w) mark |= marks[b][w];
-      if (__builtin_amdgcn_readfirstlane(mark) != 0) add_strange(at);
-    }
-    const unsigned group16 = lane >> 4, i16 = lane & 15u;
-    const unsigned vrow = 4 * (group16 >> 1) + (i16 >> 2), vpiece = 2 * (group16 & 1u) + ((i16 & 3u) >> 1);
+        for (unsigned d = 0; d < D / 32; ++d) {
 #pragma unroll
-    for (unsigned d = 0; d < D / 32; ++d) {
-#pragma unroll
-      for (unsigned j = 0; j < kSteps; ++j) {
-        s16x4 x[2];
-#pragma unroll
-        for (unsigned e = 0; e < 2; ++e) {
-          const unsigned r = 16 * j + 8 * e + vrow;
-          const _Float16* at_value = vs + r * D + 8 * value_slot(4 * d + vpiece, r) + 4 * (i16 & 1u);
-          x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(const_cast<_Float16*>(at_value)));
+          for (unsigned r = 0; r < 16; ++r) o[g][d][r] *= factor;
         }
-        const h8 v = __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[j], o[d], 0, 0, 0);
       }
     }
   };
-
-  for (;; careful = true) {
-    m = -INFINITY;
-    l = 0.0F;
+  // The weights of the tile in s and the scores of the next one, then the values of this one.
+  auto step = [&](const _Float16* next_ks, const _Float16* vs, uint32_t x, auto careful) __attribute__((always_inline)) {
+    h8 p[G][kSteps];
+    score(next_ks, s_next);
 #pragma unroll
-    for (unsigned d = 0; d < D / 32; ++d) o[d] = f16v{};
+    for (unsigned g = 0; g < G; ++g) {
+      const float floor = m[g] == -INFINITY ? 0.0F : m[g] - kLift;
+      float sum[4] = {l[g], 0.0F, 0.0F, 0.0F};
+#pragma unroll
+      for (unsigned j = 0; j < kSteps; ++j) {
+#pragma unroll
+        for (unsigned e = 0; e < 8; ++e) {
+          const float w = __builtin_amdgcn_exp2f(fmaf(s[g][j / 2][8 * (j % 2) + e], a.scale, -floor));
+          sum[e % 4] += w;
+          p[g][j][e] = static_cast<_Float16>(w);
+        }
+      }
+      l[g] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+    if constexpr (careful) {
+      uint32_t mark = 0;
+      for (unsigned w = 0; w < kWaves; ++w) mark |= marks[x & 1u][w];
+      if (__builtin_amdgcn_readfirstlane(mark) != 0) add_strange(x);
+    }
+    char* vb = const_cast<char*>(reinterpret_cast<const char*>(vs));
+#pragma unroll
+    for (unsigned j = 0; j < kSteps; ++j) {
+#pragma unroll
+      for (unsigned d = 0; d < D / 32; ++d) {
+        s16x4 y[2];
+#pragma unroll
+        for (unsigned e = 0; e < 2; ++e) {
+          y[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vb + (value_place ^ 64 * d) + (16 * j + 8 * e) * 2 * D));
+        }
+        const h8 v = __builtin_bit_cast(h8, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (unsigned g = 0; g < G; ++g) o[g][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[g][j], o[g][d], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (unsigned g = 0; g < G; ++g) {
+#pragma unroll
+      for (unsigned u = 0; u < kSub; ++u) s[g][u] = s_next[g][u];
+    }
+  };
+
+  // Tile x's V rows and tile x + 1's K rows are read while x + 1's V rows and x + 2's K rows are on their way,
+  // each into the place that was read last before the barrier.
+  auto pass = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+    for (unsigned g = 0; g < G; ++g) {
+      m[g] = -INFINITY;
+      l[g] = 0.0F;
+#pragma unroll
+      for (unsigned d = 0; d < D / 32; ++d) o[g][d] = f16v{};
+    }
     window.start(pg, slot, (from * T) >> pg.page_shift);
-    uint32_t missing0 = find_pages(from * T), missing1 = 0;
-    load(k0, v0, from * T);
+    TilePages now = find_pages(from), next = now;
+    load(k0, keys, key_part, 0, from, now);
+    wait_loads<0>();
+    __syncthreads();
+    load(v0, values, value_part, 1, from, now);
+    if (from + 1 < to) {
+      next = find_pages(from + 1);
+      load(k1, keys, key_part, 0, from + 1, next);
+    }
+    if (works) {
+      score(k0, s);
+      settle(s, from, now.missing);
+    }
+    auto turn = [&](uint32_t x, _Float16* k_free, const _Float16* k_next, const _Float16* v_now, _Float16* v_free) __attribute__((always_inline)) {
+      wait_loads<0>();
+      if (careful || now.missing != 0 || (x + 1) * T > end) repair(const_cast<_Float16*>(v_now), x, now.missing, careful);
+      __syncthreads();
+      now = next;
+      if (x + 1 < to) load(v_free, values, value_part, 1, x + 1, next);
+      if (x + 2 < to) {
+        next = find_pages(x + 2);
+        load(k_free, keys, key_part, 0, x + 2, next);
+      }
+      if (works) {
+        step(k_next, v_now, x, careful);
+        if (x + 1 < to) settle(s, x + 1, now.missing);
+      }
+    };
 #pragma unroll 1
     for (uint32_t x = from; x < to; x += 2) {
-      wait_loads<0>();
-      if (careful || missing0 != 0 || (x + 1) * T > end) {
-        repair(v0, x * T, missing0, 0);
-        wait_loads<63>();
-      }
-      __syncthreads();
-      if (x + 1 < to) {
-        missing1 = find_pages((x + 1) * T);
-        load(k1, v1, (x + 1) * T);
-      }
-      if (works) attend(k0, v0, x * T, missing0, 0);
-      if (x + 1 < to) {
-        wait_loads<0>();
-        if (careful || missing1 != 0 || (x + 2) * T > end) {
-          repair(v1, (x + 1) * T, missing1, 1);
-          wait_loads<63>();
-        }
-        __syncthreads();
-        if (x + 2 < to) {
-          missing0 = find_pages((x + 2) * T);
-          load(k0, v0, (x + 2) * T);
-        }
-        if (works) attend(k1, v1, (x + 1) * T, missing1, 1);
-      }
+      turn(x, k0, k1, v0, v1);
+      if (x + 1 < to) turn(x + 1, k1, k0, v1, v0);
     }
     // Whether an output is an infinity or NaN: finite values at weights below 2^15 make none.
     bool strange = false;
 #pragma unroll
-    for (unsigned d = 0; d < D / 32; ++d) {
+    for (unsigned g = 0; g < G; ++g) {
 #pragma unroll
-      for (unsigned r = 0; r < 16; ++r) strange |= !(fabsf(o[d][r]) < INFINITY);
+      for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+        for (unsigned r = 0; r < 16; ++r) strange |= !(fabsf(o[g][d][r]) < INFINITY);
+      }
     }
-    const bool mine = works && __any(strange);
-    if (lane == 0) again[wave] = mine ? 1u : 0u;
-    __syncthreads();
-    uint32_t found = 0;
-    for (unsigned w = 0; w < kWaves; ++w) found |= again[w];
-    if (careful || __builtin_amdgcn_readfirstlane(found) == 0) {
-      l = sum_over_halves(l);
-      // Only NaN scores, and strange values at scores of -infinity, make a NaN row rather than an empty one.
-      if ((m == -INFINITY && (l != l || (careful && strange))) || m != m) m = 0.0F;
-      break;
+    return strange;
+  };
+  // A second, careful pass follows in the rare case that an output of the first is an infinity or NaN.
+  bool strange = pass(std::false_type{});
+  const bool mine = works && __any(strange);
+  if (lane == 0) again[wave] = mine ? 1u : 0u;
+  __syncthreads();
+  uint32_t found = 0;
+  for (unsigned w = 0; w < kWaves; ++w) found |= again[w];
+  const bool careful = __builtin_amdgcn_readfirstlane(found) != 0;
+  if (__builtin_expect(careful, 0)) strange = pass(std::true_type{});
+#pragma unroll
+  for (unsigned g = 0; g < G; ++g) {
+    l[g] = sum_over_halves(l[g]);
+    // Only NaN scores, and strange values at scores of -infinity, make a NaN row rather than an empty one.
+    if ((m[g] == -INFINITY && (l[g] != l[g] || (careful && strange))) || m[g] != m[g]) m[g] = 0.0F;
+    if (out_row[g] == 0xffffffffu) continue;
+    if (a.splits > 1) {
+      const std::size_t at = static_cast<std::size_t>(out_row[g]) * a.splits + split;
+#pragma unroll
+      for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+        for (unsigned r = 0; r < 16; r += 4) {
+          *reinterpret_cast<f4*>(a.partial_o + at * D + 32 * d + 2 * r + 4 * h) = f4{o[g][d][r], o[g][d][r + 1], o[g][d][r + 2], o[g][d][r + 3]};
+        }
+      }
+      if (h == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{m[g], l[g]};
+      continue;
     }
-    __syncthreads();
-  }
-  if (row >= rows) return;
-  if (a.splits > 1) {
-    const std::size_t at = out_row * a.splits + split;
+    const bool empty = m[g] == -INFINITY;
+    const float inverse = empty ? 0.0F : 1.0F / l[g];
 #pragma unroll
     for (unsigned d = 0; d < D / 32; ++d) {
 #pragma unroll
       for (unsigned r = 0; r < 16; r += 4) {
-        *reinterpret_cast<f4*>(a.partial_o + at * D + 32 * d + 2 * r + 4 * h) = f4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+        const unsigned at = 32 * d + 2 * r + 4 * h;
+        f4 y;
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) y[e] = empty ? 0.0F : o[g][d][r + e] * inverse;
+        if (a.gate != nullptr) {
+          const f4 gate = *reinterpret_cast<const f4*>(a.gate + static_cast<std::size_t>(out_row[g]) * 2 * D + D + at);
+#pragma unroll
+          for (unsigned e = 0; e < 4; ++e) y[e] *= 1.0F / (1.0F + expf(-gate[e]));
+        }
+        h4 out;
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) out[e] = static_cast<_Float16>(y[e]);
+        *reinterpret_cast<h4*>(a.output + static_cast<std::size_t>(out_row[g]) * D + at) = out;
       }
     }
-    if (h == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{m, l};
-    return;
+    if (a.log_sums != nullptr && h == 0) a.log_sums[out_row[g]] = empty ? -INFINITY : (m[g] - kLift) * kLn2 + logf(l[g]);
   }
-  const bool empty = m == -INFINITY;
-  const float inverse = empty ? 0.0F : 1.0F / l;
-#pragma unroll
-  for (unsigned d = 0; d < D / 32; ++d) {
-#pragma unroll
-    for (unsigned r = 0; r < 16; r += 4) {
-      const unsigned at = 32 * d + 2 * r + 4 * h;
-      f4 y;
-#pragma unroll
-      for (unsigned e = 0; e < 4; ++e) y[e] = empty ? 0.0F : o[d][r + e] * inverse;
-      if (a.gate != nullptr) {
-        const f4 gate = *reinterpret_cast<const f4*>(a.gate + out_row * 2 * D + D + at);
-#pragma unroll
-        for (unsigned e = 0; e < 4; ++e) y[e] *= 1.0F / (1.0F + expf(-gate[e]));
-      }
-      h4 out;
-#pragma unroll
-      for (unsigned e = 0; e < 4; ++e) out[e] = static_cast<_Float16>(y[e]);
-      *reinterpret_cast<h4*>(a.output + out_row * D + at) = out;
-    }
-  }
-  if (a.log_sums != nullptr && h == 0) a.log_sums[out_row] = empty ? -INFINITY : (m - kLift) * kLn2 + logf(l);
 }
 
 // Merges a row's ranges of positions and applies the gate: a wave per row and query head, D / 64
@@ -377,9 +452,9 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkAttnArgs a) {
   const uint32_t row = linear / a.q_heads, i = sequence_of(a.list.first, a.list.count, row);
   const uint32_t slot = listed_slot(a.list, i), tokens = a.list.first[i + 1] - a.list.first[i];
   const uint32_t length = committed(a.pages, slot), t = row - a.list.first[i];
-  const uint32_t tile_row = (t * a.group + linear % a.q_heads % a.group) / kRows * kRows;
-  const uint32_t hi = length + (min(tokens * a.group, tile_row + kRows) - 1) / a.group + 1;
-  const uint32_t tiles = (hi + kTile<D> - 1) / kTile<D>, per = tiles_per_split(tiles, a.splits);
+  const uint32_t tile_row = (t * a.group + linear % a.q_heads % a.group) / a.tile_rows * a.tile_rows;
+  const uint32_t hi = length + (min(tokens * a.group, tile_row + a.tile_rows) - 1) / a.group + 1;
+  const uint32_t tiles = (hi + kTile - 1) / kTile, per = tiles_per_split(tiles, a.splits);
   const uint32_t used = (tiles + per - 1) / per;
   const std::size_t base = static_cast<std::size_t>(linear) * a.splits;
   float best = -INFINITY;
@@ -517,6 +592,7 @@ int32_t read_heads(const gfxinfer_kv_pages* pages, uint32_t q_heads) {
 }
 
 struct ChunkShape {
+  uint32_t groups;  // of 32 rows a wave takes
   uint32_t tiles, splits;
 };
 
@@ -524,16 +600,18 @@ ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads
                        uint32_t* first_tile) {
   ChunkShape s{};
   const uint32_t group = q_heads / kv_heads;
+  const uint64_t all_rows = static_cast<uint64_t>(list.first[kMaxChunks]) * group * kv_heads;
+  s.groups = head_size == 128 && all_rows >= 2ull * kComputeUnits * rows_of(2) ? 2 : 1;
+  const uint32_t tile_rows = rows_of(s.groups);
   for (uint32_t i = 0; i < list.count; ++i) {
     first_tile[i] = s.tiles;
     const uint64_t rows = static_cast<uint64_t>(list.first[i + 1] - list.first[i]) * group;
-    s.tiles += static_cast<uint32_t>((rows + kRows - 1) / kRows);
+    s.tiles += static_cast<uint32_t>((rows + tile_rows - 1) / tile_rows);
   }
   for (uint32_t i = list.count; i <= kMaxChunks; ++i) first_tile[i] = s.tiles;
-  const uint32_t tile = head_size == 128 ? kTile<128> : kTile<256>;
   const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift;
-  const uint64_t places = 2 * kComputeUnits, items = static_cast<uint64_t>(s.tiles) * kv_heads;
-  const uint64_t most = std::max<uint64_t>(1, capacity / (tile * kLeastTiles));
+  const uint64_t places = (head_size == 128 && s.groups == 1 ? 2 : 1) * kComputeUnits, items = static_cast<uint64_t>(s.tiles) * kv_heads;
+  const uint64_t most = std::max<uint64_t>(1, capacity / (kTile * kLeastTiles));
   s.splits = static_cast<uint32_t>(std::clamp<uint64_t>((places + items - 1) / items, 1, most));
   return s;
 }
@@ -611,13 +689,15 @@ extern "C" int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pa
     a.kv_heads = kv_heads;
     a.group = q_heads / kv_heads;
     a.splits = shape.splits;
+    a.tile_rows = rows_of(shape.groups);
     a.scale = kLog2E / std::sqrt(static_cast<float>(head_size));
     const uint64_t items = static_cast<uint64_t>(shape.tiles) * shape.splits * kv_heads;
     if (items > (1u << 30)) return fail(GFXI_INVALID_ARGUMENT, "chunk attention over too many rows for one launch");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid(static_cast<unsigned>(items)), block(kWaves * 64);
-    if (head_size == 128) hipLaunchKernelGGL(chunk_attention_kernel<128>, grid, block, 0, st, a);
-    else hipLaunchKernelGGL(chunk_attention_kernel<256>, grid, block, 0, st, a);
+    if (head_size == 256) hipLaunchKernelGGL((chunk_attention_kernel<256, 1>), grid, block, 0, st, a);
+    else if (shape.groups == 1) hipLaunchKernelGGL((chunk_attention_kernel<128, 1>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((chunk_attention_kernel<128, 2>), grid, block, 0, st, a);
     if (const int32_t s = launch_status("chunk attention launch failed"); s != GFXI_OK || shape.splits == 1) return s;
     const dim3 combine(static_cast<unsigned>((rows + 3) / 4));
     if (head_size == 128) hipLaunchKernelGGL(chunk_combine_kernel<128>, combine, dim3(256), 0, st, a);

@@ -1,7 +1,7 @@
 // Products in 8-bit integers with one scale per token and one per output channel, for any
 // number of tokens, and the quantizer of their rows.
 //
-//   s = max |x| / 127,  c = rint(x / s)                       (a row: a token, or a channel)
+//   s = max |x| * fl32(1 / 127),  c = rint(x / s)              (a row: a token, or a channel)
 //   y[t][n] = float(sum_k a[t][k] w[n][k]) * (sa[t] * sw[n])
 //
 // The integer sum is exact (columns < 2^17, codes >= -128: below 2^31), so K may be divided
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const void
 #pragma unroll
   for (unsigned w = 0; w < kQuantWaves; ++w) top = fmaxf(top, partial[w]);
   const bool broken = top == INFINITY;
-  const float scale = broken ? __builtin_nanf("") : fmaxf(top / 127.0F, 0x1p-126F);
+  const float scale = broken ? __builtin_nanf("") : fmaxf(top * (1.0F / 127.0F), 0x1p-126F);
   if (threadIdx.x == 0) scales[row] = scale;
   auto store = [&](const float (&v)[8], uint32_t unit) __attribute__((always_inline)) {
     uint64_t packed = 0;

@@ -810,8 +810,8 @@ int32_t gfxinfer_launch_kv_pages_evict(const gfxinfer_kv_pages* pages, const gfx
 
 /* Rows [rows][columns] at a pitch of row_stride elements (8 | row_stride, rows 16-byte
  * aligned) of GFXI_F16, GFXI_F32 or GFXI_BF16 to codes int8 [rows][columns] and scales fp32
- * [rows]: scale = max |x| / 127 (at least 2^-126), code = the integer nearest x / scale, ties
- * to even, within -127..127.  For tokens, and once for a matrix's output channels.  A row with
+ * [rows]: scale = max |x| times the fp32 number nearest 1 / 127, rounded (at least 2^-126), code =
+ * the integer nearest x / scale, ties to even, within -127..127.  For tokens, and once for a matrix's output channels.  A row with
  * an infinity or a NaN gets zero codes and a NaN scale.  1..2^24 rows; columns a multiple of
  * 16 below 2^17. */
 int32_t gfxinfer_launch_quantize_rows_i8(const void* input, int32_t input_type, size_t rows, size_t columns,

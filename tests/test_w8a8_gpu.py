@@ -8,13 +8,14 @@ import pytest
 from gpu_util import dev, host, say
 
 pytestmark = pytest.mark.gpu
+SCALE = np.float32(1) / np.float32(127)
 
 
 def _codes_of(x):
     """(codes, scales) by the definition: the quotient in 64 bits, where next to a half nothing is lost."""
     x = x.astype(np.float32)
     bad = ~np.isfinite(x).all(1)
-    scale = np.maximum(np.abs(np.where(bad[:, None], 0, x)).max(1) / np.float32(127), np.float32(2.0 ** -126)).astype(np.float32)
+    scale = np.maximum(np.abs(np.where(bad[:, None], 0, x)).max(1) * SCALE, np.float32(2.0 ** -126)).astype(np.float32)
     codes = np.clip(np.rint(np.where(bad[:, None], 0, x).astype(np.float64) / scale[:, None].astype(np.float64)), -127, 127)
     return codes.astype(np.int8), np.where(bad, np.float32(np.nan), scale)
 
@@ -50,13 +51,13 @@ def test_codes_next_to_a_half(device, gx):
     """Quotients whose fp32 rounding is a half although they lie beside it, and true halves, which go to even."""
     rng = np.random.default_rng(11)
     top = np.float32(rng.uniform(0.5, 2.0))
-    scale = np.float32(top / np.float32(127))
+    scale = np.float32(top * SCALE)
     half = ((np.arange(-126, 126) + 0.5) * np.float64(scale)).astype(np.float32)
     x = np.concatenate([half, np.nextafter(half, np.float32(9)), np.nextafter(half, np.float32(-9)), [top, 0, -0.0, -top]]).astype(np.float32)
     x = np.resize(x, (len(x) + 15) // 16 * 16)[None]
     ties = np.array([[127.0] + [k + 0.5 for k in range(-8, 7)]], np.float32)   # scale 1: exact halves
     for rows in (x, ties):
-        q = rows.astype(np.float32) / (np.abs(rows).max() / np.float32(127))
+        q = rows.astype(np.float32) / (np.abs(rows).max() * SCALE)
         assert np.any(np.abs(q - np.trunc(q)) == 0.5)
         codes, scales = _quantize(gx, _tensor(rows, "float32"))
         want, wanted_scales = _codes_of(rows)
