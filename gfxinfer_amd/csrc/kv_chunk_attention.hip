@@ -3,9 +3,12 @@
 // Row (t, g) of a listed sequence and a KV head, new token t at query head g of the head's
 // group, attends to the first length + t + 1 positions:
 //     o = softmax(q . K / sqrt(D)) . V * sigmoid(gate),   L = log(sum exp(q . K / sqrt(D)))
-// The rows of a sequence and KV head are one tall matrix: a workgroup takes a tile of its rows
-// and a range of positions, each of its four waves 32 or 64 of the rows, and a K / V row staged in
-// LDS serves all of them.
+// The rows of a sequence and KV head are one tall matrix, in tiles of 128: a workgroup takes a tile
+// and a range of positions, each of its four waves 32 of the rows, and a K / V row staged in LDS
+// serves them all.  A second launch joins the ranges of a tile.  (Equal shares of all work, one a
+// workgroup and cut anywhere, were slower: 2048 tokens on 30000 1630 us, not 1403.  Workgroups that
+// go over the same positions of a head at the same time read them through one L2, those shares
+// did not.)
 //
 // Scores are computed transposed, S^T = K Q^T (v_mfma_f32_32x32x16_f16), so that a lane holds
 // half of one row's scores, the running maximum takes one lane exchange, and the weights are
@@ -34,11 +37,13 @@ using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 constexpr unsigned kWaves = 4;
 constexpr float kLn2 = 0.6931471805599453F;
 
-// A row tile: G groups of 32 rows a wave.  Positions of a step, and workgroups a CU holds.
-constexpr unsigned rows_of(unsigned g) { return kWaves * 32 * g; }
-constexpr unsigned kTile = 64;
-template <unsigned D, unsigned G>
-constexpr unsigned kResident = D == 128 && G == 1 ? 2 : 1;
+constexpr unsigned kRows = kWaves * 32;    // of a row tile
+template <unsigned D>
+constexpr unsigned kTile = 8192 / D;        // positions of a step: 16 KB of K and of V; two of each in LDS
+// Workgroups a CU holds: at head size 256 the outputs and queries of 32 rows alone are 192 of the 256
+// registers that two waves of a SIMD would have each.
+template <unsigned D>
+constexpr unsigned kResident = D == 128 ? 2 : 1;
 
 // A row's weights are 2^(score - m + kLift) in fp16, scores in units of log2.  m is a maximum of
 // the row so far that moves up once it is passed by kRise, so weights stay below 2^15.  Against
@@ -54,13 +59,14 @@ struct ChunkAttnArgs {
   const float* gate;     // [rows][q_heads][2 D] or null
   __half* output;        // [rows][q_heads][D]
   float* log_sums;       // [rows][q_heads] or null
-  float* partial_o;      // [rows][q_heads][splits][D], where positions are divided
-  float* partial_ml;     // [rows][q_heads][splits][2]
-  uint32_t layer, q_heads, kv_heads, group, splits, tile_rows;
+  uint32_t* range;       // steps of a range, as the attention launch found it
+  float* partial_o;      // [rows][q_heads][ranges][D], where positions are divided
+  float* partial_ml;     // [rows][q_heads][ranges][2]
+  uint32_t layer, q_heads, kv_heads, group, ranges;
   float scale;           // log2(e) / sqrt(D)
 };
 
-// The listed sequence a row tile belongs to: one round of loads of the list instead of a search.
+// The listed sequence a row tile (a row) belongs to: one round of loads of the list, no search.
 __device__ __forceinline__ uint32_t sequence_of(const uint32_t* first, uint32_t count, uint32_t x) {
   if (count == 1) return 0;
   const unsigned lane = threadIdx.x & 63u;
@@ -71,10 +77,25 @@ __device__ __forceinline__ uint32_t sequence_of(const uint32_t* first, uint32_t 
   return __builtin_amdgcn_readfirstlane(found) - 1;
 }
 
-// Tiles of positions a range holds at least, and how a row tile's positions are divided.
-constexpr uint32_t kLeastTiles = 4;
-__device__ __forceinline__ uint32_t tiles_per_split(uint32_t tiles, uint32_t splits) {
-  return max(kLeastTiles, (tiles + splits - 1) / splits);
+// Steps a range holds at least, if there is more than one.
+constexpr uint32_t kLeastSteps = 2;
+// Ranges of equal length for all sequences: the longest one is divided into as many as the launch
+// allows, the others into as few as hold them.
+template <unsigned D>
+__device__ __forceinline__ uint32_t range_steps(const ChunkAttnArgs& a) {
+  const unsigned lane = threadIdx.x & 63u;
+  uint32_t most = 0;
+  for (uint32_t from = 0; from < a.list.count; from += 64) {
+    const uint32_t i = from + lane;
+    if (i < a.list.count) {
+      const uint32_t length = min(a.pages.lengths[a.list.slot[i]], a.pages.stride << a.pages.page_shift);
+      most = max(most, length + (a.list.first[i + 1] - a.list.first[i]));
+    }
+  }
+#pragma unroll
+  for (unsigned d = 1; d < 64; d <<= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
+  const uint32_t steps = (__builtin_amdgcn_readfirstlane(most) + kTile<D> - 1) / kTile<D>;
+  return max(kLeastSteps, (steps + a.ranges - 1) / a.ranges);
 }
 
 __device__ __forceinline__ float max_over_halves(float v) {
@@ -89,67 +110,68 @@ __device__ __forceinline__ float sum_over_halves(float v) {
 }
 
 // Sixteen-position parts of a tile: their pages, -1 where there is none.
+template <unsigned D>
 struct TilePages {
-  int32_t page[kTile / 16];
+  int32_t page[kTile<D> / 16];
   uint32_t missing;
 };
 
-// One item: a row tile of a listed sequence at KV head hk, tiles [from, to) of positions.
-template <unsigned D, unsigned G>
-__global__ __launch_bounds__(kWaves * 64, (kResident<D, G>)) void chunk_attention_kernel(ChunkAttnArgs a) {
-  constexpr unsigned T = kTile, kSub = T / 32, kSteps = T / 16, kRows = rows_of(G);
+template <unsigned D>
+__global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_kernel(ChunkAttnArgs a) {
+  constexpr unsigned T = kTile<D>, kSub = T / 32, kSteps = T / 16;
   constexpr unsigned kLoadRows = 512 / D;                   // rows a load of a wave covers
   constexpr unsigned kLoads = T / kLoadRows / kWaves;       // of K, and of V, per tile and wave
   __shared__ __align__(1024) _Float16 k0[T * D];
   __shared__ __align__(1024) _Float16 k1[T * D];
   __shared__ __align__(1024) _Float16 v0[T * D];
   __shared__ __align__(1024) _Float16 v1[T * D];
-  __shared__ uint32_t marks[2][kWaves];
-  __shared__ uint32_t again[kWaves];
+  __shared__ uint32_t again[kWaves];       // the wave's rows met an infinity or NaN
+  __shared__ uint32_t strange_tiles[32];   // bit x % 1024: a tile x holds infinities or NaNs among its values
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned n = lane & 31u, h = lane >> 5;
   const KvPages& pg = a.pages;
-
-  // KV heads vary fastest: with eight of them each XCD reads one.  Late tokens, which see most, first.
+  // KV heads vary fastest: with eight of them each XCD reads one.  Then row tiles, so that those that
+  // read the same positions run together; late tokens, which see most, first.
   const uint32_t hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  const uint32_t split = rest % a.splits, all_tiles = a.first_tile[kMaxChunks];
-  const uint32_t row_tile = all_tiles - 1 - rest / a.splits;
+  const uint32_t tiles = a.first_tile[kMaxChunks], range = rest / tiles, row_tile = tiles - 1 - rest % tiles;
   const uint32_t i = sequence_of(a.first_tile, a.list.count, row_tile);
   const uint32_t slot = listed_slot(a.list, i), first_row = a.list.first[i], tokens = a.list.first[i + 1] - first_row;
+  uint32_t per = 0xffffffffu;
+  if (a.ranges > 1) {
+    per = range_steps<D>(a);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.range = per;
+  }
   const uint32_t length = committed(pg, slot), rows = tokens * a.group;
   const uint32_t tile_row = (row_tile - a.first_tile[i]) * kRows;
   // The tile's last row sees this many positions; what lies behind the sequence's end is not read.
   const uint32_t last_row = min(rows, tile_row + kRows) - 1;
-  const uint32_t end = length + tokens, hi = length + last_row / a.group + 1;
-  const uint32_t tiles = (hi + T - 1) / T, per = tiles_per_split(tiles, a.splits);
-  const uint32_t from = split * per, to = min(from + per, tiles);
-  if (from >= tiles) return;
+  const uint32_t end = length + tokens, steps = (length + last_row / a.group + T) / T;
+  const uint32_t from = a.ranges > 1 ? range * per : 0u, to = a.ranges > 1 ? min(from + per, steps) : steps;
+  if (from >= steps) return;
 
-  const uint32_t wave_row = tile_row + wave * 32 * G;
+  const uint32_t wave_row = tile_row + wave * 32, row = wave_row + n;
   const bool works = wave_row < rows;                        // the wave has a row
   const uint32_t least_visible = length + wave_row / a.group + 1;
-  uint32_t visible[G], out_row[G];                           // out_row: [rows][q_heads], below 2^30
-  h8 q[G][D / 16];
+  const uint32_t visible = row < rows ? length + row / a.group + 1 : 0;
+  // Where the lane's row goes, [rows][q_heads], below 2^30.
+  const uint32_t out_row = row < rows ? (first_row + row / a.group) * a.q_heads + hk * a.group + row % a.group : 0xffffffffu;
+  h8 q[D / 16];
 #pragma unroll
-  for (unsigned g = 0; g < G; ++g) {
-    const uint32_t row = wave_row + 32 * g + n, t = row / a.group;
-    const bool there = row < rows;
-    visible[g] = there ? length + t + 1 : 0;
-    out_row[g] = there ? (first_row + t) * a.q_heads + hk * a.group + (row - t * a.group) : 0xffffffffu;
-#pragma unroll
-    for (unsigned s = 0; s < D / 16; ++s) {
-      q[g][s] = h8{};
-      if (there) q[g][s] = *reinterpret_cast<const h8*>(a.query + static_cast<std::size_t>(out_row[g]) * D + 16 * s + 8 * h);
-    }
+  for (unsigned st = 0; st < D / 16; ++st) {
+    q[st] = h8{};
+    if (row < rows) q[st] = *reinterpret_cast<const h8*>(a.query + static_cast<std::size_t>(out_row) * D + 16 * st + 8 * h);
+    if constexpr (D == 256) asm volatile("" : "+a"(q[st]));
   }
 
   const std::size_t layer_row = (static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) * pg.row + hk * D;
   const __half* keys = pg.key + layer_row;
   const __half* values = pg.value + layer_row;
   const uint32_t in_page = (1u << pg.page_shift) - 1;
+  f16v o[D / 32], s[kSub], s_next[kSub];
+  float m, l;
   PageWindow window;
   auto find_pages = [&](uint32_t x) __attribute__((always_inline)) {
-    TilePages p;
+    TilePages<D> p;
     p.missing = 0;
 #pragma unroll
     for (unsigned e = 0; e < T / 16; ++e) {
@@ -159,20 +181,27 @@ __global__ __launch_bounds__(kWaves * 64, (kResident<D, G>)) void chunk_attentio
     }
     return p;
   };
-  // Where the lane's piece of a load lies in memory, in elements from the first of the load's rows:
-  // this ^ 8 (row0 % 16) for K, ^ 16 (row0 % 8) for V.
-  const uint32_t load_row = lane / (D / 8);
-  const uint32_t key_part = load_row * pg.row + 8 * key_slot(lane % (D / 8), load_row);
-  const uint32_t value_part = load_row * pg.row + 8 * value_slot(lane % (D / 8), load_row);
-  // Rows of a tile into LDS.  All rows of a load are of one part; parts without a page load from page 0 of
-  // the pool (always there), and so do those past the end.
-  auto load = [&](_Float16* to_lds, const __half* pool, uint32_t part, unsigned swizzle, uint32_t x, const TilePages& p) __attribute__((always_inline)) {
+  // Where the lane's piece of a load lies in memory, in bytes from the first of the load's rows: the rows of
+  // load u of a wave are 16 or 8 u and its own, so the order of their pieces (by the row in sixteen for K,
+  // in eight for V) is that of u % 2.
+  const uint32_t load_row = lane / (D / 8), row_bytes = 2 * pg.row;
+  uint32_t key_part[2], value_part;
+#pragma unroll
+  for (unsigned e = 0; e < 2; ++e) {
+    key_part[e] = load_row * row_bytes + 16 * key_slot(lane % (D / 8), kLoadRows * (wave + kWaves * e) + load_row);
+  }
+  value_part = load_row * row_bytes + 16 * value_slot(lane % (D / 8), kLoadRows * wave + load_row);
+  // Rows of a tile into LDS, through buffer descriptors of the parts' sixteen rows (after flat loads into LDS
+  // the compiler lets every read of LDS wait for all reads before it).  Parts without a page load from page 0
+  // of the pool (always there), and so do those past the end.
+  auto load = [&](_Float16* to_lds, const __half* pool, bool key, uint32_t x, const TilePages<D>& p) __attribute__((always_inline)) {
 #pragma unroll
     for (unsigned u = 0; u < kLoads; ++u) {
       const unsigned row0 = kLoadRows * (wave + kWaves * u), e = kLoadRows * kWaves * u / 16;
-      const std::size_t base = ((static_cast<std::size_t>(max(p.page[e], 0)) << pg.page_shift) + ((x * T + row0) & in_page)) * pg.row;
-      __builtin_amdgcn_global_load_lds((global_void*)(pool + base + (part ^ 8 * (swizzle == 0 ? row0 & 15u : 2 * (row0 & 7u)))),
-                                       (lds_void*)(to_lds + row0 * D), 16, 0, 0);
+      const std::size_t base = ((static_cast<std::size_t>(max(p.page[e], 0)) << pg.page_shift) + ((x * T + 16 * e) & in_page)) * pg.row;
+      const auto rows16 = __builtin_amdgcn_make_buffer_rsrc(const_cast<__half*>(pool + base), 0, static_cast<int>(15 * row_bytes + 2 * D), 0x20000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rows16, (lds_void*)(to_lds + row0 * D), 16, static_cast<int>(key ? key_part[D == 128 ? 0 : u % 2] : value_part),
+                                               static_cast<int>((row0 & 15u) * row_bytes), 0, 0);
     }
   };
 
@@ -183,24 +212,19 @@ __global__ __launch_bounds__(kWaves * 64, (kResident<D, G>)) void chunk_attentio
   const unsigned key_place = n * (2 * D) + 16 * key_slot(h, n);
   const unsigned value_place = vrow * (2 * D) + 16 * value_slot(2 * (lane >> 4 & 1u) + ((i16 & 3u) >> 1), vrow) + 8 * (i16 & 1u);
 
-  f16v o[G][D / 32], s[G][kSub], s_next[G][kSub];
-  float m[G], l[G];
   // What a page holds past a sequence's end, and what a missing one would, may be anything, and 0 * NaN
   // is NaN: the wave's own V rows of such positions become zeros.  A careful pass also takes out
   // infinities and NaNs, and marks the tile.
-  auto repair = [&](_Float16* vs, uint32_t x, uint32_t missing, bool careful) __attribute__((always_inline)) {
+  auto repair = [&](_Float16* vs, uint32_t x, uint32_t missing, auto careful) __attribute__((always_inline)) {
     bool strange = false;
 #pragma unroll 1
     for (unsigned u = 0; u < kLoads; ++u) {
       const unsigned row0 = kLoadRows * (wave + kWaves * u);
       u32x4* piece = reinterpret_cast<u32x4*>(vs + row0 * D) + lane;
       if (x * T + row0 + load_row >= end || (missing >> row0 / 16 & 1u) != 0) *piece = u32x4{0, 0, 0, 0};
-      if (careful) strange |= take_strange(piece);
+      if constexpr (careful) strange |= take_strange(piece);
     }
-    if (careful) {
-      const bool any = __any(strange);
-      if (lane == 0) marks[x & 1u][wave] = any ? 1u : 0u;
-    }
+    if (careful && strange) atomicOr(&strange_tiles[x / 32 % 32], 1u << x % 32);
     wait_loads<63>();
   };
   // The rows that see an infinity or NaN among the values get it, whatever the weight: no weight is
@@ -217,99 +241,78 @@ __global__ __launch_bounds__(kWaves * 64, (kResident<D, G>)) void chunk_attentio
 #pragma unroll
         for (unsigned r = 0; r < 16; ++r) {
           const float y = __half2float(v[32 * d + 8 * (r / 4) + 4 * h + r % 4]);
-#pragma unroll
-          for (unsigned g = 0; g < G; ++g) {
-            if (!(fabsf(y) < INFINITY) && position < visible[g]) o[g][d][r] += y;
-          }
+          if (!(fabsf(y) < INFINITY) && position < visible) o[d][r] += y;
         }
       }
     }
-    wait_loads<0>();
   };
   // Raw products of the rows with a tile of K rows.
-  auto score = [&](const _Float16* ks, f16v (&out)[G][kSub]) __attribute__((always_inline)) {
+  auto score = [&](const _Float16* ks, f16v (&out)[kSub]) __attribute__((always_inline)) {
     const char* kb = reinterpret_cast<const char*>(ks);
 #pragma unroll
-    for (unsigned g = 0; g < G; ++g) {
-#pragma unroll
-      for (unsigned u = 0; u < kSub; ++u) out[g][u] = f16v{};
-    }
+    for (unsigned u = 0; u < kSub; ++u) out[u] = f16v{};
 #pragma unroll
     for (unsigned st = 0; st < D / 16; ++st) {
 #pragma unroll
       for (unsigned u = 0; u < kSub; ++u) {
         const h8 k = *reinterpret_cast<const h8*>(kb + (key_place ^ 32 * st) + u * 64 * D);
-#pragma unroll
-        for (unsigned g = 0; g < G; ++g) out[g][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[g][st], out[g][u], 0, 0, 0);
+        out[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[st], out[u], 0, 0, 0);
       }
     }
   };
   // Scores of a tile are ready: hides what a row does not see, and moves the maxima.
-  auto settle = [&](f16v (&sc)[G][kSub], uint32_t x, uint32_t missing) __attribute__((always_inline)) {
+  auto settle = [&](f16v (&sc)[kSub], uint32_t x, uint32_t missing) __attribute__((always_inline)) {
     if (x * T + T > least_visible || missing != 0) {
 #pragma unroll
-      for (unsigned g = 0; g < G; ++g) {
+      for (unsigned u = 0; u < kSub; ++u) {
 #pragma unroll
-        for (unsigned u = 0; u < kSub; ++u) {
-#pragma unroll
-          for (unsigned r = 0; r < 16; ++r) {
-            const unsigned p = 32 * u + 8 * (r / 4) + 4 * h + r % 4;
-            if (x * T + p >= visible[g] || (missing >> (2 * u + r / 8) & 1u) != 0) sc[g][u][r] = -INFINITY;
-          }
+        for (unsigned r = 0; r < 16; ++r) {
+          const unsigned p = 32 * u + 8 * (r / 4) + 4 * h + r % 4;
+          if (x * T + p >= visible || (missing >> (2 * u + r / 8) & 1u) != 0) sc[u][r] = -INFINITY;
         }
       }
     }
     // (A NaN score makes the maximum NaN and the row's result with it, as it has to.)
-    float top[G];
-    bool rises = false;
+    float best = sc[0][0];
 #pragma unroll
-    for (unsigned g = 0; g < G; ++g) {
-      float best = sc[g][0][0];
+    for (unsigned e = 1; e < 16 * kSub; ++e) best = __builtin_elementwise_maximum(best, sc[e / 16][e % 16]);
+    const float top = max_over_halves(best) * a.scale;
+    if (__any(!(top <= m + kRise))) {
+      const float next = top <= m + kRise ? m : top;
+      // From nothing to something: there is nothing to scale yet.
+      const float factor = next == m || m == -INFINITY ? 1.0F : rescale_factor(m, next);
+      m = next;
+      l *= factor;
 #pragma unroll
-      for (unsigned e = 1; e < 16 * kSub; ++e) best = __builtin_elementwise_maximum(best, sc[g][e / 16][e % 16]);
-      top[g] = max_over_halves(best) * a.scale;
-      rises |= !(top[g] <= m[g] + kRise);
-    }
-    if (__any(rises)) {
+      for (unsigned d = 0; d < D / 32; ++d) {
 #pragma unroll
-      for (unsigned g = 0; g < G; ++g) {
-        const float next = top[g] <= m[g] + kRise ? m[g] : top[g];
-        // From nothing to something: there is nothing to scale yet.
-        const float factor = next == m[g] || m[g] == -INFINITY ? 1.0F : rescale_factor(m[g], next);
-        m[g] = next;
-        l[g] *= factor;
-#pragma unroll
-        for (unsigned d = 0; d < D / 32; ++d) {
-#pragma unroll
-          for (unsigned r = 0; r < 16; ++r) o[g][d][r] *= factor;
-        }
+        for (unsigned r = 0; r < 16; ++r) o[d][r] *= factor;
       }
     }
   };
   // The weights of the tile in s and the scores of the next one, then the values of this one.
-  auto step = [&](const _Float16* next_ks, const _Float16* vs, uint32_t x, auto careful) __attribute__((always_inline)) {
-    h8 p[G][kSteps];
+  auto step = [&](const _Float16* next_ks, const _Float16* vs) __attribute__((always_inline)) {
+    h8 p[kSteps];
+    if constexpr (D == 256) {
+      // The outputs and queries belong into the accumulation registers: left to itself the compiler counts
+      // them among the others and reads every operand right before its product (4 prompts of 300 on
+      // 1500..6000: 226 us, not 211).
+#pragma unroll
+      for (unsigned d = 0; d < D / 32; ++d) asm volatile("" : "+a"(o[d]));
+    }
     score(next_ks, s_next);
+    const float floor = m == -INFINITY ? 0.0F : m - kLift;
+    float sum[4] = {l, 0.0F, 0.0F, 0.0F};
 #pragma unroll
-    for (unsigned g = 0; g < G; ++g) {
-      const float floor = m[g] == -INFINITY ? 0.0F : m[g] - kLift;
-      float sum[4] = {l[g], 0.0F, 0.0F, 0.0F};
+    for (unsigned j = 0; j < kSteps; ++j) {
 #pragma unroll
-      for (unsigned j = 0; j < kSteps; ++j) {
-#pragma unroll
-        for (unsigned e = 0; e < 8; ++e) {
-          const float w = __builtin_amdgcn_exp2f(fmaf(s[g][j / 2][8 * (j % 2) + e], a.scale, -floor));
-          sum[e % 4] += w;
-          p[g][j][e] = static_cast<_Float16>(w);
-        }
+      for (unsigned e = 0; e < 8; ++e) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[j / 2][8 * (j % 2) + e], a.scale, -floor));
+        sum[e % 4] += w;
+        p[j][e] = static_cast<_Float16>(w);
       }
-      l[g] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
-    if constexpr (careful) {
-      uint32_t mark = 0;
-      for (unsigned w = 0; w < kWaves; ++w) mark |= marks[x & 1u][w];
-      if (__builtin_amdgcn_readfirstlane(mark) != 0) add_strange(x);
-    }
+    l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     char* vb = const_cast<char*>(reinterpret_cast<const char*>(vs));
 #pragma unroll
     for (unsigned j = 0; j < kSteps; ++j) {
@@ -321,53 +324,64 @@ __global__ __launch_bounds__(kWaves * 64, (kResident<D, G>)) void chunk_attentio
           y[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vb + (value_place ^ 64 * d) + (16 * j + 8 * e) * 2 * D));
         }
         const h8 v = __builtin_bit_cast(h8, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (unsigned g = 0; g < G; ++g) o[g][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[g][j], o[g][d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[j], o[d], 0, 0, 0);
       }
     }
+    // The order of all this: operands are read eight ahead of the products, and exponentials go
+    // between the products of the next tile's scores.
+    constexpr unsigned kScores = kSub * D / 16, kAhead = 8;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
-    for (unsigned g = 0; g < G; ++g) {
-#pragma unroll
-      for (unsigned u = 0; u < kSub; ++u) s[g][u] = s_next[g][u];
+    for (unsigned e = 0; e < kScores; ++e) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x400, 16 * kSub / kScores, 0);
+      __builtin_amdgcn_sched_group_barrier(0x2, 3 * 16 * kSub / kScores, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
+#pragma unroll
+    for (unsigned e = 0; e < kSteps * D / 32; ++e) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+#pragma unroll
+    for (unsigned u = 0; u < kSub; ++u) s[u] = s_next[u];
   };
 
   // Tile x's V rows and tile x + 1's K rows are read while x + 1's V rows and x + 2's K rows are on their way,
   // each into the place that was read last before the barrier.
   auto pass = [&](auto careful) __attribute__((always_inline)) {
+    m = -INFINITY;
+    l = 0.0F;
 #pragma unroll
-    for (unsigned g = 0; g < G; ++g) {
-      m[g] = -INFINITY;
-      l[g] = 0.0F;
-#pragma unroll
-      for (unsigned d = 0; d < D / 32; ++d) o[g][d] = f16v{};
-    }
+    for (unsigned d = 0; d < D / 32; ++d) o[d] = f16v{};
     window.start(pg, slot, (from * T) >> pg.page_shift);
-    TilePages now = find_pages(from), next = now;
-    load(k0, keys, key_part, 0, from, now);
+    TilePages<D> now = find_pages(from), next = now;
+    if (careful && threadIdx.x < 32) strange_tiles[threadIdx.x] = 0;
+    __syncthreads();  // the tile before this one is done with
+    load(k0, keys, true, from, now);
     wait_loads<0>();
     __syncthreads();
-    load(v0, values, value_part, 1, from, now);
+    load(v0, values, false, from, now);
     if (from + 1 < to) {
       next = find_pages(from + 1);
-      load(k1, keys, key_part, 0, from + 1, next);
+      load(k1, keys, true, from + 1, next);
     }
     if (works) {
       score(k0, s);
       settle(s, from, now.missing);
     }
-    auto turn = [&](uint32_t x, _Float16* k_free, const _Float16* k_next, const _Float16* v_now, _Float16* v_free) __attribute__((always_inline)) {
+    auto turn = [&](uint32_t x, _Float16* k_free, const _Float16* k_next, _Float16* v_now, _Float16* v_free) __attribute__((always_inline)) {
       wait_loads<0>();
-      if (careful || now.missing != 0 || (x + 1) * T > end) repair(const_cast<_Float16*>(v_now), x, now.missing, careful);
+      if (careful || now.missing != 0 || (x + 1) * T > end) repair(v_now, x, now.missing, careful);
       __syncthreads();
       now = next;
-      if (x + 1 < to) load(v_free, values, value_part, 1, x + 1, next);
+      if (x + 1 < to) load(v_free, values, false, x + 1, next);
       if (x + 2 < to) {
         next = find_pages(x + 2);
-        load(k_free, keys, key_part, 0, x + 2, next);
+        load(k_free, keys, true, x + 2, next);
       }
       if (works) {
-        step(k_next, v_now, x, careful);
+        step(k_next, v_now);
         if (x + 1 < to) settle(s, x + 1, now.missing);
       }
     };
@@ -376,106 +390,119 @@ __global__ __launch_bounds__(kWaves * 64, (kResident<D, G>)) void chunk_attentio
       turn(x, k0, k1, v0, v1);
       if (x + 1 < to) turn(x + 1, k1, k0, v1, v0);
     }
-    // Whether an output is an infinity or NaN: finite values at weights below 2^15 make none.
+  };
+  // Whether an output is an infinity or NaN: finite values at weights below 2^15 make none.
+  auto is_strange = [&]() __attribute__((always_inline)) {
     bool strange = false;
 #pragma unroll
-    for (unsigned g = 0; g < G; ++g) {
+    for (unsigned d = 0; d < D / 32; ++d) {
 #pragma unroll
-      for (unsigned d = 0; d < D / 32; ++d) {
-#pragma unroll
-        for (unsigned r = 0; r < 16; ++r) strange |= !(fabsf(o[g][d][r]) < INFINITY);
-      }
+      for (unsigned r = 0; r < 16; ++r) strange |= !(fabsf(o[d][r]) < INFINITY);
     }
     return strange;
   };
+
+  pass(std::false_type{});
+  bool strange = is_strange();
   // A second, careful pass follows in the rare case that an output of the first is an infinity or NaN.
-  bool strange = pass(std::false_type{});
-  const bool mine = works && __any(strange);
+  const bool mine = __any(strange);
   if (lane == 0) again[wave] = mine ? 1u : 0u;
   __syncthreads();
   uint32_t found = 0;
   for (unsigned w = 0; w < kWaves; ++w) found |= again[w];
   const bool careful = __builtin_amdgcn_readfirstlane(found) != 0;
-  if (__builtin_expect(careful, 0)) strange = pass(std::true_type{});
-#pragma unroll
-  for (unsigned g = 0; g < G; ++g) {
-    l[g] = sum_over_halves(l[g]);
-    // Only NaN scores, and strange values at scores of -infinity, make a NaN row rather than an empty one.
-    if ((m[g] == -INFINITY && (l[g] != l[g] || (careful && strange))) || m[g] != m[g]) m[g] = 0.0F;
-    if (out_row[g] == 0xffffffffu) continue;
-    if (a.splits > 1) {
-      const std::size_t at = static_cast<std::size_t>(out_row[g]) * a.splits + split;
-#pragma unroll
-      for (unsigned d = 0; d < D / 32; ++d) {
-#pragma unroll
-        for (unsigned r = 0; r < 16; r += 4) {
-          *reinterpret_cast<f4*>(a.partial_o + at * D + 32 * d + 2 * r + 4 * h) = f4{o[g][d][r], o[g][d][r + 1], o[g][d][r + 2], o[g][d][r + 3]};
-        }
-      }
-      if (h == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{m[g], l[g]};
-      continue;
+  if (__builtin_expect(careful, 0)) {
+    pass(std::true_type{});
+    for (uint32_t x = from; x < to; ++x) {
+      if ((__builtin_amdgcn_readfirstlane(strange_tiles[x / 32 % 32]) >> x % 32 & 1u) != 0) add_strange(x);
     }
-    const bool empty = m[g] == -INFINITY;
-    const float inverse = empty ? 0.0F : 1.0F / l[g];
+    strange = is_strange();
+  }
+  l = sum_over_halves(l);
+  // Only NaN scores, and strange values at scores of -infinity, make a NaN row rather than an empty one.
+  if ((m == -INFINITY && (l != l || (careful && strange))) || m != m) m = 0.0F;
+  if (out_row == 0xffffffffu) return;
+  if (a.ranges > 1) {
+    const std::size_t at = static_cast<std::size_t>(out_row) * a.ranges + range;
 #pragma unroll
     for (unsigned d = 0; d < D / 32; ++d) {
 #pragma unroll
       for (unsigned r = 0; r < 16; r += 4) {
-        const unsigned at = 32 * d + 2 * r + 4 * h;
-        f4 y;
-#pragma unroll
-        for (unsigned e = 0; e < 4; ++e) y[e] = empty ? 0.0F : o[g][d][r + e] * inverse;
-        if (a.gate != nullptr) {
-          const f4 gate = *reinterpret_cast<const f4*>(a.gate + static_cast<std::size_t>(out_row[g]) * 2 * D + D + at);
-#pragma unroll
-          for (unsigned e = 0; e < 4; ++e) y[e] *= 1.0F / (1.0F + expf(-gate[e]));
-        }
-        h4 out;
-#pragma unroll
-        for (unsigned e = 0; e < 4; ++e) out[e] = static_cast<_Float16>(y[e]);
-        *reinterpret_cast<h4*>(a.output + static_cast<std::size_t>(out_row[g]) * D + at) = out;
+        *reinterpret_cast<f4*>(a.partial_o + at * D + 32 * d + 2 * r + 4 * h) = f4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
       }
     }
-    if (a.log_sums != nullptr && h == 0) a.log_sums[out_row[g]] = empty ? -INFINITY : (m[g] - kLift) * kLn2 + logf(l[g]);
+    if (h == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{m, l};
+    return;
   }
+  const bool empty = m == -INFINITY;
+  const float inverse = empty ? 0.0F : 1.0F / l;
+#pragma unroll
+  for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+    for (unsigned r = 0; r < 16; r += 4) {
+      const unsigned at = 32 * d + 2 * r + 4 * h;
+      f4 y;
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) y[e] = empty ? 0.0F : o[d][r + e] * inverse;
+      if (a.gate != nullptr) {
+        const f4 gate = *reinterpret_cast<const f4*>(a.gate + static_cast<std::size_t>(out_row) * 2 * D + D + at);
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) y[e] *= 1.0F / (1.0F + expf(-gate[e]));
+      }
+      h4 out;
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) out[e] = static_cast<_Float16>(y[e]);
+      *reinterpret_cast<h4*>(a.output + static_cast<std::size_t>(out_row) * D + at) = out;
+    }
+  }
+  if (a.log_sums != nullptr && h == 0) a.log_sums[out_row] = empty ? -INFINITY : (m - kLift) * kLn2 + logf(l);
 }
 
-// Merges a row's ranges of positions and applies the gate: a wave per row and query head, D / 64
-// dims a lane.
+// Joins the ranges of a row and applies the gate: a wave per row and query head, D / 64 dims a lane.
 template <unsigned D>
-__global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkAttnArgs a) {
+__global__ __launch_bounds__(256) void chunk_join_kernel(ChunkAttnArgs a) {
   constexpr unsigned J = D / 64;
+  using vec = float __attribute__((ext_vector_type(J)));
+  using hvec = _Float16 __attribute__((ext_vector_type(J)));
   const unsigned lane = threadIdx.x & 63u;
-  const uint32_t rows = a.list.first[kMaxChunks] * a.q_heads;
   const uint32_t linear = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
-  if (linear >= rows) return;
+  if (linear >= a.list.first[kMaxChunks] * a.q_heads) return;
   const uint32_t row = linear / a.q_heads, i = sequence_of(a.list.first, a.list.count, row);
-  const uint32_t slot = listed_slot(a.list, i), tokens = a.list.first[i + 1] - a.list.first[i];
-  const uint32_t length = committed(a.pages, slot), t = row - a.list.first[i];
-  const uint32_t tile_row = (t * a.group + linear % a.q_heads % a.group) / a.tile_rows * a.tile_rows;
-  const uint32_t hi = length + (min(tokens * a.group, tile_row + a.tile_rows) - 1) / a.group + 1;
-  const uint32_t tiles = (hi + kTile - 1) / kTile, per = tiles_per_split(tiles, a.splits);
-  const uint32_t used = (tiles + per - 1) / per;
-  const std::size_t base = static_cast<std::size_t>(linear) * a.splits;
-  float best = -INFINITY;
-  for (uint32_t s = 0; s < used; ++s) best = fmaxf(best, a.partial_ml[2 * (base + s)]);
-  float total = 0.0F, y[J] = {};
-  for (uint32_t s = 0; s < used; ++s) {
-    const float2 x = *reinterpret_cast<const float2*>(a.partial_ml + 2 * (base + s));
+  const std::size_t base = static_cast<std::size_t>(linear) * a.ranges;
+  vec g = {};
+  if (a.gate != nullptr) g = *reinterpret_cast<const vec*>(a.gate + static_cast<std::size_t>(linear) * 2 * D + D + J * lane);
+  const uint32_t slot = listed_slot(a.list, i), tokens = a.list.first[i + 1] - a.list.first[i], t = row - a.list.first[i];
+  const uint32_t tile_row = (t * a.group + linear % a.q_heads % a.group) / kRows * kRows;
+  const uint32_t last_row = min(tokens * a.group, tile_row + kRows) - 1;
+  const uint32_t steps = (committed(a.pages, slot) + last_row / a.group + kTile<D>) / kTile<D>, per = *a.range;
+  const uint32_t used = (steps + per - 1) / per;
+  float best = -INFINITY, sum = 0.0F;
+  vec y = {};
+  for (uint32_t r = 0; r < used; ++r) {
+    const float2 x = *reinterpret_cast<const float2*>(a.partial_ml + 2 * (base + r));
+    const vec o = *reinterpret_cast<const vec*>(a.partial_o + (base + r) * D + J * lane);
     if (x.x == -INFINITY) continue;
-    const float w = rescale_factor(x.x, best);
-    total += x.y * w;
-#pragma unroll
-    for (unsigned j = 0; j < J; ++j) y[j] = fmaf(a.partial_o[(base + s) * D + J * lane + j], w, y[j]);
+    const float next = fmaxf(best, x.x), w = rescale_factor(x.x, next);
+    if (best == -INFINITY) {
+      sum = x.y * w;
+      y = o * w;
+    } else {
+      const float keep = rescale_factor(best, next);
+      sum = sum * keep + x.y * w;
+      y = y * keep + o * w;
+    }
+    best = next;
   }
   const bool empty = best == -INFINITY;
+  hvec out;
 #pragma unroll
   for (unsigned j = 0; j < J; ++j) {
-    y[j] = empty ? 0.0F : y[j] / total;
-    if (a.gate != nullptr) y[j] *= 1.0F / (1.0F + expf(-a.gate[static_cast<std::size_t>(linear) * 2 * D + D + J * lane + j]));
-    a.output[static_cast<std::size_t>(linear) * D + J * lane + j] = to_half(y[j]);
+    float v = empty ? 0.0F : y[j] / sum;
+    if (a.gate != nullptr) v *= 1.0F / (1.0F + expf(-g[j]));
+    out[j] = static_cast<_Float16>(v);
   }
-  if (a.log_sums != nullptr && lane == 0) a.log_sums[linear] = empty ? -INFINITY : (best - kLift) * kLn2 + logf(total);
+  *reinterpret_cast<hvec*>(a.output + static_cast<std::size_t>(linear) * D + J * lane) = out;
+  if (a.log_sums != nullptr && lane == 0) a.log_sums[linear] = empty ? -INFINITY : (best - kLift) * kLn2 + logf(sum);
 }
 
 // ---- the weight that each position receives ---------------------------------------------
@@ -592,32 +619,31 @@ int32_t read_heads(const gfxinfer_kv_pages* pages, uint32_t q_heads) {
 }
 
 struct ChunkShape {
-  uint32_t groups;  // of 32 rows a wave takes
-  uint32_t tiles, splits;
+  uint32_t tiles, ranges;
 };
 
+// Row tiles, and the ranges that the longest sequence's positions are divided into: two workgroups
+// for each place, as far as full tables hold so many.
 ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads, uint32_t head_size,
                        uint32_t* first_tile) {
   ChunkShape s{};
   const uint32_t group = q_heads / kv_heads;
-  const uint64_t all_rows = static_cast<uint64_t>(list.first[kMaxChunks]) * group * kv_heads;
-  s.groups = head_size == 128 && all_rows >= 2ull * kComputeUnits * rows_of(2) ? 2 : 1;
-  const uint32_t tile_rows = rows_of(s.groups);
   for (uint32_t i = 0; i < list.count; ++i) {
     first_tile[i] = s.tiles;
-    const uint64_t rows = static_cast<uint64_t>(list.first[i + 1] - list.first[i]) * group;
-    s.tiles += static_cast<uint32_t>((rows + tile_rows - 1) / tile_rows);
+    s.tiles += ((list.first[i + 1] - list.first[i]) * group + kRows - 1) / kRows;
   }
   for (uint32_t i = list.count; i <= kMaxChunks; ++i) first_tile[i] = s.tiles;
-  const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift;
-  const uint64_t places = (head_size == 128 && s.groups == 1 ? 2 : 1) * kComputeUnits, items = static_cast<uint64_t>(s.tiles) * kv_heads;
-  const uint64_t most = std::max<uint64_t>(1, capacity / (kTile * kLeastTiles));
-  s.splits = static_cast<uint32_t>(std::clamp<uint64_t>((places + items - 1) / items, 1, most));
+  const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift, items = static_cast<uint64_t>(s.tiles) * kv_heads;
+  const uint64_t places = (head_size == 128 ? kResident<128> : kResident<256>) * kComputeUnits;
+  const uint64_t most = std::max<uint64_t>(1, capacity / ((head_size == 128 ? kTile<128> : kTile<256>) * kLeastSteps));
+  s.ranges = static_cast<uint32_t>(std::clamp<uint64_t>((2 * places + items - 1) / items, 1, most));
   return s;
 }
 
+constexpr std::size_t kRangeWord = 256;  // bytes before the results
 std::size_t chunk_bytes(const ChunkShape& s, const ChunkList& list, uint32_t q_heads, uint32_t head_size) {
-  return s.splits == 1 ? 0 : static_cast<std::size_t>(list.first[kMaxChunks]) * q_heads * s.splits * (head_size + 2) * sizeof(float);
+  if (s.ranges == 1) return 0;
+  return kRangeWord + static_cast<std::size_t>(list.first[kMaxChunks]) * q_heads * s.ranges * (head_size + 2) * sizeof(float);
 }
 
 uint32_t weight_parts(const KvPages& p, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads, uint32_t& columns) {
@@ -649,8 +675,7 @@ extern "C" size_t gfxinfer_kv_pages_chunk_attention_workspace_bytes(const gfxinf
     // The slots do not matter here: every entry names the first one.
     const std::vector<uint32_t> any(std::min(count, kMaxChunks + 1), 0u);
     if (const int32_t s = read_chunks(a.pages, any.data(), tokens, count, false, a.list); s != GFXI_OK) return s;
-    const ChunkShape shape = chunk_shape(a.pages, a.list, q_heads, pages->kv_heads, pages->head_size, a.first_tile);
-    bytes = chunk_bytes(shape, a.list, q_heads, pages->head_size);
+    bytes = chunk_bytes(chunk_shape(a.pages, a.list, q_heads, pages->kv_heads, pages->head_size, a.first_tile), a.list, q_heads, pages->head_size);
     return GFXI_OK;
   });
   return bytes;
@@ -677,32 +702,32 @@ extern "C" int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pa
     if (need != 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need)) {
       return fail(GFXI_INVALID_ARGUMENT, "chunk attention workspace is null, not 16-byte aligned or too small");
     }
+    const uint64_t items = static_cast<uint64_t>(shape.tiles) * shape.ranges * kv_heads;
     const std::size_t rows = static_cast<std::size_t>(a.list.first[kMaxChunks]) * q_heads;
+    if (items > (1u << 30)) return fail(GFXI_INVALID_ARGUMENT, "chunk attention over too many rows for one launch");
     a.query = reinterpret_cast<const __half*>(query);
     a.gate = gate;
     a.output = reinterpret_cast<__half*>(output);
     a.log_sums = log_sums;
-    a.partial_o = workspace;
-    a.partial_ml = workspace == nullptr ? nullptr : workspace + rows * shape.splits * head_size;
+    if (need != 0) {
+      a.range = reinterpret_cast<uint32_t*>(workspace);
+      a.partial_o = workspace + kRangeWord / sizeof(float);
+      a.partial_ml = a.partial_o + rows * shape.ranges * head_size;
+    }
     a.layer = layer;
     a.q_heads = q_heads;
     a.kv_heads = kv_heads;
     a.group = q_heads / kv_heads;
-    a.splits = shape.splits;
-    a.tile_rows = rows_of(shape.groups);
+    a.ranges = shape.ranges;
     a.scale = kLog2E / std::sqrt(static_cast<float>(head_size));
-    const uint64_t items = static_cast<uint64_t>(shape.tiles) * shape.splits * kv_heads;
-    if (items > (1u << 30)) return fail(GFXI_INVALID_ARGUMENT, "chunk attention over too many rows for one launch");
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid(static_cast<unsigned>(items)), block(kWaves * 64);
-    if (head_size == 256) hipLaunchKernelGGL((chunk_attention_kernel<256, 1>), grid, block, 0, st, a);
-    else if (shape.groups == 1) hipLaunchKernelGGL((chunk_attention_kernel<128, 1>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((chunk_attention_kernel<128, 2>), grid, block, 0, st, a);
-    if (const int32_t s = launch_status("chunk attention launch failed"); s != GFXI_OK || shape.splits == 1) return s;
-    const dim3 combine(static_cast<unsigned>((rows + 3) / 4));
-    if (head_size == 128) hipLaunchKernelGGL(chunk_combine_kernel<128>, combine, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(chunk_combine_kernel<256>, combine, dim3(256), 0, st, a);
-    return launch_status("chunk attention combine launch failed");
+    const dim3 grid(static_cast<unsigned>(items)), block(kWaves * 64), join(static_cast<unsigned>((rows + 3) / 4));
+    if (head_size == 128) hipLaunchKernelGGL(chunk_attention_kernel<128>, grid, block, 0, st, a);
+    else hipLaunchKernelGGL(chunk_attention_kernel<256>, grid, block, 0, st, a);
+    if (const int32_t s = launch_status("chunk attention launch failed"); s != GFXI_OK || a.ranges == 1) return s;
+    if (head_size == 128) hipLaunchKernelGGL(chunk_join_kernel<128>, join, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(chunk_join_kernel<256>, join, dim3(256), 0, st, a);
+    return launch_status("chunk attention join launch failed");
   });
 }
 

@@ -745,8 +745,9 @@ size_t gfxinfer_kv_pages_chunk_attention_workspace_bytes(const gfxinfer_kv_pages
  * head row used, or NULL for no gate; output fp16 [rows][q_heads][hd]; log_sums fp32
  * [rows][q_heads], or NULL: the natural logarithm of the sum of exp(score) of a row, -inf for
  * a row that sees nothing (its output is zeros).  A position without a page is not seen.
- * The order of fp32 additions depends on the shape of the call (token counts, q_heads,
- * table_stride) and on the row's own position. */
+ * Where a row's positions are cut for different workgroups, and so the order of its fp32
+ * additions, depends on the token counts and lengths of all listed sequences: equal calls give
+ * equal bits, a row beside other sequences may differ in the last ones. */
 int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pages* pages, uint32_t layer, const uint16_t* query,
                                                  const float* gate, uint16_t* output, float* log_sums,
                                                  const uint32_t* sequences, const uint32_t* tokens, uint32_t count,

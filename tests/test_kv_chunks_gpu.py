@@ -271,17 +271,25 @@ def test_missing_pages_are_not_seen(device, gx, heads, page, wide):
 
 
 def test_one_sequence_several_times_and_orders(device, gx):
-    """A list may name a sequence twice; its order is the order of the rows."""
+    """A list may name a sequence twice; its order is the order of the rows; a call repeated gives the same bits."""
     rng = np.random.default_rng(14)
     c = Chunks(rng, A, 16, [333, 50], [6, 6])
     say("order of the list")
-    got, _ = c.run(gx)
-    c.query, c.gate = (np.concatenate([x[6:], x[:6]]) for x in (c.query, c.gate))
-    other, _ = c.run(gx, listed=[1, 0])
-    assert np.array_equal(other[6:], got[:6]) and np.array_equal(other[:6], got[6:])
-    c.query[:6], c.gate[:6] = c.query[6:], c.gate[6:]
-    twice, _ = c.run(gx, listed=[0, 0])
-    assert np.array_equal(twice[:6], twice[6:]) and np.array_equal(twice[:6], got[:6])
+    got, sums = c.run(gx)
+    c.check(got, sums)
+    again, again_sums = c.run(gx)
+    assert np.array_equal(got, again) and np.array_equal(sums, again_sums)
+    query, gate = c.query, c.gate
+    swapped = lambda x: np.concatenate([x[6:], x[:6]])  # noqa: E731
+    c.query, c.gate = swapped(query), swapped(gate)
+    other, other_sums = c.run(gx, listed=[1, 0])
+    c.query, c.gate = query, gate
+    c.check(swapped(other), swapped(other_sums))
+    c.query, c.gate = (np.concatenate([x[:6], x[:6]]) for x in (query, gate))
+    twice, twice_sums = c.run(gx, listed=[0, 0])
+    c.query, c.gate = query, gate
+    for half in (slice(0, 6), slice(6, 12)):
+        c.check(np.concatenate([twice[half], got[6:]]), np.concatenate([twice_sums[half], sums[6:]]))
 
 
 def test_offsets_past_32_bits(device, gx):
