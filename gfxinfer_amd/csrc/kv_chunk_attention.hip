@@ -59,43 +59,44 @@ struct ChunkAttnArgs {
   const float* gate;     // [rows][q_heads][2 D] or null
   __half* output;        // [rows][q_heads][D]
   float* log_sums;       // [rows][q_heads] or null
-  uint32_t* range;       // steps of a range, as the attention launch found it
   float* partial_o;      // [rows][q_heads][ranges][D], where positions are divided
-  float* partial_ml;     // [rows][q_heads][ranges][2]
+  float* partial_ml;     // [rows][q_heads][ranges][2]: maximum (-inf: the row has nothing there), sum
   uint32_t layer, q_heads, kv_heads, group, ranges;
   float scale;           // log2(e) / sqrt(D)
 };
 
-// The listed sequence a row tile (a row) belongs to: one round of loads of the list, no search.
-__device__ __forceinline__ uint32_t sequence_of(const uint32_t* first, uint32_t count, uint32_t x) {
-  if (count == 1) return 0;
-  const unsigned lane = threadIdx.x & 63u;
-  uint32_t found = 0;
-  for (uint32_t from = 0; from < count; from += 64) {
-    found += static_cast<uint32_t>(__popcll(__ballot(from + lane < count && first[min(from + lane, kMaxChunks)] <= x)));
-  }
-  return __builtin_amdgcn_readfirstlane(found) - 1;
-}
-
 // Steps a range holds at least, if there is more than one.
 constexpr uint32_t kLeastSteps = 2;
-// Ranges of equal length for all sequences: the longest one is divided into as many as the launch
-// allows, the others into as few as hold them.
+
+// The listed sequence of a row tile, and the steps of a range: ranges are of equal length for all
+// sequences, the longest one is divided into as many as the launch allows and the others into as few
+// as hold them.  The list and the lengths take one round of loads each, a lane a sequence.
+struct Listed {
+  uint32_t slot, length, first_row, tokens, first_tile, per;
+};
 template <unsigned D>
-__device__ __forceinline__ uint32_t range_steps(const ChunkAttnArgs& a) {
+__device__ __forceinline__ Listed find_listed(const ChunkAttnArgs& a, uint32_t row_tile) {
   const unsigned lane = threadIdx.x & 63u;
+  Listed found{};
   uint32_t most = 0;
   for (uint32_t from = 0; from < a.list.count; from += 64) {
-    const uint32_t i = from + lane;
-    if (i < a.list.count) {
-      const uint32_t length = min(a.pages.lengths[a.list.slot[i]], a.pages.stride << a.pages.page_shift);
-      most = max(most, length + (a.list.first[i + 1] - a.list.first[i]));
+    const uint32_t i = min(from + lane, a.list.count - 1);
+    const uint32_t slot = a.list.slot[i], row = a.list.first[i], tokens = a.list.first[i + 1] - row;
+    const uint32_t tile = a.first_tile[i], next_tile = a.first_tile[i + 1];
+    const uint32_t length = min(a.pages.lengths[slot], a.pages.stride << a.pages.page_shift);
+    most = max(most, length + tokens);
+    const uint64_t here = __ballot(from + lane < a.list.count && tile <= row_tile && row_tile < next_tile);
+    if (here != 0) {
+      const int at = __ffsll(static_cast<unsigned long long>(here)) - 1;
+      auto take = [&](uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), at)); };
+      found = Listed{take(slot), take(length), take(row), take(tokens), take(tile), 0};
     }
   }
 #pragma unroll
   for (unsigned d = 1; d < 64; d <<= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
   const uint32_t steps = (__builtin_amdgcn_readfirstlane(most) + kTile<D> - 1) / kTile<D>;
-  return max(kLeastSteps, (steps + a.ranges - 1) / a.ranges);
+  found.per = max(kLeastSteps, (steps + a.ranges - 1) / a.ranges);
+  return found;
 }
 
 __device__ __forceinline__ float max_over_halves(float v) {
@@ -107,6 +108,274 @@ __device__ __forceinline__ float sum_over_halves(float v) {
   const unsigned u = __float_as_uint(v);
   const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// What the waves of a workgroup need of a range of positions of one row tile.
+struct Range {
+  uint32_t slot, end, from, to, hk;  // steps [from, to)
+  uint32_t least;                    // positions that all rows see
+};
+
+// Where a lane's part of the first output tile of 16 V rows lies in LDS, in bytes; output tile d is at
+// the place ^ 64 d (see the attention kernel).
+template <unsigned D>
+__device__ __forceinline__ unsigned value_place_of(unsigned lane) {
+  const unsigned i16 = lane & 15u, vrow = 4 * (lane >> 5) + (i16 >> 2);
+  return vrow * (2 * D) + 16 * value_slot(2 * (lane >> 4 & 1u) + ((i16 & 3u) >> 1), vrow) + 8 * (i16 & 1u);
+}
+
+// Output tiles first .. first + 3 of 16 V rows in LDS, complete when they return.  (The compiler would let
+// reads of its own wait for the next block's loads into LDS, which it cannot tell from this block's.)
+template <unsigned D, unsigned Rows>
+__device__ __forceinline__ void read_tiles(unsigned place, unsigned first, h8 (&v)[4]) {
+  s16x4 x[8];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+      : "v"(place ^ 64 * first), "v"(place ^ 64 * (first + 1)), "v"(place ^ 64 * (first + 2)), "v"(place ^ 64 * (first + 3)),
+        "n"(Rows * 2 * D), "n"((Rows + 8) * 2 * D)
+      : "memory");
+#pragma unroll
+  for (unsigned d = 0; d < 4; ++d) {
+    v[d] = __builtin_bit_cast(h8, __builtin_shufflevector(x[2 * d], x[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+
+// A tile of at most 32 rows, as a decoding sequence has: all waves take the same rows and divide the
+// positions, blocks of 32 in turn.  K goes straight into registers, V through a part of LDS of the
+// wave's own, both a block ahead and without a barrier.  The waves' results meet in LDS at the end;
+// wave w leaves with output tiles w, w + 4 .. of all 32 rows in o[0], o[1] .., and with the rows'
+// maxima and sums.
+template <unsigned D>
+__device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& w, const h8 (&q)[D / 16], uint32_t visible,
+                                           _Float16* (&lds)[kWaves], f16v (&o)[D / 32], float& m, float& l) {
+  constexpr unsigned kBlock = 32, kLoadRows = 512 / D, kLoads = kBlock / kLoadRows;
+  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned n = lane & 31u, h = lane >> 5;
+  const KvPages& pg = a.pages;
+  const uint32_t in_page = (1u << pg.page_shift) - 1, row_bytes = 2 * pg.row;
+  const std::size_t layer_row = (static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) * pg.row + w.hk * D;
+  const __half* keys = pg.key + layer_row;
+  const __half* values = pg.value + layer_row;
+  _Float16* vs = wave == 0 ? lds[0] : wave == 1 ? lds[1] : wave == 2 ? lds[2] : lds[3];  // two blocks
+  const uint32_t load_row = lane / (D / 8);
+  const uint32_t value_part = load_row * row_bytes + 16 * value_slot(lane % (D / 8), load_row);
+  const unsigned value_place = lds_address(vs) + value_place_of<D>(lane);
+  const uint32_t first = w.from * kTile<D> / kBlock + wave, last = min(w.to * kTile<D>, w.end + kBlock - 1) / kBlock;
+  PageWindow window;
+  h8 k[D / 16];
+  int32_t page[2];  // of the block's halves, -1: none; these load from page 0 of the pool (always there)
+  // Block b's K rows into k, its V rows into the part `to`.
+  auto load = [&](uint32_t b, unsigned to) __attribute__((always_inline)) {
+    const uint32_t at = b * kBlock;
+#pragma unroll
+    for (unsigned e = 0; e < 2; ++e) page[e] = at + 16 * e < w.end ? window.find(pg, w.slot, (at + 16 * e) >> pg.page_shift) : -1;
+    const uint32_t p = static_cast<uint32_t>(max(n < 16 ? page[0] : page[1], 0));
+    const __half* row = keys + ((static_cast<std::size_t>(p) << pg.page_shift) + ((at + n) & in_page)) * pg.row + 8 * h;
+#pragma unroll
+    for (unsigned st = 0; st < D / 16; ++st) k[st] = *reinterpret_cast<const h8*>(row + 16 * st);
+#pragma unroll
+    for (unsigned u = 0; u < kLoads; ++u) {
+      const unsigned row0 = kLoadRows * u, e = row0 / 16;
+      const std::size_t base = ((static_cast<std::size_t>(max(page[e], 0)) << pg.page_shift) + ((at + 16 * e) & in_page)) * pg.row;
+      const auto rows16 = __builtin_amdgcn_make_buffer_rsrc(const_cast<__half*>(values + base), 0, static_cast<int>(15 * row_bytes + 2 * D), 0x20000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rows16, (lds_void*)(vs + (to * kBlock + row0) * D), 16, static_cast<int>(value_part ^ 32 * (row0 & 7u)),
+                                               static_cast<int>((row0 & 15u) * row_bytes), 0, 0);
+    }
+  };
+  bool careful = false, strange;
+#pragma unroll 1
+  for (;; careful = true) {
+    m = -INFINITY;
+    l = 0.0F;
+#pragma unroll
+    for (unsigned d = 0; d < D / 32; ++d) o[d] = f16v{};
+    window.start(pg, w.slot, first * kBlock >> pg.page_shift);
+    if (first < last) load(first, 0);
+    unsigned in = 0;
+#pragma unroll 1
+    for (uint32_t b = first; b < last; b += kWaves, in ^= 1) {
+      const uint32_t at = b * kBlock;
+      const int32_t here[2] = {page[0], page[1]};
+      f16v s = {};
+#pragma unroll
+      for (unsigned st = 0; st < D / 16; ++st) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[st], q[st], s, 0, 0, 0);
+      const bool more = b + kWaves < last;
+      if (more) load(b + kWaves, in ^ 1);
+      if (at + kBlock > w.least || here[0] < 0 || here[1] < 0) {
+#pragma unroll
+        for (unsigned r = 0; r < 16; ++r) {
+          if (at + 8 * (r / 4) + 4 * h + r % 4 >= visible || here[r / 8] < 0) s[r] = -INFINITY;
+        }
+      }
+      float best = s[0];
+#pragma unroll
+      for (unsigned r = 1; r < 16; ++r) best = __builtin_elementwise_maximum(best, s[r]);
+      const float top = max_over_halves(best) * a.scale;
+      if (__any(!(top <= m + kRise))) {
+        const float next = top <= m + kRise ? m : top;
+        const float factor = next == m || m == -INFINITY ? 1.0F : rescale_factor(m, next);
+        m = next;
+        l *= factor;
+#pragma unroll
+        for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+          for (unsigned r = 0; r < 16; ++r) o[d][r] *= factor;
+        }
+      }
+      const float floor = m == -INFINITY ? 0.0F : m - kLift;
+      h8 p[2];
+#pragma unroll
+      for (unsigned r = 0; r < 16; ++r) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale, -floor));
+        l += x;
+        p[r / 8][r % 8] = static_cast<_Float16>(x);
+      }
+      // The block's V rows are there when only the next block's loads are on their way.
+      if (more) wait_loads<D / 16 + kLoads>();
+      else wait_loads<0>();
+      if (careful || at + kBlock > w.end || here[0] < 0 || here[1] < 0) {  // as in the attention kernel
+#pragma unroll 1
+        for (unsigned u = 0; u < kLoads; ++u) {
+          const unsigned row0 = kLoadRows * u;
+          u32x4* piece = reinterpret_cast<u32x4*>(vs + (in * kBlock + row0) * D) + lane;
+          if (at + row0 + load_row >= w.end || (row0 < 16 ? here[0] : here[1]) < 0) *piece = u32x4{0, 0, 0, 0};
+          if (careful) take_strange(piece);
+        }
+        wait_loads<63>();
+      }
+      const unsigned place = value_place + in * (kBlock * 2 * D);
+#pragma unroll
+      for (unsigned d = 0; d < D / 32; d += 4) {
+        h8 v[4];
+        read_tiles<D, 0>(place, d, v);
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) o[d + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[e], p[0], o[d + e], 0, 0, 0);
+        read_tiles<D, 16>(place, d, v);
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) o[d + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[e], p[1], o[d + e], 0, 0, 0);
+      }
+      if (careful) {
+        // The rows that see an infinity or NaN among the values get it, whatever the weight.
+#pragma unroll 1
+        for (unsigned x = 0; x < kBlock; ++x) {
+          const int32_t one = x < 16 ? here[0] : here[1];
+          if (at + x >= w.end || one < 0) continue;
+          const __half* v = values + ((static_cast<std::size_t>(one) << pg.page_shift) + ((at + x) & in_page)) * pg.row;
+#pragma unroll
+          for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+            for (unsigned r = 0; r < 16; ++r) {
+              const float y = __half2float(v[32 * d + 8 * (r / 4) + 4 * h + r % 4]);
+              if (!(fabsf(y) < INFINITY) && at + x < visible) o[d][r] += y;
+              asm volatile("" ::: "memory");
+            }
+          }
+        }
+      }
+    }
+    strange = false;
+#pragma unroll
+    for (unsigned d = 0; d < D / 32; ++d) {
+#pragma unroll
+      for (unsigned r = 0; r < 16; ++r) strange |= !(fabsf(o[d][r]) < INFINITY);
+    }
+    if (careful || !__any(strange)) break;
+  }
+  l = sum_over_halves(l);
+  if ((m == -INFINITY && (l != l || (careful && strange))) || m != m) m = 0.0F;
+  // The waves' results, four output tiles at a time.
+  float2* ml = reinterpret_cast<float2*>(lds[0]);  // [waves][32], once V is no longer needed
+  __syncthreads();
+  if (h == 0) ml[wave * 32 + n] = float2{m, l};
+  __syncthreads();
+  float2 part[kWaves];
+  float all = -INFINITY, total = 0.0F, factor[kWaves];
+#pragma unroll
+  for (unsigned v = 0; v < kWaves; ++v) {
+    part[v] = ml[v * 32 + n];
+    all = fmaxf(all, part[v].x);
+  }
+#pragma unroll
+  for (unsigned v = 0; v < kWaves; ++v) {
+    factor[v] = part[v].x == -INFINITY ? 0.0F : rescale_factor(part[v].x, all);
+    if (part[v].x != -INFINITY) total += part[v].y * factor[v];
+  }
+  m = all;
+  l = total;
+  f16v sum[D / 128];
+#pragma unroll
+  for (unsigned g = 0; g < D / 128; ++g) {
+    __syncthreads();
+    f4* mine = reinterpret_cast<f4*>(vs);
+#pragma unroll
+    for (unsigned d = 0; d < 4; ++d) {
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) mine[(4 * d + e) * 64 + lane] = f4{o[4 * g + d][4 * e], o[4 * g + d][4 * e + 1], o[4 * g + d][4 * e + 2], o[4 * g + d][4 * e + 3]};
+    }
+    __syncthreads();
+    sum[g] = f16v{};
+#pragma unroll
+    for (unsigned v = 0; v < kWaves; ++v) {
+      const f4* other = reinterpret_cast<const f4*>(lds[v]);
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) {
+        const f4 x = other[(4 * wave + e) * 64 + lane];
+#pragma unroll
+        for (unsigned c = 0; c < 4; ++c) {
+          if (factor[v] != 0.0F) sum[g][4 * e + c] += x[c] * factor[v];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (unsigned g = 0; g < D / 128; ++g) o[g] = sum[g];
+}
+
+// Output tiles of a row: a range's part, or the row itself with the gate applied.  o[i] is output tile
+// first + i * step.
+template <unsigned D, unsigned N>
+__device__ __forceinline__ void write_row(const ChunkAttnArgs& a, uint32_t out_row, uint32_t range, const f16v* o, unsigned first,
+                                          unsigned step, float m, float l, bool sums) {
+  const unsigned h = (threadIdx.x & 63u) >> 5;
+  if (a.ranges > 1) {
+    const std::size_t at = static_cast<std::size_t>(out_row) * a.ranges + range;
+#pragma unroll
+    for (unsigned i = 0; i < N; ++i) {
+#pragma unroll
+      for (unsigned r = 0; r < 16; r += 4) {
+        *reinterpret_cast<f4*>(a.partial_o + at * D + 32 * (first + i * step) + 2 * r + 4 * h) = f4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+      }
+    }
+    if (sums) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{m, l};
+    return;
+  }
+  const bool empty = m == -INFINITY;
+  const float inverse = empty ? 0.0F : 1.0F / l;
+#pragma unroll
+  for (unsigned i = 0; i < N; ++i) {
+#pragma unroll
+    for (unsigned r = 0; r < 16; r += 4) {
+      const unsigned at = 32 * (first + i * step) + 2 * r + 4 * h;
+      f4 y;
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) y[e] = empty ? 0.0F : o[i][r + e] * inverse;
+      if (a.gate != nullptr) {
+        const f4 gate = *reinterpret_cast<const f4*>(a.gate + static_cast<std::size_t>(out_row) * 2 * D + D + at);
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) y[e] *= 1.0F / (1.0F + expf(-gate[e]));
+      }
+      h4 out;
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) out[e] = static_cast<_Float16>(y[e]);
+      *reinterpret_cast<h4*>(a.output + static_cast<std::size_t>(out_row) * D + at) = out;
+    }
+  }
+  if (a.log_sums != nullptr && sums) a.log_sums[out_row] = empty ? -INFINITY : (m - kLift) * kLn2 + logf(l);
 }
 
 // Sixteen-position parts of a tile: their pages, -1 where there is none.
@@ -121,10 +390,12 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   constexpr unsigned T = kTile<D>, kSub = T / 32, kSteps = T / 16;
   constexpr unsigned kLoadRows = 512 / D;                   // rows a load of a wave covers
   constexpr unsigned kLoads = T / kLoadRows / kWaves;       // of K, and of V, per tile and wave
-  __shared__ __align__(1024) _Float16 k0[T * D];
-  __shared__ __align__(1024) _Float16 k1[T * D];
-  __shared__ __align__(1024) _Float16 v0[T * D];
-  __shared__ __align__(1024) _Float16 v1[T * D];
+  // Two tiles of K and of V; with few rows two blocks of V of a wave each.
+  constexpr unsigned kPart = T * D > 2 * 32 * D ? T * D : 2 * 32 * D;
+  __shared__ __align__(1024) _Float16 k0[kPart];
+  __shared__ __align__(1024) _Float16 k1[kPart];
+  __shared__ __align__(1024) _Float16 v0[kPart];
+  __shared__ __align__(1024) _Float16 v1[kPart];
   __shared__ uint32_t again[kWaves];       // the wave's rows met an infinity or NaN
   __shared__ uint32_t strange_tiles[32];   // bit x % 1024: a tile x holds infinities or NaNs among its values
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -134,22 +405,25 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   // read the same positions run together; late tokens, which see most, first.
   const uint32_t hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
   const uint32_t tiles = a.first_tile[kMaxChunks], range = rest / tiles, row_tile = tiles - 1 - rest % tiles;
-  const uint32_t i = sequence_of(a.first_tile, a.list.count, row_tile);
-  const uint32_t slot = listed_slot(a.list, i), first_row = a.list.first[i], tokens = a.list.first[i + 1] - first_row;
-  uint32_t per = 0xffffffffu;
-  if (a.ranges > 1) {
-    per = range_steps<D>(a);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.range = per;
-  }
-  const uint32_t length = committed(pg, slot), rows = tokens * a.group;
-  const uint32_t tile_row = (row_tile - a.first_tile[i]) * kRows;
+  const Listed listed = find_listed<D>(a, row_tile);
+  const uint32_t slot = listed.slot, first_row = listed.first_row, tokens = listed.tokens, length = listed.length;
+  const uint32_t rows = tokens * a.group, tile_row = (row_tile - listed.first_tile) * kRows;
   // The tile's last row sees this many positions; what lies behind the sequence's end is not read.
   const uint32_t last_row = min(rows, tile_row + kRows) - 1;
   const uint32_t end = length + tokens, steps = (length + last_row / a.group + T) / T;
-  const uint32_t from = a.ranges > 1 ? range * per : 0u, to = a.ranges > 1 ? min(from + per, steps) : steps;
-  if (from >= steps) return;
+  const uint32_t from = a.ranges > 1 ? range * listed.per : 0u, to = a.ranges > 1 ? min(from + listed.per, steps) : steps;
+  if (from >= steps) {  // (there is more than one range)
+    const uint32_t row = tile_row + threadIdx.x;
+    if (threadIdx.x < kRows && row < rows) {
+      const std::size_t at = (static_cast<std::size_t>(first_row + row / a.group) * a.q_heads + hk * a.group + row % a.group) * a.ranges + range;
+      *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{-INFINITY, 0.0F};
+    }
+    return;
+  }
 
-  const uint32_t wave_row = tile_row + wave * 32, row = wave_row + n;
+  // With few rows all waves take the same ones and divide the positions.
+  const bool few = min(rows, tile_row + kRows) - tile_row <= 32;
+  const uint32_t wave_row = few ? tile_row : tile_row + wave * 32, row = wave_row + n;
   const bool works = wave_row < rows;                        // the wave has a row
   const uint32_t least_visible = length + wave_row / a.group + 1;
   const uint32_t visible = row < rows ? length + row / a.group + 1 : 0;
@@ -162,13 +436,19 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
     if (row < rows) q[st] = *reinterpret_cast<const h8*>(a.query + static_cast<std::size_t>(out_row) * D + 16 * st + 8 * h);
     if constexpr (D == 256) asm volatile("" : "+a"(q[st]));
   }
-
+  f16v o[D / 32];
+  float m, l;
+  if (few) {
+    _Float16* lds[kWaves] = {k0, k1, v0, v1};
+    attend_few<D>(a, Range{slot, end, from, to, hk, least_visible}, q, visible, lds, o, m, l);
+    if (out_row != 0xffffffffu) write_row<D, D / 128>(a, out_row, range, o, wave, 4, m, l, wave == 0 && h == 0);
+    return;
+  }
   const std::size_t layer_row = (static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) * pg.row + hk * D;
   const __half* keys = pg.key + layer_row;
   const __half* values = pg.value + layer_row;
   const uint32_t in_page = (1u << pg.page_shift) - 1;
-  f16v o[D / 32], s[kSub], s_next[kSub];
-  float m, l;
+  f16v s[kSub], s_next[kSub];
   PageWindow window;
   auto find_pages = [&](uint32_t x) __attribute__((always_inline)) {
     TilePages<D> p;
@@ -208,9 +488,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   // Where the lane's part of the first score operand of 32 K rows, and of the first output tile of
   // 16 V rows, lies in bytes.  Operand s is at the place ^ 32 s, output tile d at the place ^ 64 d:
   // the slots of a row are permuted by exclusive or, and rows start at multiples of their size.
-  const unsigned i16 = lane & 15u, vrow = 4 * h + (i16 >> 2);
-  const unsigned key_place = n * (2 * D) + 16 * key_slot(h, n);
-  const unsigned value_place = vrow * (2 * D) + 16 * value_slot(2 * (lane >> 4 & 1u) + ((i16 & 3u) >> 1), vrow) + 8 * (i16 & 1u);
+  const unsigned key_place = n * (2 * D) + 16 * key_slot(h, n), value_place = value_place_of<D>(lane);
 
   // What a page holds past a sequence's end, and what a missing one would, may be anything, and 0 * NaN
   // is NaN: the wave's own V rows of such positions become zeros.  A careful pass also takes out
@@ -421,88 +699,67 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   l = sum_over_halves(l);
   // Only NaN scores, and strange values at scores of -infinity, make a NaN row rather than an empty one.
   if ((m == -INFINITY && (l != l || (careful && strange))) || m != m) m = 0.0F;
-  if (out_row == 0xffffffffu) return;
-  if (a.ranges > 1) {
-    const std::size_t at = static_cast<std::size_t>(out_row) * a.ranges + range;
-#pragma unroll
-    for (unsigned d = 0; d < D / 32; ++d) {
-#pragma unroll
-      for (unsigned r = 0; r < 16; r += 4) {
-        *reinterpret_cast<f4*>(a.partial_o + at * D + 32 * d + 2 * r + 4 * h) = f4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
-      }
-    }
-    if (h == 0) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{m, l};
-    return;
-  }
-  const bool empty = m == -INFINITY;
-  const float inverse = empty ? 0.0F : 1.0F / l;
-#pragma unroll
-  for (unsigned d = 0; d < D / 32; ++d) {
-#pragma unroll
-    for (unsigned r = 0; r < 16; r += 4) {
-      const unsigned at = 32 * d + 2 * r + 4 * h;
-      f4 y;
-#pragma unroll
-      for (unsigned e = 0; e < 4; ++e) y[e] = empty ? 0.0F : o[d][r + e] * inverse;
-      if (a.gate != nullptr) {
-        const f4 gate = *reinterpret_cast<const f4*>(a.gate + static_cast<std::size_t>(out_row) * 2 * D + D + at);
-#pragma unroll
-        for (unsigned e = 0; e < 4; ++e) y[e] *= 1.0F / (1.0F + expf(-gate[e]));
-      }
-      h4 out;
-#pragma unroll
-      for (unsigned e = 0; e < 4; ++e) out[e] = static_cast<_Float16>(y[e]);
-      *reinterpret_cast<h4*>(a.output + static_cast<std::size_t>(out_row) * D + at) = out;
-    }
-  }
-  if (a.log_sums != nullptr && h == 0) a.log_sums[out_row] = empty ? -INFINITY : (m - kLift) * kLn2 + logf(l);
+  if (out_row != 0xffffffffu) write_row<D, D / 32>(a, out_row, range, o, 0, 1, m, l, h == 0);
 }
 
 // Joins the ranges of a row and applies the gate: a wave per row and query head, D / 64 dims a lane.
+// Lane r holds range r's maximum and sum; the outputs of the first two ranges are loaded beside them.
 template <unsigned D>
-__global__ __launch_bounds__(256) void chunk_join_kernel(ChunkAttnArgs a) {
+__global__ __launch_bounds__(256) void chunk_join_kernel(ChunkAttnArgs a, uint32_t rows) {
   constexpr unsigned J = D / 64;
   using vec = float __attribute__((ext_vector_type(J)));
   using hvec = _Float16 __attribute__((ext_vector_type(J)));
   const unsigned lane = threadIdx.x & 63u;
-  const uint32_t linear = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
-  if (linear >= a.list.first[kMaxChunks] * a.q_heads) return;
-  const uint32_t row = linear / a.q_heads, i = sequence_of(a.list.first, a.list.count, row);
-  const std::size_t base = static_cast<std::size_t>(linear) * a.ranges;
+  const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
+  if (row >= rows) return;
+  const std::size_t base = static_cast<std::size_t>(row) * a.ranges;
+  const float* parts = a.partial_o + base * D + J * lane;
   vec g = {};
-  if (a.gate != nullptr) g = *reinterpret_cast<const vec*>(a.gate + static_cast<std::size_t>(linear) * 2 * D + D + J * lane);
-  const uint32_t slot = listed_slot(a.list, i), tokens = a.list.first[i + 1] - a.list.first[i], t = row - a.list.first[i];
-  const uint32_t tile_row = (t * a.group + linear % a.q_heads % a.group) / kRows * kRows;
-  const uint32_t last_row = min(tokens * a.group, tile_row + kRows) - 1;
-  const uint32_t steps = (committed(a.pages, slot) + last_row / a.group + kTile<D>) / kTile<D>, per = *a.range;
-  const uint32_t used = (steps + per - 1) / per;
+  if (a.gate != nullptr) g = *reinterpret_cast<const vec*>(a.gate + static_cast<std::size_t>(row) * 2 * D + D + J * lane);
+  const vec first[2] = {*reinterpret_cast<const vec*>(parts), *reinterpret_cast<const vec*>(parts + D)};
   float best = -INFINITY, sum = 0.0F;
   vec y = {};
-  for (uint32_t r = 0; r < used; ++r) {
-    const float2 x = *reinterpret_cast<const float2*>(a.partial_ml + 2 * (base + r));
-    const vec o = *reinterpret_cast<const vec*>(a.partial_o + (base + r) * D + J * lane);
-    if (x.x == -INFINITY) continue;
-    const float next = fmaxf(best, x.x), w = rescale_factor(x.x, next);
-    if (best == -INFINITY) {
-      sum = x.y * w;
-      y = o * w;
-    } else {
+  for (uint32_t from = 0; from < a.ranges; from += 64) {
+    const uint32_t here = min(64u, a.ranges - from);
+    float2 x = {-INFINITY, 0.0F};
+    if (lane < here) x = *reinterpret_cast<const float2*>(a.partial_ml + 2 * (base + from + lane));
+    const float next = fmaxf(best, wave_max(x.x));
+    if (next == -INFINITY) continue;
+    const float w = x.x == -INFINITY ? 0.0F : rescale_factor(x.x, next);
+    if (best != -INFINITY) {
       const float keep = rescale_factor(best, next);
-      sum = sum * keep + x.y * w;
-      y = y * keep + o * w;
+      sum *= keep;
+      y *= keep;
     }
     best = next;
+    sum += wave_sum(w == 0.0F ? 0.0F : x.y * w);
+    for (uint64_t left = __ballot(w != 0.0F); left != 0;) {
+      constexpr unsigned kBatch = 4;
+      vec v[kBatch];
+      float wv[kBatch];
+#pragma unroll
+      for (unsigned e = 0; e < kBatch; ++e) {
+        const int r = left != 0 ? __ffsll(static_cast<unsigned long long>(left)) - 1 : -1;
+        wv[e] = r < 0 ? 0.0F : lane_value(w, r);
+        left &= left - 1;
+        if (r < 0) v[e] = vec{};
+        else if (from + r < 2) v[e] = r == 0 ? first[0] : first[1];
+        else v[e] = *reinterpret_cast<const vec*>(parts + static_cast<std::size_t>(from + r) * D);
+      }
+#pragma unroll
+      for (unsigned e = 0; e < kBatch; ++e) y += v[e] * wv[e];
+    }
   }
   const bool empty = best == -INFINITY;
   hvec out;
 #pragma unroll
   for (unsigned j = 0; j < J; ++j) {
-    float v = empty ? 0.0F : y[j] / sum;
-    if (a.gate != nullptr) v *= 1.0F / (1.0F + expf(-g[j]));
-    out[j] = static_cast<_Float16>(v);
+    float z = empty ? 0.0F : y[j] / sum;
+    if (a.gate != nullptr) z *= 1.0F / (1.0F + expf(-g[j]));
+    out[j] = static_cast<_Float16>(z);
   }
-  *reinterpret_cast<hvec*>(a.output + static_cast<std::size_t>(linear) * D + J * lane) = out;
-  if (a.log_sums != nullptr && lane == 0) a.log_sums[linear] = empty ? -INFINITY : (best - kLift) * kLn2 + logf(sum);
+  *reinterpret_cast<hvec*>(a.output + static_cast<std::size_t>(row) * D + J * lane) = out;
+  if (a.log_sums != nullptr && lane == 0) a.log_sums[row] = empty ? -INFINITY : (best - kLift) * kLn2 + logf(sum);
 }
 
 // ---- the weight that each position receives ---------------------------------------------
@@ -636,14 +893,13 @@ ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads
   const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift, items = static_cast<uint64_t>(s.tiles) * kv_heads;
   const uint64_t places = (head_size == 128 ? kResident<128> : kResident<256>) * kComputeUnits;
   const uint64_t most = std::max<uint64_t>(1, capacity / ((head_size == 128 ? kTile<128> : kTile<256>) * kLeastSteps));
-  s.ranges = static_cast<uint32_t>(std::clamp<uint64_t>((2 * places + items - 1) / items, 1, most));
+  s.ranges = static_cast<uint32_t>(std::clamp<uint64_t>((places * (head_size == 128 ? 3 : 4) / 2 + items - 1) / items, 1, most));
   return s;
 }
 
-constexpr std::size_t kRangeWord = 256;  // bytes before the results
 std::size_t chunk_bytes(const ChunkShape& s, const ChunkList& list, uint32_t q_heads, uint32_t head_size) {
   if (s.ranges == 1) return 0;
-  return kRangeWord + static_cast<std::size_t>(list.first[kMaxChunks]) * q_heads * s.ranges * (head_size + 2) * sizeof(float);
+  return static_cast<std::size_t>(list.first[kMaxChunks]) * q_heads * s.ranges * (head_size + 2) * sizeof(float);
 }
 
 uint32_t weight_parts(const KvPages& p, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads, uint32_t& columns) {
@@ -710,8 +966,7 @@ extern "C" int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pa
     a.output = reinterpret_cast<__half*>(output);
     a.log_sums = log_sums;
     if (need != 0) {
-      a.range = reinterpret_cast<uint32_t*>(workspace);
-      a.partial_o = workspace + kRangeWord / sizeof(float);
+      a.partial_o = workspace;
       a.partial_ml = a.partial_o + rows * shape.ranges * head_size;
     }
     a.layer = layer;
@@ -725,8 +980,8 @@ extern "C" int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pa
     if (head_size == 128) hipLaunchKernelGGL(chunk_attention_kernel<128>, grid, block, 0, st, a);
     else hipLaunchKernelGGL(chunk_attention_kernel<256>, grid, block, 0, st, a);
     if (const int32_t s = launch_status("chunk attention launch failed"); s != GFXI_OK || a.ranges == 1) return s;
-    if (head_size == 128) hipLaunchKernelGGL(chunk_join_kernel<128>, join, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(chunk_join_kernel<256>, join, dim3(256), 0, st, a);
+    if (head_size == 128) hipLaunchKernelGGL(chunk_join_kernel<128>, join, dim3(256), 0, st, a, static_cast<uint32_t>(rows));
+    else hipLaunchKernelGGL(chunk_join_kernel<256>, join, dim3(256), 0, st, a, static_cast<uint32_t>(rows));
     return launch_status("chunk attention join launch failed");
   });
 }
