@@ -51,6 +51,8 @@ constexpr unsigned kResident = D == 128 ? 2 : 1;
 // counted: the one rounding of the weights is half the size of the output's own.
 constexpr float kLift = 11.0F, kRise = 4.0F;
 
+constexpr float kWritten = -1.0F;  // in the place of range 0's sum: the row is complete, nothing to join
+
 struct ChunkAttnArgs {
   KvPages pages;
   ChunkList list;
@@ -95,7 +97,7 @@ __device__ __forceinline__ Listed find_listed(const ChunkAttnArgs& a, uint32_t r
 #pragma unroll
   for (unsigned d = 1; d < 64; d <<= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
   const uint32_t steps = (__builtin_amdgcn_readfirstlane(most) + kTile<D> - 1) / kTile<D>;
-  found.per = max(kLeastSteps, (steps + a.ranges - 1) / a.ranges);
+  found.per = a.ranges == 1 ? 0xffffffu : max(kLeastSteps, (steps + a.ranges - 1) / a.ranges);
   return found;
 }
 
@@ -336,14 +338,14 @@ __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& 
   for (unsigned g = 0; g < D / 128; ++g) o[g] = sum[g];
 }
 
-// Output tiles of a row: a range's part, or the row itself with the gate applied.  o[i] is output tile
-// first + i * step.
+// Output tiles of a row: a range's part, or, where one range holds all positions, the row itself with
+// the gate applied.  o[i] is output tile first + i * step.
 template <unsigned D, unsigned N>
-__device__ __forceinline__ void write_row(const ChunkAttnArgs& a, uint32_t out_row, uint32_t range, const f16v* o, unsigned first,
-                                          unsigned step, float m, float l, bool sums) {
+__device__ __forceinline__ void write_row(const ChunkAttnArgs& a, uint32_t out_row, uint32_t range, bool whole, const f16v* o,
+                                          unsigned first, unsigned step, float m, float l, bool sums) {
   const unsigned h = (threadIdx.x & 63u) >> 5;
-  if (a.ranges > 1) {
-    const std::size_t at = static_cast<std::size_t>(out_row) * a.ranges + range;
+  const std::size_t at = static_cast<std::size_t>(out_row) * a.ranges + range;
+  if (!whole) {
 #pragma unroll
     for (unsigned i = 0; i < N; ++i) {
 #pragma unroll
@@ -375,7 +377,8 @@ __device__ __forceinline__ void write_row(const ChunkAttnArgs& a, uint32_t out_r
       *reinterpret_cast<h4*>(a.output + static_cast<std::size_t>(out_row) * D + at) = out;
     }
   }
-  if (a.log_sums != nullptr && sums) a.log_sums[out_row] = empty ? -INFINITY : (m - kLift) * kLn2 + logf(l);
+  if (sums && a.ranges > 1) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{0.0F, kWritten};
+  if (sums && a.log_sums != nullptr) a.log_sums[out_row] = empty ? -INFINITY : (m - kLift) * kLn2 + logf(l);
 }
 
 // Sixteen-position parts of a tile: their pages, -1 where there is none.
@@ -411,8 +414,10 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   // The tile's last row sees this many positions; what lies behind the sequence's end is not read.
   const uint32_t last_row = min(rows, tile_row + kRows) - 1;
   const uint32_t end = length + tokens, steps = (length + last_row / a.group + T) / T;
-  const uint32_t from = a.ranges > 1 ? range * listed.per : 0u, to = a.ranges > 1 ? min(from + listed.per, steps) : steps;
-  if (from >= steps) {  // (there is more than one range)
+  // As few ranges as hold them, of equal length.
+  const uint32_t used = (steps - 1) / listed.per + 1, per = (steps + used - 1) / used;
+  const uint32_t from = range * per, to = min(from + per, steps);
+  if (from >= steps) {
     const uint32_t row = tile_row + threadIdx.x;
     if (threadIdx.x < kRows && row < rows) {
       const std::size_t at = (static_cast<std::size_t>(first_row + row / a.group) * a.q_heads + hk * a.group + row % a.group) * a.ranges + range;
@@ -440,8 +445,10 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   float m, l;
   if (few) {
     _Float16* lds[kWaves] = {k0, k1, v0, v1};
+    // (Few rows are left to the join even if one range holds them: its waves divide the gate among more
+    // lanes, eight decoding sequences 12.9 us, not 14.4.)
     attend_few<D>(a, Range{slot, end, from, to, hk, least_visible}, q, visible, lds, o, m, l);
-    if (out_row != 0xffffffffu) write_row<D, D / 128>(a, out_row, range, o, wave, 4, m, l, wave == 0 && h == 0);
+    if (out_row != 0xffffffffu) write_row<D, D / 128>(a, out_row, range, a.ranges == 1, o, wave, 4, m, l, wave == 0 && h == 0);
     return;
   }
   const std::size_t layer_row = (static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) * pg.row + hk * D;
@@ -699,8 +706,10 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   l = sum_over_halves(l);
   // Only NaN scores, and strange values at scores of -infinity, make a NaN row rather than an empty one.
   if ((m == -INFINITY && (l != l || (careful && strange))) || m != m) m = 0.0F;
-  if (out_row != 0xffffffffu) write_row<D, D / 32>(a, out_row, range, o, 0, 1, m, l, h == 0);
+  if (out_row != 0xffffffffu) write_row<D, D / 32>(a, out_row, range, used == 1, o, 0, 1, m, l, h == 0);
 }
+
+constexpr uint32_t kJoinRows = 4096;
 
 // Joins the ranges of a row and applies the gate: a wave per row and query head, D / 64 dims a lane.
 // Lane r holds range r's maximum and sum; the outputs of the first two ranges are loaded beside them.
@@ -714,6 +723,8 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkAttnArgs a, uint32
   if (row >= rows) return;
   const std::size_t base = static_cast<std::size_t>(row) * a.ranges;
   const float* parts = a.partial_o + base * D + J * lane;
+  // Many rows: complete ones are not worth the loads that cover the look.
+  if (rows > kJoinRows && __builtin_amdgcn_readfirstlane(__float_as_int(a.partial_ml[2 * base + 1])) == __float_as_int(kWritten)) return;
   vec g = {};
   if (a.gate != nullptr) g = *reinterpret_cast<const vec*>(a.gate + static_cast<std::size_t>(row) * 2 * D + D + J * lane);
   const vec first[2] = {*reinterpret_cast<const vec*>(parts), *reinterpret_cast<const vec*>(parts + D)};
@@ -723,6 +734,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkAttnArgs a, uint32
     const uint32_t here = min(64u, a.ranges - from);
     float2 x = {-INFINITY, 0.0F};
     if (lane < here) x = *reinterpret_cast<const float2*>(a.partial_ml + 2 * (base + from + lane));
+    if (from == 0 && lane_value(x.y, 0) == kWritten) return;
     const float next = fmaxf(best, wave_max(x.x));
     if (next == -INFINITY) continue;
     const float w = x.x == -INFINITY ? 0.0F : rescale_factor(x.x, next);
