@@ -19,12 +19,12 @@ namespace gfx950 {
 namespace {
 
 using i32x4 = int __attribute__((ext_vector_type(4)));
+using i32x16 = int __attribute__((ext_vector_type(16)));
 using u32x4 = unsigned __attribute__((ext_vector_type(4)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
 using h16x4 = _Float16 __attribute__((ext_vector_type(4)));
 using h16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using lds_void = __attribute__((address_space(3))) void;
-using global_void = __attribute__((address_space(1))) void;
 
 // ---- quantizer -------------------------------------------------------------------------
 
@@ -55,7 +55,7 @@ __device__ __forceinline__ void load8(const void* input, std::size_t at, float (
 
 // rint of the exact quotient: where the rounded quotient is a half, the sign of the remainder
 // says on which side of it the exact one lies (zero: on it, and ties go to even).
-__device__ __forceinline__ int code_of(float x, float scale) {
+__device__ __forceinline__ float exact_code(float x, float scale) {
   const float q = x / scale;
   float c = rintf(q);
   if (fabsf(q - truncf(q)) == 0.5F) {
@@ -63,7 +63,30 @@ __device__ __forceinline__ int code_of(float x, float scale) {
     if (rest > 0.0F) c = ceilf(q);
     if (rest < 0.0F) c = floorf(q);
   }
-  return static_cast<int>(fminf(fmaxf(c, -127.0F), 127.0F));
+  return c;
+}
+
+// Four codes.  x times the reciprocal is within 2^-16 of the quotient (two roundings of numbers below
+// 127.1), so only where it lies that close to a half the quotient is needed: one code in 30000.
+__device__ __forceinline__ uint32_t four_codes(const float (&x)[8], unsigned first, float scale, float inverse) {
+  float c[4];
+  bool close = false;
+#pragma unroll
+  for (unsigned e = 0; e < 4; ++e) {
+    const float q = x[first + e] * inverse;
+    c[e] = rintf(q);
+    close |= fabsf(q - c[e]) > 0.5F - 0x1p-15F;
+  }
+  if (close) {
+#pragma unroll
+    for (unsigned e = 0; e < 4; ++e) c[e] = exact_code(x[first + e], scale);
+  }
+  uint32_t packed = 0;
+#pragma unroll
+  for (unsigned e = 0; e < 4; ++e) {
+    packed |= (static_cast<uint32_t>(static_cast<int>(__builtin_amdgcn_fmed3f(c[e], -127.0F, 127.0F))) & 0xffu) << 8 * e;
+  }
+  return packed;
 }
 
 constexpr unsigned kQuantThreads = 256, kQuantWaves = kQuantThreads / 64;
@@ -109,14 +132,12 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const void
   for (unsigned w = 0; w < kQuantWaves; ++w) top = fmaxf(top, partial[w]);
   const bool broken = top == INFINITY;
   const float scale = broken ? __builtin_nanf("") : fmaxf(top * (1.0F / 127.0F), 0x1p-126F);
+  const float inverse = 1.0F / scale;
   if (threadIdx.x == 0) scales[row] = scale;
   auto store = [&](const float (&v)[8], uint32_t unit) __attribute__((always_inline)) {
-    uint64_t packed = 0;
-    if (!broken) {
-#pragma unroll
-      for (unsigned e = 0; e < 8; ++e) packed |= static_cast<uint64_t>(static_cast<uint8_t>(code_of(v[e], scale))) << 8 * e;
-    }
-    *reinterpret_cast<uint64_t*>(codes + row * columns + 8 * unit) = packed;
+    uint2 packed = {0, 0};
+    if (!broken) packed = uint2{four_codes(v, 0, scale, inverse), four_codes(v, 4, scale, inverse)};
+    *reinterpret_cast<uint2*>(codes + row * columns + 8 * unit) = packed;
   };
 #pragma unroll
   for (unsigned u = 0; u < kQuantUnits; ++u) {
@@ -172,96 +193,138 @@ __device__ __forceinline__ void write_output(const ProductArgs& a, uint32_t toke
   }
 }
 
-// Few tokens: the weights are streamed once, straight into registers.  A workgroup holds
-// 16 R channels and 16 T tokens; its waves divide K and add their sums in LDS.
-template <unsigned T, unsigned R, unsigned Waves, unsigned Steps>
+// Operand tiles (16 rows, 128 bytes of K) first and second of a stage in LDS, both 64-byte steps of
+// each, complete when they return.  (The compiler would let reads of its own wait for the later stages'
+// loads into LDS, which it cannot tell from this one's.)
+__device__ __forceinline__ void read_pair(unsigned first, unsigned second, i32x4 (&x)[2], i32x4 (&y)[2]) {
+  asm volatile(
+      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\tds_read_b128 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(y[0]), "=&v"(y[1])
+      : "v"(first), "v"(first ^ 64u), "v"(second), "v"(second ^ 64u)
+      : "memory");
+}
+
+// At most Loads of the wave's loads are on their way.
+template <unsigned Loads>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(Loads < 64);
+  __builtin_amdgcn_s_waitcnt((Loads & 15u) | (Loads >> 4) << 14 | 0xfu << 8 | 7u << 4);
+  asm volatile("" ::: "memory");
+}
+
+// Few tokens: the weights are streamed once.  A workgroup holds 16 R channels and 16 T tokens; its
+// waves divide K, each with a ring of Depth stages of 128 bytes in LDS for itself, and add their sums
+// at the end.  Loads cover whole lines of memory, eight rows of 128 bytes each: straight into the
+// registers of an operand they would be sixteen rows of 64 (17408 x 5120, one token: 27 us, not 21).
+// Piece c of row r lies in slot c ^ (r % 8), see below.
+template <unsigned T, unsigned R, unsigned Waves, unsigned Depth>
 __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
-  __shared__ i32x4 sums[Waves][R * T][64];
+  constexpr unsigned kTiles = R + T, kStageBytes = kTiles * 2048;
+  constexpr unsigned kSums = R * T * 1024;
+  __shared__ __align__(1024) int8_t ring[Waves * (Depth * kStageBytes > kSums ? Depth * kStageBytes : kSums)];
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned n = lane & 15u, q = lane >> 4;
   const uint32_t first = blockIdx.x * 16 * R;
-  const int8_t* w[R];
-  const int8_t* x[T];
+  int8_t* mine = ring + wave * (Depth * kStageBytes);
+  const auto weights = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.weights) + static_cast<std::size_t>(first) * a.columns, 0,
+                                                         static_cast<int>(min(16 * R, a.rows - first) * a.columns), 0x20000);
+  const auto codes = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.codes), 0, static_cast<int>(min(16 * T, a.tokens) * a.columns), 0x20000);
+  // Load u covers rows 8 u .. of the channels, then of the tokens; rows past the last one load that one.
+  const unsigned piece = (lane & 7u) ^ (lane >> 3);
+  uint32_t source[2 * kTiles];
 #pragma unroll
-  for (unsigned r = 0; r < R; ++r) w[r] = a.weights + static_cast<std::size_t>(min(first + 16 * r + n, a.rows - 1)) * a.columns + 16 * q;
-#pragma unroll
-  for (unsigned t = 0; t < T; ++t) x[t] = a.codes + static_cast<std::size_t>(min(16 * t + n, a.tokens - 1)) * a.columns + 16 * q;
-  const uint32_t steps = (a.columns + 63) / 64, per = (steps + Waves - 1) / Waves;
-  const uint32_t from = wave * per, to = min(from + per, steps);
-  i32x4 acc[R][T] = {};
-  i32x4 wv[2][Steps][R], xv[2][Steps][T];
-  auto load = [&](uint32_t step, unsigned b) __attribute__((always_inline)) {
-#pragma unroll
-    for (unsigned s = 0; s < Steps; ++s) {
-      const uint32_t k = (step + s) * 64;
-      const bool there = step + s < to && k + 16 * q < a.columns;
-#pragma unroll
-      for (unsigned r = 0; r < R; ++r) {
-        wv[b][s][r] = i32x4{0, 0, 0, 0};
-        if (there) wv[b][s][r] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(w[r] + k));
-      }
-#pragma unroll
-      for (unsigned t = 0; t < T; ++t) {
-        xv[b][s][t] = i32x4{0, 0, 0, 0};
-        if (there) xv[b][s][t] = *reinterpret_cast<const i32x4*>(x[t] + k);
-      }
-    }
-  };
-  auto multiply = [&](unsigned b) __attribute__((always_inline)) {
-#pragma unroll
-    for (unsigned s = 0; s < Steps; ++s) {
-#pragma unroll
-      for (unsigned r = 0; r < R; ++r) {
-#pragma unroll
-        for (unsigned t = 0; t < T; ++t) {
-          acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[b][s][r], xv[b][s][t], acc[r][t], 0, 0, 0);
-        }
-      }
-    }
-  };
-  if (from < to) load(from, 0);
-  for (uint32_t step = from; step < to; step += 2 * Steps) {
-    if (step + Steps < to) load(step + Steps, 1);
-    multiply(0);
-    if (step + Steps < to) {
-      if (step + 2 * Steps < to) load(step + 2 * Steps, 0);
-      multiply(1);
-    }
+  for (unsigned u = 0; u < 2 * kTiles; ++u) {
+    const unsigned r = 8 * u + lane / 8;
+    source[u] = (u < 2 * R ? min(r, a.rows - first - 1) : min(r - 16 * R, a.tokens - 1)) * a.columns;
   }
+  const uint32_t stages = (a.columns + 127) / 128, per = (stages + Waves - 1) / Waves;
+  const uint32_t from = wave * per, to = min(from + per, stages);
+  auto load = [&](uint32_t s, unsigned slot) __attribute__((always_inline)) {
+    const uint32_t at = min(s * 128 + 16 * piece, a.columns - 16);  // past the row: anything of it, see below
+#pragma unroll
+    for (unsigned u = 0; u < 2 * kTiles; ++u) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(u < 2 * R ? weights : codes, (lds_void*)(mine + slot * kStageBytes + u * 1024), 16,
+                                               static_cast<int>(source[u] + at), 0, 0, 0);
+    }
+  };
+  i32x4 acc[R][T] = {};
+#pragma unroll
+  for (unsigned d = 0; d + 1 < Depth; ++d) {
+    if (from + d < to) load(from + d, d);
+  }
+  const unsigned place = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)mine)) + n * 128 + 16 * (q ^ (n & 7u));
+  unsigned slot = 0;
+#pragma unroll 1
+  for (uint32_t s = from; s < to; ++s) {
+    // This stage has arrived when only the later ones are on their way.
+    if (s + Depth - 1 <= to) wait_loads<(Depth - 2) * 2 * kTiles>();
+    else wait_loads<0>();
+    if (s + 1 == stages && a.columns % 128 != 0) {
+      // The tokens' pieces past the end of a row become zeros, each by the lane that loaded it.
+      if (s * 128 + 16 * piece >= a.columns) {
+#pragma unroll
+        for (unsigned u = 2 * R; u < 2 * kTiles; ++u) *reinterpret_cast<i32x4*>(mine + slot * kStageBytes + u * 1024 + 16 * lane) = i32x4{0, 0, 0, 0};
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    // The stage before this one has been read: its slot takes the next loads.
+    const unsigned before = slot == 0 ? Depth - 1 : slot - 1;
+    if (s + Depth - 1 < to) load(s + Depth - 1, before);
+    const unsigned at = place + slot * kStageBytes;
+    i32x4 w[R + R % 2][2], x[T + T % 2][2];
+    // Pairs of tiles: channels, then tokens (an odd one is read twice).
+#pragma unroll
+    for (unsigned r = 0; r < R; r += 2) read_pair(at + r * 2048, at + (r + 1 < R ? r + 1 : r) * 2048, w[r], w[r + 1]);
+#pragma unroll
+    for (unsigned t = 0; t < T; t += 2) read_pair(at + (R + t) * 2048, at + (R + (t + 1 < T ? t + 1 : t)) * 2048, x[t], x[t + 1]);
+#pragma unroll
+    for (unsigned k = 0; k < 2; ++k) {
+#pragma unroll
+      for (unsigned r = 0; r < R; ++r) {
+#pragma unroll
+        for (unsigned t = 0; t < T; ++t) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[r][k], x[t][k], acc[r][t], 0, 0, 0);
+      }
+    }
+    slot = slot + 1 == Depth ? 0 : slot + 1;
+  }
+  __syncthreads();  // the rings are done with
+  i32x4* sums = reinterpret_cast<i32x4*>(ring);  // [waves][R T][64]
 #pragma unroll
   for (unsigned r = 0; r < R; ++r) {
 #pragma unroll
-    for (unsigned t = 0; t < T; ++t) sums[wave][r * T + t][lane] = acc[r][t];
+    for (unsigned t = 0; t < T; ++t) sums[(wave * R * T + r * T + t) * 64 + lane] = acc[r][t];
   }
   __syncthreads();
   for (unsigned i = wave; i < R * T; i += Waves) {
-    i32x4 total = sums[0][i][lane];
+    i32x4 total = sums[i * 64 + lane];
 #pragma unroll
-    for (unsigned v = 1; v < Waves; ++v) total += sums[v][i][lane];
+    for (unsigned v = 1; v < Waves; ++v) total += sums[(v * R * T + i) * 64 + lane];
     write_output(a, 16 * (i % T) + n, first + 16 * (i / T) + 4 * q, total);
   }
 }
 
 // Many tokens: tiles of BN channels and BM tokens, K in stages of 128 bytes that go straight
-// from memory into LDS, one ahead of the products.
+// from memory into LDS, one ahead of the products (v_mfma_i32_32x32x32_i8).
 //
 // A stage's row is 128 bytes, eight pieces of 16; piece c of row r lies in slot c ^ (r % 8)
 // (the address a lane loads from is permuted, since loads into LDS fill it lane after lane),
 // so the rows of an operand fall on different banks.
 constexpr unsigned kStage = 128;
+constexpr unsigned kGroup = 8;  // token tiles that run beside each other
 
 template <unsigned BN, unsigned BM, unsigned WN, unsigned WM>
 __global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs a, uint32_t row_tiles, uint32_t token_tiles) {
   constexpr unsigned kWaves = WN * WM;
-  constexpr unsigned R = BN / WN / 16, T = BM / WM / 16;   // 16 x 16 tiles of a wave
+  constexpr unsigned R = BN / WN / 32, T = BM / WM / 32;   // 32 x 32 tiles of a wave
   constexpr unsigned kLoads = (BN + BM) * kStage / 16 / (kWaves * 64);
   static_assert(BN * kStage / 16 % (kWaves * 64) == 0 && BM * kStage / 16 % (kWaves * 64) == 0);
   __shared__ __align__(1024) int8_t stage0[(BN + BM) * kStage];
   __shared__ __align__(1024) int8_t stage1[(BN + BM) * kStage];
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned n = lane & 15u, q = lane >> 4;
-  // Consecutive workgroups go to the eight XCDs in turn: each XCD takes a run of the tiles, in
-  // columns of all token tiles, so that weights are read into one L2.
+  const unsigned n = lane & 31u, h = lane >> 5;
+  // Consecutive workgroups go to the eight XCDs in turn: each XCD takes a run of the tiles, in groups of
+  // eight token tiles by all row tiles, so that the 32 tiles it works on at once share their operands
+  // through its L2.
   const uint32_t tiles = row_tiles * token_tiles, all = tiles * a.splits;
   uint32_t id = blockIdx.x;
   {
@@ -269,43 +332,56 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs 
     id = xcd * per + min(xcd, rest) + at;
   }
   const uint32_t split = id / tiles, tile = id - split * tiles;
-  const uint32_t row0 = tile / token_tiles * BN, token0 = tile % token_tiles * BM;
+  const uint32_t group = tile / (kGroup * row_tiles), in_group = tile - group * kGroup * row_tiles;
+  const uint32_t wide = min(kGroup, token_tiles - group * kGroup);
+  const uint32_t row0 = in_group / wide * BN, token0 = (group * kGroup + in_group % wide) * BM;
   const uint32_t stages = (a.columns + kStage - 1) / kStage, per_split = (stages + a.splits - 1) / a.splits;
   const uint32_t from = split * per_split, to = min(from + per_split, stages);
 
-  // Load u of a wave covers 8 rows (lane / 8) of eight pieces each.
-  const int8_t* source[kLoads];
+  // Load u of a wave covers 8 rows (lane / 8) of eight pieces each; rows past the last one load that one.
+  const auto weights = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.weights) + static_cast<std::size_t>(row0) * a.columns, 0,
+                                                         static_cast<int>(min(BN, a.rows - row0) * a.columns), 0x20000);
+  const auto codes = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.codes) + static_cast<std::size_t>(token0) * a.columns, 0,
+                                                       static_cast<int>(min(BM, a.tokens - token0) * a.columns), 0x20000);
+  uint32_t source[kLoads];
   const unsigned piece = (lane & 7u) ^ (lane >> 3);
 #pragma unroll
   for (unsigned u = 0; u < kLoads; ++u) {
     const unsigned r = 8 * (wave + kWaves * u) + lane / 8;
-    source[u] = r < BN ? a.weights + static_cast<std::size_t>(min(row0 + r, a.rows - 1)) * a.columns
-                       : a.codes + static_cast<std::size_t>(min(token0 + r - BN, a.tokens - 1)) * a.columns;
+    source[u] = (r < BN ? min(r, a.rows - row0 - 1) : min(r - BN, a.tokens - token0 - 1)) * a.columns;
   }
   auto load = [&](int8_t* stage, uint32_t s) __attribute__((always_inline)) {
-    const uint32_t k = s * kStage + 16 * piece;
-    const uint32_t at = min(k, a.columns - 16);  // past the row: anything of it, see below
+    const uint32_t at = min(s * kStage + 16 * piece, a.columns - 16);  // past the row: anything of it, see below
 #pragma unroll
     for (unsigned u = 0; u < kLoads; ++u) {
-      __builtin_amdgcn_global_load_lds((global_void*)(source[u] + at), (lds_void*)(stage + 8 * (wave + kWaves * u) * kStage), 16, 0, 0);
+      const unsigned r = 8 * (wave + kWaves * u);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r < BN ? weights : codes, (lds_void*)(stage + r * kStage), 16, static_cast<int>(source[u] + at), 0, 0, 0);
     }
   };
-  i32x4 acc[R][T] = {};
+  i32x16 acc[R][T] = {};
   const unsigned wrow = wave / WM * (BN / WN), trow = BN + wave % WM * (BM / WM);
+  const unsigned place = n * kStage + 16 * (h ^ (n & 7u));  // step k is at the place ^ 32 k
   auto multiply = [&](const int8_t* stage) __attribute__((always_inline)) {
 #pragma unroll
-    for (unsigned k = 0; k < 2; ++k) {
-      const unsigned slot = 16 * ((4 * k + q) ^ (n & 7u));
+    for (unsigned k = 0; k < kStage / 32; ++k) {
       i32x4 w[R], x[T];
 #pragma unroll
-      for (unsigned r = 0; r < R; ++r) w[r] = *reinterpret_cast<const i32x4*>(stage + (wrow + 16 * r + n) * kStage + slot);
+      for (unsigned t = 0; t < T; ++t) x[t] = *reinterpret_cast<const i32x4*>(stage + (trow + 32 * t) * kStage + (place ^ 32 * k));
 #pragma unroll
-      for (unsigned t = 0; t < T; ++t) x[t] = *reinterpret_cast<const i32x4*>(stage + (trow + 16 * t + n) * kStage + slot);
+      for (unsigned r = 0; r < R; ++r) w[r] = *reinterpret_cast<const i32x4*>(stage + (wrow + 32 * r) * kStage + (place ^ 32 * k));
 #pragma unroll
       for (unsigned r = 0; r < R; ++r) {
 #pragma unroll
-        for (unsigned t = 0; t < T; ++t) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[r], x[t], acc[r][t], 0, 0, 0);
+        for (unsigned t = 0; t < T; ++t) acc[r][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[r], x[t], acc[r][t], 0, 0, 0);
       }
+    }
+    // Operands are read two ahead of a step's products.
+    constexpr unsigned kReads = kStage / 32 * (R + T), kAhead = R + T + 2;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (unsigned e = 0; e < kReads - kAhead; ++e) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
   };
   // The tokens' pieces past the end of a row become zeros, each by the lane that loaded it.
@@ -320,6 +396,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs 
   };
   const bool ragged = a.columns % kStage != 0;
   if (from < to) load(stage0, from);
+#pragma unroll 1
   for (uint32_t s = from; s < to; s += 2) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // loads into LDS have arrived
     if (ragged && s + 1 == stages) clear_tail(stage0);
@@ -338,17 +415,21 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs 
   for (unsigned t = 0; t < T; ++t) {
 #pragma unroll
     for (unsigned r = 0; r < R; ++r) {
-      const uint32_t token = token0 + (trow - BN) + 16 * t + n, row = row0 + wrow + 16 * r + 4 * q;
-      if (a.splits == 1) {
-        write_output(a, token, row, acc[r][t]);
-      } else if (token < a.tokens) {
-        int32_t* plane = a.partial + (static_cast<std::size_t>(split) * a.tokens + token) * a.rows;
-        if (a.rows % 4 == 0) {
-          if (row < a.rows) *reinterpret_cast<i32x4*>(plane + row) = acc[r][t];
-        } else {
 #pragma unroll
-          for (unsigned e = 0; e < 4; ++e) {
-            if (row + e < a.rows) plane[row + e] = acc[r][t][e];
+      for (unsigned e = 0; e < 16; e += 4) {
+        const uint32_t token = token0 + (trow - BN) + 32 * t + n, row = row0 + wrow + 32 * r + 2 * e + 4 * h;
+        const i32x4 sum = {acc[r][t][e], acc[r][t][e + 1], acc[r][t][e + 2], acc[r][t][e + 3]};
+        if (a.splits == 1) {
+          write_output(a, token, row, sum);
+        } else if (token < a.tokens) {
+          int32_t* plane = a.partial + (static_cast<std::size_t>(split) * a.tokens + token) * a.rows;
+          if (a.rows % 4 == 0) {
+            if (row < a.rows) *reinterpret_cast<i32x4*>(plane + row) = sum;
+          } else {
+#pragma unroll
+            for (unsigned c = 0; c < 4; ++c) {
+              if (row + c < a.rows) plane[row + c] = sum[c];
+            }
           }
         }
       }
@@ -414,9 +495,9 @@ bool product_sizes(std::size_t rows, std::size_t columns, std::size_t tokens) {
 
 bool aligned(const void* p, std::size_t bytes) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-template <unsigned T, unsigned R, unsigned Waves, unsigned Steps>
+template <unsigned T, unsigned R, unsigned Waves, unsigned Depth>
 void launch_few(const ProductArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((w8a8_few_kernel<T, R, Waves, Steps>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(Waves * 64), 0, stream, a);
+  hipLaunchKernelGGL((w8a8_few_kernel<T, R, Waves, Depth>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(Waves * 64), 0, stream, a);
 }
 
 }  // namespace
@@ -476,9 +557,9 @@ extern "C" int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float*
                         output_type == GFXI_F16 ? 1u : 0u};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (s.tile == 0) {
-      if (tokens <= 16) launch_few<1, 1, 8, 4>(a, st);
-      else if (tokens <= 32) launch_few<2, 2, 8, 2>(a, st);
-      else launch_few<4, 2, 8, 2>(a, st);
+      if (tokens <= 16) launch_few<1, 1, 4, 4>(a, st);
+      else if (tokens <= 32) launch_few<2, 2, 4, 3>(a, st);
+      else launch_few<4, 2, 4, 3>(a, st);
       return launch_status("8-bit product launch failed");
     }
     const dim3 grid(static_cast<unsigned>(groups));
