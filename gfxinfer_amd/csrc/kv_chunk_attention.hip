@@ -112,6 +112,10 @@ __device__ __forceinline__ float sum_over_halves(float v) {
   return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
+// V rows in LDS: piece c of row r lies in slot c ^ 4 (r % 4), so that the four rows of 64 bytes that half
+// a wave reads at once (a transposing read of 32 columns) fall on different banks.
+__device__ __forceinline__ unsigned value_slot4(unsigned piece, unsigned row) { return piece ^ 4 * (row & 3u); }
+
 // What the waves of a workgroup need of a range of positions of one row tile.
 struct Range {
   uint32_t slot, end, from, to, hk;  // steps [from, to)
@@ -123,7 +127,7 @@ struct Range {
 template <unsigned D>
 __device__ __forceinline__ unsigned value_place_of(unsigned lane) {
   const unsigned i16 = lane & 15u, vrow = 4 * (lane >> 5) + (i16 >> 2);
-  return vrow * (2 * D) + 16 * value_slot(2 * (lane >> 4 & 1u) + ((i16 & 3u) >> 1), vrow) + 8 * (i16 & 1u);
+  return vrow * (2 * D) + 16 * value_slot4(2 * (lane >> 4 & 1u) + ((i16 & 3u) >> 1), vrow) + 8 * (i16 & 1u);
 }
 
 // Output tiles first .. first + 3 of 16 V rows in LDS, complete when they return.  (The compiler would let
@@ -165,7 +169,7 @@ __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& 
   const __half* values = pg.value + layer_row;
   _Float16* vs = wave == 0 ? lds[0] : wave == 1 ? lds[1] : wave == 2 ? lds[2] : lds[3];  // two blocks
   const uint32_t load_row = lane / (D / 8);
-  const uint32_t value_part = load_row * row_bytes + 16 * value_slot(lane % (D / 8), load_row);
+  const uint32_t value_part = load_row * row_bytes + 16 * value_slot4(lane % (D / 8), load_row);
   const unsigned value_place = lds_address(vs) + value_place_of<D>(lane);
   const uint32_t first = w.from * kTile<D> / kBlock + wave, last = min(w.to * kTile<D>, w.end + kBlock - 1) / kBlock;
   PageWindow window;
@@ -185,7 +189,7 @@ __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& 
       const unsigned row0 = kLoadRows * u, e = row0 / 16;
       const std::size_t base = ((static_cast<std::size_t>(max(page[e], 0)) << pg.page_shift) + ((at + 16 * e) & in_page)) * pg.row;
       const auto rows16 = __builtin_amdgcn_make_buffer_rsrc(const_cast<__half*>(values + base), 0, static_cast<int>(15 * row_bytes + 2 * D), 0x20000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rows16, (lds_void*)(vs + (to * kBlock + row0) * D), 16, static_cast<int>(value_part ^ 32 * (row0 & 7u)),
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rows16, (lds_void*)(vs + (to * kBlock + row0) * D), 16, static_cast<int>(value_part ^ 64 * (row0 & 3u)),
                                                static_cast<int>((row0 & 15u) * row_bytes), 0, 0);
     }
   };
@@ -470,14 +474,14 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   };
   // Where the lane's piece of a load lies in memory, in bytes from the first of the load's rows: the rows of
   // load u of a wave are 16 or 8 u and its own, so the order of their pieces (by the row in sixteen for K,
-  // in eight for V) is that of u % 2.
+  // in four for V) is that of u % 2.
   const uint32_t load_row = lane / (D / 8), row_bytes = 2 * pg.row;
   uint32_t key_part[2], value_part;
 #pragma unroll
   for (unsigned e = 0; e < 2; ++e) {
     key_part[e] = load_row * row_bytes + 16 * key_slot(lane % (D / 8), kLoadRows * (wave + kWaves * e) + load_row);
   }
-  value_part = load_row * row_bytes + 16 * value_slot(lane % (D / 8), kLoadRows * wave + load_row);
+  value_part = load_row * row_bytes + 16 * value_slot4(lane % (D / 8), kLoadRows * wave + load_row);
   // Rows of a tile into LDS, through buffer descriptors of the parts' sixteen rows (after flat loads into LDS
   // the compiler lets every read of LDS wait for all reads before it).  Parts without a page load from page 0
   // of the pool (always there), and so do those past the end.

@@ -216,7 +216,7 @@ __device__ __forceinline__ void wait_loads() {
 // waves divide K, each with a ring of Depth stages of 128 bytes in LDS for itself, and add their sums
 // at the end.  Loads cover whole lines of memory, eight rows of 128 bytes each: straight into the
 // registers of an operand they would be sixteen rows of 64 (17408 x 5120, one token: 27 us, not 21).
-// Piece c of row r lies in slot c ^ (r % 8), see below.
+// Piece c of row r lies in slot c ^ (r / 2 % 8), see below.
 template <unsigned T, unsigned R, unsigned Waves, unsigned Depth>
 __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
   constexpr unsigned kTiles = R + T, kStageBytes = kTiles * 2048;
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
                                                          static_cast<int>(min(16 * R, a.rows - first) * a.columns), 0x20000);
   const auto codes = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.codes), 0, static_cast<int>(min(16 * T, a.tokens) * a.columns), 0x20000);
   // Load u covers rows 8 u .. of the channels, then of the tokens; rows past the last one load that one.
-  const unsigned piece = (lane & 7u) ^ (lane >> 3);
+  const unsigned piece[2] = {(lane & 7u) ^ (lane >> 4), (lane & 7u) ^ (4 + (lane >> 4))};  // of even and odd loads
   uint32_t source[2 * kTiles];
 #pragma unroll
   for (unsigned u = 0; u < 2 * kTiles; ++u) {
@@ -240,11 +240,14 @@ __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
   const uint32_t stages = (a.columns + 127) / 128, per = (stages + Waves - 1) / Waves;
   const uint32_t from = wave * per, to = min(from + per, stages);
   auto load = [&](uint32_t s, unsigned slot) __attribute__((always_inline)) {
-    const uint32_t at = min(s * 128 + 16 * piece, a.columns - 16);  // past the row: anything of it, see below
+    // Past the row: anything of it, see below.
+    uint32_t at[2];
+#pragma unroll
+    for (unsigned e = 0; e < 2; ++e) at[e] = min(s * 128 + 16 * piece[e], a.columns - 16);
 #pragma unroll
     for (unsigned u = 0; u < 2 * kTiles; ++u) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(u < 2 * R ? weights : codes, (lds_void*)(mine + slot * kStageBytes + u * 1024), 16,
-                                               static_cast<int>(source[u] + at), 0, 0, 0);
+                                               static_cast<int>(source[u] + at[u % 2]), 0, 0, 0);
     }
   };
   i32x4 acc[R][T] = {};
@@ -252,7 +255,7 @@ __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
   for (unsigned d = 0; d + 1 < Depth; ++d) {
     if (from + d < to) load(from + d, d);
   }
-  const unsigned place = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)mine)) + n * 128 + 16 * (q ^ (n & 7u));
+  const unsigned place = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)mine)) + n * 128 + 16 * (q ^ (n >> 1));
   unsigned slot = 0;
 #pragma unroll 1
   for (uint32_t s = from; s < to; ++s) {
@@ -261,9 +264,9 @@ __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
     else wait_loads<0>();
     if (s + 1 == stages && a.columns % 128 != 0) {
       // The tokens' pieces past the end of a row become zeros, each by the lane that loaded it.
-      if (s * 128 + 16 * piece >= a.columns) {
 #pragma unroll
-        for (unsigned u = 2 * R; u < 2 * kTiles; ++u) *reinterpret_cast<i32x4*>(mine + slot * kStageBytes + u * 1024 + 16 * lane) = i32x4{0, 0, 0, 0};
+      for (unsigned u = 2 * R; u < 2 * kTiles; ++u) {
+        if (s * 128 + 16 * piece[u % 2] >= a.columns) *reinterpret_cast<i32x4*>(mine + slot * kStageBytes + u * 1024 + 16 * lane) = i32x4{0, 0, 0, 0};
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
@@ -306,9 +309,9 @@ __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
 // Many tokens: tiles of BN channels and BM tokens, K in stages of 128 bytes that go straight
 // from memory into LDS, one ahead of the products (v_mfma_i32_32x32x32_i8).
 //
-// A stage's row is 128 bytes, eight pieces of 16; piece c of row r lies in slot c ^ (r % 8)
+// A stage's row is 128 bytes, eight pieces of 16; piece c of row r lies in slot c ^ (r / 2 % 8)
 // (the address a lane loads from is permuted, since loads into LDS fill it lane after lane),
-// so the rows of an operand fall on different banks.
+// so sixteen rows of an operand, two of which lie side by side in the banks, fall on different ones.
 constexpr unsigned kStage = 128;
 constexpr unsigned kGroup = 8;  // token tiles that run beside each other
 
@@ -344,7 +347,8 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs 
   const auto codes = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.codes) + static_cast<std::size_t>(token0) * a.columns, 0,
                                                        static_cast<int>(min(BM, a.tokens - token0) * a.columns), 0x20000);
   uint32_t source[kLoads];
-  const unsigned piece = (lane & 7u) ^ (lane >> 3);
+  static_assert(kWaves % 2 == 0);  // loads of a wave are all of even or all of odd groups of eight rows
+  const unsigned piece = (lane & 7u) ^ (4 * (wave & 1u) + (lane >> 4));
 #pragma unroll
   for (unsigned u = 0; u < kLoads; ++u) {
     const unsigned r = 8 * (wave + kWaves * u) + lane / 8;
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs 
   };
   i32x16 acc[R][T] = {};
   const unsigned wrow = wave / WM * (BN / WN), trow = BN + wave % WM * (BM / WM);
-  const unsigned place = n * kStage + 16 * (h ^ (n & 7u));  // step k is at the place ^ 32 k
+  const unsigned place = n * kStage + 16 * (h ^ (n >> 1 & 7u));  // step k is at the place ^ 32 k
   auto multiply = [&](const int8_t* stage) __attribute__((always_inline)) {
 #pragma unroll
     for (unsigned k = 0; k < kStage / 32; ++k) {
@@ -557,8 +561,9 @@ extern "C" int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float*
                         output_type == GFXI_F16 ? 1u : 0u};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (s.tile == 0) {
-      if (tokens <= 16) launch_few<1, 1, 4, 4>(a, st);
+      if (tokens <= 16) launch_few<1, 1, 4, 3>(a, st);
       else if (tokens <= 32) launch_few<2, 2, 4, 3>(a, st);
+      else if (tokens <= 48) launch_few<3, 2, 4, 3>(a, st);
       else launch_few<4, 2, 4, 3>(a, st);
       return launch_status("8-bit product launch failed");
     }
