@@ -89,16 +89,15 @@ __device__ __forceinline__ uint32_t four_codes(const float (&x)[8], unsigned fir
   return packed;
 }
 
-constexpr unsigned kQuantThreads = 256, kQuantWaves = kQuantThreads / 64;
-constexpr unsigned kQuantUnits = 8;  // of eight values a thread keeps: rows up to 16384 are read once
+constexpr unsigned kQuantUnits = 4;  // of eight values a thread keeps
 
 // A workgroup a row.  A row that holds an infinity or a NaN gets a NaN scale and zero codes,
 // so every product with it is NaN; a row of zeros the smallest normal scale.
-template <int Type>
-__global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const void* __restrict__ input, std::size_t stride,
-                                                                      uint32_t columns, int8_t* __restrict__ codes,
-                                                                      float* __restrict__ scales) {
-  __shared__ float partial[kQuantWaves];
+template <int Type, unsigned Threads>
+__global__ __launch_bounds__(Threads) void quantize_rows_kernel(const void* __restrict__ input, std::size_t stride,
+                                                                uint32_t columns, int8_t* __restrict__ codes,
+                                                                float* __restrict__ scales) {
+  __shared__ float partial[Threads / 64];
   const std::size_t row = blockIdx.x;
   const uint32_t units = columns / 8;
   float x[kQuantUnits][8];
@@ -113,14 +112,14 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const void
   };
 #pragma unroll
   for (unsigned u = 0; u < kQuantUnits; ++u) {
-    const uint32_t unit = threadIdx.x + u * kQuantThreads;
+    const uint32_t unit = threadIdx.x + u * Threads;
     if (unit < units) load8<Type>(input, row * stride + 8 * unit, x[u]);
   }
 #pragma unroll
   for (unsigned u = 0; u < kQuantUnits; ++u) {
-    if (threadIdx.x + u * kQuantThreads < units) measure(x[u]);
+    if (threadIdx.x + u * Threads < units) measure(x[u]);
   }
-  for (uint32_t unit = threadIdx.x + kQuantUnits * kQuantThreads; unit < units; unit += kQuantThreads) {
+  for (uint32_t unit = threadIdx.x + kQuantUnits * Threads; unit < units; unit += Threads) {
     float v[8];
     load8<Type>(input, row * stride + 8 * unit, v);
     measure(v);
@@ -129,7 +128,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const void
   if ((threadIdx.x & 63u) == 0) partial[threadIdx.x >> 6] = top;
   __syncthreads();
 #pragma unroll
-  for (unsigned w = 0; w < kQuantWaves; ++w) top = fmaxf(top, partial[w]);
+  for (unsigned w = 0; w < Threads / 64; ++w) top = fmaxf(top, partial[w]);
   const bool broken = top == INFINITY;
   const float scale = broken ? __builtin_nanf("") : fmaxf(top * (1.0F / 127.0F), 0x1p-126F);
   const float inverse = 1.0F / scale;
@@ -141,10 +140,10 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const void
   };
 #pragma unroll
   for (unsigned u = 0; u < kQuantUnits; ++u) {
-    const uint32_t unit = threadIdx.x + u * kQuantThreads;
+    const uint32_t unit = threadIdx.x + u * Threads;
     if (unit < units) store(x[u], unit);
   }
-  for (uint32_t unit = threadIdx.x + kQuantUnits * kQuantThreads; unit < units; unit += kQuantThreads) {
+  for (uint32_t unit = threadIdx.x + kQuantUnits * Threads; unit < units; unit += Threads) {
     float v[8];
     load8<Type>(input, row * stride + 8 * unit, v);
     store(v, unit);
@@ -212,6 +211,9 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("" ::: "memory");
 }
 
+// All of the wave's LDS accesses are complete.
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // Few tokens: the weights are streamed once.  A workgroup holds 16 R channels and 16 T tokens; its
 // waves divide K, each with a ring of Depth stages of 128 bytes in LDS for itself, and add their sums
 // at the end.  Loads cover whole lines of memory, eight rows of 128 bytes each: straight into the
@@ -268,7 +270,7 @@ __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
       for (unsigned u = 2 * R; u < 2 * kTiles; ++u) {
         if (s * 128 + 16 * piece[u % 2] >= a.columns) *reinterpret_cast<i32x4*>(mine + slot * kStageBytes + u * 1024 + 16 * lane) = i32x4{0, 0, 0, 0};
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      wait_reads();
     }
     // The stage before this one has been read: its slot takes the next loads.
     const unsigned before = slot == 0 ? Depth - 1 : slot - 1;
@@ -315,14 +317,19 @@ __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
 constexpr unsigned kStage = 128;
 constexpr unsigned kGroup = 8;  // token tiles that run beside each other
 
-template <unsigned BN, unsigned BM, unsigned WN, unsigned WM>
+template <unsigned BN, unsigned BM, unsigned WN, unsigned WM, unsigned Depth>
 __global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs a, uint32_t row_tiles, uint32_t token_tiles) {
   constexpr unsigned kWaves = WN * WM;
   constexpr unsigned R = BN / WN / 32, T = BM / WM / 32;   // 32 x 32 tiles of a wave
   constexpr unsigned kLoads = (BN + BM) * kStage / 16 / (kWaves * 64);
   static_assert(BN * kStage / 16 % (kWaves * 64) == 0 && BM * kStage / 16 % (kWaves * 64) == 0);
-  __shared__ __align__(1024) int8_t stage0[(BN + BM) * kStage];
-  __shared__ __align__(1024) int8_t stage1[(BN + BM) * kStage];
+  // (Arrays of their own, so that the compiler can tell one stage's reads from another's loads.)
+  constexpr unsigned kBytes = (BN + BM) * kStage;
+  __shared__ __align__(1024) int8_t stage0[kBytes];
+  __shared__ __align__(1024) int8_t stage1[kBytes];
+  __shared__ __align__(1024) int8_t stage2[Depth > 2 ? kBytes : 16];
+  __shared__ __align__(1024) int8_t stage3[Depth > 3 ? kBytes : 16];
+  int8_t* const ring[4] = {stage0, stage1, stage2, stage3};
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned n = lane & 31u, h = lane >> 5;
   // Consecutive workgroups go to the eight XCDs in turn: each XCD takes a run of the tiles, in groups of
@@ -399,22 +406,33 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs 
     }
   };
   const bool ragged = a.columns % kStage != 0;
-  if (from < to) load(stage0, from);
+  // Stages past the last one load that one again: with no branch around the loads the compiler can count
+  // them, too.
+#pragma unroll
+  for (unsigned d = 0; d + 1 < Depth; ++d) load(ring[d], min(from + d, to - 1));
+  auto turn = [&](uint32_t s, unsigned d) __attribute__((always_inline)) {
+    // This stage has arrived when only the later ones are on their way.
+    wait_loads<(Depth - 2) * kLoads>();
+    if (ragged && s + 1 == stages) clear_tail(ring[d]);
+    wait_reads();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // Every wave has read the stage before this one: its place takes the next loads.
+    load(ring[(d + Depth - 1) % Depth], min(s + Depth - 1, to - 1));
+    multiply(ring[d]);
+  };
+  uint32_t s = from;
 #pragma unroll 1
-  for (uint32_t s = from; s < to; s += 2) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // loads into LDS have arrived
-    if (ragged && s + 1 == stages) clear_tail(stage0);
-    __syncthreads();
-    if (s + 1 < to) load(stage1, s + 1);
-    multiply(stage0);
-    if (s + 1 < to) {
-      __builtin_amdgcn_s_waitcnt(0x0f70);
-      if (ragged && s + 2 == stages) clear_tail(stage1);
-      __syncthreads();
-      if (s + 2 < to) load(stage0, s + 2);
-      multiply(stage1);
-    }
+  for (; s + Depth <= to; s += Depth) {
+#pragma unroll
+    for (unsigned d = 0; d < Depth; ++d) turn(s + d, d);
   }
+#pragma unroll
+  for (unsigned d = 0; d + 1 < Depth; ++d) {
+    if (s + d < to) turn(s + d, d);
+  }
+  // The loads of no stage write into this workgroup's LDS, so it stays until they have.
+  wait_loads<0>();
 #pragma unroll
   for (unsigned t = 0; t < T; ++t) {
 #pragma unroll
@@ -464,25 +482,47 @@ __global__ __launch_bounds__(256) void w8a8_join_kernel(ProductArgs a) {
 constexpr uint32_t kFewTokens = 64;
 
 struct ProductShape {
-  uint32_t tile;  // channels and tokens of a tile; 0: the kernel for few tokens
+  uint32_t tile_rows;  // channels of a tile, see below; 0: the kernel for few tokens
   uint32_t row_tiles, token_tiles, splits;
 };
 
+// The tile shapes, with the time in nanoseconds that a round of their workgroups takes by itself and for each
+// stage of 128 columns, fitted to what 900 products of 65 to 4096 tokens and 1024 to 34816 rows took.
+struct TileShape {
+  uint32_t rows, tokens, places;
+  double round, stage;
+};
+constexpr TileShape kTileShapes[] = {
+    {64, 64, 2 * kComputeUnits, 600, 370},
+    {128, 128, kComputeUnits, 2700, 470},
+    {256, 128, kComputeUnits, 4500, 620},
+};
+// Joining splits takes 8.5 us and 1.34 ps for each sum.
+constexpr double kJoinTime = 8500, kJoinSum = 0.00134;
+constexpr uint32_t kMaxSplits = 8;
+
+// The shape and the number of splits that take the shortest time: the rounds that the chip needs for the
+// workgroups times the time of one. Against the best of all on the same 78 sizes the choice costs 2.3 % on
+// average and 16 % at worst. 5120 x 5120 and 160 tokens: 12.6 us in tiles of 64, 18.4 of 128, 28 of 256; 17408 x 5120 and 1024
+// tokens: 197, 162 and 127; 5120 x 17408 and 320 tokens: 48 in four splits of 256, 55 in three, 75 in tiles of 64 without.
 ProductShape product_shape(std::size_t rows, std::size_t columns, std::size_t tokens) {
   ProductShape s{};
   s.splits = 1;
   if (tokens <= kFewTokens) return s;
-  auto tiles = [&](uint32_t size) { return ((rows + size - 1) / size) * ((tokens + size - 1) / size); };
-  s.tile = tiles(256) >= kComputeUnits ? 256 : 128;
-  s.row_tiles = static_cast<uint32_t>((rows + s.tile - 1) / s.tile);
-  s.token_tiles = static_cast<uint32_t>((tokens + s.tile - 1) / s.tile);
-  if (s.tile == 128) {
-    const std::size_t places = 2 * kComputeUnits, stages = (columns + kStage - 1) / kStage;
-    const std::size_t want = std::max<std::size_t>(1, places / tiles(128));
-    s.splits = static_cast<uint32_t>(std::max<std::size_t>(1, std::min(want, stages / 8)));
-    // Every split has a stage to do.
-    const std::size_t per = (stages + s.splits - 1) / s.splits;
-    s.splits = static_cast<uint32_t>((stages + per - 1) / per);
+  const std::size_t stages = (columns + kStage - 1) / kStage;
+  double best = 0;
+  for (const TileShape& t : kTileShapes) {
+    const std::size_t row_tiles = (rows + t.rows - 1) / t.rows, token_tiles = (tokens + t.tokens - 1) / t.tokens;
+    for (uint32_t want = 1; want <= std::min<std::size_t>(kMaxSplits, stages); ++want) {
+      // Every split has a stage to do.
+      const std::size_t per = (stages + want - 1) / want, splits = (stages + per - 1) / per;
+      const std::size_t rounds = (row_tiles * token_tiles * splits + t.places - 1) / t.places;
+      double time = static_cast<double>(rounds) * (t.round + static_cast<double>(per) * t.stage);
+      if (splits > 1) time += kJoinTime + kJoinSum * static_cast<double>(splits * rows * tokens);
+      if (s.tile_rows != 0 && time >= best) continue;
+      best = time;
+      s = {t.rows, static_cast<uint32_t>(row_tiles), static_cast<uint32_t>(token_tiles), static_cast<uint32_t>(splits)};
+    }
   }
   return s;
 }
@@ -504,6 +544,18 @@ void launch_few(const ProductArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((w8a8_few_kernel<T, R, Waves, Depth>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(Waves * 64), 0, stream, a);
 }
 
+// Rows up to 8192 values fit the registers of four waves, up to 32768 those of sixteen; longer ones are read twice.
+template <int Type>
+void launch_quantize(const void* input, std::size_t rows, std::size_t stride, uint32_t columns, int8_t* codes, float* scales,
+                     hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(rows));
+  if (columns <= 256 * 8 * kQuantUnits) {
+    hipLaunchKernelGGL((quantize_rows_kernel<Type, 256>), grid, dim3(256), 0, stream, input, stride, columns, codes, scales);
+  } else {
+    hipLaunchKernelGGL((quantize_rows_kernel<Type, 1024>), grid, dim3(1024), 0, stream, input, stride, columns, codes, scales);
+  }
+}
+
 }  // namespace
 }  // namespace gfx950
 
@@ -521,12 +573,11 @@ extern "C" int32_t gfxinfer_launch_quantize_rows_i8(const void* input, int32_t i
     if (!aligned(input, 16) || !aligned(codes, 16) || !aligned(scales, 4)) {
       return fail(GFXI_INVALID_ARGUMENT, "row quantizer: input and codes are 16-byte aligned, scales are set");
     }
-    const dim3 grid(static_cast<unsigned>(rows)), block(kQuantThreads);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const uint32_t n = static_cast<uint32_t>(columns);
-    if (input_type == GFXI_F16) hipLaunchKernelGGL(quantize_rows_kernel<GFXI_F16>, grid, block, 0, st, input, row_stride, n, codes, scales);
-    else if (input_type == GFXI_F32) hipLaunchKernelGGL(quantize_rows_kernel<GFXI_F32>, grid, block, 0, st, input, row_stride, n, codes, scales);
-    else hipLaunchKernelGGL(quantize_rows_kernel<GFXI_BF16>, grid, block, 0, st, input, row_stride, n, codes, scales);
+    if (input_type == GFXI_F16) launch_quantize<GFXI_F16>(input, rows, row_stride, n, codes, scales, st);
+    else if (input_type == GFXI_F32) launch_quantize<GFXI_F32>(input, rows, row_stride, n, codes, scales, st);
+    else launch_quantize<GFXI_BF16>(input, rows, row_stride, n, codes, scales, st);
     return launch_status("row quantizer launch failed");
   });
 }
@@ -560,7 +611,7 @@ extern "C" int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float*
                         static_cast<uint32_t>(rows), static_cast<uint32_t>(columns), static_cast<uint32_t>(tokens), s.splits,
                         output_type == GFXI_F16 ? 1u : 0u};
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (s.tile == 0) {
+    if (s.tile_rows == 0) {
       if (tokens <= 16) launch_few<1, 1, 4, 3>(a, st);
       else if (tokens <= 32) launch_few<2, 2, 4, 3>(a, st);
       else if (tokens <= 48) launch_few<3, 2, 4, 3>(a, st);
@@ -568,8 +619,9 @@ extern "C" int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float*
       return launch_status("8-bit product launch failed");
     }
     const dim3 grid(static_cast<unsigned>(groups));
-    if (s.tile == 256) hipLaunchKernelGGL((w8a8_tile_kernel<256, 256, 2, 4>), grid, dim3(512), 0, st, a, s.row_tiles, s.token_tiles);
-    else hipLaunchKernelGGL((w8a8_tile_kernel<128, 128, 2, 2>), grid, dim3(256), 0, st, a, s.row_tiles, s.token_tiles);
+    if (s.tile_rows == 64) hipLaunchKernelGGL((w8a8_tile_kernel<64, 64, 2, 2, 4>), grid, dim3(256), 0, st, a, s.row_tiles, s.token_tiles);
+    else if (s.tile_rows == 128) hipLaunchKernelGGL((w8a8_tile_kernel<128, 128, 2, 4, 4>), grid, dim3(512), 0, st, a, s.row_tiles, s.token_tiles);
+    else hipLaunchKernelGGL((w8a8_tile_kernel<256, 128, 4, 2, 3>), grid, dim3(512), 0, st, a, s.row_tiles, s.token_tiles);
     if (const int32_t status = launch_status("8-bit product launch failed"); status != GFXI_OK || s.splits == 1) return status;
     const std::size_t quads = (rows + 3) / 4 * tokens;
     hipLaunchKernelGGL(w8a8_join_kernel, dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(256), 0, st, a);

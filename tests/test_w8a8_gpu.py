@@ -118,6 +118,17 @@ def test_products_equal_the_definition(device, gx, half, tokens, rows, columns):
     assert np.array_equal(_product(gx, w, ws, a, s, half), _want(w, ws, a, s, half))
 
 
+@pytest.mark.parametrize("tokens,rows,columns", [
+    (65, 1999, 528), (65, 1999, 4112), (65, 17001, 1040), (65, 7000, 8208), (1000, 7000, 528), (65, 17001, 8208), (2000, 5000, 656)])
+def test_every_tile_shape(device, gx, tokens, rows, columns):
+    """Small, middle and large tiles, in one piece and with K divided among workgroups, all with a ragged edge."""
+    rng = np.random.default_rng(tokens + rows + columns)
+    say("8-bit product", tokens, rows, columns)
+    a, w = (rng.integers(-128, 128, (x, columns), dtype=np.int8) for x in (tokens, rows))
+    s, ws = ((rng.random(x) + 0.5).astype(np.float32) for x in (tokens, rows))
+    assert np.array_equal(_product(gx, w, ws, a, s, False), _want(w, ws, a, s, False))
+
+
 @pytest.mark.parametrize("tokens", [1, 64, 70])
 def test_the_largest_sums(device, gx, tokens):
     """All codes -128 at the longest K: 128 * 128 * 131056 is the largest sum a call can make, below 2^31."""
