@@ -97,7 +97,7 @@ __device__ __forceinline__ Listed find_listed(const ChunkAttnArgs& a, uint32_t r
 #pragma unroll
   for (unsigned d = 1; d < 64; d <<= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
   const uint32_t steps = (__builtin_amdgcn_readfirstlane(most) + kTile<D> - 1) / kTile<D>;
-  found.per = a.ranges == 1 ? 0xffffffu : max(kLeastSteps, (steps + a.ranges - 1) / a.ranges);
+  found.per = a.ranges == 1 ? 0xffffffffu : max(kLeastSteps, (steps + a.ranges - 1) / a.ranges);
   return found;
 }
 
@@ -792,93 +792,313 @@ struct WeightArgs {
   float scale;
 };
 
-constexpr unsigned kWeightPositions = 128;  // of a workgroup: 32 a wave
-constexpr unsigned kWeightRows = 32;        // rows staged at a time
+// Sums of N registers over the 32 lanes of a half: at each exchange a lane keeps the registers whose
+// number has its own bit, so that register r of lane n ends as the whole sum of number n % N.
+template <unsigned N, unsigned Distance = 1>
+__device__ __forceinline__ float sum_lanes(const float (&sum)[N]) {
+  const bool odd = (threadIdx.x & Distance) != 0;
+  float half[N > 1 ? N / 2 : 1];
+  if constexpr (N == 1) {
+    half[0] = sum[0] + __shfl_xor(sum[0], Distance);  // fewer registers than lanes
+  } else {
+#pragma unroll
+    for (unsigned r = 0; r < N / 2; ++r) half[r] = (odd ? sum[2 * r + 1] : sum[2 * r]) + __shfl_xor(odd ? sum[2 * r] : sum[2 * r + 1], Distance);
+  }
+  if constexpr (Distance == 16) return half[0];
+  else return sum_lanes<(N > 1 ? N / 2 : 1), 2 * Distance>(half);
+}
 
-// A wave holds 32 positions of K as the A operand; the rows of a KV head pass through LDS, 32
-// at a time, and each score's exponential is added to the lane's sum of its position.
+// The K row of a position, or one that is always there.
+__device__ __forceinline__ const __half* key_row(const WeightArgs& a, uint32_t slot, uint32_t position, uint32_t end) {
+  const KvPages& pg = a.pages;
+  const int32_t page = position < end ? table_page(pg, slot, position >> pg.page_shift) : -1;
+  const std::size_t row = (static_cast<std::size_t>(max(page, 0)) << pg.page_shift) + (page < 0 ? 0 : position & ((1u << pg.page_shift) - 1));
+  return pg.key + ((static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) + row) * pg.row;
+}
+
+constexpr uint32_t kFewRows = 32;  // of a sequence and KV head
+
+// Sequences of at most 32 rows, as a decoding one has: a workgroup takes 32 positions and all KV
+// heads, a wave every fourth one, and adds the sum over all of them.
 template <unsigned D>
-__global__ __launch_bounds__(256) void weight_kernel(WeightArgs a) {
-  __shared__ __align__(1024) _Float16 rows0[kWeightRows * D];
+__global__ __launch_bounds__(256) void few_weight_kernel(WeightArgs a) {
+  __shared__ float parts[4][32];
+  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned n = lane & 31u, h = lane >> 5;
+  const KvPages& pg = a.pages;
+  const uint32_t i = blockIdx.y, slot = listed_slot(a.list, i), first_row = a.list.first[i], tokens = a.list.first[i + 1] - first_row;
+  const uint32_t rows = tokens * a.group;
+  if (rows == 0 || rows > kFewRows) return;
+  const uint32_t length = committed(pg, slot), capacity = pg.stride << pg.page_shift, end = min(length + tokens, capacity);
+  const uint32_t t = min(n, rows - 1) / a.group;
+  const std::size_t out_row = (static_cast<std::size_t>(first_row) + t) * a.q_heads + (min(n, rows - 1) - t * a.group);
+  for (uint32_t at = blockIdx.x * 32; at < end; at += gridDim.x * 32) {
+    const __half* keys = key_row(a, slot, at + n, end) + 8 * h;
+    float sum[16] = {};
+    for (uint32_t hk = wave; hk < a.kv_heads; hk += 4) {
+      const std::size_t row = out_row + hk * a.group;
+      h8 k[D / 16], q[D / 16];
+#pragma unroll
+      for (unsigned s = 0; s < D / 16; ++s) k[s] = *reinterpret_cast<const h8*>(keys + hk * D + 16 * s);
+#pragma unroll
+      for (unsigned s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const h8*>(a.query + row * D + 16 * s + 8 * h);
+      const float level = a.log_sums[row] * kLog2E;
+      const uint32_t visible = n < rows && level > -INFINITY ? length + t + 1 : 0;  // not of a row that sees nothing, or a NaN
+      f16v s = f16v{};
+#pragma unroll
+      for (unsigned st = 0; st < D / 16; ++st) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[st], q[st], s, 0, 0, 0);
+#pragma unroll
+      for (unsigned r = 0; r < 16; ++r) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale, -level));
+        sum[r] += at + 8 * (r / 4) + 4 * h + r % 4 < visible ? w : 0.0F;
+      }
+    }
+    const float mine = sum_lanes(sum);
+    // Lane n has the sum of register n % 16: position 8 (r / 4) + 4 h + r % 4.
+    if (n < 16) parts[wave][8 * (n / 4) + 4 * h + n % 4] = mine;
+    __syncthreads();
+    if (threadIdx.x < 32 && at + threadIdx.x < end && table_page(pg, slot, (at + threadIdx.x) >> pg.page_shift) >= 0) {
+      float total = 0.0F;
+#pragma unroll
+      for (unsigned v = 0; v < 4; ++v) total += parts[v][threadIdx.x];
+      a.weights.weight[static_cast<std::size_t>(slot) * capacity + at + threadIdx.x] += total;
+    }
+    __syncthreads();
+  }
+}
+
+constexpr unsigned kWeightPositions = 256;  // of a workgroup: 64 a wave
+constexpr unsigned kWeightRows = 32;        // rows of a step
+// Workgroups a CU holds.
+template <unsigned D>
+constexpr unsigned kWeightResident = D == 128 ? 2 : 1;
+constexpr unsigned kWeightRing = 4;         // steps in LDS: one is read, two are on their way
+
+// Rows of a step on their way to LDS, and the log sums of its lane's row: each lane walks from a row to
+// the one 32 further on without dividing.
+struct RowWalk {
+  uint32_t head;    // the row's query head of the group
+  uint32_t offset;  // from the step's first token, in units of the caller
+  __device__ __forceinline__ void start(uint32_t row, uint32_t token, uint32_t group, uint32_t token_step, uint32_t head_step) {
+    const uint32_t t = row / group;
+    head = row - t * group;
+    offset = (t - token) * token_step + head * head_step;
+  }
+  // `by` = 32 % group; `wrapped`: the step's first token moved on by 32 / group + 1 tokens, not 32 / group.
+  __device__ __forceinline__ void step(uint32_t by, bool wrapped, uint32_t group, uint32_t token_step, uint32_t head_step) {
+    head += by;
+    offset += by * head_step - (wrapped ? token_step : 0);
+    const bool over = head >= group;
+    head -= over ? group : 0;
+    offset += over ? token_step - group * head_step : 0;
+  }
+};
+
+// A wave holds 64 positions of K as the A operand.  The rows of a KV head pass through LDS, 32 at a time,
+// three steps ahead, and serve all waves; the exponentials of a step, each added to the lane's sum of
+// its position, go between the next step's products.
+template <unsigned D>
+__global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightArgs a) {
+  constexpr unsigned P = kWeightPositions / 4 / 32;
+  constexpr unsigned kLoadRows = 512 / D, kLoads = kWeightRows / kLoadRows / 4;
+  // (Arrays of their own, so that the compiler can tell one step's reads from another's loads.)
+  __shared__ __align__(1024) _Float16 step0[kWeightRows * D], step1[kWeightRows * D], step2[kWeightRows * D], step3[kWeightRows * D];
+  _Float16* const ring[kWeightRing] = {step0, step1, step2, step3};
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned n = lane & 31u, h = lane >> 5;
   const KvPages& pg = a.pages;
   const uint32_t hk = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads % a.parts;
   const uint32_t column = blockIdx.x / a.kv_heads / a.parts, i = blockIdx.y;
   const uint32_t slot = listed_slot(a.list, i), first_row = a.list.first[i], tokens = a.list.first[i + 1] - first_row;
-  const uint32_t length = committed(pg, slot), end = min(length + tokens, pg.stride << pg.page_shift);
   const uint32_t rows = tokens * a.group, all = (rows + kWeightRows - 1) / kWeightRows;
-  const uint32_t per = (all + a.parts - 1) / a.parts, from = part * per, to = min(from + per, all);
-  const uint32_t in_page = (1u << pg.page_shift) - 1;
-  const __half* keys = pg.key + (static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) * pg.row + hk * D;
+  if (rows <= kFewRows) return;
+  const uint32_t length = committed(pg, slot), end = min(length + tokens, pg.stride << pg.page_shift);
+  const uint32_t per = (all + a.parts - 1) / a.parts, to = min(part * per + per, all);
+  const uint32_t token_bytes = a.q_heads * D * 2;
   const std::size_t plane = (static_cast<std::size_t>(i) * a.kv_heads + hk) * a.parts + part;
   float* sums = a.partial + plane * (static_cast<std::size_t>(pg.stride) << pg.page_shift);
   for (uint32_t at = column * kWeightPositions; at < end; at += a.columns * kWeightPositions) {
-    const uint32_t mine = at + 32 * wave, position = mine + n;
-    const int32_t page = position < end ? table_page(pg, slot, position >> pg.page_shift) : -1;
-    const __half* source = keys + ((static_cast<std::size_t>(max(page, 0)) << pg.page_shift) + (page < 0 ? 0 : position & in_page)) * pg.row;
-    h8 k[D / 16];
+    const uint32_t mine = at + 32 * P * wave;
+    // The step of token x's first row, of all those of a part at most.
+    auto step_of = [&](uint32_t x) { return static_cast<uint32_t>(min(static_cast<uint64_t>(x) * a.group / kWeightRows, static_cast<uint64_t>(to))); };
+    // Rows of tokens before length + t = at see nothing of these positions, those from seen on all of them.
+    const uint32_t from = max(part * per, at > length ? step_of(at - length) : 0u);
+    const uint32_t sees = min(at + kWeightPositions, end), seen = sees > length + 1 ? step_of(sees - length - 1 + (kWeightRows - 1) / a.group + 1) : 0;
+    float sum[16 * P] = {};
+    h8 k[P][D / 16];
+    if (from < to) {
 #pragma unroll
-    for (unsigned s = 0; s < D / 16; ++s) k[s] = *reinterpret_cast<const h8*>(source + 16 * s + 8 * h);
-    float sum[16] = {};
-    for (uint32_t x = from; x < to; ++x) {
-      const uint32_t row0 = x * kWeightRows;
-      // Rows before the tile's first position see nothing of it.
-      if (length + min(rows, row0 + kWeightRows) / a.group + 1 <= at) continue;
+      for (unsigned p = 0; p < P; ++p) {
+        const __half* row = key_row(a, slot, mine + 32 * p + n, end) + hk * D + 8 * h;
+#pragma unroll
+        for (unsigned st = 0; st < D / 16; ++st) k[p][st] = *reinterpret_cast<const h8*>(row + 16 * st);
+      }
+    }
+    // Steps [first, last).  Without `masked` every row of them sees every position; false: a row among them
+    // has a log sum that is not a number to subtract.
+    auto pass = [&](auto masked, uint32_t first, uint32_t last) __attribute__((always_inline)) {
+      if (first >= last) return true;
+      // The step whose rows are loaded next, its first row's token and head, and the lanes' rows.
+      uint32_t ahead = first, token = first * kWeightRows / a.group, head = first * kWeightRows - token * a.group;
+      RowWalk walk[kLoads], sum_walk;
+#pragma unroll
+      for (unsigned u = 0; u < kLoads; ++u) {
+        walk[u].start(first * kWeightRows + (wave + 4 * u) * kLoadRows + lane / (D / 8), token, a.group, token_bytes, 2 * D);
+      }
+      sum_walk.start(first * kWeightRows + n, token, a.group, a.q_heads * 4, 4);
+      // (Rows past the last one load that one.)
+      auto load = [&](_Float16* step, float& level) __attribute__((always_inline)) {
+        const std::size_t row = (static_cast<std::size_t>(first_row) + token) * a.q_heads + hk * a.group;
+        const uint32_t there = min(kWeightRows, tokens - 1 - token) * a.q_heads + a.group;  // rows from this one on
+        const auto queries = __builtin_amdgcn_make_buffer_rsrc(const_cast<__half*>(a.query + row * D), 0, static_cast<int>(there * (2 * D)), 0x20000);
+        const auto levels = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.log_sums + row), 0, static_cast<int>(there * 4), 0x20000);
+        level = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(levels, static_cast<int>(min(sum_walk.offset, there * 4 - 4)), 0, 0));
+#pragma unroll
+        for (unsigned u = 0; u < kLoads; ++u) {
+          const unsigned r = (wave + 4 * u) * kLoadRows + lane / (D / 8);
+          const unsigned piece = 16 * key_slot(lane % (D / 8), r);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(queries, (lds_void*)(step + (wave + 4 * u) * kLoadRows * D), 16,
+                                                   static_cast<int>(min(walk[u].offset, (there - 1) * (2 * D)) + piece), 0, 0, 0);
+        }
+        const bool more = ++ahead < last;
+        const uint32_t by = more ? kWeightRows % a.group : 0;
+        head += by;
+        const bool wrapped = head >= a.group;
+        head -= wrapped ? a.group : 0;
+        token += (more ? kWeightRows / a.group : 0) + (wrapped ? 1 : 0);
+#pragma unroll
+        for (unsigned u = 0; u < kLoads; ++u) walk[u].step(by, wrapped, a.group, token_bytes, 2 * D);
+        sum_walk.step(by, wrapped, a.group, a.q_heads * 4, 4);
+      };
+      f16v s[2][P] = {};
+      float level[kWeightRing] = {};
+      bool plain = true;
+      auto multiply = [&](unsigned d) __attribute__((always_inline)) {
+        // (Computed anew for each step: 32 addresses of 4 steps would take the registers of as many operands.)
+        unsigned place = n * (2 * D) + 16 * key_slot(h, n);
+        asm volatile("" : "+v"(place));
+#pragma unroll
+        for (unsigned st = 0; st < D / 16; ++st) {
+          const h8 q = *reinterpret_cast<const h8*>(reinterpret_cast<const char*>(ring[d]) + (place ^ 32 * st));
+#pragma unroll
+          for (unsigned p = 0; p < P; ++p) s[d % 2][p] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[p][st], q, st == 0 ? f16v{} : s[d % 2][p], 0, 0, 0);
+        }
+      };
+      // What the rows of s[d % 2] give to the positions.
+      auto add = [&](unsigned d, float level) __attribute__((always_inline)) {
+#pragma unroll
+        for (unsigned p = 0; p < P; ++p) {
+#pragma unroll
+          for (unsigned r = 0; r < 16; ++r) sum[16 * p + r] += __builtin_amdgcn_exp2f(fmaf(s[d % 2][p][r], a.scale, -level));
+        }
+      };
+      auto add_masked = [&](uint32_t x, unsigned d, float level) __attribute__((always_inline)) {
+        const uint32_t row = x * kWeightRows + n;
+        const int32_t visible = row < rows && level > -INFINITY  // not of a row that sees nothing, or a NaN
+                                    ? static_cast<int32_t>(length + row / a.group + 1 - mine - 4 * h) : 0;
+#pragma unroll
+        for (unsigned p = 0; p < P; ++p) {
+#pragma unroll
+          for (unsigned r = 0; r < 16; ++r) {
+            const float w = __builtin_amdgcn_exp2f(fmaf(s[d % 2][p][r], a.scale, -level));
+            sum[16 * p + r] += static_cast<int32_t>(32 * p + 8 * (r / 4) + r % 4) < visible ? w : 0.0F;
+          }
+        }
+      };
+#pragma unroll
+      for (unsigned d = 0; d + 1 < kWeightRing; ++d) {
+        load(ring[d], level[d]);
+        asm volatile("" ::: "memory");  // in this order: the waits below count them
+      }
+      auto turn = [&](uint32_t x, unsigned d) __attribute__((always_inline)) {
+        // This step has arrived when only the later ones are on their way.
+        wait_loads<2 * (kLoads + 1)>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const unsigned before = (d + kWeightRing - 1) % kWeightRing;
+        // Nothing yet before the first step: exponentials of zeros less infinity.
+        const float old = x == first ? INFINITY : level[before] * kLog2E;
+        if constexpr (!masked.value) plain &= x == first || fabsf(old) < INFINITY;
+        // Every wave has read the step before this one: its place takes the next loads.
+        load(ring[before], level[before]);
+        multiply(d);
+        if constexpr (masked.value) {
+          add_masked(x, d, level[d] * kLog2E);
+        } else {
+          add(d + 1, old);
+          constexpr unsigned kProducts = P * D / 16, kAhead = 4;
+          __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+          for (unsigned e = 0; e < kProducts; ++e) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x400, 16 * P / kProducts, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, 2 * 16 * P / kProducts + 1, 0);
+            if (e % P == 0) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          }
+        }
+        // (In this turn: left to itself the compiler moves all turns' exponentials behind the last one's products.)
+#pragma unroll
+        for (unsigned r = 0; r < 16 * P; ++r) asm volatile("" : "+v"(sum[r]));
+      };
+      uint32_t x = first;
+#pragma unroll 1
+      for (; x + kWeightRing <= last; x += kWeightRing) {
+#pragma unroll
+        for (unsigned d = 0; d < kWeightRing; ++d) turn(x + d, d);
+      }
+#pragma unroll
+      for (unsigned d = 0; d < kWeightRing; ++d) {
+        if (x + d < last) {
+          turn(x + d, d);
+        } else if (!masked.value && x + d == last) {
+          const float old = level[(d + kWeightRing - 1) % kWeightRing] * kLog2E;
+          plain &= fabsf(old) < INFINITY;
+          add(d + 1, old);
+        }
+      }
+      // No load writes into LDS when the next rows, or another workgroup's, come there.
+      wait_loads<0>();
       __syncthreads();
+      return plain;
+    };
+    // The steps without a mask, and those before and behind them; all with masks where that did not do.
+    uint32_t low = max(from, min(seen, to)), high = max(low, min(to, rows / kWeightRows));
+    if (__syncthreads_or(!pass(std::false_type{}, low, high))) {
 #pragma unroll
-      for (unsigned u = threadIdx.x; u < kWeightRows * D / 8; u += 256) {
-        const uint32_t r = u / (D / 8), c = u % (D / 8), row = min(row0 + r, rows - 1), t = row / a.group;
-        const std::size_t out_row = (static_cast<std::size_t>(first_row) + t) * a.q_heads + hk * a.group + (row - t * a.group);
-        *reinterpret_cast<u32x4*>(rows0 + r * D + 8 * key_slot(c, r)) = *reinterpret_cast<const u32x4*>(a.query + out_row * D + 8 * c);
-      }
-      __syncthreads();
-      const uint32_t row = row0 + n, t = row / a.group;
-      float level = INFINITY;
-      uint32_t visible = 0;
-      if (row < rows) {
-        level = a.log_sums[(static_cast<std::size_t>(first_row) + t) * a.q_heads + hk * a.group + (row - t * a.group)] * kLog2E;
-        visible = level > -INFINITY ? length + t + 1 : 0;   // a row that sees nothing, or a NaN
-      }
-      f16v s = f16v{};
-#pragma unroll
-      for (unsigned st = 0; st < D / 16; ++st) {
-        const h8 q = *reinterpret_cast<const h8*>(rows0 + n * D + 8 * key_slot(2 * st + h, n));
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[st], q, s, 0, 0, 0);
-      }
-#pragma unroll
-      for (unsigned r = 0; r < 16; ++r) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale, -level));
-        sum[r] += mine + 8 * (r / 4) + 4 * h + r % 4 < visible ? w : 0.0F;
-      }
+      for (unsigned r = 0; r < 16 * P; ++r) sum[r] = 0.0F;
+      low = high = to;
     }
-    // A position's sum lies over the 32 lanes of a half.
-#pragma unroll
-    for (unsigned r = 0; r < 16; ++r) {
-#pragma unroll
-      for (unsigned d = 1; d < 32; d <<= 1) sum[r] += __shfl_xor(sum[r], d);
-    }
-#pragma unroll
-    for (unsigned r = 0; r < 16; ++r) {
-      const uint32_t p = mine + 8 * (r / 4) + 4 * h + r % 4;
-      if (n == r && p < end) sums[p] = sum[r];
-    }
+#pragma unroll 1
+    for (unsigned e = 0; e < 2; ++e) pass(std::true_type{}, e == 0 ? from : high, e == 0 ? low : to);
+    // Lane n has the sum of register n of the 32: position 32 (r / 16) + 8 (r / 4 % 4) + 4 h + r % 4.
+    const float total = sum_lanes(sum);
+    const uint32_t position = mine + 32 * (n / 16) + 8 * (n / 4 % 4) + 4 * h + n % 4;
+    if (position < end) sums[position] = total;
   }
 }
 
-// Adds the planes of the KV heads and row parts, in their order, to what the positions have.
+// Adds the planes of the KV heads and row parts, in their order, to what the positions have: a lane a
+// position, a wave a quarter of the planes.
 __global__ __launch_bounds__(256) void weight_join_kernel(WeightArgs a) {
+  __shared__ float parts[4][64];
   const KvPages& pg = a.pages;
+  const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint32_t i = blockIdx.y, slot = listed_slot(a.list, i), tokens = a.list.first[i + 1] - a.list.first[i];
+  if (tokens * a.group <= kFewRows) return;
   const uint32_t capacity = pg.stride << pg.page_shift, end = min(committed(pg, slot) + tokens, capacity);
-  if (tokens == 0) return;
-  const uint32_t planes = a.kv_heads * a.parts;
-  for (uint32_t p = blockIdx.x * 256 + threadIdx.x; p < end; p += gridDim.x * 256) {
-    if (table_page(pg, slot, p >> pg.page_shift) < 0) continue;
-    const float* at = a.partial + static_cast<std::size_t>(i) * planes * capacity + p;
+  const uint32_t planes = a.kv_heads * a.parts, quarter = (planes + 3) / 4;
+  for (uint32_t at = blockIdx.x * 64; at < end; at += gridDim.x * 64) {
+    const uint32_t p = at + lane;
+    const float* source = a.partial + static_cast<std::size_t>(i) * planes * capacity + min(p, end - 1);
     float sum = 0.0F;
-    for (uint32_t x = 0; x < planes; ++x) sum += at[static_cast<std::size_t>(x) * capacity];
-    a.weights.weight[static_cast<std::size_t>(slot) * capacity + p] += sum;
+#pragma unroll 8
+    for (uint32_t x = wave * quarter; x < min(wave * quarter + quarter, planes); ++x) sum += source[static_cast<std::size_t>(x) * capacity];
+    parts[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && p < end && table_page(pg, slot, p >> pg.page_shift) >= 0) {
+      a.weights.weight[static_cast<std::size_t>(slot) * capacity + p] += parts[0][lane] + parts[1][lane] + parts[2][lane] + parts[3][lane];
+    }
+    __syncthreads();
   }
 }
 
@@ -918,18 +1138,37 @@ std::size_t chunk_bytes(const ChunkShape& s, const ChunkList& list, uint32_t q_h
   return static_cast<std::size_t>(list.first[kMaxChunks]) * q_heads * s.ranges * (head_size + 2) * sizeof(float);
 }
 
-uint32_t weight_parts(const KvPages& p, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads, uint32_t& columns) {
+// How the rows of the long chunks are divided: workgroups along the positions, and parts of the rows.
+struct WeightShape {
+  uint32_t columns, parts;
+  bool few, many;  // sequences of at most kFewRows rows, of more
+};
+
+WeightShape weight_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads) {
+  WeightShape s{};
   const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift;
-  columns = static_cast<uint32_t>(std::min<uint64_t>((capacity + kWeightPositions - 1) / kWeightPositions, 1024));
-  uint32_t most = 0;
-  for (uint32_t i = 0; i < list.count; ++i) most = std::max(most, list.first[i + 1] - list.first[i]);
+  s.columns = static_cast<uint32_t>(std::min<uint64_t>((capacity + kWeightPositions - 1) / kWeightPositions, 1024));
+  uint32_t most = 0, long_ones = 0;
+  for (uint32_t i = 0; i < list.count; ++i) {
+    const uint32_t tokens = list.first[i + 1] - list.first[i];
+    most = std::max(most, tokens);
+    const bool many = static_cast<uint64_t>(tokens) * (q_heads / kv_heads) > kFewRows;
+    s.few |= !many && tokens != 0;
+    s.many |= many;
+    long_ones += many;
+  }
+  s.parts = 1;
+  if (!s.many) return s;
   const uint64_t blocks = (static_cast<uint64_t>(most) * (q_heads / kv_heads) + kWeightRows - 1) / kWeightRows;
-  const uint64_t items = static_cast<uint64_t>(columns) * kv_heads * list.count;
-  return static_cast<uint32_t>(std::clamp<uint64_t>(4 * kComputeUnits / items, 1, std::max<uint64_t>(1, blocks / 4)));
+  const uint64_t items = static_cast<uint64_t>(s.columns) * kv_heads * long_ones;
+  s.parts = static_cast<uint32_t>(std::clamp<uint64_t>(4 * kComputeUnits / items, 1, std::max<uint64_t>(1, blocks / 8)));
+  return s;
 }
 
-std::size_t weight_bytes(const KvPages& p, const ChunkList& list, uint32_t kv_heads, uint32_t parts) {
-  return static_cast<std::size_t>(list.count) * kv_heads * parts * (static_cast<std::size_t>(p.stride) << p.page_shift) * sizeof(float);
+// (At least a little, also where nothing is divided: a workspace is always given.)
+std::size_t weight_bytes(const KvPages& p, const ChunkList& list, uint32_t kv_heads, const WeightShape& s) {
+  if (!s.many) return 16;
+  return static_cast<std::size_t>(list.count) * kv_heads * s.parts * (static_cast<std::size_t>(p.stride) << p.page_shift) * sizeof(float);
 }
 
 }  // namespace
@@ -1012,8 +1251,7 @@ extern "C" size_t gfxinfer_kv_weights_workspace_bytes(const gfxinfer_kv_pages* p
     if (const int32_t s = read_heads(pages, q_heads); s != GFXI_OK) return s;
     const std::vector<uint32_t> any(std::min(count, kMaxChunks + 1), 0u);
     if (const int32_t s = read_chunks(p, any.data(), tokens, count, false, list); s != GFXI_OK) return s;
-    uint32_t columns;
-    bytes = weight_bytes(p, list, pages->kv_heads, weight_parts(p, list, q_heads, pages->kv_heads, columns));
+    bytes = weight_bytes(p, list, pages->kv_heads, weight_shape(p, list, q_heads, pages->kv_heads));
     return GFXI_OK;
   });
   return bytes;
@@ -1034,8 +1272,10 @@ extern "C" int32_t gfxinfer_launch_kv_weights_add(const gfxinfer_kv_pages* pages
       return fail(GFXI_INVALID_ARGUMENT, "weights need a layer of the cache, 16-byte aligned queries and their log sums");
     }
     a.kv_heads = pages->kv_heads;
-    a.parts = weight_parts(a.pages, a.list, q_heads, a.kv_heads, a.columns);
-    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < weight_bytes(a.pages, a.list, a.kv_heads, a.parts)) {
+    const WeightShape shape = weight_shape(a.pages, a.list, q_heads, a.kv_heads);
+    a.parts = shape.parts;
+    a.columns = shape.columns;
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < weight_bytes(a.pages, a.list, a.kv_heads, shape)) {
       return fail(GFXI_INVALID_ARGUMENT, "K/V weights workspace is null, not 16-byte aligned or too small");
     }
     a.query = reinterpret_cast<const __half*>(query);
@@ -1046,12 +1286,19 @@ extern "C" int32_t gfxinfer_launch_kv_weights_add(const gfxinfer_kv_pages* pages
     a.group = q_heads / a.kv_heads;
     a.scale = kLog2E / std::sqrt(static_cast<float>(pages->head_size));
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    const uint64_t capacity = static_cast<uint64_t>(a.pages.stride) << a.pages.page_shift;
+    if (shape.few) {
+      const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((capacity + 31) / 32, 1024)), count);
+      if (pages->head_size == 128) hipLaunchKernelGGL(few_weight_kernel<128>, grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL(few_weight_kernel<256>, grid, dim3(256), 0, st, a);
+      if (const int32_t s = launch_status("K/V weights launch failed"); s != GFXI_OK) return s;
+    }
+    if (!shape.many) return GFXI_OK;
     const dim3 grid(a.columns * a.kv_heads * a.parts, count);
     if (pages->head_size == 128) hipLaunchKernelGGL(weight_kernel<128>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(weight_kernel<256>, grid, dim3(256), 0, st, a);
     if (const int32_t s = launch_status("K/V weights launch failed"); s != GFXI_OK) return s;
-    const uint64_t capacity = static_cast<uint64_t>(a.pages.stride) << a.pages.page_shift;
-    hipLaunchKernelGGL(weight_join_kernel, dim3(static_cast<unsigned>(std::min<uint64_t>((capacity + 255) / 256, 1024)), count),
+    hipLaunchKernelGGL(weight_join_kernel, dim3(static_cast<unsigned>(std::min<uint64_t>((capacity + 63) / 64, 1024)), count),
                        dim3(256), 0, st, a);
     return launch_status("K/V weights join launch failed");
   });
