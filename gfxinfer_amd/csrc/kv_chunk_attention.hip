@@ -934,6 +934,14 @@ __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightA
         for (unsigned st = 0; st < D / 16; ++st) k[p][st] = *reinterpret_cast<const h8*>(row + 16 * st);
       }
     }
+    if constexpr (D == 256) {
+      // (K in accumulation registers, which leaves the others to the scores and sums.)
+#pragma unroll
+      for (unsigned p = 0; p < P; ++p) {
+#pragma unroll
+        for (unsigned st = 0; st < D / 16; ++st) asm volatile("" : "+a"(k[p][st]));
+      }
+    }
     // Steps [first, last).  Without `masked` every row of them sees every position; false: a row among them
     // has a log sum that is not a number to subtract.
     auto pass = [&](auto masked, uint32_t first, uint32_t last) __attribute__((always_inline)) {
@@ -946,51 +954,59 @@ __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightA
         walk[u].start(first * kWeightRows + (wave + 4 * u) * kLoadRows + lane / (D / 8), token, a.group, token_bytes, 2 * D);
       }
       sum_walk.start(first * kWeightRows + n, token, a.group, a.q_heads * 4, 4);
-      // (Rows past the last one load that one.)
+      // Where the lanes' parts of the step are (rows past the last one load that one).
+      uint32_t there, part_at[kLoads], level_at;  // rows from the step's first one on; bytes
+      const uint32_t load_row = wave * kLoadRows + lane / (D / 8);
+      auto place_part = [&](unsigned u) __attribute__((always_inline)) {
+        part_at[u] = min(walk[u].offset, (there - 1) * (2 * D)) + 16 * key_slot(lane % (D / 8), load_row + 4 * u * kLoadRows);
+      };
+      auto place_level = [&] { level_at = min(sum_walk.offset, there * 4 - 4); };
+      auto count = [&] { there = min(kWeightRows, tokens - 1 - token) * a.q_heads + a.group; };
       auto load = [&](_Float16* step, float& level) __attribute__((always_inline)) {
         const std::size_t row = (static_cast<std::size_t>(first_row) + token) * a.q_heads + hk * a.group;
-        const uint32_t there = min(kWeightRows, tokens - 1 - token) * a.q_heads + a.group;  // rows from this one on
         const auto queries = __builtin_amdgcn_make_buffer_rsrc(const_cast<__half*>(a.query + row * D), 0, static_cast<int>(there * (2 * D)), 0x20000);
         const auto levels = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.log_sums + row), 0, static_cast<int>(there * 4), 0x20000);
-        level = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(levels, static_cast<int>(min(sum_walk.offset, there * 4 - 4)), 0, 0));
+        level = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(levels, static_cast<int>(level_at), 0, 0));
 #pragma unroll
         for (unsigned u = 0; u < kLoads; ++u) {
-          const unsigned r = (wave + 4 * u) * kLoadRows + lane / (D / 8);
-          const unsigned piece = 16 * key_slot(lane % (D / 8), r);
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(queries, (lds_void*)(step + (wave + 4 * u) * kLoadRows * D), 16,
-                                                   static_cast<int>(min(walk[u].offset, (there - 1) * (2 * D)) + piece), 0, 0, 0);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(queries, (lds_void*)(step + (wave + 4 * u) * kLoadRows * D), 16, static_cast<int>(part_at[u]), 0, 0, 0);
         }
-        const bool more = ++ahead < last;
-        const uint32_t by = more ? kWeightRows % a.group : 0;
-        head += by;
-        const bool wrapped = head >= a.group;
-        head -= wrapped ? a.group : 0;
-        token += (more ? kWeightRows / a.group : 0) + (wrapped ? 1 : 0);
-#pragma unroll
-        for (unsigned u = 0; u < kLoads; ++u) walk[u].step(by, wrapped, a.group, token_bytes, 2 * D);
-        sum_walk.step(by, wrapped, a.group, a.q_heads * 4, 4);
       };
+      // On to the next step, in kLoads + 2 pieces of work.
+      uint32_t by = 0;
+      bool wrapped = false;
+      auto advance = [&](unsigned piece) __attribute__((always_inline)) {
+        if (piece == 0) {
+          const bool more = ++ahead < last;
+          by = more ? kWeightRows % a.group : 0;
+          head += by;
+          wrapped = head >= a.group;
+          head -= wrapped ? a.group : 0;
+          token += (more ? kWeightRows / a.group : 0) + (wrapped ? 1 : 0);
+          count();
+        } else if (piece <= kLoads) {
+          walk[piece - 1].step(by, wrapped, a.group, token_bytes, 2 * D);
+          place_part(piece - 1);
+        } else {
+          sum_walk.step(by, wrapped, a.group, a.q_heads * 4, 4);
+          place_level();
+        }
+      };
+      count();
+#pragma unroll
+      for (unsigned u = 0; u < kLoads; ++u) place_part(u);
+      place_level();
       f16v s[2][P] = {};
       float level[kWeightRing] = {};
       bool plain = true;
-      auto multiply = [&](unsigned d) __attribute__((always_inline)) {
-        // (Computed anew for each step: 32 addresses of 4 steps would take the registers of as many operands.)
-        unsigned place = n * (2 * D) + 16 * key_slot(h, n);
-        asm volatile("" : "+v"(place));
-#pragma unroll
-        for (unsigned st = 0; st < D / 16; ++st) {
-          const h8 q = *reinterpret_cast<const h8*>(reinterpret_cast<const char*>(ring[d]) + (place ^ 32 * st));
-#pragma unroll
-          for (unsigned p = 0; p < P; ++p) s[d % 2][p] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[p][st], q, st == 0 ? f16v{} : s[d % 2][p], 0, 0, 0);
-        }
+      // A piece of the step's rows: the B operand of product st.
+      auto read = [&](unsigned d, unsigned place, unsigned st) __attribute__((always_inline)) {
+        return *reinterpret_cast<const h8*>(reinterpret_cast<const char*>(ring[d]) + (place ^ 32 * st));
       };
-      // What the rows of s[d % 2] give to the positions.
-      auto add = [&](unsigned d, float level) __attribute__((always_inline)) {
+      // What rows n of s[d % 2] give to positions 4 h + [first, last) in the accumulators' order.
+      auto add = [&](unsigned d, float level, unsigned first, unsigned last) __attribute__((always_inline)) {
 #pragma unroll
-        for (unsigned p = 0; p < P; ++p) {
-#pragma unroll
-          for (unsigned r = 0; r < 16; ++r) sum[16 * p + r] += __builtin_amdgcn_exp2f(fmaf(s[d % 2][p][r], a.scale, -level));
-        }
+        for (unsigned e = first; e < last; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(s[d % 2][e / 16][e % 16], a.scale, -level));
       };
       auto add_masked = [&](uint32_t x, unsigned d, float level) __attribute__((always_inline)) {
         const uint32_t row = x * kWeightRows + n;
@@ -1009,6 +1025,8 @@ __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightA
       for (unsigned d = 0; d + 1 < kWeightRing; ++d) {
         load(ring[d], level[d]);
         asm volatile("" ::: "memory");  // in this order: the waits below count them
+#pragma unroll
+        for (unsigned e = 0; e < kLoads + 2; ++e) advance(e);
       }
       auto turn = [&](uint32_t x, unsigned d) __attribute__((always_inline)) {
         // This step has arrived when only the later ones are on their way.
@@ -1019,22 +1037,32 @@ __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightA
         // Nothing yet before the first step: exponentials of zeros less infinity.
         const float old = x == first ? INFINITY : level[before] * kLog2E;
         if constexpr (!masked.value) plain &= x == first || fabsf(old) < INFINITY;
+        // (Computed anew for each step: 32 addresses of 4 steps would take the registers of as many operands.)
+        unsigned place = n * (2 * D) + 16 * key_slot(h, n);
+        asm volatile("" : "+v"(place));
+        constexpr unsigned kSteps = D / 16, kAhead = 3, kEach = 16 * P / kSteps;
+        h8 q[kAhead + 1];
+#pragma unroll
+        for (unsigned st = 0; st < kAhead; ++st) q[st] = read(d, place, st);
+        __builtin_amdgcn_sched_barrier(0);
         // Every wave has read the step before this one: its place takes the next loads.
         load(ring[before], level[before]);
-        multiply(d);
-        if constexpr (masked.value) {
-          add_masked(x, d, level[d] * kLog2E);
-        } else {
-          add(d + 1, old);
-          constexpr unsigned kProducts = P * D / 16, kAhead = 4;
-          __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+        // Products, reads three ahead of them and the last step's exponentials, in this order.
 #pragma unroll
-          for (unsigned e = 0; e < kProducts; ++e) {
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x400, 16 * P / kProducts, 0);
-            __builtin_amdgcn_sched_group_barrier(0x2, 2 * 16 * P / kProducts + 1, 0);
-            if (e % P == 0) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          }
+        for (unsigned st = 0; st < kSteps; ++st) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (st + kAhead < kSteps) q[(st + kAhead) % (kAhead + 1)] = read(d, place, st + kAhead);
+#pragma unroll
+          for (unsigned p = 0; p < P; ++p) s[d % 2][p] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[p][st], q[st % (kAhead + 1)], st == 0 ? f16v{} : s[d % 2][p], 0, 0, 0);
+          if constexpr (!masked.value) add(d + 1, old, kEach * st, kEach * st + kEach);
+          if (st < kLoads + 2) advance(st);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (masked.value) add_masked(x, d, level[d] * kLog2E);
+        if constexpr (D == 256) {
+          // (In the registers that the vector unit reads.)
+#pragma unroll
+          for (unsigned p = 0; p < P; ++p) asm volatile("" : "+v"(s[d % 2][p]));
         }
         // (In this turn: left to itself the compiler moves all turns' exponentials behind the last one's products.)
 #pragma unroll
@@ -1053,7 +1081,7 @@ __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightA
         } else if (!masked.value && x + d == last) {
           const float old = level[(d + kWeightRing - 1) % kWeightRing] * kLog2E;
           plain &= fabsf(old) < INFINITY;
-          add(d + 1, old);
+          add(d + 1, old, 0, 16 * P);
         }
       }
       // No load writes into LDS when the next rows, or another workgroup's, come there.
@@ -1161,7 +1189,7 @@ WeightShape weight_shape(const KvPages& p, const ChunkList& list, uint32_t q_hea
   if (!s.many) return s;
   const uint64_t blocks = (static_cast<uint64_t>(most) * (q_heads / kv_heads) + kWeightRows - 1) / kWeightRows;
   const uint64_t items = static_cast<uint64_t>(s.columns) * kv_heads * long_ones;
-  s.parts = static_cast<uint32_t>(std::clamp<uint64_t>(4 * kComputeUnits / items, 1, std::max<uint64_t>(1, blocks / 8)));
+  s.parts = static_cast<uint32_t>(std::clamp<uint64_t>(6 * kComputeUnits / items, 1, std::max<uint64_t>(1, blocks / 8)));
   return s;
 }
 
