@@ -11,6 +11,7 @@
 // commits (move_kernel).
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "kv_weights.hpp"
 
@@ -19,7 +20,7 @@ namespace {
 
 using u32x4 = unsigned __attribute__((ext_vector_type(4)));
 
-constexpr unsigned kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
+constexpr unsigned kGrantThreads = 1024;
 
 // The workspace: a header per sequence, then its moves and its copies, then the bits of kept
 // rows.  All offsets by the host's sizes alone.
@@ -53,7 +54,7 @@ struct EvictArgs {
   int32_t* status;
 };
 
-__device__ __forceinline__ uint32_t capacity_of(const KvPages& p) { return p.stride << p.page_shift; }
+__host__ __device__ __forceinline__ uint32_t capacity_of(const KvPages& p) { return p.stride << p.page_shift; }
 
 // Order of weights as unsigned numbers; NaN above all, the zeros equal.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -62,20 +63,37 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
 }
 
+// Sum over the lanes up to this one: within rows of 16, then the rows before (no trips through LDS).
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
+  auto from = [](uint32_t x, auto control, auto rows) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), control.value, rows.value, 0xf, false));
+  };
+  using Shift1 = std::integral_constant<int, 0x111>;
+  using Shift2 = std::integral_constant<int, 0x112>;
+  using Shift4 = std::integral_constant<int, 0x114>;
+  using Shift8 = std::integral_constant<int, 0x118>;
+  using Last15 = std::integral_constant<int, 0x142>;  // a row's last lane to the next row
+  using Last31 = std::integral_constant<int, 0x143>;  // lane 31 to the upper rows
+  using All = std::integral_constant<int, 0xf>;
+  v += from(v, Shift1{}, All{});
+  v += from(v, Shift2{}, All{});
+  v += from(v, Shift4{}, All{});
+  v += from(v, Shift8{}, All{});
+  v += from(v, Last15{}, std::integral_constant<int, 0xa>{});
+  v += from(v, Last31{}, std::integral_constant<int, 0xc>{});
+  return v;
+}
+
+template <unsigned Waves>
 __device__ __forceinline__ uint32_t scan_waves(uint32_t v, uint32_t* partial, uint32_t& total) {
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  uint32_t sum = v;
-#pragma unroll
-  for (unsigned d = 1; d < 64; d <<= 1) {
-    const uint32_t o = __shfl_up(sum, d);
-    if (lane >= d) sum += o;
-  }
+  const uint32_t sum = scan_lanes(v);
   if (lane == 63u) partial[wave] = sum;
   __syncthreads();
   uint32_t before = 0;
   total = 0;
 #pragma unroll
-  for (unsigned w = 0; w < kSelectWaves; ++w) {
+  for (unsigned w = 0; w < Waves; ++w) {
     const uint32_t part = partial[w];
     if (w < wave) before += part;
     total += part;
@@ -84,128 +102,201 @@ __device__ __forceinline__ uint32_t scan_waves(uint32_t v, uint32_t* partial, ui
   return before + sum - v;
 }
 
+constexpr unsigned kSelectKeys = 4;  // of a thread
+
+// Numbers of the lanes' flags among those of a block of rows, of keys e * threads + thread in this order: the
+// flags before a lane's own.  counts has room for each wave's of each key; one barrier.
+template <unsigned Waves>
+__device__ __forceinline__ void rank_flags(const bool (&flag)[kSelectKeys], uint32_t* counts, uint32_t (&rank)[kSelectKeys], uint32_t& total) {
+  static_assert(kSelectKeys * Waves <= 64);
+  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+  for (unsigned e = 0; e < kSelectKeys; ++e) {
+    const uint64_t bits = __ballot(flag[e]);
+    rank[e] = static_cast<uint32_t>(__popcll(bits & ((1ull << lane) - 1)));
+    if (lane == 0) counts[e * Waves + wave] = static_cast<uint32_t>(__popcll(bits));
+  }
+  __syncthreads();
+  const uint32_t mine = lane < kSelectKeys * Waves ? counts[lane] : 0;
+  const uint32_t upto = scan_lanes(mine);
+#pragma unroll
+  for (unsigned e = 0; e < kSelectKeys; ++e) rank[e] += __builtin_amdgcn_readlane(upto - mine, e * Waves + wave);
+  total = __builtin_amdgcn_readlane(upto, 63);
+}
+
 // Chooses the rows of one sequence: the number of rows that stay for their position, then the
 // key of the last row that fits (a radix select over 8 bits a pass, largest first), then in row
-// order which rows stay, and the lists of holes and movers.
-__global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictArgs a) {
-  __shared__ uint32_t histogram[256];
-  __shared__ uint32_t partial[kSelectWaves];
-  __shared__ uint32_t chosen[3];  // digit, how many of it are wanted
-  const unsigned tid = threadIdx.x, lane = tid & 63u;
+// order which rows stay, and the lists of holes and movers.  Up to four rows a thread lie in
+// registers all the while; each pass has one barrier, its own counts and every wave looks for the digit.
+template <unsigned Threads>
+__global__ __launch_bounds__(Threads) void select_kernel(EvictArgs a) {
+  constexpr unsigned kWaves = Threads / 64;
+  constexpr uint32_t kRows = Threads * kSelectKeys;
+  constexpr unsigned kCopies = 4;  // of the counts, one for every fourth wave: the first digits of many weights are the same
+  __shared__ uint32_t histogram[4][kCopies][256];
+  __shared__ uint32_t partial[kWaves];
+  __shared__ uint32_t counts[3][64];
+  const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const KvPages& pg = a.pages;
   const uint32_t i = blockIdx.x, slot = listed_slot(a.list, i);
-  const uint32_t capacity = capacity_of(pg), n = min(pg.lengths[slot], capacity);
+  const uint32_t capacity = capacity_of(pg), n = min(pg.lengths[slot], capacity), dropped = a.weights.dropped[slot];
+  const std::size_t base = static_cast<std::size_t>(slot) * capacity;
+  const float* weight = a.weights.weight + base;
+  const int32_t* position = a.weights.position + base;
+  float w[kSelectKeys];
+  int32_t p[kSelectKeys];
+  auto fetch = [&](uint32_t from) __attribute__((always_inline)) {
+#pragma unroll
+    for (unsigned e = 0; e < kSelectKeys; ++e) {
+      const uint32_t row = min(from + e * Threads + tid, capacity - 1);
+      w[e] = weight[row];
+      p[e] = position[row];
+    }
+  };
+  // All that the choice reads is asked for before the length is there.
+  fetch(0);
+  const uint32_t columns = pages_for(a.budget, pg.page_shift), page_tokens = 1u << pg.page_shift;
+  const int32_t first_page = tid < min(columns, pg.stride) ? table_page(pg, slot, tid) : -1;
+  const uint32_t first_holders = first_page >= 0 ? pg.references[first_page] : 0;
   if (n <= a.budget) {
     if (tid == 0) a.headers[i] = EvictHeader{0, 0, 0, 0};
     return;
   }
-  const std::size_t base = static_cast<std::size_t>(slot) * capacity;
-  const float* weight = a.weights.weight + base;
-  const int32_t* position = a.weights.position + base;
-  const int64_t last = static_cast<int64_t>(n) + a.weights.dropped[slot] - a.recent;  // positions from here on stay
-  auto fixed = [&](uint32_t row) __attribute__((always_inline)) {
-    const int32_t p = position[row];
-    return p < static_cast<int64_t>(a.first) || p >= last;
+  const int64_t last = static_cast<int64_t>(n) + dropped - a.recent;  // positions from here on stay
+  uint32_t key[kSelectKeys];
+  bool fixed[kSelectKeys], there[kSelectKeys];
+  auto take = [&](uint32_t from) __attribute__((always_inline)) {
+#pragma unroll
+    for (unsigned e = 0; e < kSelectKeys; ++e) {
+      there[e] = from + e * Threads + tid < n;
+      key[e] = order_of(w[e]);
+      fixed[e] = there[e] && (p[e] < static_cast<int64_t>(a.first) || p[e] >= last);
+    }
   };
+  auto load = [&](uint32_t from) __attribute__((always_inline)) {
+    fetch(from);
+    take(from);
+  };
+  if constexpr (Threads == 256) __builtin_assume(n <= kRows);  // the table holds no more
+  const bool resident = n <= kRows;
+  for (uint32_t x = tid; x < 4 * kCopies * 256; x += Threads) (&histogram[0][0][0])[x] = 0;
   uint32_t mine = 0;
-  for (uint32_t row = tid; row < n; row += kSelectThreads) mine += fixed(row) ? 1u : 0u;
-  uint32_t protected_rows;
-  scan_waves(mine, partial, protected_rows);
-  // At most first + recent <= budget where positions are distinct, as begin makes them.
-  const uint32_t room = a.budget - min(protected_rows, a.budget);
-  const bool crowded = protected_rows > a.budget;  // damaged positions: then none is protected
-  uint32_t wanted = crowded ? a.budget : room, prefix = 0;
-  bool none = wanted == 0;
-  for (int shift = 24; shift >= 0 && !none; shift -= 8) {
-    if (tid < 256) histogram[tid] = 0;
-    __syncthreads();
-    const uint32_t high = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (uint32_t row = tid; row < n; row += kSelectThreads) {
-      const uint32_t key = order_of(weight[row]);
-      if ((key & high) == prefix && (crowded || !fixed(row))) atomicAdd(&histogram[key >> shift & 255u], 1u);
-    }
-    __syncthreads();
-    // The digit in which the wanted-th largest lies: the first wave sums from the top.
-    if (tid < 64) {
-      uint32_t four[4], sum = 0;
+#pragma unroll 1
+  for (uint32_t from = 0; from < n; from += kRows) {
+    if (from != 0) fetch(from);
+    take(from);
 #pragma unroll
-      for (unsigned e = 0; e < 4; ++e) {
-        four[e] = histogram[255u - (4 * lane + e)];
-        sum += four[e];
-      }
-      uint32_t upto = sum;
-#pragma unroll
-      for (unsigned d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(upto, d);
-        if (lane >= d) upto += o;
-      }
-      uint32_t before = upto - sum;
-#pragma unroll
-      for (unsigned e = 0; e < 4; ++e) {
-        if (before < wanted && wanted <= before + four[e]) {
-          chosen[0] = 255u - (4 * lane + e);
-          chosen[1] = wanted - before;
-        }
-        before += four[e];
-      }
-    }
-    __syncthreads();
-    prefix |= chosen[0] << shift;
-    wanted = chosen[1];
-    __syncthreads();
+    for (unsigned e = 0; e < kSelectKeys; ++e) mine += fixed[e] ? 1u : 0u;
   }
-  // Rows above the key stay, and the first `wanted` of those at it.
-  const uint32_t key_at = prefix;
+  uint32_t protected_rows;
+  scan_waves<kWaves>(mine, partial, protected_rows);
+  // At most first + recent <= budget where positions are distinct, as begin makes them.
+  const bool crowded = protected_rows > a.budget;  // damaged positions: then none is protected
+  uint32_t wanted = crowded ? a.budget : a.budget - protected_rows, prefix = 0, high = 0;
+  const bool none = wanted == 0;
+  bool exact = none;  // all rows of this prefix stay, later digits do not matter
+#pragma unroll 1
+  for (int shift = 24; shift >= 0 && !exact; shift -= 8) {
+    uint32_t (&own)[256] = histogram[shift / 8][wave % kCopies];
+#pragma unroll 1
+    for (uint32_t from = 0; from < n; from += kRows) {
+      if (!resident) load(from);
+#pragma unroll
+      for (unsigned e = 0; e < kSelectKeys; ++e) {
+        if (there[e] && (key[e] & high) == prefix && (crowded || !fixed[e])) atomicAdd(&own[key[e] >> shift & 255u], 1u);
+      }
+    }
+    __syncthreads();
+    // The digit in which the wanted-th largest lies: sums from the top, four digits a lane.
+    uint32_t four[4] = {}, sum = 0;
+#pragma unroll
+    for (unsigned c = 0; c < kCopies; ++c) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(&histogram[shift / 8][c][252u - 4 * lane]);
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) four[e] += x[3 - e];
+    }
+#pragma unroll
+    for (unsigned e = 0; e < 4; ++e) sum += four[e];
+    const uint32_t upto = scan_lanes(sum);
+    uint32_t before = upto - sum, digit = 0, rest = 0;
+    bool found = false, all = false;
+#pragma unroll
+    for (unsigned e = 0; e < 4; ++e) {
+      if (before < wanted && wanted <= before + four[e]) {
+        found = true;
+        digit = 255u - (4 * lane + e);
+        rest = wanted - before;
+        all = rest == four[e];
+      }
+      before += four[e];
+    }
+    // (One lane finds it: there are more rows than wanted.)
+    const int at = __ffsll(static_cast<unsigned long long>(__ballot(found))) - 1;
+    prefix |= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(digit), at)) << shift;
+    wanted = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rest), at));
+    exact = __builtin_amdgcn_readlane(all ? 1 : 0, at) != 0;
+    high |= 255u << shift;
+  }
+  // Rows above the prefix stay, and the first `wanted` of those at it.
   uint32_t* kept_bits = a.kept + static_cast<std::size_t>(i) * a.kept_words;
   RowMove* moves = a.moves + static_cast<std::size_t>(i) * a.most_moves;
   uint32_t ties = 0, holes = 0, movers = 0;
-  for (uint32_t from = 0; from < n; from += kSelectThreads) {
-    const uint32_t row = from + tid;
-    bool stays = false, tie = false;
-    if (row < n) {
-      const bool stands = !crowded && fixed(row);
-      const uint32_t key = order_of(weight[row]);
-      stays = stands || (!none && key > key_at);
-      tie = !stands && !none && key == key_at;
+#pragma unroll 1
+  for (uint32_t from = 0; from < n; from += kRows) {
+    if (!resident) load(from);
+    bool stays[kSelectKeys], tie[kSelectKeys];
+#pragma unroll
+    for (unsigned e = 0; e < kSelectKeys; ++e) {
+      const bool stands = there[e] && !crowded && fixed[e];
+      stays[e] = stands || (there[e] && !none && (key[e] & high) > prefix);
+      tie[e] = there[e] && !stands && !none && (key[e] & high) == prefix;
     }
-    uint32_t total;
-    const uint32_t rank = ties + scan_waves(tie ? 1u : 0u, partial, total);
+    uint32_t rank[kSelectKeys], total;
+    rank_flags<kWaves>(tie, counts[0], rank, total);
+    bool hole[kSelectKeys], mover[kSelectKeys];
+#pragma unroll
+    for (unsigned e = 0; e < kSelectKeys; ++e) {
+      const uint32_t first = from + e * Threads + 64 * wave, row = first + lane;  // 32 | first
+      stays[e] |= tie[e] && ties + rank[e] < wanted;
+      hole[e] = row < a.budget && !stays[e];
+      mover[e] = row >= a.budget && stays[e];
+      const uint64_t bits = __ballot(stays[e] && row < a.budget);
+      if (lane == 0 && first / 32 < a.kept_words) kept_bits[first / 32] = static_cast<uint32_t>(bits);
+      if (lane == 32 && first / 32 + 1 < a.kept_words) kept_bits[first / 32 + 1] = static_cast<uint32_t>(bits >> 32);
+    }
     ties += total;
-    stays |= tie && rank < wanted;
-    const bool hole = row < a.budget && !stays, mover = row >= a.budget && row < n && stays;
-    const uint64_t bits = __ballot(stays && row < a.budget);
-    if (lane == 0 && row / 32 < a.kept_words) kept_bits[row / 32] = static_cast<uint32_t>(bits);
-    if (lane == 32 && row / 32 < a.kept_words) kept_bits[row / 32] = static_cast<uint32_t>(bits >> 32);
-    // Holes in the low half, movers in the high half: at most 1024 each.
-    const uint32_t both = scan_waves((hole ? 1u : 0u) | (mover ? 1u : 0u) << 16, partial, total);
-    if (hole) {
-      const uint32_t at = holes + (both & 0xffffu);
-      if (at < a.most_moves) moves[at].target = row;
+    rank_flags<kWaves>(hole, counts[1], rank, total);
+#pragma unroll
+    for (unsigned e = 0; e < kSelectKeys; ++e) {
+      if (hole[e] && holes + rank[e] < a.most_moves) moves[holes + rank[e]].target = from + e * Threads + tid;
     }
-    if (mover) {
-      const uint32_t at = movers + (both >> 16);
-      if (at < a.most_moves) {
-        moves[at].page = table_page(pg, slot, row >> pg.page_shift);
-        moves[at].row = row & ((1u << pg.page_shift) - 1);
-        moves[at].source = row;
+    holes += total;
+    rank_flags<kWaves>(mover, counts[2], rank, total);
+#pragma unroll
+    for (unsigned e = 0; e < kSelectKeys; ++e) {
+      const uint32_t row = from + e * Threads + tid;
+      if (mover[e] && movers + rank[e] < a.most_moves) {
+        RowMove& move = moves[movers + rank[e]];
+        move.page = table_page(pg, slot, row >> pg.page_shift);
+        move.row = row & ((1u << pg.page_shift) - 1);
+        move.source = row;
       }
     }
-    holes += total & 0xffffu;
-    movers += total >> 16;
+    movers += total;
   }
   __threadfence_block();
   __syncthreads();
   // Pages with a hole that other sequences hold too.
   PageCopy* copies = a.copies + static_cast<std::size_t>(i) * a.most_copies;
-  const uint32_t columns = pages_for(a.budget, pg.page_shift), page_tokens = 1u << pg.page_shift;
   uint32_t found = 0;
-  for (uint32_t from = 0; from < columns; from += kSelectThreads) {
+#pragma unroll 1
+  for (uint32_t from = 0; from < columns; from += Threads) {
     const uint32_t column = from + tid;
     int32_t page = -1;
     bool copy = false;
     if (column < columns) {
-      page = table_page(pg, slot, column);
-      if (page >= 0 && pg.references[page] > 1) {
+      page = from == 0 ? first_page : table_page(pg, slot, column);
+      if (page >= 0 && (from == 0 ? first_holders : pg.references[page]) > 1) {
         // A row of the page before the budget whose bit is off.
         const uint32_t begin = column << pg.page_shift, end = min(begin + page_tokens, a.budget);
         for (uint32_t r = begin; r < end; r += 32) {  // begin is a multiple of 16
@@ -217,7 +308,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictArgs a) {
       }
     }
     uint32_t total;
-    const uint32_t at = found + scan_waves(copy ? 1u : 0u, partial, total);
+    const uint32_t at = found + scan_waves<kWaves>(copy ? 1u : 0u, partial, total);
     if (copy) copies[at] = PageCopy{column, page, -1, 0};
     found += total;
   }
@@ -226,13 +317,13 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictArgs a) {
 
 // One workgroup gives every copy a free page, lowest first, sequence by sequence, or fails the
 // call as a whole; then it renames the pages.
-__global__ __launch_bounds__(kSelectThreads) void grant_kernel(EvictArgs a) {
-  __shared__ uint32_t partial[kSelectWaves];
+__global__ __launch_bounds__(kGrantThreads) void grant_kernel(EvictArgs a) {
+  __shared__ uint32_t partial[kGrantThreads / 64];
   __shared__ uint32_t start[kMaxListed + 1];
   const unsigned tid = threadIdx.x;
   const KvPages& pg = a.pages;
   uint32_t total;
-  const uint32_t before = scan_waves(tid < a.list.count ? a.headers[tid].copies : 0u, partial, total);
+  const uint32_t before = scan_waves<kGrantThreads / 64>(tid < a.list.count ? a.headers[tid].copies : 0u, partial, total);
   if (tid < a.list.count) start[tid] = before;
   if (tid == 0) start[a.list.count] = total;
   __syncthreads();
@@ -242,9 +333,9 @@ __global__ __launch_bounds__(kSelectThreads) void grant_kernel(EvictArgs a) {
   }
   // Twice over the counts: is there enough, then who gets what.
   uint32_t available = 0;
-  for (uint32_t from = 0; from < pg.page_count && available < total; from += kSelectThreads) {
+  for (uint32_t from = 0; from < pg.page_count && available < total; from += kGrantThreads) {
     uint32_t found;
-    scan_waves(from + tid < pg.page_count && pg.references[from + tid] == 0 ? 1u : 0u, partial, found);
+    scan_waves<kGrantThreads / 64>(from + tid < pg.page_count && pg.references[from + tid] == 0 ? 1u : 0u, partial, found);
     available += found;
   }
   if (tid == 0) {
@@ -253,11 +344,11 @@ __global__ __launch_bounds__(kSelectThreads) void grant_kernel(EvictArgs a) {
   }
   if (available < total) return;
   uint32_t given = 0;
-  for (uint32_t from = 0; from < pg.page_count && given < total; from += kSelectThreads) {
+  for (uint32_t from = 0; from < pg.page_count && given < total; from += kGrantThreads) {
     const uint32_t page = from + tid;
     const bool free = page < pg.page_count && pg.references[page] == 0;
     uint32_t found;
-    const uint32_t rank = given + scan_waves(free ? 1u : 0u, partial, found);
+    const uint32_t rank = given + scan_waves<kGrantThreads / 64>(free ? 1u : 0u, partial, found);
     if (free && rank < total) {
       uint32_t low = 0, high = a.list.count;  // the last sequence whose start is <= rank
       while (high - low > 1) {
@@ -276,7 +367,7 @@ __global__ __launch_bounds__(kSelectThreads) void grant_kernel(EvictArgs a) {
   // them leave is free for the next call, not for this one.
   __syncthreads();
   for (uint32_t i = 0; i < a.list.count; ++i) {
-    for (uint32_t c = tid; c < start[i + 1] - start[i]; c += kSelectThreads) {
+    for (uint32_t c = tid; c < start[i + 1] - start[i]; c += kGrantThreads) {
       atomicSub(&pg.references[a.copies[static_cast<std::size_t>(i) * a.most_copies + c].from], 1u);
     }
   }
@@ -456,9 +547,12 @@ extern "C" int32_t gfxinfer_launch_kv_pages_evict(const gfxinfer_kv_pages* pages
     a.recent = recent;
     a.status = status;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(select_kernel, dim3(count), dim3(kSelectThreads), 0, st, a);
+    // A wave's instructions are what the choice takes its time with, and sixteen waves share a CU's four vector
+    // units: tables of few rows take four (501 rows: XX us, with sixteen 11.1).
+    if (capacity_of(a.pages) <= 256 * kSelectKeys) hipLaunchKernelGGL(select_kernel<256>, dim3(count), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(select_kernel<1024>, dim3(count), dim3(1024), 0, st, a);
     if (const int32_t s = launch_status("K/V eviction launch failed"); s != GFXI_OK) return s;
-    hipLaunchKernelGGL(grant_kernel, dim3(1), dim3(kSelectThreads), 0, st, a);
+    hipLaunchKernelGGL(grant_kernel, dim3(1), dim3(kGrantThreads), 0, st, a);
     if (const int32_t s = launch_status("K/V eviction launch failed"); s != GFXI_OK) return s;
     hipLaunchKernelGGL(move_kernel, dim3(std::max(1u, kMoveWorkgroups / count), count), dim3(kMoveThreads), 0, st, a);
     return launch_status("K/V eviction launch failed");
