@@ -12,6 +12,7 @@ There is no fallback: if the library is missing, importing the wrappers fails.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import re
 import subprocess
@@ -614,21 +615,22 @@ def launch_kv_pages_evict(pages, weights, sequences, budget, first, recent, stat
 
 # ---- products in 8-bit integers, any number of tokens ----------------------------
 
+@functools.cache
 def _types():
     import torch
-    return {torch.float16: TYPE_F16, torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16}
+    return {torch.float16: TYPE_F16, torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16}, (torch.int8,)
 
 
 def launch_quantize_rows_i8(x, codes, scales, stream=None):
     """x [rows, columns], fp16, fp32 or bf16 with dense rows; codes int8 [rows, columns]; scales fp32 [rows]."""
-    import torch
+    types, integers = _types()
     rows, columns = x.shape
-    L, device, kind = lib(), x.get_device(), _types().get(x.dtype)
+    L, device, kind = lib(), x.get_device(), types.get(x.dtype)
     if kind is None or x.stride(1) != 1 or not x.is_cuda:
         raise ValueError("row quantizer: x is fp16, fp32 or bf16 [rows, columns] on a GPU, with dense rows")
     check(L.gfxinfer_launch_quantize_rows_i8(
         x.data_ptr(), kind, rows, columns, x.stride(0) if rows > 1 else -(-columns // 8) * 8,
-        _operand(codes, (torch.int8,), rows * columns, device, "codes"), _operand(scales, _real, 4 * rows, device, "scales"),
+        _operand(codes, integers, rows * columns, device, "codes"), _operand(scales, _real, 4 * rows, device, "scales"),
         _launch_stream(device, stream)))
 
 
@@ -639,14 +641,14 @@ def w8a8_gemm_workspace_bytes(rows, columns, tokens) -> int:
 def launch_w8a8_gemm(weights, weight_scales, codes, scales, output, workspace, stream=None):
     """weights int8 [rows, columns], weight_scales fp32 [rows], codes int8 [tokens, columns], scales fp32 [tokens], output fp32
     or fp16 [tokens, rows]; workspace may be None where w8a8_gemm_workspace_bytes is 0."""
-    import torch
+    types, integers = _types()
     (rows, columns), tokens, L = weights.shape, codes.shape[0], lib()
-    device, kind = weights.get_device(), _types().get(output.dtype)
+    device, kind = weights.get_device(), types.get(output.dtype)
     if not weights.is_cuda or tuple(codes.shape) != (tokens, columns) or tuple(output.shape) != (tokens, rows) or kind in (None, TYPE_BF16):
         raise ValueError("8-bit product: weights [rows, columns] on a GPU, codes [tokens, columns], output fp32 or fp16 [tokens, rows]")
     check(L.gfxinfer_launch_w8a8_gemm(
-        _operand(weights, (torch.int8,), rows * columns, device, "weights"), _operand(weight_scales, _real, 4 * rows, device, "weight_scales"),
-        _operand(codes, (torch.int8,), tokens * columns, device, "codes"), _operand(scales, _real, 4 * tokens, device, "scales"),
+        _operand(weights, integers, rows * columns, device, "weights"), _operand(weight_scales, _real, 4 * rows, device, "weight_scales"),
+        _operand(codes, integers, tokens * columns, device, "codes"), _operand(scales, _real, 4 * tokens, device, "scales"),
         _operand(output, (output.dtype,), tokens * rows * output.element_size(), device, "output"), kind, rows, columns, tokens,
         *_scratch(workspace, device), _launch_stream(device, stream)))
 
