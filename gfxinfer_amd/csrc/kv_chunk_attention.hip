@@ -549,6 +549,15 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
       }
     }
   };
+  // The outputs and queries belong into the accumulation registers: left to itself the compiler counts them
+  // among the others and reads every operand right before its product (4 prompts of 300 on 1500..6000:
+  // 226 us, not 211), or moves all of them there and back where maxima might move.
+  auto keep_outputs = [&]() __attribute__((always_inline)) {
+    if constexpr (D == 256) {
+#pragma unroll
+      for (unsigned d = 0; d < D / 32; ++d) asm volatile("" : "+a"(o[d]));
+    }
+  };
   // Scores of a tile are ready: hides what a row does not see, and moves the maxima.
   auto settle = [&](f16v (&sc)[kSub], uint32_t x, uint32_t missing) __attribute__((always_inline)) {
     if (x * T + T > least_visible || missing != 0) {
@@ -566,6 +575,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
 #pragma unroll
     for (unsigned e = 1; e < 16 * kSub; ++e) best = __builtin_elementwise_maximum(best, sc[e / 16][e % 16]);
     const float top = max_over_halves(best) * a.scale;
+    keep_outputs();
     if (__any(!(top <= m + kRise))) {
       const float next = top <= m + kRise ? m : top;
       // From nothing to something: there is nothing to scale yet.
@@ -577,18 +587,14 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
 #pragma unroll
         for (unsigned r = 0; r < 16; ++r) o[d][r] *= factor;
       }
+      keep_outputs();
     }
+    keep_outputs();
   };
   // The weights of the tile in s and the scores of the next one, then the values of this one.
   auto step = [&](const _Float16* next_ks, const _Float16* vs) __attribute__((always_inline)) {
     h8 p[kSteps];
-    if constexpr (D == 256) {
-      // The outputs and queries belong into the accumulation registers: left to itself the compiler counts
-      // them among the others and reads every operand right before its product (4 prompts of 300 on
-      // 1500..6000: 226 us, not 211).
-#pragma unroll
-      for (unsigned d = 0; d < D / 32; ++d) asm volatile("" : "+a"(o[d]));
-    }
+    keep_outputs();
     score(next_ks, s_next);
     const float floor = m == -INFINITY ? 0.0F : m - kLift;
     float sum[4] = {l, 0.0F, 0.0F, 0.0F};
@@ -633,7 +639,10 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
 #pragma unroll
-    for (unsigned u = 0; u < kSub; ++u) s[u] = s_next[u];
+    for (unsigned u = 0; u < kSub; ++u) {
+      s[u] = s_next[u];
+      if constexpr (D == 256) asm volatile("" : "+v"(s[u]));  // for the vector unit
+    }
   };
 
   // Tile x's V rows and tile x + 1's K rows are read while x + 1's V rows and x + 2's K rows are on their way,
