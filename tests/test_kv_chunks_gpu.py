@@ -380,6 +380,19 @@ def test_weights_equal_the_definition(device, gx, heads, page, lengths, tokens):
     assert np.array_equal(got, _weights(c, gx, sums, before))  # the same bits every time
 
 
+def test_weights_of_long_caches(device, gx):
+    """More positions than a launch has workgroups for: a chunk's (256 each) and a decoding sequence's (32 each)."""
+    rng = np.random.default_rng(24)
+    c = Chunks(rng, (1, 1, 128), 4096, [262300, 33000], [40, 1], gate=False, gap=0)
+    say("received weights of long caches")
+    sums = np.zeros((41, 1), np.float32)
+    for i, t in enumerate(c.tokens):
+        s = c.rows_of(i, 0)[0]
+        sums[c.first(i):c.first(i) + t, 0] = s.max(1) + np.log(np.exp(s - s.max(1, keepdims=True)).sum(1))
+    before = rng.random((3, c.table.shape[1] * 4096)).astype(np.float32)
+    _check_weights(c, _weights(c, gx, sums, before), sums, before)
+
+
 @pytest.mark.parametrize("heads", [A, B])
 def test_weights_of_missing_pages_and_rows_that_see_nothing(device, gx, heads):
     rng = np.random.default_rng(21)
