@@ -67,7 +67,7 @@ def test_bad_attention_is_refused(gx, cache, change):  # noqa: F811
 
 
 @pytest.mark.parametrize("change", SHARED + [
-    dict(layer=2), dict(query=None), dict(sums=None), dict(q_heads=0), dict(q_heads=3), dict(workspace=None), dict(bytes=100),
+    dict(layer=2), dict(query=None), dict(sums=None), dict(q_heads=0), dict(q_heads=3), dict(workspace=None), dict(bytes=8),
     dict(query=_aligned(4096).ctypes.data + 2), dict(sums=_aligned(4096).ctypes.data + 2), dict(ids=_ids(1, 1)),
     dict(workspace=_aligned(4096).ctypes.data + 8)])
 def test_bad_weights_are_refused(gx, cache, weights, change):  # noqa: F811
