@@ -318,7 +318,7 @@ constexpr unsigned kStage = 128;
 constexpr unsigned kGroup = 8;  // token tiles that run beside each other
 
 template <unsigned BN, unsigned BM, unsigned WN, unsigned WM, unsigned Depth>
-__global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs a, uint32_t row_tiles, uint32_t token_tiles) {
+__global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs a, uint32_t first_row, uint32_t row_tiles, uint32_t token_tiles) {
   constexpr unsigned kWaves = WN * WM;
   constexpr unsigned R = BN / WN / 32, T = BM / WM / 32;   // 32 x 32 tiles of a wave
   constexpr unsigned kLoads = (BN + BM) * kStage / 16 / (kWaves * 64);
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void w8a8_tile_kernel(ProductArgs 
   const uint32_t split = id / tiles, tile = id - split * tiles;
   const uint32_t group = tile / (kGroup * row_tiles), in_group = tile - group * kGroup * row_tiles;
   const uint32_t wide = min(kGroup, token_tiles - group * kGroup);
-  const uint32_t row0 = in_group / wide * BN, token0 = (group * kGroup + in_group % wide) * BM;
+  const uint32_t row0 = first_row + in_group / wide * BN, token0 = (group * kGroup + in_group % wide) * BM;
   const uint32_t stages = (a.columns + kStage - 1) / kStage, per_split = (stages + a.splits - 1) / a.splits;
   const uint32_t from = split * per_split, to = min(from + per_split, stages);
 
@@ -482,6 +482,7 @@ __global__ __launch_bounds__(256) void w8a8_join_kernel(ProductArgs a) {
 constexpr uint32_t kFewTokens = 64;
 
 struct ProductShape {
+  uint32_t main_tiles;  // of 256 channels, which run first
   uint32_t tile_rows;  // channels of a tile, see below; 0: the kernel for few tokens
   uint32_t row_tiles, token_tiles, splits;
 };
@@ -500,20 +501,19 @@ constexpr TileShape kTileShapes[] = {
 // Joining splits takes 8.5 us and 1.34 ps for each sum.
 constexpr double kJoinTime = 8500, kJoinSum = 0.00134;
 constexpr uint32_t kMaxSplits = 8;
+constexpr std::size_t kMainTile = 256;
 
 // The shape and the number of splits that take the shortest time: the rounds that the chip needs for the
 // workgroups times the time of one. Against the best of all on the same 78 sizes the choice costs 2.3 % on
 // average and 16 % at worst. 5120 x 5120 and 160 tokens: 12.6 us in tiles of 64, 18.4 of 128, 28 of 256; 17408 x 5120 and 1024
 // tokens: 197, 162 and 127; 5120 x 17408 and 320 tokens: 48 in four splits of 256, 55 in three, 75 in tiles of 64 without.
-ProductShape product_shape(std::size_t rows, std::size_t columns, std::size_t tokens) {
+ProductShape best_shape(std::size_t rows, std::size_t columns, std::size_t tokens, uint32_t most_splits) {
   ProductShape s{};
-  s.splits = 1;
-  if (tokens <= kFewTokens) return s;
   const std::size_t stages = (columns + kStage - 1) / kStage;
   double best = 0;
   for (const TileShape& t : kTileShapes) {
     const std::size_t row_tiles = (rows + t.rows - 1) / t.rows, token_tiles = (tokens + t.tokens - 1) / t.tokens;
-    for (uint32_t want = 1; want <= std::min<std::size_t>(kMaxSplits, stages); ++want) {
+    for (uint32_t want = 1; want <= std::min<std::size_t>(most_splits, stages); ++want) {
       // Every split has a stage to do.
       const std::size_t per = (stages + want - 1) / want, splits = (stages + per - 1) / per;
       const std::size_t rounds = (row_tiles * token_tiles * splits + t.places - 1) / t.places;
@@ -521,9 +521,25 @@ ProductShape product_shape(std::size_t rows, std::size_t columns, std::size_t to
       if (splits > 1) time += kJoinTime + kJoinSum * static_cast<double>(splits * rows * tokens);
       if (s.tile_rows != 0 && time >= best) continue;
       best = time;
-      s = {t.rows, static_cast<uint32_t>(row_tiles), static_cast<uint32_t>(token_tiles), static_cast<uint32_t>(splits)};
+      s = {0, t.rows, static_cast<uint32_t>(row_tiles), static_cast<uint32_t>(token_tiles), static_cast<uint32_t>(splits)};
     }
   }
+  return s;
+}
+
+// Tiles of 256 x 256 take the least time for their size, but a last round of few of them takes as long as a full
+// one.  So they take the channels that make whole rounds, and the others follow in the shape that is best for them: 17408 x 5120
+// with 4096 tokens 419 us, in one launch of 256 x 128 457; 34816 x 5120 with 509 tokens 120, not 151; 5120 x 5120 with 8192
+// tokens 234, not 247; where what is left is more than half a round it is about even (27392 x 5120 with 1500 tokens 279, not 269).
+ProductShape product_shape(std::size_t rows, std::size_t columns, std::size_t tokens) {
+  ProductShape s{};
+  s.splits = 1;
+  if (tokens <= kFewTokens) return s;
+  const std::size_t wide = (tokens + kMainTile - 1) / kMainTile, rounds = wide * (rows / kMainTile) / kComputeUnits;
+  const std::size_t first = rounds * kComputeUnits / wide;
+  if (first == 0) return best_shape(rows, columns, tokens, kMaxSplits);
+  if (first * kMainTile < rows) s = best_shape(rows - first * kMainTile, columns, tokens, 1);
+  s.main_tiles = static_cast<uint32_t>(first);
   return s;
 }
 
@@ -611,17 +627,24 @@ extern "C" int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float*
                         static_cast<uint32_t>(rows), static_cast<uint32_t>(columns), static_cast<uint32_t>(tokens), s.splits,
                         output_type == GFXI_F16 ? 1u : 0u};
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (s.tile_rows == 0) {
+    if (tokens <= kFewTokens) {
       if (tokens <= 16) launch_few<1, 1, 4, 3>(a, st);
       else if (tokens <= 32) launch_few<2, 2, 4, 3>(a, st);
       else if (tokens <= 48) launch_few<3, 2, 4, 3>(a, st);
       else launch_few<4, 2, 4, 3>(a, st);
       return launch_status("8-bit product launch failed");
     }
+    uint32_t first_row = 0;
+    if (s.main_tiles != 0) {
+      const uint32_t token_tiles = static_cast<uint32_t>((tokens + kMainTile - 1) / kMainTile);
+      hipLaunchKernelGGL((w8a8_tile_kernel<256, 256, 2, 4, 2>), dim3(s.main_tiles * token_tiles), dim3(512), 0, st, a, 0u, s.main_tiles, token_tiles);
+      if (const int32_t status = launch_status("8-bit product launch failed"); status != GFXI_OK || s.tile_rows == 0) return status;
+      first_row = s.main_tiles * kMainTile;
+    }
     const dim3 grid(static_cast<unsigned>(groups));
-    if (s.tile_rows == 64) hipLaunchKernelGGL((w8a8_tile_kernel<64, 64, 2, 2, 4>), grid, dim3(256), 0, st, a, s.row_tiles, s.token_tiles);
-    else if (s.tile_rows == 128) hipLaunchKernelGGL((w8a8_tile_kernel<128, 128, 2, 4, 4>), grid, dim3(512), 0, st, a, s.row_tiles, s.token_tiles);
-    else hipLaunchKernelGGL((w8a8_tile_kernel<256, 128, 4, 2, 3>), grid, dim3(512), 0, st, a, s.row_tiles, s.token_tiles);
+    if (s.tile_rows == 64) hipLaunchKernelGGL((w8a8_tile_kernel<64, 64, 2, 2, 4>), grid, dim3(256), 0, st, a, first_row, s.row_tiles, s.token_tiles);
+    else if (s.tile_rows == 128) hipLaunchKernelGGL((w8a8_tile_kernel<128, 128, 2, 4, 4>), grid, dim3(512), 0, st, a, first_row, s.row_tiles, s.token_tiles);
+    else hipLaunchKernelGGL((w8a8_tile_kernel<256, 128, 4, 2, 3>), grid, dim3(512), 0, st, a, first_row, s.row_tiles, s.token_tiles);
     if (const int32_t status = launch_status("8-bit product launch failed"); status != GFXI_OK || s.splits == 1) return status;
     const std::size_t quads = (rows + 3) / 4 * tokens;
     hipLaunchKernelGGL(w8a8_join_kernel, dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(256), 0, st, a);

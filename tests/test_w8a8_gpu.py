@@ -119,9 +119,11 @@ def test_products_equal_the_definition(device, gx, half, tokens, rows, columns):
 
 
 @pytest.mark.parametrize("tokens,rows,columns", [
-    (65, 1999, 528), (65, 1999, 4112), (65, 17001, 1040), (65, 7000, 8208), (1000, 7000, 528), (65, 17001, 8208), (2000, 5000, 656)])
+    (65, 1999, 528), (65, 1999, 4112), (65, 17001, 1040), (65, 7000, 8208), (1000, 7000, 528), (65, 17001, 8208), (2000, 5000, 656),
+    (4096, 4096, 144), (300, 33025, 272)])
 def test_every_tile_shape(device, gx, tokens, rows, columns):
-    """Small, middle and large tiles, in one piece and with K divided among workgroups, all with a ragged edge."""
+    """Small, middle and large tiles, in one piece and with K divided among workgroups, most with a ragged edge; whole rounds of
+    the largest tiles alone and with other tiles behind them."""
     rng = np.random.default_rng(tokens + rows + columns)
     say("8-bit product", tokens, rows, columns)
     a, w = (rng.integers(-128, 128, (x, columns), dtype=np.int8) for x in (tokens, rows))
