@@ -528,16 +528,18 @@ ProductShape best_shape(std::size_t rows, std::size_t columns, std::size_t token
 }
 
 // Tiles of 256 x 256 take the least time for their size, but a last round of few of them takes as long as a full
-// one.  So they take the channels that make whole rounds, and the others follow in the shape that is best for them: 17408 x 5120
-// with 4096 tokens 419 us, in one launch of 256 x 128 457; 34816 x 5120 with 509 tokens 120, not 151; 5120 x 5120 with 8192
-// tokens 234, not 247; where what is left is more than half a round it is about even (27392 x 5120 with 1500 tokens 279, not 269).
+// one, and so does a tile with few tokens.  So where they pad the tokens no further than tiles of 128 would, they take the channels
+// that make whole rounds, and the others follow in the shape that is best for them.  17408 x 5120 with 4096 tokens: 419 us, in one
+// launch of 256 x 128 457; 34816 x 5120 with 509 tokens 120, not 151; 5120 x 5120 with 8192 tokens 234, not 247.  With more
+// padding (34816 x 5120 and 300 tokens) it took 111 us and one launch 97; where more than half a round is left it is about even
+// (27392 x 5120 with 1024 tokens 199 and 203, 34816 x 5120 with 768 200 and 186).
 ProductShape product_shape(std::size_t rows, std::size_t columns, std::size_t tokens) {
   ProductShape s{};
   s.splits = 1;
   if (tokens <= kFewTokens) return s;
   const std::size_t wide = (tokens + kMainTile - 1) / kMainTile, rounds = wide * (rows / kMainTile) / kComputeUnits;
   const std::size_t first = rounds * kComputeUnits / wide;
-  if (first == 0) return best_shape(rows, columns, tokens, kMaxSplits);
+  if (first == 0 || (tokens + 127) / 128 % 2 != 0) return best_shape(rows, columns, tokens, kMaxSplits);
   if (first * kMainTile < rows) s = best_shape(rows - first * kMainTile, columns, tokens, 1);
   s.main_tiles = static_cast<uint32_t>(first);
   return s;
