@@ -19,6 +19,11 @@
 // The scores of a tile of positions are computed beside the exponentials of the tile before it:
 // the exponentials alone take a wave's vector unit nearly as long as both products take the
 // matrix unit.
+//
+// 2048 tokens on 30000, 40 x 8 x 128: 1381 us, 942 TFLOP/s (a large fp16 product: 1.28 PFLOP/s); the matrix units
+// are busy 48 % of the time, waits take 23 % of the waves'.  24 x 4 x 256: 1856 us, 841 TFLOP/s: the outputs of 32 rows
+// leave room for one wave a SIMD, and nothing covers its waits.  31 sequences that decode on 200 .. 4090 and a chunk of
+// 509: 77 us, 3.7 TB/s.  Eight that decode on up to 600: 13.4 us, two launches of dependent reads.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -551,7 +556,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   };
   // The outputs and queries belong into the accumulation registers: left to itself the compiler counts them
   // among the others and reads every operand right before its product (4 prompts of 300 on 1500..6000:
-  // 226 us, not 211), or moves all of them there and back where maxima might move.
+  // 226 us, not 211), or moves all of them there and back where maxima might move (204, not 182).
   auto keep_outputs = [&]() __attribute__((always_inline)) {
     if constexpr (D == 256) {
 #pragma unroll
@@ -828,7 +833,9 @@ __device__ __forceinline__ const __half* key_row(const WeightArgs& a, uint32_t s
 constexpr uint32_t kFewRows = 32;  // of a sequence and KV head
 
 // Sequences of at most 32 rows, as a decoding one has: a workgroup takes 32 positions and all KV
-// heads, a wave every fourth one, and adds the sum over all of them.
+// heads, a wave every fourth one, and adds the sum over all of them.  A position's row holds the heads side by side, so
+// a workgroup reads whole rows, and one launch does (sixteen on up to 4090, 24 x 4 x 256: 16.1 us, 3.9 TB/s; with
+// a sum for each KV head and a second launch 24.6).
 template <unsigned D>
 __global__ __launch_bounds__(256) void few_weight_kernel(WeightArgs a) {
   __shared__ float parts[4][32];
@@ -905,7 +912,9 @@ struct RowWalk {
 
 // A wave holds 64 positions of K as the A operand.  The rows of a KV head pass through LDS, 32 at a time,
 // three steps ahead, and serve all waves; the exponentials of a step, each added to the lane's sum of
-// its position, go between the next step's products.
+// its position, go between the next step's products.  64 positions a wave, not 32: a step's operands are read
+// from LDS by every wave, which at 32 takes as long as its products.  2048 tokens on 8000: 40 x 8 x 128 227 us, 832
+// TFLOP/s, the matrix units busy 47 % of the time, the vector unit 36 %; 24 x 4 x 256 322 us, 706 TFLOP/s.
 template <unsigned D>
 __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightArgs a) {
   constexpr unsigned P = kWeightPositions / 4 / 32;

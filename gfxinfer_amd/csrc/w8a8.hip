@@ -9,6 +9,11 @@
 // a lane's 16 bytes of the v_mfma_i32_16x16x64_i8 operand are contiguous in a row.
 // Channels are the A operand and tokens the B operand, so a lane ends up with four
 // neighbouring channels of one token.
+//
+// What bounds it: with few tokens the weights' bytes (5120 x 5120, one token: 6.9 us, 3.8 TB/s; 17408 x
+// 5120, 37 tokens: 25 us, 3.6 TB/s), with many the matrix instructions and the waits between their stages
+// (17408 x 5120, 4096 tokens: 393 us, 1.86 POP/s, where a large library product of one size reaches 2.25;
+// the matrix units are busy 43 % of the time at about 2.0 GHz, LDS reads have no bank conflicts).
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -91,7 +96,8 @@ __device__ __forceinline__ uint32_t four_codes(const float (&x)[8], unsigned fir
 
 constexpr unsigned kQuantUnits = 4;  // of eight values a thread keeps
 
-// A workgroup a row.  A row that holds an infinity or a NaN gets a NaN scale and zero codes,
+// A workgroup a row, read once and kept in registers: bytes, 4096 rows of 5120 in fp16 15 us (4.1 TB/s), one
+// row 3.3 us, the time of a launch and three dependent steps.  A row that holds an infinity or a NaN gets a NaN scale and zero codes,
 // so every product with it is NaN; a row of zeros the smallest normal scale.
 template <int Type, unsigned Threads>
 __global__ __launch_bounds__(Threads) void quantize_rows_kernel(const void* __restrict__ input, std::size_t stride,
@@ -309,7 +315,8 @@ __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
 }
 
 // Many tokens: tiles of BN channels and BM tokens, K in stages of 128 bytes that go straight
-// from memory into LDS, one ahead of the products (v_mfma_i32_32x32x32_i8).
+// from memory into LDS, Depth - 1 ahead of the products (v_mfma_i32_32x32x32_i8).  Two stages ahead instead
+// of one: 5120 x 17408 and 509 tokens 65 us, not 77; the tiles of 256 x 256 have room in LDS for one ahead.
 //
 // A stage's row is 128 bytes, eight pieces of 16; piece c of row r lies in slot c ^ (r / 2 % 8)
 // (the address a lane loads from is permuted, since loads into LDS fill it lane after lane),
@@ -479,7 +486,11 @@ __global__ __launch_bounds__(256) void w8a8_join_kernel(ProductArgs a) {
   write_output(a, token, row, sum);
 }
 
-constexpr uint32_t kFewTokens = 64;
+// Up to 48 tokens, and up to 64 of small matrices: 5120 x 5120 and 64 tokens 10.1 us, in tiles 11.8; 5120 x 17408
+// 35.6 and 30.7, with 40 tokens 31.5 and 27.6; 34816 x 5120 and 64 tokens 61.6 and 56.9, with 40 52.2 and 54.5.
+bool few_tokens(std::size_t rows, std::size_t columns, std::size_t tokens) {
+  return tokens <= 48 || (tokens <= 64 && rows * columns < (1u << 26));
+}
 
 struct ProductShape {
   uint32_t main_tiles;  // of 256 channels, which run first
@@ -536,7 +547,7 @@ ProductShape best_shape(std::size_t rows, std::size_t columns, std::size_t token
 ProductShape product_shape(std::size_t rows, std::size_t columns, std::size_t tokens) {
   ProductShape s{};
   s.splits = 1;
-  if (tokens <= kFewTokens) return s;
+  if (few_tokens(rows, columns, tokens)) return s;
   const std::size_t wide = (tokens + kMainTile - 1) / kMainTile, rounds = wide * (rows / kMainTile) / kComputeUnits;
   const std::size_t first = rounds * kComputeUnits / wide;
   if (first == 0 || (tokens + 127) / 128 % 2 != 0) return best_shape(rows, columns, tokens, kMaxSplits);
@@ -629,7 +640,7 @@ extern "C" int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float*
                         static_cast<uint32_t>(rows), static_cast<uint32_t>(columns), static_cast<uint32_t>(tokens), s.splits,
                         output_type == GFXI_F16 ? 1u : 0u};
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (tokens <= kFewTokens) {
+    if (few_tokens(rows, columns, tokens)) {
       if (tokens <= 16) launch_few<1, 1, 4, 3>(a, st);
       else if (tokens <= 32) launch_few<2, 2, 4, 3>(a, st);
       else if (tokens <= 48) launch_few<3, 2, 4, 3>(a, st);
