@@ -800,10 +800,12 @@ struct WeightArgs {
   ChunkList list;
   const __half* query;
   const float* log_sums;
-  float* partial;  // [count][kv_heads * parts][capacity]
+  float* partial;  // [sequences with many rows][kv_heads * parts][capacity]
   uint32_t layer, q_heads, kv_heads, group, parts;
   uint32_t columns;  // workgroups along the positions
+  uint32_t many;     // sequences with more than kFewRows rows
   float scale;
+  uint16_t order[kMaxChunks];  // of the listed sequences: those, then the others with rows
 };
 
 // Sums of N registers over the 32 lanes of a half: at each exchange a lane keeps the registers whose
@@ -842,9 +844,8 @@ __global__ __launch_bounds__(256) void few_weight_kernel(WeightArgs a) {
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned n = lane & 31u, h = lane >> 5;
   const KvPages& pg = a.pages;
-  const uint32_t i = blockIdx.y, slot = listed_slot(a.list, i), first_row = a.list.first[i], tokens = a.list.first[i + 1] - first_row;
-  const uint32_t rows = tokens * a.group;
-  if (rows == 0 || rows > kFewRows) return;
+  const uint32_t i = a.order[a.many + blockIdx.y], slot = listed_slot(a.list, i), first_row = a.list.first[i];
+  const uint32_t tokens = a.list.first[i + 1] - first_row, rows = tokens * a.group;
   const uint32_t length = committed(pg, slot), capacity = pg.stride << pg.page_shift, end = min(length + tokens, capacity);
   const uint32_t t = min(n, rows - 1) / a.group;
   const std::size_t out_row = (static_cast<std::size_t>(first_row) + t) * a.q_heads + (min(n, rows - 1) - t * a.group);
@@ -926,14 +927,13 @@ __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightA
   const unsigned n = lane & 31u, h = lane >> 5;
   const KvPages& pg = a.pages;
   const uint32_t hk = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads % a.parts;
-  const uint32_t column = blockIdx.x / a.kv_heads / a.parts, i = blockIdx.y;
+  const uint32_t column = blockIdx.x / a.kv_heads / a.parts, i = a.order[blockIdx.y];
   const uint32_t slot = listed_slot(a.list, i), first_row = a.list.first[i], tokens = a.list.first[i + 1] - first_row;
   const uint32_t rows = tokens * a.group, all = (rows + kWeightRows - 1) / kWeightRows;
-  if (rows <= kFewRows) return;
   const uint32_t length = committed(pg, slot), end = min(length + tokens, pg.stride << pg.page_shift);
   const uint32_t per = (all + a.parts - 1) / a.parts, to = min(part * per + per, all);
   const uint32_t token_bytes = a.q_heads * D * 2;
-  const std::size_t plane = (static_cast<std::size_t>(i) * a.kv_heads + hk) * a.parts + part;
+  const std::size_t plane = (static_cast<std::size_t>(blockIdx.y) * a.kv_heads + hk) * a.parts + part;
   float* sums = a.partial + plane * (static_cast<std::size_t>(pg.stride) << pg.page_shift);
   for (uint32_t at = column * kWeightPositions; at < end; at += a.columns * kWeightPositions) {
     const uint32_t mine = at + 32 * P * wave;
@@ -1129,13 +1129,12 @@ __global__ __launch_bounds__(256) void weight_join_kernel(WeightArgs a) {
   __shared__ float parts[4][64];
   const KvPages& pg = a.pages;
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t i = blockIdx.y, slot = listed_slot(a.list, i), tokens = a.list.first[i + 1] - a.list.first[i];
-  if (tokens * a.group <= kFewRows) return;
+  const uint32_t i = a.order[blockIdx.y], slot = listed_slot(a.list, i), tokens = a.list.first[i + 1] - a.list.first[i];
   const uint32_t capacity = pg.stride << pg.page_shift, end = min(committed(pg, slot) + tokens, capacity);
   const uint32_t planes = a.kv_heads * a.parts, quarter = (planes + 3) / 4;
   for (uint32_t at = blockIdx.x * 64; at < end; at += gridDim.x * 64) {
     const uint32_t p = at + lane;
-    const float* source = a.partial + static_cast<std::size_t>(i) * planes * capacity + min(p, end - 1);
+    const float* source = a.partial + static_cast<std::size_t>(blockIdx.y) * planes * capacity + min(p, end - 1);
     float sum = 0.0F;
 #pragma unroll 8
     for (uint32_t x = wave * quarter; x < min(wave * quarter + quarter, planes); ++x) sum += source[static_cast<std::size_t>(x) * capacity];
@@ -1187,34 +1186,33 @@ std::size_t chunk_bytes(const ChunkShape& s, const ChunkList& list, uint32_t q_h
 // How the rows of the long chunks are divided: workgroups along the positions, and parts of the rows.
 struct WeightShape {
   uint32_t columns, parts;
-  bool few, many;  // sequences of at most kFewRows rows, of more
+  uint32_t few, many;  // sequences of 1 .. kFewRows rows, of more
 };
 
 WeightShape weight_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads) {
   WeightShape s{};
   const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift;
   s.columns = static_cast<uint32_t>(std::min<uint64_t>((capacity + kWeightPositions - 1) / kWeightPositions, 1024));
-  uint32_t most = 0, long_ones = 0;
+  uint32_t most = 0;
   for (uint32_t i = 0; i < list.count; ++i) {
     const uint32_t tokens = list.first[i + 1] - list.first[i];
     most = std::max(most, tokens);
     const bool many = static_cast<uint64_t>(tokens) * (q_heads / kv_heads) > kFewRows;
-    s.few |= !many && tokens != 0;
-    s.many |= many;
-    long_ones += many;
+    s.few += !many && tokens != 0;
+    s.many += many;
   }
   s.parts = 1;
-  if (!s.many) return s;
+  if (s.many == 0) return s;
   const uint64_t blocks = (static_cast<uint64_t>(most) * (q_heads / kv_heads) + kWeightRows - 1) / kWeightRows;
-  const uint64_t items = static_cast<uint64_t>(s.columns) * kv_heads * long_ones;
+  const uint64_t items = static_cast<uint64_t>(s.columns) * kv_heads * s.many;
   s.parts = static_cast<uint32_t>(std::clamp<uint64_t>(6 * kComputeUnits / items, 1, std::max<uint64_t>(1, blocks / 8)));
   return s;
 }
 
 // (At least a little, also where nothing is divided: a workspace is always given.)
-std::size_t weight_bytes(const KvPages& p, const ChunkList& list, uint32_t kv_heads, const WeightShape& s) {
-  if (!s.many) return 16;
-  return static_cast<std::size_t>(list.count) * kv_heads * s.parts * (static_cast<std::size_t>(p.stride) << p.page_shift) * sizeof(float);
+std::size_t weight_bytes(const KvPages& p, uint32_t kv_heads, const WeightShape& s) {
+  if (s.many == 0) return 16;
+  return static_cast<std::size_t>(s.many) * kv_heads * s.parts * (static_cast<std::size_t>(p.stride) << p.page_shift) * sizeof(float);
 }
 
 }  // namespace
@@ -1297,7 +1295,7 @@ extern "C" size_t gfxinfer_kv_weights_workspace_bytes(const gfxinfer_kv_pages* p
     if (const int32_t s = read_heads(pages, q_heads); s != GFXI_OK) return s;
     const std::vector<uint32_t> any(std::min(count, kMaxChunks + 1), 0u);
     if (const int32_t s = read_chunks(p, any.data(), tokens, count, false, list); s != GFXI_OK) return s;
-    bytes = weight_bytes(p, list, pages->kv_heads, weight_shape(p, list, q_heads, pages->kv_heads));
+    bytes = weight_bytes(p, pages->kv_heads, weight_shape(p, list, q_heads, pages->kv_heads));
     return GFXI_OK;
   });
   return bytes;
@@ -1321,7 +1319,13 @@ extern "C" int32_t gfxinfer_launch_kv_weights_add(const gfxinfer_kv_pages* pages
     const WeightShape shape = weight_shape(a.pages, a.list, q_heads, a.kv_heads);
     a.parts = shape.parts;
     a.columns = shape.columns;
-    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < weight_bytes(a.pages, a.list, a.kv_heads, shape)) {
+    a.many = shape.many;
+    for (uint32_t i = 0, many = 0, few = shape.many; i < count; ++i) {
+      const uint64_t rows = static_cast<uint64_t>(a.list.first[i + 1] - a.list.first[i]) * (q_heads / a.kv_heads);
+      if (rows > kFewRows) a.order[many++] = static_cast<uint16_t>(i);
+      else if (rows != 0) a.order[few++] = static_cast<uint16_t>(i);
+    }
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < weight_bytes(a.pages, a.kv_heads, shape)) {
       return fail(GFXI_INVALID_ARGUMENT, "K/V weights workspace is null, not 16-byte aligned or too small");
     }
     a.query = reinterpret_cast<const __half*>(query);
@@ -1333,18 +1337,18 @@ extern "C" int32_t gfxinfer_launch_kv_weights_add(const gfxinfer_kv_pages* pages
     a.scale = kLog2E / std::sqrt(static_cast<float>(pages->head_size));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const uint64_t capacity = static_cast<uint64_t>(a.pages.stride) << a.pages.page_shift;
-    if (shape.few) {
-      const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((capacity + 31) / 32, 1024)), count);
+    if (shape.few != 0) {
+      const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((capacity + 31) / 32, 1024)), shape.few);
       if (pages->head_size == 128) hipLaunchKernelGGL(few_weight_kernel<128>, grid, dim3(256), 0, st, a);
       else hipLaunchKernelGGL(few_weight_kernel<256>, grid, dim3(256), 0, st, a);
       if (const int32_t s = launch_status("K/V weights launch failed"); s != GFXI_OK) return s;
     }
-    if (!shape.many) return GFXI_OK;
-    const dim3 grid(a.columns * a.kv_heads * a.parts, count);
+    if (shape.many == 0) return GFXI_OK;
+    const dim3 grid(a.columns * a.kv_heads * a.parts, shape.many);
     if (pages->head_size == 128) hipLaunchKernelGGL(weight_kernel<128>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(weight_kernel<256>, grid, dim3(256), 0, st, a);
     if (const int32_t s = launch_status("K/V weights launch failed"); s != GFXI_OK) return s;
-    hipLaunchKernelGGL(weight_join_kernel, dim3(static_cast<unsigned>(std::min<uint64_t>((capacity + 63) / 64, 1024)), count),
+    hipLaunchKernelGGL(weight_join_kernel, dim3(static_cast<unsigned>(std::min<uint64_t>((capacity + 63) / 64, 1024)), shape.many),
                        dim3(256), 0, st, a);
     return launch_status("K/V weights join launch failed");
   });

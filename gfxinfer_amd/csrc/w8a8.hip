@@ -633,7 +633,8 @@ extern "C" int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float*
       return fail(GFXI_INVALID_ARGUMENT, "8-bit product: workspace is null, not 16-byte aligned or too small");
     }
     const uint64_t groups = static_cast<uint64_t>(s.row_tiles) * s.token_tiles * s.splits;
-    if (groups > (1u << 30) || (s.splits > 1 && static_cast<uint64_t>(rows) * tokens > (1ull << 38))) {
+    const uint64_t main_groups = static_cast<uint64_t>(s.main_tiles) * ((tokens + kMainTile - 1) / kMainTile);
+    if (groups > (1u << 30) || main_groups > (1u << 30) || (s.splits > 1 && static_cast<uint64_t>(rows) * tokens > (1ull << 38))) {
       return fail(GFXI_INVALID_ARGUMENT, "8-bit product: too large for one launch");
     }
     const ProductArgs a{weights, weight_scales, codes, scales, output, static_cast<int32_t*>(workspace),

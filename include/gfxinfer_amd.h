@@ -776,8 +776,8 @@ size_t gfxinfer_kv_weights_workspace_bytes(const gfxinfer_kv_pages* pages, const
 /* weight[s][j] += sum of exp(score - log_sum) over the chunk's tokens and query heads that see
  * position j, for each listed sequence (distinct) and one layer; query, log_sums and tokens as
  * given to and by gfxinfer_launch_kv_pages_chunk_attention.  Rows whose log_sum is -inf or NaN
- * add nothing; positions without a page are left as they are.  No atomics: the sums' order
- * depends on the shape of the call alone. */
+ * add nothing; positions without a page are left as they are.  No atomics: a call repeated
+ * gives the same bits. */
 int32_t gfxinfer_launch_kv_weights_add(const gfxinfer_kv_pages* pages, const gfxinfer_kv_weights* weights, uint32_t layer,
                                        const uint16_t* query, const float* log_sums, const uint32_t* sequences,
                                        const uint32_t* tokens, uint32_t count, uint32_t q_heads, void* workspace,

@@ -20,6 +20,7 @@ def _product(gx, **change):
     dict(rows=(1 << 24) + 1), dict(columns=0), dict(columns=24), dict(columns=1 << 17), dict(tokens=0), dict(tokens=(1 << 24) + 1),
     dict(weights=_aligned(4096).ctypes.data + 8), dict(codes=_aligned(4096).ctypes.data + 4),
     dict(output=_aligned(4096).ctypes.data + 8), dict(scales=_aligned(4096).ctypes.data + 2),
+    dict(rows=1 << 24, columns=16, tokens=1 << 24),           # more tiles than a launch has workgroups
     dict(tokens=300, rows=256, columns=8192), dict(tokens=300, rows=256, columns=8192, workspace=_aligned(64), bytes=64)])
 def test_bad_products_are_refused(gx, change):
     assert _product(gx, **change) == gx.INVALID_ARGUMENT
