@@ -25,7 +25,9 @@
 // leave room for one wave a SIMD, and nothing covers its waits.  31 sequences that decode on 200 .. 4090 and a chunk of
 // 509: 77 us, 3.7 TB/s.  Eight that decode on up to 600: 13.4 us, two launches of dependent reads.
 #include <algorithm>
+#include <array>
 #include <cmath>
+#include <numeric>
 #include <type_traits>
 #include <vector>
 
@@ -61,7 +63,8 @@ constexpr float kWritten = -1.0F;  // in the place of range 0's sum: the row is 
 struct ChunkAttnArgs {
   KvPages pages;
   ChunkList list;
-  uint32_t first_tile[kMaxChunks + 1];  // of the listed sequences' row tiles
+  uint32_t first_tile[kMaxChunks];  // of the listed sequences' row tiles
+  uint32_t tiles;
   const __half* query;   // [rows][q_heads][D]
   const float* gate;     // [rows][q_heads][2 D] or null
   __half* output;        // [rows][q_heads][D]
@@ -89,7 +92,7 @@ __device__ __forceinline__ Listed find_listed(const ChunkAttnArgs& a, uint32_t r
   for (uint32_t from = 0; from < a.list.count; from += 64) {
     const uint32_t i = min(from + lane, a.list.count - 1);
     const uint32_t slot = a.list.slot[i], row = a.list.first[i], tokens = a.list.first[i + 1] - row;
-    const uint32_t tile = a.first_tile[i], next_tile = a.first_tile[i + 1];
+    const uint32_t tile = a.first_tile[i], next_tile = tile + (tokens * a.group + kRows - 1) / kRows;
     const uint32_t length = min(a.pages.lengths[slot], a.pages.stride << a.pages.page_shift);
     most = max(most, length + tokens);
     const uint64_t here = __ballot(from + lane < a.list.count && tile <= row_tile && row_tile < next_tile);
@@ -416,7 +419,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   // KV heads vary fastest: with eight of them each XCD reads one.  Then row tiles, so that those that
   // read the same positions run together; late tokens, which see most, first.
   const uint32_t hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  const uint32_t tiles = a.first_tile[kMaxChunks], range = rest / tiles, row_tile = tiles - 1 - rest % tiles;
+  const uint32_t tiles = a.tiles, range = rest / tiles, row_tile = tiles - 1 - rest % tiles;
   const Listed listed = find_listed<D>(a, row_tile);
   const uint32_t slot = listed.slot, first_row = listed.first_row, tokens = listed.tokens, length = listed.length;
   const uint32_t rows = tokens * a.group, tile_row = (row_tile - listed.first_tile) * kRows;
@@ -1166,11 +1169,16 @@ ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads
                        uint32_t* first_tile) {
   ChunkShape s{};
   const uint32_t group = q_heads / kv_heads;
-  for (uint32_t i = 0; i < list.count; ++i) {
-    first_tile[i] = s.tiles;
-    s.tiles += ((list.first[i + 1] - list.first[i]) * group + kRows - 1) / kRows;
+  // Tiles run from the last to the first: sequences with few new tokens get the last ones.  (31 that decode and a
+  // chunk behind them in the list: 88 us, in the list's order, with the chunk's tiles first, 93.)
+  std::array<uint16_t, kMaxChunks> order;
+  std::iota(order.begin(), order.begin() + list.count, uint16_t{0});
+  auto tokens = [&](uint32_t i) { return list.first[i + 1] - list.first[i]; };
+  std::stable_sort(order.begin(), order.begin() + list.count, [&](uint32_t a, uint32_t b) { return tokens(a) > tokens(b); });
+  for (uint32_t e = 0; e < list.count; ++e) {
+    first_tile[order[e]] = s.tiles;
+    s.tiles += (tokens(order[e]) * group + kRows - 1) / kRows;
   }
-  for (uint32_t i = list.count; i <= kMaxChunks; ++i) first_tile[i] = s.tiles;
   const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift, items = static_cast<uint64_t>(s.tiles) * kv_heads;
   const uint64_t places = (head_size == 128 ? kResident<128> : kResident<256>) * kComputeUnits;
   const uint64_t most = std::max<uint64_t>(1, capacity / ((head_size == 128 ? kTile<128> : kTile<256>) * kLeastSteps));
@@ -1273,6 +1281,7 @@ extern "C" int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pa
     a.kv_heads = kv_heads;
     a.group = q_heads / kv_heads;
     a.ranges = shape.ranges;
+    a.tiles = shape.tiles;
     a.scale = kLog2E / std::sqrt(static_cast<float>(head_size));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid(static_cast<unsigned>(items)), block(kWaves * 64), join(static_cast<unsigned>((rows + 3) / 4));
