@@ -10,9 +10,10 @@
 // pages for private copies (grant_kernel), and a grid that fills the GPU moves rows and
 // commits (move_kernel).
 //
-// Four sequences that lose a row each take 6.8 + 2.1 + 4.9 us, chains of dependent reads in one
-// workgroup a sequence; eight that lose 512 rows of 16 layers 9.8 + 5.2 + 98 us, the moves' 418 MB
-// at 4.3 TB/s.
+// Few sequences in small tables are chosen and granted by one workgroup (select_grant_kernel).
+//
+// Four sequences that lose a row each take 10.8 + 4.5 us, chains of dependent steps in one workgroup;
+// eight that lose 512 rows of 16 layers 9.8 + 5.2 + 98 us, the moves' 418 MB at 4.3 TB/s.
 #include <algorithm>
 #include <string>
 #include <type_traits>
@@ -88,9 +89,10 @@ __device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
   return v;
 }
 
+// Of the threads of so many waves; with several such groups in a workgroup each has its own partial sums.
 template <unsigned Waves>
 __device__ __forceinline__ uint32_t scan_waves(uint32_t v, uint32_t* partial, uint32_t& total) {
-  const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const unsigned lane = threadIdx.x & 63u, wave = (threadIdx.x >> 6) % Waves;
   const uint32_t sum = scan_lanes(v);
   if (lane == 63u) partial[wave] = sum;
   __syncthreads();
@@ -107,13 +109,15 @@ __device__ __forceinline__ uint32_t scan_waves(uint32_t v, uint32_t* partial, ui
 }
 
 constexpr unsigned kSelectKeys = 4;  // of a thread
+constexpr unsigned kSmallThreads = 256;
+constexpr unsigned kSmallSequences = kGrantThreads / kSmallThreads;
 
 // Numbers of the lanes' flags among those of a block of rows, of keys e * threads + thread in this order: the
 // flags before a lane's own.  counts has room for each wave's of each key; one barrier.
 template <unsigned Waves>
 __device__ __forceinline__ void rank_flags(const bool (&flag)[kSelectKeys], uint32_t* counts, uint32_t (&rank)[kSelectKeys], uint32_t& total) {
   static_assert(kSelectKeys * Waves <= 64);
-  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % Waves;
 #pragma unroll
   for (unsigned e = 0; e < kSelectKeys; ++e) {
     const uint64_t bits = __ballot(flag[e]);
@@ -132,18 +136,28 @@ __device__ __forceinline__ void rank_flags(const bool (&flag)[kSelectKeys], uint
 // key of the last row that fits (a radix select over 8 bits a pass, largest first, until a digit's
 // rows all stay), then in row order which rows stay, and the lists of holes and movers.  Up to four rows a thread lie in
 // registers all the while; each pass has one barrier, its own counts and every wave looks for the digit.
+//
+// A group of threads a sequence; several groups of a workgroup go through the same barriers, those
+// without a sequence or with nothing to drop among them (Groups: then four rows a thread are all).
+constexpr unsigned kCopies = 4;  // of the counts, one for every fourth wave: the first digits of many weights are the same
 template <unsigned Threads>
-__global__ __launch_bounds__(Threads) void select_kernel(EvictArgs a) {
+struct SelectShared {
+  uint32_t histogram[4][kCopies][256];
+  uint32_t partial[Threads / 64];
+  uint32_t counts[3][64];
+};
+
+template <unsigned Threads, bool Groups>
+__device__ __forceinline__ void select_rows(const EvictArgs& a, uint32_t listed, SelectShared<Threads>& lds, uint32_t (*open)[kSmallSequences]) {
   constexpr unsigned kWaves = Threads / 64;
   constexpr uint32_t kRows = Threads * kSelectKeys;
-  constexpr unsigned kCopies = 4;  // of the counts, one for every fourth wave: the first digits of many weights are the same
-  __shared__ uint32_t histogram[4][kCopies][256];
-  __shared__ uint32_t partial[kWaves];
-  __shared__ uint32_t counts[3][64];
-  const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const unsigned tid = threadIdx.x % Threads, lane = tid & 63u, wave = tid >> 6;
+  auto& histogram = lds.histogram;
+  auto& partial = lds.partial;
+  auto& counts = lds.counts;
   const KvPages& pg = a.pages;
-  const uint32_t i = blockIdx.x, slot = listed_slot(a.list, i);
-  const uint32_t capacity = capacity_of(pg), n = min(pg.lengths[slot], capacity), dropped = a.weights.dropped[slot];
+  const uint32_t i = Groups ? min(listed, a.list.count - 1) : listed, slot = listed_slot(a.list, i);
+  const uint32_t capacity = capacity_of(pg), length = min(pg.lengths[slot], capacity), dropped = a.weights.dropped[slot];
   const std::size_t base = static_cast<std::size_t>(slot) * capacity;
   const float* weight = a.weights.weight + base;
   const int32_t* position = a.weights.position + base;
@@ -162,13 +176,15 @@ __global__ __launch_bounds__(Threads) void select_kernel(EvictArgs a) {
   const uint32_t columns = pages_for(a.budget, pg.page_shift), page_tokens = 1u << pg.page_shift;
   const int32_t first_page = tid < min(columns, pg.stride) ? table_page(pg, slot, tid) : -1;
   const uint32_t first_holders = first_page >= 0 ? pg.references[first_page] : 0;
-  if (n <= a.budget) {
-    if (tid == 0) a.headers[i] = EvictHeader{0, 0, 0, 0};
-    return;
+  const bool over = length > a.budget && i == listed;
+  if (!over) {
+    if (tid == 0 && i == listed) a.headers[i] = EvictHeader{0, 0, 0, 0};
+    if constexpr (!Groups) return;
   }
+  const uint32_t n = over ? length : 0;
   const int64_t last = static_cast<int64_t>(n) + dropped - a.recent;  // positions from here on stay
-  uint32_t key[kSelectKeys];
-  bool fixed[kSelectKeys], there[kSelectKeys];
+  uint32_t key[kSelectKeys] = {};
+  bool fixed[kSelectKeys] = {}, there[kSelectKeys] = {};
   auto take = [&](uint32_t from) __attribute__((always_inline)) {
 #pragma unroll
     for (unsigned e = 0; e < kSelectKeys; ++e) {
@@ -181,7 +197,7 @@ __global__ __launch_bounds__(Threads) void select_kernel(EvictArgs a) {
     fetch(from);
     take(from);
   };
-  if constexpr (Threads == 256) __builtin_assume(n <= kRows);  // the table holds no more
+  if constexpr (Threads == kSmallThreads) __builtin_assume(n <= kRows);  // the table holds no more
   const bool resident = n <= kRows;
   for (uint32_t x = tid; x < 4 * kCopies * 256; x += Threads) (&histogram[0][0][0])[x] = 0;
   uint32_t mine = 0;
@@ -198,19 +214,27 @@ __global__ __launch_bounds__(Threads) void select_kernel(EvictArgs a) {
   const bool crowded = protected_rows > a.budget;  // damaged positions: then none is protected
   uint32_t wanted = crowded ? a.budget : a.budget - protected_rows, prefix = 0, high = 0;
   const bool none = wanted == 0;
-  bool exact = none;  // all rows of this prefix stay, later digits do not matter
+  bool exact = none || !over;  // all rows of this prefix stay, later digits do not matter
 #pragma unroll 1
-  for (int shift = 24; shift >= 0 && !exact; shift -= 8) {
+  for (int shift = 24; shift >= 0 && (Groups || !exact); shift -= 8) {
     uint32_t (&own)[256] = histogram[shift / 8][wave % kCopies];
 #pragma unroll 1
     for (uint32_t from = 0; from < n; from += kRows) {
       if (!resident) load(from);
 #pragma unroll
       for (unsigned e = 0; e < kSelectKeys; ++e) {
-        if (there[e] && (key[e] & high) == prefix && (crowded || !fixed[e])) atomicAdd(&own[key[e] >> shift & 255u], 1u);
+        if ((!Groups || !exact) && there[e] && (key[e] & high) == prefix && (crowded || !fixed[e])) atomicAdd(&own[key[e] >> shift & 255u], 1u);
       }
     }
+    if (Groups && tid == 0) open[shift / 8][listed] = exact ? 0 : 1;
     __syncthreads();
+    if constexpr (Groups) {
+      uint32_t any = 0;
+#pragma unroll
+      for (unsigned g = 0; g < kSmallSequences; ++g) any |= open[shift / 8][g];
+      if (__builtin_amdgcn_readfirstlane(any) == 0) break;
+      if (exact) continue;
+    }
     // The digit in which the wanted-th largest lies: sums from the top, four digits a lane.
     uint32_t four[4] = {}, sum = 0;
 #pragma unroll
@@ -246,7 +270,7 @@ __global__ __launch_bounds__(Threads) void select_kernel(EvictArgs a) {
   RowMove* moves = a.moves + static_cast<std::size_t>(i) * a.most_moves;
   uint32_t ties = 0, holes = 0, movers = 0;
 #pragma unroll 1
-  for (uint32_t from = 0; from < n; from += kRows) {
+  for (uint32_t from = 0; from < (Groups ? 1 : n); from += kRows) {
     if (!resident) load(from);
     bool stays[kSelectKeys], tie[kSelectKeys];
 #pragma unroll
@@ -262,11 +286,11 @@ __global__ __launch_bounds__(Threads) void select_kernel(EvictArgs a) {
     for (unsigned e = 0; e < kSelectKeys; ++e) {
       const uint32_t first = from + e * Threads + 64 * wave, row = first + lane;  // 32 | first
       stays[e] |= tie[e] && ties + rank[e] < wanted;
-      hole[e] = row < a.budget && !stays[e];
+      hole[e] = over && row < a.budget && !stays[e];
       mover[e] = row >= a.budget && stays[e];
       const uint64_t bits = __ballot(stays[e] && row < a.budget);
-      if (lane == 0 && first / 32 < a.kept_words) kept_bits[first / 32] = static_cast<uint32_t>(bits);
-      if (lane == 32 && first / 32 + 1 < a.kept_words) kept_bits[first / 32 + 1] = static_cast<uint32_t>(bits >> 32);
+      if (over && lane == 0 && first / 32 < a.kept_words) kept_bits[first / 32] = static_cast<uint32_t>(bits);
+      if (over && lane == 32 && first / 32 + 1 < a.kept_words) kept_bits[first / 32 + 1] = static_cast<uint32_t>(bits >> 32);
     }
     ties += total;
     rank_flags<kWaves>(hole, counts[1], rank, total);
@@ -298,7 +322,7 @@ __global__ __launch_bounds__(Threads) void select_kernel(EvictArgs a) {
     const uint32_t column = from + tid;
     int32_t page = -1;
     bool copy = false;
-    if (column < columns) {
+    if (over && column < columns) {
       page = from == 0 ? first_page : table_page(pg, slot, column);
       if (page >= 0 && (from == 0 ? first_holders : pg.references[page]) > 1) {
         // A row of the page before the budget whose bit is off.
@@ -316,14 +340,24 @@ __global__ __launch_bounds__(Threads) void select_kernel(EvictArgs a) {
     if (copy) copies[at] = PageCopy{column, page, -1, 0};
     found += total;
   }
-  if (tid == 0) a.headers[i] = EvictHeader{min(holes, movers), found, n, 0};
+  if (tid == 0 && over) a.headers[i] = EvictHeader{min(holes, movers), found, n, 0};
+}
+
+template <unsigned Threads>
+__global__ __launch_bounds__(Threads) void select_kernel(EvictArgs a) {
+  __shared__ SelectShared<Threads> lds;
+  select_rows<Threads, false>(a, blockIdx.x, lds, nullptr);
 }
 
 // One workgroup gives every copy a free page, lowest first, sequence by sequence, or fails the
-// call as a whole; then it renames the pages.
-__global__ __launch_bounds__(kGrantThreads) void grant_kernel(EvictArgs a) {
-  __shared__ uint32_t partial[kGrantThreads / 64];
-  __shared__ uint32_t start[kMaxListed + 1];
+// call as a whole (false); then it renames the pages.
+struct GrantShared {
+  uint32_t partial[kGrantThreads / 64];
+  uint32_t start[kMaxListed + 1];
+};
+__device__ __forceinline__ bool grant_pages(const EvictArgs& a, GrantShared& lds) {
+  auto& partial = lds.partial;
+  auto& start = lds.start;
   const unsigned tid = threadIdx.x;
   const KvPages& pg = a.pages;
   uint32_t total;
@@ -333,7 +367,7 @@ __global__ __launch_bounds__(kGrantThreads) void grant_kernel(EvictArgs a) {
   __syncthreads();
   if (total == 0) {
     if (tid == 0) *a.status = 0;
-    return;
+    return true;
   }
   // Twice over the counts: is there enough, then who gets what.
   uint32_t available = 0;
@@ -346,7 +380,7 @@ __global__ __launch_bounds__(kGrantThreads) void grant_kernel(EvictArgs a) {
     *a.status = available < total ? 1 : 0;
     if (available < total) a.headers[0].failed = 1;
   }
-  if (available < total) return;
+  if (available < total) return false;
   uint32_t given = 0;
   for (uint32_t from = 0; from < pg.page_count && given < total; from += kGrantThreads) {
     const uint32_t page = from + tid;
@@ -375,6 +409,26 @@ __global__ __launch_bounds__(kGrantThreads) void grant_kernel(EvictArgs a) {
       atomicSub(&pg.references[a.copies[static_cast<std::size_t>(i) * a.most_copies + c].from], 1u);
     }
   }
+  return true;
+}
+
+__global__ __launch_bounds__(kGrantThreads) void grant_kernel(EvictArgs a) {
+  __shared__ GrantShared lds;
+  grant_pages(a, lds);
+}
+
+// Both for up to four sequences whose tables hold at most 1024 rows, a launch less, which is the host's time (four
+// sequences, a row each, with all calls of the step: 31.2 us, not 36.0; replayed from a graph 23.2 and 21.8).
+
+__global__ __launch_bounds__(kGrantThreads) void select_grant_kernel(EvictArgs a) {
+  __shared__ SelectShared<kSmallThreads> chosen[kSmallSequences];
+  __shared__ GrantShared granted;
+  __shared__ uint32_t open[4][kSmallSequences];  // whether a pass has anything to do for a group
+  const unsigned group = threadIdx.x / kSmallThreads;
+  select_rows<kSmallThreads, true>(a, group, chosen[group], open);
+  __threadfence_block();
+  __syncthreads();
+  grant_pages(a, granted);
 }
 
 constexpr unsigned kMoveThreads = 256, kMoveWorkgroups = 2048;
@@ -553,10 +607,15 @@ extern "C" int32_t gfxinfer_launch_kv_pages_evict(const gfxinfer_kv_pages* pages
     const hipStream_t st = static_cast<hipStream_t>(stream);
     // A wave's instructions are what the choice takes its time with, and sixteen waves share a CU's four vector
     // units: tables of few rows take four (501 rows: 8.5 us, with sixteen 11.1).
-    if (capacity_of(a.pages) <= 256 * kSelectKeys) hipLaunchKernelGGL(select_kernel<256>, dim3(count), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(select_kernel<1024>, dim3(count), dim3(1024), 0, st, a);
-    if (const int32_t s = launch_status("K/V eviction launch failed"); s != GFXI_OK) return s;
-    hipLaunchKernelGGL(grant_kernel, dim3(1), dim3(kGrantThreads), 0, st, a);
+    const bool small = capacity_of(a.pages) <= kSmallThreads * kSelectKeys;
+    if (small && count <= kSmallSequences) {
+      hipLaunchKernelGGL(select_grant_kernel, dim3(1), dim3(kGrantThreads), 0, st, a);
+    } else {
+      if (small) hipLaunchKernelGGL(select_kernel<kSmallThreads>, dim3(count), dim3(kSmallThreads), 0, st, a);
+      else hipLaunchKernelGGL(select_kernel<1024>, dim3(count), dim3(1024), 0, st, a);
+      if (const int32_t s = launch_status("K/V eviction launch failed"); s != GFXI_OK) return s;
+      hipLaunchKernelGGL(grant_kernel, dim3(1), dim3(kGrantThreads), 0, st, a);
+    }
     if (const int32_t s = launch_status("K/V eviction launch failed"); s != GFXI_OK) return s;
     hipLaunchKernelGGL(move_kernel, dim3(std::max(1u, kMoveWorkgroups / count), count), dim3(kMoveThreads), 0, st, a);
     return launch_status("K/V eviction launch failed");

@@ -147,6 +147,21 @@ def test_eviction_equals_the_model(device, gx, layers, page, heads, lengths, bud
     cache.check()                                              # nothing is left to do
 
 
+@pytest.mark.parametrize("page,lengths,stride,budget,shared", [
+    (16, [100, 37, 64, 50, 38, 90, 0, 200], 16, 37, 0),        # more sequences than one workgroup chooses for
+    (16, [120, 37, 1000, 90], 64, 40, 0), (16, [120, 37, 90], 70, 40, 32), (16, [90, 800], 64, 700, 32)])
+def test_tables_of_many_sizes(device, gx, page, lengths, stride, budget, shared):
+    rng = np.random.default_rng(budget + stride)
+    m = _filled(rng, 2, page, (1, 128), lengths, stride, spare=20, shared=shared)
+    cache = Cache(gx, m)
+    say("tables of many sizes", lengths, stride, budget, shared)
+    for _ in range(2):                                         # the second time there is nothing to do
+        sequences = rng.permutation(len(lengths)).tolist()
+        assert m.evict(sequences, budget, 3, 9) == 0
+        assert cache.evict(sequences, budget, 3, 9) == 0
+        cache.check()
+
+
 def test_ties_zeros_infinities_and_nan(device, gx):
     rng = np.random.default_rng(31)
     for values in ([0.0], [-0.0, 0.0], [1.0, 1.0, 2.0], [np.nan, 1.0, np.inf], [np.nan], [np.inf, -np.inf, -1.0], [1e-45, 0.0, 2e-45],
