@@ -20,8 +20,8 @@
 // the exponentials alone take a wave's vector unit nearly as long as both products take the
 // matrix unit.
 //
-// 2048 tokens on 30000, 40 x 8 x 128: 1381 us, 942 TFLOP/s (a large fp16 product: 1.28 PFLOP/s); the matrix units
-// are busy 48 % of the time, waits take 23 % of the waves'.  24 x 4 x 256: 1856 us, 841 TFLOP/s: the outputs of 32 rows
+// 2048 tokens on 30000, 40 x 8 x 128: 1369 us, 950 TFLOP/s (a large fp16 product: 1.28 PFLOP/s); the matrix units
+// are busy 48 % of the time, waits take 23 % of the waves'.  24 x 4 x 256: 1842 us, 848 TFLOP/s: the outputs of 32 rows
 // leave room for one wave a SIMD, and nothing covers its waits.  31 sequences that decode on 200 .. 4090 and a chunk of
 // 509: 77 us, 3.7 TB/s.  Eight that decode on up to 600: 13.4 us, two launches of dependent reads.
 #include <algorithm>
@@ -65,6 +65,7 @@ struct ChunkAttnArgs {
   ChunkList list;
   uint32_t first_tile[kMaxChunks];  // of the listed sequences' row tiles
   uint32_t tiles;
+  uint32_t whole;        // tiles and KV heads that run first and are not divided
   const __half* query;   // [rows][q_heads][D]
   const float* gate;     // [rows][q_heads][2 D] or null
   __half* output;        // [rows][q_heads][D]
@@ -427,7 +428,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   const uint32_t last_row = min(rows, tile_row + kRows) - 1;
   const uint32_t end = length + tokens, steps = (length + last_row / a.group + T) / T;
   // As few ranges as hold them, of equal length.
-  const uint32_t used = (steps - 1) / listed.per + 1, per = (steps + used - 1) / used;
+  const uint32_t used = blockIdx.x % (tiles * a.kv_heads) < a.whole ? 1 : (steps - 1) / listed.per + 1, per = (steps + used - 1) / used;
   const uint32_t from = range * per, to = min(from + per, steps);
   if (from >= steps) {
     const uint32_t row = tile_row + threadIdx.x;
@@ -1160,11 +1161,14 @@ int32_t read_heads(const gfxinfer_kv_pages* pages, uint32_t q_heads) {
 }
 
 struct ChunkShape {
-  uint32_t tiles, ranges;
+  uint32_t tiles, ranges, whole;
 };
 
-// Row tiles, and the ranges that the longest sequence's positions are divided into: two workgroups
-// for each place, as far as full tables hold so many.
+// Row tiles, and the ranges that the longest sequence's positions are divided into: one and a half workgroups
+// for each place (two at head size 256), as far as full tables hold so many.  Where there are tiles for all places, those that
+// make whole rounds are not divided, and the rest only as far as it fills one more round: parts cost a trip through memory
+// (2048 tokens on 30000 in 640 tiles: 1369 us, all of them in two ranges 1412; 3000 on 8000 at head size 256: 912, undivided 1096).
+constexpr uint64_t kMostOfRest = 4;
 ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads, uint32_t head_size,
                        uint32_t* first_tile) {
   ChunkShape s{};
@@ -1182,7 +1186,13 @@ ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads
   const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift, items = static_cast<uint64_t>(s.tiles) * kv_heads;
   const uint64_t places = (head_size == 128 ? kResident<128> : kResident<256>) * kComputeUnits;
   const uint64_t most = std::max<uint64_t>(1, capacity / ((head_size == 128 ? kTile<128> : kTile<256>) * kLeastSteps));
-  s.ranges = static_cast<uint32_t>(std::clamp<uint64_t>((places * (head_size == 128 ? 3 : 4) / 2 + items - 1) / items, 1, most));
+  if (items < places) {
+    s.ranges = static_cast<uint32_t>(std::clamp<uint64_t>((places * (head_size == 128 ? 3 : 4) / 2 + items - 1) / items, 1, most));
+  } else {
+    s.whole = static_cast<uint32_t>(items / places * places);
+    const uint64_t rest = items - s.whole;
+    s.ranges = rest == 0 ? 1 : static_cast<uint32_t>(std::min({places / rest, most, kMostOfRest}));
+  }
   return s;
 }
 
@@ -1282,6 +1292,7 @@ extern "C" int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pa
     a.group = q_heads / kv_heads;
     a.ranges = shape.ranges;
     a.tiles = shape.tiles;
+    a.whole = shape.whole;
     a.scale = kLog2E / std::sqrt(static_cast<float>(head_size));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid(static_cast<unsigned>(items)), block(kWaves * 64), join(static_cast<unsigned>((rows + 3) / 4));

@@ -157,6 +157,14 @@ def test_attention_equals_the_definition(device, gx, heads, page, lengths, token
     c.check(got, sums if gate else None)
 
 
+@pytest.mark.parametrize("heads,page,lengths,tokens", [((32, 1, 256), 32, [100, 60], [1050, 1]), ((32, 1, 128), 64, [300, 5], [2070, 2])])
+def test_more_tiles_than_places(device, gx, heads, page, lengths, tokens):
+    """Tiles that are not divided beside a rest that is, a decoding sequence's few rows among them."""
+    c = Chunks(np.random.default_rng(sum(tokens)), heads, page, lengths, tokens)
+    say("more tiles than places", heads, page, lengths, tokens)
+    c.check(*c.run(gx))
+
+
 @pytest.mark.parametrize("heads", [A, B])
 def test_a_wide_table_divides_the_positions(device, gx, heads):
     """The same rows with a table that leaves room: other ranges, the same result within its tolerance."""
