@@ -81,12 +81,13 @@ constexpr uint32_t kLeastSteps = 2;
 
 // The listed sequence of a row tile, and the steps of a range: ranges are of equal length for all
 // sequences, the longest one is divided into as many as the launch allows and the others into as few
-// as hold them.  The list and the lengths take one round of loads each, a lane a sequence.
+// as hold them.  The list and the lengths take one round of loads each, a lane a sequence; the first pages of the
+// sequence's table come beside its length.
 struct Listed {
   uint32_t slot, length, first_row, tokens, first_tile, per;
 };
 template <unsigned D>
-__device__ __forceinline__ Listed find_listed(const ChunkAttnArgs& a, uint32_t row_tile) {
+__device__ __forceinline__ Listed find_listed(const ChunkAttnArgs& a, uint32_t row_tile, PageWindow& window) {
   const unsigned lane = threadIdx.x & 63u;
   Listed found{};
   uint32_t most = 0;
@@ -94,14 +95,14 @@ __device__ __forceinline__ Listed find_listed(const ChunkAttnArgs& a, uint32_t r
     const uint32_t i = min(from + lane, a.list.count - 1);
     const uint32_t slot = a.list.slot[i], row = a.list.first[i], tokens = a.list.first[i + 1] - row;
     const uint32_t tile = a.first_tile[i], next_tile = tile + (tokens * a.group + kRows - 1) / kRows;
-    const uint32_t length = min(a.pages.lengths[slot], a.pages.stride << a.pages.page_shift);
-    most = max(most, length + tokens);
+    const uint32_t committed = a.pages.lengths[slot];
     const uint64_t here = __ballot(from + lane < a.list.count && tile <= row_tile && row_tile < next_tile);
-    if (here != 0) {
-      const int at = __ffsll(static_cast<unsigned long long>(here)) - 1;
-      auto take = [&](uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), at)); };
-      found = Listed{take(slot), take(length), take(row), take(tokens), take(tile), 0};
-    }
+    const int at = here != 0 ? __ffsll(static_cast<unsigned long long>(here)) - 1 : 0;
+    auto take = [&](uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), at)); };
+    if (here != 0) window.start(a.pages, take(slot), 0);
+    const uint32_t length = min(committed, a.pages.stride << a.pages.page_shift);
+    most = max(most, length + tokens);
+    if (here != 0) found = Listed{take(slot), take(length), take(row), take(tokens), take(tile), 0};
   }
 #pragma unroll
   for (unsigned d = 1; d < 64; d <<= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
@@ -167,7 +168,7 @@ __device__ __forceinline__ void read_tiles(unsigned place, unsigned first, h8 (&
 // maxima and sums.
 template <unsigned D>
 __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& w, const h8 (&q)[D / 16], uint32_t visible,
-                                           _Float16* (&lds)[kWaves], f16v (&o)[D / 32], float& m, float& l) {
+                                           _Float16* (&lds)[kWaves], PageWindow& window, f16v (&o)[D / 32], float& m, float& l) {
   constexpr unsigned kBlock = 32, kLoadRows = 512 / D, kLoads = kBlock / kLoadRows;
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned n = lane & 31u, h = lane >> 5;
@@ -181,7 +182,6 @@ __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& 
   const uint32_t value_part = load_row * row_bytes + 16 * value_slot4(lane % (D / 8), load_row);
   const unsigned value_place = lds_address(vs) + value_place_of<D>(lane);
   const uint32_t first = w.from * kTile<D> / kBlock + wave, last = min(w.to * kTile<D>, w.end + kBlock - 1) / kBlock;
-  PageWindow window;
   h8 k[D / 16];
   int32_t page[2];  // of the block's halves, -1: none; these load from page 0 of the pool (always there)
   // Block b's K rows into k, its V rows into the part `to`.
@@ -209,7 +209,6 @@ __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& 
     l = 0.0F;
 #pragma unroll
     for (unsigned d = 0; d < D / 32; ++d) o[d] = f16v{};
-    window.start(pg, w.slot, first * kBlock >> pg.page_shift);
     if (first < last) load(first, 0);
     unsigned in = 0;
 #pragma unroll 1
@@ -421,7 +420,8 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   // read the same positions run together; late tokens, which see most, first.
   const uint32_t hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
   const uint32_t tiles = a.tiles, range = rest / tiles, row_tile = tiles - 1 - rest % tiles;
-  const Listed listed = find_listed<D>(a, row_tile);
+  PageWindow window;
+  const Listed listed = find_listed<D>(a, row_tile, window);
   const uint32_t slot = listed.slot, first_row = listed.first_row, tokens = listed.tokens, length = listed.length;
   const uint32_t rows = tokens * a.group, tile_row = (row_tile - listed.first_tile) * kRows;
   // The tile's last row sees this many positions; what lies behind the sequence's end is not read.
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
     _Float16* lds[kWaves] = {k0, k1, v0, v1};
     // (Few rows are left to the join even if one range holds them: its waves divide the gate among more
     // lanes, eight decoding sequences 12.9 us, not 14.4.)
-    attend_few<D>(a, Range{slot, end, from, to, hk, least_visible}, q, visible, lds, o, m, l);
+    attend_few<D>(a, Range{slot, end, from, to, hk, least_visible}, q, visible, lds, window, o, m, l);
     if (out_row != 0xffffffffu) write_row<D, D / 128>(a, out_row, range, a.ranges == 1, o, wave, 4, m, l, wave == 0 && h == 0);
     return;
   }
@@ -469,7 +469,6 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   const __half* values = pg.value + layer_row;
   const uint32_t in_page = (1u << pg.page_shift) - 1;
   f16v s[kSub], s_next[kSub];
-  PageWindow window;
   auto find_pages = [&](uint32_t x) __attribute__((always_inline)) {
     TilePages<D> p;
     p.missing = 0;
@@ -661,7 +660,6 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
     l = 0.0F;
 #pragma unroll
     for (unsigned d = 0; d < D / 32; ++d) o[d] = f16v{};
-    window.start(pg, slot, (from * T) >> pg.page_shift);
     TilePages<D> now = find_pages(from), next = now;
     if (careful && threadIdx.x < 32) strange_tiles[threadIdx.x] = 0;
     __syncthreads();  // the tile before this one is done with
@@ -798,18 +796,20 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkAttnArgs a, uint32
 
 // ---- the weight that each position receives ---------------------------------------------
 
+// A listed sequence, all that one load of the arguments has to bring.
+struct WeightItem {
+  uint32_t slot, first_row, tokens;
+};
 struct WeightArgs {
   KvPages pages;
   KvWeights weights;
-  ChunkList list;
   const __half* query;
   const float* log_sums;
   float* partial;  // [sequences with many rows][kv_heads * parts][capacity]
   uint32_t layer, q_heads, kv_heads, group, parts;
   uint32_t columns;  // workgroups along the positions
-  uint32_t many;     // sequences with more than kFewRows rows
   float scale;
-  uint16_t order[kMaxChunks];  // of the listed sequences: those, then the others with rows
+  WeightItem item[kMaxChunks];  // of the launch's sequences: those with more than kFewRows rows, or the others
 };
 
 // Sums of N registers over the 32 lanes of a half: at each exchange a lane keeps the registers whose
@@ -828,13 +828,14 @@ __device__ __forceinline__ float sum_lanes(const float (&sum)[N]) {
   else return sum_lanes<(N > 1 ? N / 2 : 1), 2 * Distance>(half);
 }
 
-// The K row of a position, or one that is always there.
-__device__ __forceinline__ const __half* key_row(const WeightArgs& a, uint32_t slot, uint32_t position, uint32_t end) {
+// The K row of a position on its page (-1: none), or one that is always there.
+__device__ __forceinline__ const __half* key_row(const WeightArgs& a, int32_t page, uint32_t position) {
   const KvPages& pg = a.pages;
-  const int32_t page = position < end ? table_page(pg, slot, position >> pg.page_shift) : -1;
   const std::size_t row = (static_cast<std::size_t>(max(page, 0)) << pg.page_shift) + (page < 0 ? 0 : position & ((1u << pg.page_shift) - 1));
   return pg.key + ((static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) + row) * pg.row;
 }
+
+static_assert(sizeof(WeightArgs) <= 4096);  // arguments of a launch
 
 constexpr uint32_t kFewRows = 32;  // of a sequence and KV head
 
@@ -848,13 +849,18 @@ __global__ __launch_bounds__(256) void few_weight_kernel(WeightArgs a) {
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned n = lane & 31u, h = lane >> 5;
   const KvPages& pg = a.pages;
-  const uint32_t i = a.order[a.many + blockIdx.y], slot = listed_slot(a.list, i), first_row = a.list.first[i];
-  const uint32_t tokens = a.list.first[i + 1] - first_row, rows = tokens * a.group;
-  const uint32_t length = committed(pg, slot), capacity = pg.stride << pg.page_shift, end = min(length + tokens, capacity);
-  const uint32_t t = min(n, rows - 1) / a.group;
+  const WeightItem item = a.item[blockIdx.y];
+  const uint32_t slot = item.slot, first_row = item.first_row, tokens = item.tokens, rows = tokens * a.group;
+  const uint32_t capacity = pg.stride << pg.page_shift, t = min(n, rows - 1) / a.group;
   const std::size_t out_row = (static_cast<std::size_t>(first_row) + t) * a.q_heads + (min(n, rows - 1) - t * a.group);
+  float* weights = a.weights.weight + static_cast<std::size_t>(slot) * capacity;
+  const uint32_t length = committed(pg, slot), end = min(length + tokens, capacity);
+  // (Pages and weights are not asked for before the length is there: half of the workgroups have no
+  // positions, 19.9 us, not 18.6.)
   for (uint32_t at = blockIdx.x * 32; at < end; at += gridDim.x * 32) {
-    const __half* keys = key_row(a, slot, at + n, end) + 8 * h;
+    const int32_t page = table_page(pg, slot, (at + n) >> pg.page_shift);
+    const bool there = at + n < end && page >= 0;
+    const __half* keys = key_row(a, there ? page : -1, at + n) + 8 * h;
     float sum[16] = {};
     for (uint32_t hk = wave; hk < a.kv_heads; hk += 4) {
       const std::size_t row = out_row + hk * a.group;
@@ -878,11 +884,11 @@ __global__ __launch_bounds__(256) void few_weight_kernel(WeightArgs a) {
     // Lane n has the sum of register n % 16: position 8 (r / 4) + 4 h + r % 4.
     if (n < 16) parts[wave][8 * (n / 4) + 4 * h + n % 4] = mine;
     __syncthreads();
-    if (threadIdx.x < 32 && at + threadIdx.x < end && table_page(pg, slot, (at + threadIdx.x) >> pg.page_shift) >= 0) {
+    if (threadIdx.x < 32 && there) {
       float total = 0.0F;
 #pragma unroll
       for (unsigned v = 0; v < 4; ++v) total += parts[v][threadIdx.x];
-      a.weights.weight[static_cast<std::size_t>(slot) * capacity + at + threadIdx.x] += total;
+      weights[at + threadIdx.x] += total;
     }
     __syncthreads();
   }
@@ -931,9 +937,10 @@ __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightA
   const unsigned n = lane & 31u, h = lane >> 5;
   const KvPages& pg = a.pages;
   const uint32_t hk = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads % a.parts;
-  const uint32_t column = blockIdx.x / a.kv_heads / a.parts, i = a.order[blockIdx.y];
-  const uint32_t slot = listed_slot(a.list, i), first_row = a.list.first[i], tokens = a.list.first[i + 1] - first_row;
-  const uint32_t rows = tokens * a.group, all = (rows + kWeightRows - 1) / kWeightRows;
+  const uint32_t column = blockIdx.x / a.kv_heads / a.parts;
+  const WeightItem item = a.item[blockIdx.y];
+  const uint32_t slot = item.slot, first_row = item.first_row, tokens = item.tokens, rows = tokens * a.group;
+  const uint32_t all = (rows + kWeightRows - 1) / kWeightRows;
   const uint32_t length = committed(pg, slot), end = min(length + tokens, pg.stride << pg.page_shift);
   const uint32_t per = (all + a.parts - 1) / a.parts, to = min(part * per + per, all);
   const uint32_t token_bytes = a.q_heads * D * 2;
@@ -951,7 +958,9 @@ __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightA
     if (from < to) {
 #pragma unroll
       for (unsigned p = 0; p < P; ++p) {
-        const __half* row = key_row(a, slot, mine + 32 * p + n, end) + hk * D + 8 * h;
+        const uint32_t position = mine + 32 * p + n;
+        const int32_t page = position < end ? table_page(pg, slot, position >> pg.page_shift) : -1;
+        const __half* row = key_row(a, page, position) + hk * D + 8 * h;
 #pragma unroll
         for (unsigned st = 0; st < D / 16; ++st) k[p][st] = *reinterpret_cast<const h8*>(row + 16 * st);
       }
@@ -1133,7 +1142,7 @@ __global__ __launch_bounds__(256) void weight_join_kernel(WeightArgs a) {
   __shared__ float parts[4][64];
   const KvPages& pg = a.pages;
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t i = a.order[blockIdx.y], slot = listed_slot(a.list, i), tokens = a.list.first[i + 1] - a.list.first[i];
+  const uint32_t slot = a.item[blockIdx.y].slot, tokens = a.item[blockIdx.y].tokens;
   const uint32_t capacity = pg.stride << pg.page_shift, end = min(committed(pg, slot) + tokens, capacity);
   const uint32_t planes = a.kv_heads * a.parts, quarter = (planes + 3) / 4;
   for (uint32_t at = blockIdx.x * 64; at < end; at += gridDim.x * 64) {
@@ -1330,21 +1339,16 @@ extern "C" int32_t gfxinfer_launch_kv_weights_add(const gfxinfer_kv_pages* pages
     if (const int32_t s = read_pages(pages, a.pages); s != GFXI_OK) return s;
     if (const int32_t s = read_weights(weights, a.weights); s != GFXI_OK) return s;
     if (const int32_t s = read_heads(pages, q_heads); s != GFXI_OK) return s;
-    if (const int32_t s = read_chunks(a.pages, sequences, tokens, count, true, a.list); s != GFXI_OK) return s;
+    ChunkList list;
+    if (const int32_t s = read_chunks(a.pages, sequences, tokens, count, true, list); s != GFXI_OK) return s;
     if (layer >= a.pages.layers || query == nullptr || log_sums == nullptr || !aligned16(query) ||
         (reinterpret_cast<uintptr_t>(log_sums) & 3u) != 0) {
       return fail(GFXI_INVALID_ARGUMENT, "weights need a layer of the cache, 16-byte aligned queries and their log sums");
     }
     a.kv_heads = pages->kv_heads;
-    const WeightShape shape = weight_shape(a.pages, a.list, q_heads, a.kv_heads);
+    const WeightShape shape = weight_shape(a.pages, list, q_heads, a.kv_heads);
     a.parts = shape.parts;
     a.columns = shape.columns;
-    a.many = shape.many;
-    for (uint32_t i = 0, many = 0, few = shape.many; i < count; ++i) {
-      const uint64_t rows = static_cast<uint64_t>(a.list.first[i + 1] - a.list.first[i]) * (q_heads / a.kv_heads);
-      if (rows > kFewRows) a.order[many++] = static_cast<uint16_t>(i);
-      else if (rows != 0) a.order[few++] = static_cast<uint16_t>(i);
-    }
     if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < weight_bytes(a.pages, a.kv_heads, shape)) {
       return fail(GFXI_INVALID_ARGUMENT, "K/V weights workspace is null, not 16-byte aligned or too small");
     }
@@ -1357,13 +1361,23 @@ extern "C" int32_t gfxinfer_launch_kv_weights_add(const gfxinfer_kv_pages* pages
     a.scale = kLog2E / std::sqrt(static_cast<float>(pages->head_size));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const uint64_t capacity = static_cast<uint64_t>(a.pages.stride) << a.pages.page_shift;
+    // A launch's sequences in the order of the list; only then is the place of one known without another load.
+    auto list_items = [&](bool few) {
+      for (uint32_t i = 0, at = 0; i < count; ++i) {
+        const WeightItem item{list.slot[i], list.first[i], list.first[i + 1] - list.first[i]};
+        const bool few_rows = static_cast<uint64_t>(item.tokens) * a.group <= kFewRows;
+        if (few_rows == few && item.tokens != 0) a.item[at++] = item;
+      }
+    };
     if (shape.few != 0) {
+      list_items(true);
       const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((capacity + 31) / 32, 1024)), shape.few);
       if (pages->head_size == 128) hipLaunchKernelGGL(few_weight_kernel<128>, grid, dim3(256), 0, st, a);
       else hipLaunchKernelGGL(few_weight_kernel<256>, grid, dim3(256), 0, st, a);
       if (const int32_t s = launch_status("K/V weights launch failed"); s != GFXI_OK) return s;
     }
     if (shape.many == 0) return GFXI_OK;
+    list_items(false);
     const dim3 grid(a.columns * a.kv_heads * a.parts, shape.many);
     if (pages->head_size == 128) hipLaunchKernelGGL(weight_kernel<128>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(weight_kernel<256>, grid, dim3(256), 0, st, a);
