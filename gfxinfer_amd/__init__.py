@@ -626,7 +626,7 @@ def launch_quantize_rows_i8(x, codes, scales, stream=None):
     types, integers = _types()
     rows, columns = x.shape
     L, device, kind = lib(), x.get_device(), types.get(x.dtype)
-    if kind is None or x.stride(1) != 1 or not x.is_cuda:
+    if kind is None or x.stride(1) != 1 or device < 0:
         raise ValueError("row quantizer: x is fp16, fp32 or bf16 [rows, columns] on a GPU, with dense rows")
     check(L.gfxinfer_launch_quantize_rows_i8(
         x.data_ptr(), kind, rows, columns, x.stride(0) if rows > 1 else -(-columns // 8) * 8,
@@ -644,7 +644,7 @@ def launch_w8a8_gemm(weights, weight_scales, codes, scales, output, workspace, s
     types, integers = _types()
     (rows, columns), tokens, L = weights.shape, codes.shape[0], lib()
     device, kind = weights.get_device(), types.get(output.dtype)
-    if not weights.is_cuda or tuple(codes.shape) != (tokens, columns) or tuple(output.shape) != (tokens, rows) or kind in (None, TYPE_BF16):
+    if device < 0 or codes.shape != (tokens, columns) or output.shape != (tokens, rows) or kind is None or kind == TYPE_BF16:
         raise ValueError("8-bit product: weights [rows, columns] on a GPU, codes [tokens, columns], output fp32 or fp16 [tokens, rows]")
     check(L.gfxinfer_launch_w8a8_gemm(
         _operand(weights, integers, rows * columns, device, "weights"), _operand(weight_scales, _real, 4 * rows, device, "weight_scales"),

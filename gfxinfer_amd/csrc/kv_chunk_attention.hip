@@ -841,7 +841,7 @@ constexpr uint32_t kFewRows = 32;  // of a sequence and KV head
 
 // Sequences of at most 32 rows, as a decoding one has: a workgroup takes 32 positions and all KV
 // heads, a wave every fourth one, and adds the sum over all of them.  A position's row holds the heads side by side, so
-// a workgroup reads whole rows, and one launch does (sixteen on up to 4090, 24 x 4 x 256: 16.1 us, 3.9 TB/s; with
+// a workgroup reads whole rows, and one launch does (sixteen on up to 4090, 24 x 4 x 256: 15.7 us, 4.0 TB/s; with
 // a sum for each KV head and a second launch 24.6).
 template <unsigned D>
 __global__ __launch_bounds__(256) void few_weight_kernel(WeightArgs a) {
@@ -924,7 +924,7 @@ struct RowWalk {
 // A wave holds 64 positions of K as the A operand.  The rows of a KV head pass through LDS, 32 at a time,
 // three steps ahead, and serve all waves; the exponentials of a step, each added to the lane's sum of
 // its position, go between the next step's products.  64 positions a wave, not 32: a step's operands are read
-// from LDS by every wave, which at 32 takes as long as its products.  2048 tokens on 8000: 40 x 8 x 128 227 us, 832
+// from LDS by every wave, which at 32 takes as long as its products.  2048 tokens on 8000: 40 x 8 x 128 225 us, 842
 // TFLOP/s, the matrix units busy 47 % of the time, the vector unit 36 %; 24 x 4 x 256 322 us, 706 TFLOP/s.
 template <unsigned D>
 __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightArgs a) {
