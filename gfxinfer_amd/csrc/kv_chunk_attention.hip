@@ -1041,14 +1041,14 @@ __global__ __launch_bounds__(256, kWeightResident<D>) void weight_kernel(WeightA
       };
       auto add_masked = [&](uint32_t x, unsigned d, float level) __attribute__((always_inline)) {
         const uint32_t row = x * kWeightRows + n;
-        const int32_t visible = row < rows && level > -INFINITY  // not of a row that sees nothing, or a NaN
-                                    ? static_cast<int32_t>(length + row / a.group + 1 - mine - 4 * h) : 0;
+        const uint32_t base = mine + 4 * h, end_row = length + row / a.group + 1;
+        const uint32_t visible = row < rows && level > -INFINITY && end_row > base ? end_row - base : 0;  // not of a row that sees nothing, or a NaN
 #pragma unroll
         for (unsigned p = 0; p < P; ++p) {
 #pragma unroll
           for (unsigned r = 0; r < 16; ++r) {
             const float w = __builtin_amdgcn_exp2f(fmaf(s[d % 2][p][r], a.scale, -level));
-            sum[16 * p + r] += static_cast<int32_t>(32 * p + 8 * (r / 4) + r % 4) < visible ? w : 0.0F;
+            sum[16 * p + r] += 32 * p + 8 * (r / 4) + r % 4 < visible ? w : 0.0F;
           }
         }
       };

@@ -486,10 +486,12 @@ __global__ __launch_bounds__(256) void w8a8_join_kernel(ProductArgs a) {
   write_output(a, token, row, sum);
 }
 
-// Up to 48 tokens, and up to 64 of small matrices: 5120 x 5120 and 64 tokens 10.1 us, in tiles 11.8; 5120 x 17408
-// 35.6 and 30.7, with 40 tokens 31.5 and 27.6; 34816 x 5120 and 64 tokens 61.6 and 56.9, with 40 52.2 and 54.5.
+// Up to 64 tokens of small matrices, up to 48 of large ones, up to 8 where there are so few channels that their workgroups
+// leave CUs without work over a long K: 5120 x 5120 and 64 tokens 10.1 us, in tiles 11.8; 34816 x 5120 61.6 and 56.9, with
+// 40 tokens 52.2 and 54.5; 5120 x 17408 with 16 tokens 27.0 and 25.2, with 40 31.5 and 27.6.
 bool few_tokens(std::size_t rows, std::size_t columns, std::size_t tokens) {
-  return tokens <= 48 || (tokens <= 64 && rows * columns < (1u << 26));
+  if (rows * columns < (1u << 26)) return tokens <= 64;
+  return tokens <= (rows < 32 * kComputeUnits ? 8 : 48);
 }
 
 struct ProductShape {
@@ -642,7 +644,10 @@ extern "C" int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float*
                         output_type == GFXI_F16 ? 1u : 0u};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (few_tokens(rows, columns, tokens)) {
-      if (tokens <= 16) launch_few<1, 1, 4, 3>(a, st);
+      // (With few tokens the weights' rows are all that a workgroup reads, with more its tokens' are worth reading for 32 of
+      // them: 17408 x 5120 19.5 us for one token with 16 channels a workgroup, 21.7 with 32; 16 tokens 23.2 and 21.8.)
+      if (tokens <= 4) launch_few<1, 1, 4, 3>(a, st);
+      else if (tokens <= 16) launch_few<1, 2, 4, 3>(a, st);
       else if (tokens <= 32) launch_few<2, 2, 4, 3>(a, st);
       else if (tokens <= 48) launch_few<3, 2, 4, 3>(a, st);
       else launch_few<4, 2, 4, 3>(a, st);

@@ -388,6 +388,18 @@ def test_weights_equal_the_definition(device, gx, heads, page, lengths, tokens):
     assert np.array_equal(got, _weights(c, gx, sums, before))  # the same bits every time
 
 
+@pytest.mark.parametrize("heads", [(40, 1, 128), (33, 1, 256), (128, 2, 128)])
+def test_weights_of_wide_groups(device, gx, heads):
+    """More query heads to a KV head than rows are staged at a time: a step lies within a token, or in two."""
+    rng = np.random.default_rng(sum(heads))
+    c = Chunks(rng, heads, 16, [300, 3, 0], [9, 1, 20], gate=False)
+    say("received weights of wide groups", heads)
+    got, sums = c.run(gx)
+    c.check(got, sums)
+    before = rng.random((4, c.table.shape[1] * 16)).astype(np.float32)
+    _check_weights(c, _weights(c, gx, sums, before), sums, before)
+
+
 def test_weights_of_long_caches(device, gx):
     """More positions than a launch has workgroups for: a chunk's (256 each) and a decoding sequence's (32 each)."""
     rng = np.random.default_rng(24)

@@ -120,7 +120,7 @@ def test_products_equal_the_definition(device, gx, half, tokens, rows, columns):
 
 @pytest.mark.parametrize("tokens,rows,columns", [
     (65, 1999, 528), (65, 1999, 4112), (65, 17001, 1040), (65, 7000, 8208), (1000, 7000, 528), (65, 17001, 8208), (2000, 5000, 656),
-    (4096, 4096, 144), (300, 33025, 272), (400, 33025, 272), (50, 33025, 2064)])
+    (4096, 4096, 144), (300, 33025, 272), (400, 33025, 272), (50, 33025, 2064), (17, 5001, 16400), (9, 5001, 16400), (4, 77, 1040), (5, 77, 1040)])
 def test_every_tile_shape(device, gx, tokens, rows, columns):
     """Small, middle and large tiles, in one piece and with K divided among workgroups, most with a ragged edge; whole rounds of
     the largest tiles alone and with other tiles behind them."""
