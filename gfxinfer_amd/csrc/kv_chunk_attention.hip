@@ -52,11 +52,23 @@ constexpr unsigned kTile = 8192 / D;        // positions of a step: 16 KB of K a
 template <unsigned D>
 constexpr unsigned kResident = D == 128 ? 2 : 1;
 
-// A row's weights are 2^(score - m + kLift) in fp16, scores in units of log2.  m is a maximum of
-// the row so far that moves up once it is passed by kRise, so weights stay below 2^15.  Against
-// the row's largest, weights down to 2^-25 keep fp16's 11 bits and those below 2^-36 are not
-// counted: the one rounding of the weights is half the size of the output's own.
-constexpr float kLift = 11.0F, kRise = 4.0F;
+// A row's weights are 2^(score - m + kLift), scores in units of log2.  m is a maximum of the row so far that moves up
+// once it is passed by kRise, so weights stay below 2^15.  Tiles of more than 32 rows carry a weight as one fp16
+// number: 11 bits, half the size of the output's own rounding, where a second product for 22 bits would take half
+// as much again of the matrix units' time.  Tiles of at most 32 rows wait for memory and carry pairs.
+//
+// fp16 rounds weights below 2^kSmall by 2^-25 and drops those below that.  Beside peaks whose values are near zero they
+// may be all that carries the output (26 nats below a peak, 42 % of 4096 of them was lost).  So a row is open until
+// its weights below 2^kPeak sum up to n kMean, n the positions beside one that it sees: then less than 2^-10 of their sum is
+// lost where they spread by 3 nats, nothing where they spread by one, and 2^-7 were one weight the sum and all others just too
+// small.  (Or until all its weights sum up to kMany: then 16 positions or more are peaks.)  Steps look for that
+// until a row has kAmple times as much.  Where small weights were met and the row is open to the end, two more passes
+// over the range take what lies below the peaks, with a maximum of its own, and the peaks.
+//
+// (Products of their own for small weights where they are met took 5 to 17 % of all calls' time by their presence alone,
+// as a branch between the products of a step.  A call takes as long as its slowest tile, so what one tile goes over again
+// shows: 2048 tokens on 30000 with scores that spread by 3 nats 1590 us, not 1530; by 6 nats 3600, not 1490.)
+constexpr float kLift = 11.0F, kRise = 4.0F, kSmall = -14.0F, kPeak = 8.0F, kMean = 0x1p-18F, kMany = 0x1p19F, kAmple = 256.0F;
 
 constexpr float kWritten = -1.0F;  // in the place of range 0's sum: the row is complete, nothing to join
 
@@ -122,6 +134,79 @@ __device__ __forceinline__ float sum_over_halves(float v) {
   return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
+// A row's maximum, and whether its small weights may matter.  What is seldom needed lies in LDS: registers, scalar ones
+// too, are all taken.
+struct Peaks {
+  struct Found {
+    float others;  // the sum of weights below 2^kPeak as far as it was looked for
+    float small;   // 1: small weights were met on the way
+  };
+  float m;
+  Found* found;
+  bool looks;  // a row of the wave looks for more
+
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    *found = Found{0.0F, 0.0F};
+    looks = false;
+  }
+  __device__ __forceinline__ bool moves(float top) const { return __any(!(top <= m + kRise)) || looks; }
+  // Whether a row has `share` times what it needs.  all: the sum of its weights; positions: what it sees in all steps, one at
+  // least.
+  __device__ __forceinline__ bool has(float share, float others, float all, uint32_t positions) const {
+    return m == -INFINITY || others >= kMean * share * static_cast<float>(positions - 1) || all >= kMany;
+  }
+  // A step that moves: the raw scores s(0) .. s(N - 1) of a lane's half of its row, the largest of the row, `top`, and the
+  // lane's sum of weights before this step.  Returns the factor of the sums so far.
+  template <bool Look, unsigned N, typename Score>
+  __device__ __forceinline__ float move(Score s, float scale, float top, uint32_t positions, float before) {
+    const float next = top <= m + kRise ? m : top;
+    // From nothing to something: there is nothing to scale yet.
+    const float factor = next == m || m == -INFINITY ? 1.0F : rescale_factor(m, next);
+    if constexpr (Look) {
+      Found now = *found;
+      const float all = sum_over_halves(before) * factor;
+      // After a rise by so much none of the weights so far is a peak.
+      now.others = m != -INFINITY && next - m >= kLift + kRise - kPeak ? all : now.others * factor;
+      m = next;
+      looks = !__all(has(kAmple, now.others, all, positions));
+      if (looks) {
+        float here = 0.0F;
+        bool small = false;
+#pragma unroll
+        for (unsigned e = 0; e < N; ++e) {
+          const float x = fmaf(s(e), scale, kLift - m);
+          here += x < kPeak ? __builtin_amdgcn_exp2f(x) : 0.0F;
+          small |= x < kSmall && x > -INFINITY;
+        }
+        now.others += sum_over_halves(here);
+        if (small) now.small = 1.0F;
+        looks = !__all(has(kAmple, now.others, all, positions));
+      }
+      *found = now;
+    }
+    m = next;
+    return factor;
+  }
+  // Rows that do not have enough where small weights were met, a bit a lane.
+  __device__ __forceinline__ uint64_t open(float all, uint32_t positions) const {
+    const Found now = *found;
+    const uint64_t small = __ballot(now.small != 0.0F);
+    return (small | small >> 32 | small << 32) & ~__ballot(has(1.0F, now.others, sum_over_halves(all), positions));
+  }
+};
+
+// The scores that a careful pass takes, of a lane's row: above x, up to y.  In LDS.
+struct Limits {
+  float2* scores;
+  // All, but for the rows `taken`: those below their peaks.
+  __device__ __forceinline__ void below_peaks(float m, uint64_t taken) const {
+    scores[threadIdx.x] = float2{-INFINITY, (taken >> (threadIdx.x & 63u) & 1u) != 0 ? m - kLift + kPeak : INFINITY};
+  }
+  // The peaks; none of the other rows, which are complete.
+  __device__ __forceinline__ void peaks() const { scores[threadIdx.x] = float2{scores[threadIdx.x].y, INFINITY}; }
+};
+
 // V rows in LDS: piece c of row r lies in slot c ^ 4 (r % 4), so that the four rows of 64 bytes that half
 // a wave reads at once (a transposing read of 32 columns) fall on different banks.
 __device__ __forceinline__ unsigned value_slot4(unsigned piece, unsigned row) { return piece ^ 4 * (row & 3u); }
@@ -168,7 +253,7 @@ __device__ __forceinline__ void read_tiles(unsigned place, unsigned first, h8 (&
 // maxima and sums.
 template <unsigned D>
 __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& w, const h8 (&q)[D / 16], uint32_t visible,
-                                           _Float16* (&lds)[kWaves], PageWindow& window, f16v (&o)[D / 32], float& m, float& l) {
+                                           _Float16* (&lds)[kWaves], Peaks::Found* found, const Limits& limit, PageWindow& window, f16v (&o)[D / 32], float& m, float& l) {
   constexpr unsigned kBlock = 32, kLoadRows = 512 / D, kLoads = kBlock / kLoadRows;
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned n = lane & 31u, h = lane >> 5;
@@ -202,63 +287,79 @@ __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& 
                                                static_cast<int>((row0 & 15u) * row_bytes), 0, 0);
     }
   };
-  bool careful = false, strange;
-#pragma unroll 1
-  for (;; careful = true) {
-    m = -INFINITY;
-    l = 0.0F;
+  Peaks row{-INFINITY, found + 64 * wave + lane, false};
+  // A weight is high + low, both rounded to nearest: off by 2^-23 of itself, or by 2^-25 if that is more.
+  auto rest_of = [](float x, _Float16 high) __attribute__((always_inline)) { return static_cast<_Float16>(x - static_cast<float>(high)); };
+  // What a row sees of the wave's blocks: whole ones, and one in part.
+  const uint32_t cut = visible / kBlock, whole = cut > first ? (min(cut, last) - first + kWaves - 1) / kWaves * kBlock : 0;
+  const uint32_t positions = max(1u, whole + (cut < last && cut % kWaves == first % kWaves ? visible % kBlock : 0));
+  // Passes: the first one; a careful one, without the peaks of rows whose small weights may matter; those peaks.
+  bool careful = false, apart = false, strange;
+  row.clear();
+  l = 0.0F;
 #pragma unroll
-    for (unsigned d = 0; d < D / 32; ++d) o[d] = f16v{};
+  for (unsigned d = 0; d < D / 32; ++d) o[d] = f16v{};
+#pragma unroll 1
+  for (;;) {
     if (first < last) load(first, 0);
     unsigned in = 0;
 #pragma unroll 1
     for (uint32_t b = first; b < last; b += kWaves, in ^= 1) {
       const uint32_t at = b * kBlock;
-      const int32_t here[2] = {page[0], page[1]};
+      const bool gone = page[0] < 0, upper_gone = page[1] < 0;  // of the halves
       f16v s = {};
 #pragma unroll
       for (unsigned st = 0; st < D / 16; ++st) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[st], q[st], s, 0, 0, 0);
       const bool more = b + kWaves < last;
       if (more) load(b + kWaves, in ^ 1);
-      if (at + kBlock > w.least || here[0] < 0 || here[1] < 0) {
+      if (at + kBlock > w.least || gone || upper_gone) {
 #pragma unroll
         for (unsigned r = 0; r < 16; ++r) {
-          if (at + 8 * (r / 4) + 4 * h + r % 4 >= visible || here[r / 8] < 0) s[r] = -INFINITY;
+          if (at + 8 * (r / 4) + 4 * h + r % 4 >= visible || (r < 8 ? gone : upper_gone)) s[r] = -INFINITY;
+        }
+      }
+      if (careful) {
+        const float2 limits = limit.scores[threadIdx.x];
+#pragma unroll
+        for (unsigned r = 0; r < 16; ++r) {
+          if (s[r] * a.scale <= limits.x || s[r] * a.scale > limits.y) s[r] = -INFINITY;  // (not NaN)
         }
       }
       float best = s[0];
 #pragma unroll
       for (unsigned r = 1; r < 16; ++r) best = __builtin_elementwise_maximum(best, s[r]);
       const float top = max_over_halves(best) * a.scale;
-      if (__any(!(top <= m + kRise))) {
-        const float next = top <= m + kRise ? m : top;
-        const float factor = next == m || m == -INFINITY ? 1.0F : rescale_factor(m, next);
-        m = next;
+      if (row.moves(top)) {
+        const float factor = row.move<true, 16>([&](unsigned e) { return s[e]; }, a.scale, top, positions, l);
         l *= factor;
+        if (__any(factor != 1.0F)) {
 #pragma unroll
-        for (unsigned d = 0; d < D / 32; ++d) {
+          for (unsigned d = 0; d < D / 32; ++d) {
 #pragma unroll
-          for (unsigned r = 0; r < 16; ++r) o[d][r] *= factor;
+            for (unsigned r = 0; r < 16; ++r) o[d][r] *= factor;
+          }
         }
       }
-      const float floor = m == -INFINITY ? 0.0F : m - kLift;
-      h8 p[2];
+      const float floor = row.m == -INFINITY ? 0.0F : row.m - kLift;
+      h8 high[2], low[2];
 #pragma unroll
       for (unsigned r = 0; r < 16; ++r) {
         const float x = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale, -floor));
         l += x;
-        p[r / 8][r % 8] = static_cast<_Float16>(x);
+        high[r / 8][r % 8] = static_cast<_Float16>(x);
+        low[r / 8][r % 8] = rest_of(x, high[r / 8][r % 8]);
       }
       // The block's V rows are there when only the next block's loads are on their way.
       if (more) wait_loads<D / 16 + kLoads>();
       else wait_loads<0>();
-      if (careful || at + kBlock > w.end || here[0] < 0 || here[1] < 0) {  // as in the attention kernel
+      bool odd = false;
+      if (careful || at + kBlock > w.end || gone || upper_gone) {  // as in the attention kernel
 #pragma unroll 1
         for (unsigned u = 0; u < kLoads; ++u) {
           const unsigned row0 = kLoadRows * u;
           u32x4* piece = reinterpret_cast<u32x4*>(vs + (in * kBlock + row0) * D) + lane;
-          if (at + row0 + load_row >= w.end || (row0 < 16 ? here[0] : here[1]) < 0) *piece = u32x4{0, 0, 0, 0};
-          if (careful) take_strange(piece);
+          if (at + row0 + load_row >= w.end || (row0 < 16 ? gone : upper_gone)) *piece = u32x4{0, 0, 0, 0};
+          if (careful) odd |= take_strange(piece);
         }
         wait_loads<63>();
       }
@@ -266,19 +367,23 @@ __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& 
 #pragma unroll
       for (unsigned d = 0; d < D / 32; d += 4) {
         h8 v[4];
+        auto add = [&](unsigned half) __attribute__((always_inline)) {
+#pragma unroll
+          for (unsigned e = 0; e < 4; ++e) o[d + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[e], low[half], o[d + e], 0, 0, 0);
+#pragma unroll
+          for (unsigned e = 0; e < 4; ++e) o[d + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[e], high[half], o[d + e], 0, 0, 0);
+        };
         read_tiles<D, 0>(place, d, v);
-#pragma unroll
-        for (unsigned e = 0; e < 4; ++e) o[d + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[e], p[0], o[d + e], 0, 0, 0);
+        add(0);
         read_tiles<D, 16>(place, d, v);
-#pragma unroll
-        for (unsigned e = 0; e < 4; ++e) o[d + e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[e], p[1], o[d + e], 0, 0, 0);
+        add(1);
       }
-      if (careful) {
+      if (__any(odd)) {
         // The rows that see an infinity or NaN among the values get it, whatever the weight.
 #pragma unroll 1
         for (unsigned x = 0; x < kBlock; ++x) {
-          const int32_t one = x < 16 ? here[0] : here[1];
-          if (at + x >= w.end || one < 0) continue;
+          const int32_t one = at + x < w.end ? table_page(pg, w.slot, (at + x) >> pg.page_shift) : -1;
+          if (one < 0) continue;
           const __half* v = values + ((static_cast<std::size_t>(one) << pg.page_shift) + ((at + x) & in_page)) * pg.row;
 #pragma unroll
           for (unsigned d = 0; d < D / 32; ++d) {
@@ -298,9 +403,25 @@ __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& 
 #pragma unroll
       for (unsigned r = 0; r < 16; ++r) strange |= !(fabsf(o[d][r]) < INFINITY);
     }
-    if (careful || !__any(strange)) break;
+    if (!careful) {
+      const uint64_t taken = row.open(l, positions);
+      if (!__any(strange) && taken == 0) break;
+      careful = true;
+      apart = taken != 0;
+      limit.below_peaks(row.m, taken);
+      row.clear();
+      l = 0.0F;
+#pragma unroll
+      for (unsigned d = 0; d < D / 32; ++d) o[d] = f16v{};
+    } else if (apart) {
+      apart = false;
+      limit.peaks();  // added to what is there
+    } else {
+      break;
+    }
   }
   l = sum_over_halves(l);
+  m = row.m;
   if ((m == -INFINITY && (l != l || (careful && strange))) || m != m) m = 0.0F;
   // The waves' results, four output tiles at a time.
   float2* ml = reinterpret_cast<float2*>(lds[0]);  // [waves][32], once V is no longer needed
@@ -411,8 +532,11 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   __shared__ __align__(1024) _Float16 k1[kPart];
   __shared__ __align__(1024) _Float16 v0[kPart];
   __shared__ __align__(1024) _Float16 v1[kPart];
+  __shared__ Peaks::Found found[kWaves * 64];
+  __shared__ float2 taken_scores[kWaves * 64];
   __shared__ uint32_t again[kWaves];       // the wave's rows met an infinity or NaN
   __shared__ uint32_t strange_tiles[32];   // bit x % 1024: a tile x holds infinities or NaNs among its values
+  const Limits limit{taken_scores};
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned n = lane & 31u, h = lane >> 5;
   const KvPages& pg = a.pages;
@@ -460,7 +584,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
     _Float16* lds[kWaves] = {k0, k1, v0, v1};
     // (Few rows are left to the join even if one range holds them: its waves divide the gate among more
     // lanes, eight decoding sequences 12.9 us, not 14.4.)
-    attend_few<D>(a, Range{slot, end, from, to, hk, least_visible}, q, visible, lds, window, o, m, l);
+    attend_few<D>(a, Range{slot, end, from, to, hk, least_visible}, q, visible, lds, found, limit, window, o, m, l);
     if (out_row != 0xffffffffu) write_row<D, D / 128>(a, out_row, range, a.ranges == 1, o, wave, 4, m, l, wave == 0 && h == 0);
     return;
   }
@@ -469,6 +593,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   const __half* values = pg.value + layer_row;
   const uint32_t in_page = (1u << pg.page_shift) - 1;
   f16v s[kSub], s_next[kSub];
+  Peaks peaks{-INFINITY, found + threadIdx.x, false};
   auto find_pages = [&](uint32_t x) __attribute__((always_inline)) {
     TilePages<D> p;
     p.missing = 0;
@@ -512,16 +637,16 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   // What a page holds past a sequence's end, and what a missing one would, may be anything, and 0 * NaN
   // is NaN: the wave's own V rows of such positions become zeros.  A careful pass also takes out
   // infinities and NaNs, and marks the tile.
-  auto repair = [&](_Float16* vs, uint32_t x, uint32_t missing, auto careful) __attribute__((always_inline)) {
+  auto repair = [&](_Float16* vs, uint32_t x, uint32_t missing, bool careful) __attribute__((always_inline)) {
     bool strange = false;
 #pragma unroll 1
     for (unsigned u = 0; u < kLoads; ++u) {
       const unsigned row0 = kLoadRows * (wave + kWaves * u);
       u32x4* piece = reinterpret_cast<u32x4*>(vs + row0 * D) + lane;
       if (x * T + row0 + load_row >= end || (missing >> row0 / 16 & 1u) != 0) *piece = u32x4{0, 0, 0, 0};
-      if constexpr (careful) strange |= take_strange(piece);
+      if (careful) strange |= take_strange(piece);
     }
-    if (careful && strange) atomicOr(&strange_tiles[x / 32 % 32], 1u << x % 32);
+    if (strange) atomicOr(&strange_tiles[x / 32 % 32], 1u << x % 32);
     wait_loads<63>();
   };
   // The rows that see an infinity or NaN among the values get it, whatever the weight: no weight is
@@ -567,7 +692,8 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
     }
   };
   // Scores of a tile are ready: hides what a row does not see, and moves the maxima.
-  auto settle = [&](f16v (&sc)[kSub], uint32_t x, uint32_t missing) __attribute__((always_inline)) {
+  auto positions = [&] { return max(min(visible, to * T), from * T + 1) - from * T; };
+  auto settle = [&](f16v (&sc)[kSub], uint32_t x, uint32_t missing, auto careful) __attribute__((always_inline)) {
     if (x * T + T > least_visible || missing != 0) {
 #pragma unroll
       for (unsigned u = 0; u < kSub; ++u) {
@@ -578,22 +704,30 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
         }
       }
     }
+    if constexpr (careful) {
+      const float2 limits = taken_scores[threadIdx.x];
+#pragma unroll
+      for (unsigned e = 0; e < 16 * kSub; ++e) {
+        const float score = sc[e / 16][e % 16] * a.scale;
+        if (score <= limits.x || score > limits.y) sc[e / 16][e % 16] = -INFINITY;  // (not NaN)
+      }
+    }
     // (A NaN score makes the maximum NaN and the row's result with it, as it has to.)
     float best = sc[0][0];
 #pragma unroll
     for (unsigned e = 1; e < 16 * kSub; ++e) best = __builtin_elementwise_maximum(best, sc[e / 16][e % 16]);
     const float top = max_over_halves(best) * a.scale;
     keep_outputs();
-    if (__any(!(top <= m + kRise))) {
-      const float next = top <= m + kRise ? m : top;
-      // From nothing to something: there is nothing to scale yet.
-      const float factor = next == m || m == -INFINITY ? 1.0F : rescale_factor(m, next);
-      m = next;
-      l *= factor;
+    if (peaks.moves(top)) {
+      const float factor = peaks.move<!careful.value, 16 * kSub>([&](unsigned e) { return sc[e / 16][e % 16]; }, a.scale, top,
+                                                 positions(), l);
+      if (__any(factor != 1.0F)) {
+        l *= factor;
 #pragma unroll
-      for (unsigned d = 0; d < D / 32; ++d) {
+        for (unsigned d = 0; d < D / 32; ++d) {
 #pragma unroll
-        for (unsigned r = 0; r < 16; ++r) o[d][r] *= factor;
+          for (unsigned r = 0; r < 16; ++r) o[d][r] *= factor;
+        }
       }
       keep_outputs();
     }
@@ -604,7 +738,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
     h8 p[kSteps];
     keep_outputs();
     score(next_ks, s_next);
-    const float floor = m == -INFINITY ? 0.0F : m - kLift;
+    const float floor = peaks.m == -INFINITY ? 0.0F : peaks.m - kLift;
     float sum[4] = {l, 0.0F, 0.0F, 0.0F};
 #pragma unroll
     for (unsigned j = 0; j < kSteps; ++j) {
@@ -655,11 +789,14 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
 
   // Tile x's V rows and tile x + 1's K rows are read while x + 1's V rows and x + 2's K rows are on their way,
   // each into the place that was read last before the barrier.
-  auto pass = [&](auto careful) __attribute__((always_inline)) {
-    m = -INFINITY;
+  auto clear = [&] {
+    peaks.clear();
     l = 0.0F;
 #pragma unroll
     for (unsigned d = 0; d < D / 32; ++d) o[d] = f16v{};
+  };
+  bool odd = false;  // infinities and NaNs among the values are looked for
+  auto pass = [&](auto careful, uint32_t from) __attribute__((always_inline)) {
     TilePages<D> now = find_pages(from), next = now;
     if (careful && threadIdx.x < 32) strange_tiles[threadIdx.x] = 0;
     __syncthreads();  // the tile before this one is done with
@@ -673,11 +810,11 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
     }
     if (works) {
       score(k0, s);
-      settle(s, from, now.missing);
+      settle(s, from, now.missing, careful);
     }
     auto turn = [&](uint32_t x, _Float16* k_free, const _Float16* k_next, _Float16* v_now, _Float16* v_free) __attribute__((always_inline)) {
       wait_loads<0>();
-      if (careful || now.missing != 0 || (x + 1) * T > end) repair(v_now, x, now.missing, careful);
+      if ((careful && odd) || now.missing != 0 || (x + 1) * T > end) repair(v_now, x, now.missing, careful && odd);
       __syncthreads();
       now = next;
       if (x + 1 < to) load(v_free, values, false, x + 1, next);
@@ -687,7 +824,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
       }
       if (works) {
         step(k_next, v_now);
-        if (x + 1 < to) settle(s, x + 1, now.missing);
+        if (x + 1 < to) settle(s, x + 1, now.missing, careful);
       }
     };
 #pragma unroll 1
@@ -707,23 +844,37 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
     return strange;
   };
 
-  pass(std::false_type{});
+  clear();
+  pass(std::false_type{}, from);
   bool strange = is_strange();
-  // A second, careful pass follows in the rare case that an output of the first is an infinity or NaN.
-  const bool mine = __any(strange);
-  if (lane == 0) again[wave] = mine ? 1u : 0u;
+  // Careful passes follow in the rare case that an output of the first is an infinity or NaN, or that a row's small weights
+  // may matter.
+  const uint64_t taken = peaks.open(l, positions());
+  const uint32_t mine = (__any(strange) ? 1u : 0u) | (taken != 0 ? 2u : 0u);
+  if (lane == 0) again[wave] = mine;
   __syncthreads();
-  uint32_t found = 0;
-  for (unsigned w = 0; w < kWaves; ++w) found |= again[w];
-  const bool careful = __builtin_amdgcn_readfirstlane(found) != 0;
+  uint32_t any = 0;
+  for (unsigned w = 0; w < kWaves; ++w) any |= again[w];
+  any = __builtin_amdgcn_readfirstlane(any);
+  const bool careful = any != 0;
   if (__builtin_expect(careful, 0)) {
-    pass(std::true_type{});
+    // Everything but the peaks of such rows, then those peaks.
+    odd = (any & 1u) != 0;
+    limit.below_peaks(peaks.m, taken);
+    clear();
+#pragma unroll 1
+    for (bool apart = any >= 2;; apart = false) {
+      pass(std::true_type{}, fresh_number(from));  // (what follows from it is not kept from one pass for the next)
+      if (!apart) break;
+      limit.peaks();  // added to what is there
+    }
     for (uint32_t x = from; x < to; ++x) {
       if ((__builtin_amdgcn_readfirstlane(strange_tiles[x / 32 % 32]) >> x % 32 & 1u) != 0) add_strange(x);
     }
     strange = is_strange();
   }
   l = sum_over_halves(l);
+  m = peaks.m;
   // Only NaN scores, and strange values at scores of -infinity, make a NaN row rather than an empty one.
   if ((m == -INFINITY && (l != l || (careful && strange))) || m != m) m = 0.0F;
   if (out_row != 0xffffffffu) write_row<D, D / 32>(a, out_row, range, used == 1, o, 0, 1, m, l, h == 0);

@@ -745,6 +745,10 @@ size_t gfxinfer_kv_pages_chunk_attention_workspace_bytes(const gfxinfer_kv_pages
  * head row used, or NULL for no gate; output fp16 [rows][q_heads][hd]; log_sums fp32
  * [rows][q_heads], or NULL: the natural logarithm of the sum of exp(score) of a row, -inf for
  * a row that sees nothing (its output is zeros).  A position without a page is not seen.
+ * A row's weights keep 11 bits each (gated_attention: 23), 22 where it is one of at most 32 in a
+ * tile, as when a sequence decodes: tokens times query heads of a KV head, in tiles of 128.
+ * The weights beside a row's largest (up to 15 of them, within 2 nats) together lose at most
+ * 2^-7 of their sum, 2^-10 where their scores spread by up to 3 nats.  Sums are fp32.
  * Where a row's positions are cut for different workgroups, and so the order of its fp32
  * additions, depends on the token counts and lengths of all listed sequences: equal calls give
  * equal bits, a row beside other sequences may differ in the last ones. */
