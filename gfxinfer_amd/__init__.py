@@ -534,7 +534,7 @@ def launch_kv_pages_gated_attention(pages, layer, query, gate, output, sequences
 class KvWeights(ctypes.Structure):
     """gfxinfer_kv_weights.  `of` describes tensors beside the pages and keeps them alive."""
     _fields_ = [("weight", P), ("position", P), ("dropped", P)]
-    device = None
+    device = shape = None  # of tensors given to `of`
 
     @classmethod
     def of(cls, pages, weight, position, dropped):
@@ -545,10 +545,19 @@ class KvWeights(ctypes.Structure):
                 or any(t.is_floating_point() for t in tensors[1:])):
             raise ValueError("K/V weights: contiguous fp32 weight and int32 position for every row of the table, int32 dropped")
         self = cls(*(_p(t) for t in tensors))
-        self.tensors, self.device = tensors, _device_of(tensors, "K/V weights")
+        self.tensors, self.shape, self.device = tensors, shape, _device_of(tensors, "K/V weights")
         if pages.device is not None and self.device not in (None, pages.device):
             raise ValueError("K/V weights: tensors of another device than the pages")
         return self
+
+
+def _weights_of(weights, pages):
+    """The address of weights that fit the pages: those of another cache have other rows."""
+    if weights.shape not in (None, (pages.sequences, pages.table_stride * pages.page_tokens)):
+        raise ValueError("K/V weights: made for pages with other sequences or another table")
+    if None not in (weights.device, pages.device) and weights.device != pages.device:
+        raise ValueError("K/V weights: tensors of another device than the pages")
+    return ctypes.byref(weights)
 
 
 def _chunk_lists(sequences, tokens):
@@ -581,7 +590,7 @@ def launch_kv_pages_chunk_attention(pages, layer, query, gate, output, log_sums,
 def launch_kv_weights_begin(pages, weights, sequences, tokens, stream=None):
     L = lib()
     _ids, _counts, at, tokens_at, count, _ = _chunk_lists(sequences, tokens)
-    check(L.gfxinfer_launch_kv_weights_begin(ctypes.byref(pages), ctypes.byref(weights), at, tokens_at, count,
+    check(L.gfxinfer_launch_kv_weights_begin(ctypes.byref(pages), _weights_of(weights, pages), at, tokens_at, count,
                                              _launch_stream(pages.device, stream)))
 
 
@@ -595,7 +604,7 @@ def launch_kv_weights_add(pages, weights, layer, query, log_sums, sequences, tok
     L, device = lib(), pages.device
     _ids, _counts, at, tokens_at, count, rows = _chunk_lists(sequences, tokens)
     check(L.gfxinfer_launch_kv_weights_add(
-        ctypes.byref(pages), ctypes.byref(weights), layer, _operand(query, _half, 2 * rows * q_heads * pages.head_size, device, "query"),
+        ctypes.byref(pages), _weights_of(weights, pages), layer, _operand(query, _half, 2 * rows * q_heads * pages.head_size, device, "query"),
         _operand(log_sums, _real, 4 * rows * q_heads, device, "log_sums"), at, tokens_at, count, q_heads,
         *_scratch(workspace, device), _launch_stream(device, stream)))
 
@@ -608,7 +617,7 @@ def launch_kv_pages_evict(pages, weights, sequences, budget, first, recent, stat
     """status: a device int32."""
     L, ids, device = lib(), _host_ids(sequences), pages.device
     at, count = ids.buffer_info()
-    check(L.gfxinfer_launch_kv_pages_evict(ctypes.byref(pages), ctypes.byref(weights), at, count, budget, first, recent,
+    check(L.gfxinfer_launch_kv_pages_evict(ctypes.byref(pages), _weights_of(weights, pages), at, count, budget, first, recent,
                                            _operand(status, _word, 4, device, "status"), *_scratch(workspace, device),
                                            _launch_stream(device, stream)))
 
