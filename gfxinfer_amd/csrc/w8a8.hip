@@ -95,16 +95,18 @@ __device__ __forceinline__ uint32_t four_codes(const float (&x)[8], unsigned fir
 }
 
 constexpr unsigned kQuantUnits = 4;  // of eight values a thread keeps
+constexpr unsigned kGridRows = 1u << 20;  // along x: a launch holds less than 2^32 threads in one dimension
 
 // A workgroup a row, read once and kept in registers: bytes, 4096 rows of 5120 in fp16 15 us (4.1 TB/s), one
 // row 3.3 us, the time of a launch and three dependent steps.  A row that holds an infinity or a NaN gets a NaN scale and zero codes,
 // so every product with it is NaN; a row of zeros the smallest normal scale.
 template <int Type, unsigned Threads>
-__global__ __launch_bounds__(Threads) void quantize_rows_kernel(const void* __restrict__ input, std::size_t stride,
+__global__ __launch_bounds__(Threads) void quantize_rows_kernel(const void* __restrict__ input, std::size_t stride, uint32_t rows,
                                                                 uint32_t columns, int8_t* __restrict__ codes,
                                                                 float* __restrict__ scales) {
   __shared__ float partial[Threads / 64];
-  const std::size_t row = blockIdx.x;
+  const std::size_t row = blockIdx.y * kGridRows + blockIdx.x;
+  if (row >= rows) return;
   const uint32_t units = columns / 8;
   float x[kQuantUnits][8];
   float top = 0.0F;
@@ -579,11 +581,12 @@ void launch_few(const ProductArgs& a, hipStream_t stream) {
 template <int Type>
 void launch_quantize(const void* input, std::size_t rows, std::size_t stride, uint32_t columns, int8_t* codes, float* scales,
                      hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(rows));
+  const uint32_t n = static_cast<uint32_t>(rows);
+  const dim3 grid(std::min(n, kGridRows), (n + kGridRows - 1) / kGridRows);
   if (columns <= 256 * 8 * kQuantUnits) {
-    hipLaunchKernelGGL((quantize_rows_kernel<Type, 256>), grid, dim3(256), 0, stream, input, stride, columns, codes, scales);
+    hipLaunchKernelGGL((quantize_rows_kernel<Type, 256>), grid, dim3(256), 0, stream, input, stride, n, columns, codes, scales);
   } else {
-    hipLaunchKernelGGL((quantize_rows_kernel<Type, 1024>), grid, dim3(1024), 0, stream, input, stride, columns, codes, scales);
+    hipLaunchKernelGGL((quantize_rows_kernel<Type, 1024>), grid, dim3(1024), 0, stream, input, stride, n, columns, codes, scales);
   }
 }
 
@@ -636,7 +639,9 @@ extern "C" int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float*
     }
     const uint64_t groups = static_cast<uint64_t>(s.row_tiles) * s.token_tiles * s.splits;
     const uint64_t main_groups = static_cast<uint64_t>(s.main_tiles) * ((tokens + kMainTile - 1) / kMainTile);
-    if (groups > (1u << 30) || main_groups > (1u << 30) || (s.splits > 1 && static_cast<uint64_t>(rows) * tokens > (1ull << 38))) {
+    // Of the launches' up to 512 threads a workgroup, or a thread for four sums.
+    const std::size_t quads = (rows + 3) / 4 * tokens;
+    if (groups >= (1u << 23) || main_groups >= (1u << 23) || (s.splits > 1 && quads > 0xffffff00u)) {
       return fail(GFXI_INVALID_ARGUMENT, "8-bit product: too large for one launch");
     }
     const ProductArgs a{weights, weight_scales, codes, scales, output, static_cast<int32_t*>(workspace),
@@ -665,7 +670,6 @@ extern "C" int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float*
     else if (s.tile_rows == 128) hipLaunchKernelGGL((w8a8_tile_kernel<128, 128, 2, 4, 4>), grid, dim3(512), 0, st, a, first_row, s.row_tiles, s.token_tiles);
     else hipLaunchKernelGGL((w8a8_tile_kernel<256, 128, 4, 2, 3>), grid, dim3(512), 0, st, a, first_row, s.row_tiles, s.token_tiles);
     if (const int32_t status = launch_status("8-bit product launch failed"); status != GFXI_OK || s.splits == 1) return status;
-    const std::size_t quads = (rows + 3) / 4 * tokens;
     hipLaunchKernelGGL(w8a8_join_kernel, dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(256), 0, st, a);
     return launch_status("8-bit product join launch failed");
   });
