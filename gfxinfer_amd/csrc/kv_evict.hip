@@ -173,8 +173,9 @@ __device__ __forceinline__ void select_rows(const EvictArgs& a, uint32_t listed,
   };
   // All that the choice reads is asked for before the length is there.
   fetch(0);
-  const uint32_t columns = pages_for(a.budget, pg.page_shift), page_tokens = 1u << pg.page_shift;
-  const int32_t first_page = tid < min(columns, pg.stride) ? table_page(pg, slot, tid) : -1;
+  // (A budget may be any number: no more columns than the table's are gone through.)
+  const uint32_t columns = min(pages_for(a.budget, pg.page_shift), pg.stride), page_tokens = 1u << pg.page_shift;
+  const int32_t first_page = tid < columns ? table_page(pg, slot, tid) : -1;
   const uint32_t first_holders = first_page >= 0 ? pg.references[first_page] : 0;
   const bool over = length > a.budget && i == listed;
   if (!over) {
