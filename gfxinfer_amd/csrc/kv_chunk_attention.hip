@@ -77,16 +77,24 @@ struct ChunkAttnArgs {
   ChunkList list;
   uint32_t first_tile[kMaxChunks];  // of the listed sequences' row tiles
   uint32_t tiles;
-  uint32_t whole;        // tiles and KV heads that run first and are not divided
+  uint32_t whole;        // tiles and KV heads that run first and are not divided, see partial_row
+  uint32_t tile_rows;    // most rows of a divided tile
   const __half* query;   // [rows][q_heads][D]
   const float* gate;     // [rows][q_heads][2 D] or null
   __half* output;        // [rows][q_heads][D]
   float* log_sums;       // [rows][q_heads] or null
-  float* partial_o;      // [rows][q_heads][ranges][D], where positions are divided
-  float* partial_ml;     // [rows][q_heads][ranges][2]: maximum (-inf: the row has nothing there), sum
+  float* partial_o;      // [partial rows][ranges][D], where positions are divided
+  float* partial_ml;     // [partial rows][ranges][2]: maximum (-inf: the row has nothing there), sum
   uint32_t layer, q_heads, kv_heads, group, ranges;
   float scale;           // log2(e) / sqrt(D)
 };
+
+// Where a row's parts are.  If all tiles are divided: by its place in the output, [rows][q_heads].  Otherwise by the
+// divided tile (and KV head) that it is in, [divided][tile_rows], so that they take no room for the whole ones (2048 tokens
+// of 40 x 8 x 128: 32 MB, by their place 163; 32800 tokens 4 MB, not 2.6 GB).
+__device__ __forceinline__ uint32_t partial_row(const ChunkAttnArgs& a, uint32_t item, uint32_t row_of_tile, uint32_t out_row) {
+  return a.whole == 0 ? out_row : (item - a.whole) * a.tile_rows + row_of_tile;
+}
 
 // Steps a range holds at least, if there is more than one.
 constexpr uint32_t kLeastSteps = 2;
@@ -472,12 +480,12 @@ __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& 
 }
 
 // Output tiles of a row: a range's part, or, where one range holds all positions, the row itself with
-// the gate applied.  o[i] is output tile first + i * step.
+// the gate applied.  o[i] is output tile first + i * step; joined: the join goes over the row.
 template <unsigned D, unsigned N>
-__device__ __forceinline__ void write_row(const ChunkAttnArgs& a, uint32_t out_row, uint32_t range, bool whole, const f16v* o,
-                                          unsigned first, unsigned step, float m, float l, bool sums) {
+__device__ __forceinline__ void write_row(const ChunkAttnArgs& a, uint32_t out_row, uint32_t part_row, uint32_t range, bool whole,
+                                          bool joined, const f16v* o, unsigned first, unsigned step, float m, float l, bool sums) {
   const unsigned h = (threadIdx.x & 63u) >> 5;
-  const std::size_t at = static_cast<std::size_t>(out_row) * a.ranges + range;
+  const std::size_t at = static_cast<std::size_t>(part_row) * a.ranges + range;
   if (!whole) {
 #pragma unroll
     for (unsigned i = 0; i < N; ++i) {
@@ -510,7 +518,7 @@ __device__ __forceinline__ void write_row(const ChunkAttnArgs& a, uint32_t out_r
       *reinterpret_cast<h4*>(a.output + static_cast<std::size_t>(out_row) * D + at) = out;
     }
   }
-  if (sums && a.ranges > 1) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{0.0F, kWritten};
+  if (sums && joined) *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{0.0F, kWritten};
   if (sums && a.log_sums != nullptr) a.log_sums[out_row] = empty ? -INFINITY : (m - kLift) * kLn2 + logf(l);
 }
 
@@ -542,8 +550,16 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   const KvPages& pg = a.pages;
   // KV heads vary fastest: with eight of them each XCD reads one.  Then row tiles, so that those that
   // read the same positions run together; late tokens, which see most, first.
-  const uint32_t hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  const uint32_t tiles = a.tiles, range = rest / tiles, row_tile = tiles - 1 - rest % tiles;
+  // The first range of all tiles, then the others of those that are divided.
+  const uint32_t items = a.tiles * a.kv_heads;
+  uint32_t item = blockIdx.x, range = 0;
+  if (item >= items) {
+    const uint32_t divided = items - a.whole;
+    range = 1 + (item - items) / divided;
+    item = a.whole + (item - items) % divided;
+  }
+  const uint32_t hk = item % a.kv_heads, row_tile = a.tiles - 1 - item / a.kv_heads;
+  const bool joined = a.ranges > 1 && item >= a.whole;
   PageWindow window;
   const Listed listed = find_listed<D>(a, row_tile, window);
   const uint32_t slot = listed.slot, first_row = listed.first_row, tokens = listed.tokens, length = listed.length;
@@ -552,12 +568,13 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   const uint32_t last_row = min(rows, tile_row + kRows) - 1;
   const uint32_t end = length + tokens, steps = (length + last_row / a.group + T) / T;
   // As few ranges as hold them, of equal length.
-  const uint32_t used = blockIdx.x % (tiles * a.kv_heads) < a.whole ? 1 : (steps - 1) / listed.per + 1, per = (steps + used - 1) / used;
+  const uint32_t used = joined ? (steps - 1) / listed.per + 1 : 1, per = (steps + used - 1) / used;
   const uint32_t from = range * per, to = min(from + per, steps);
   if (from >= steps) {
     const uint32_t row = tile_row + threadIdx.x;
     if (threadIdx.x < kRows && row < rows) {
-      const std::size_t at = (static_cast<std::size_t>(first_row + row / a.group) * a.q_heads + hk * a.group + row % a.group) * a.ranges + range;
+      const uint32_t out_row = (first_row + row / a.group) * a.q_heads + hk * a.group + row % a.group;
+      const std::size_t at = static_cast<std::size_t>(partial_row(a, item, threadIdx.x, out_row)) * a.ranges + range;
       *reinterpret_cast<float2*>(a.partial_ml + 2 * at) = float2{-INFINITY, 0.0F};
     }
     return;
@@ -585,7 +602,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
     // (Few rows are left to the join even if one range holds them: its waves divide the gate among more
     // lanes, eight decoding sequences 12.9 us, not 14.4.)
     attend_few<D>(a, Range{slot, end, from, to, hk, least_visible}, q, visible, lds, found, limit, window, o, m, l);
-    if (out_row != 0xffffffffu) write_row<D, D / 128>(a, out_row, range, a.ranges == 1, o, wave, 4, m, l, wave == 0 && h == 0);
+    if (out_row != 0xffffffffu) write_row<D, D / 128>(a, out_row, partial_row(a, item, n, out_row), range, !joined, joined, o, wave, 4, m, l, wave == 0 && h == 0);
     return;
   }
   const std::size_t layer_row = (static_cast<std::size_t>(a.layer) * pg.page_count << pg.page_shift) * pg.row + hk * D;
@@ -877,25 +894,43 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   m = peaks.m;
   // Only NaN scores, and strange values at scores of -infinity, make a NaN row rather than an empty one.
   if ((m == -INFINITY && (l != l || (careful && strange))) || m != m) m = 0.0F;
-  if (out_row != 0xffffffffu) write_row<D, D / 32>(a, out_row, range, used == 1, o, 0, 1, m, l, h == 0);
+  if (out_row != 0xffffffffu) write_row<D, D / 32>(a, out_row, partial_row(a, item, wave * 32 + n, out_row), range, used == 1, joined, o, 0, 1, m, l, h == 0);
 }
 
 constexpr uint32_t kJoinRows = 4096;
 
 // Joins the ranges of a row and applies the gate: a wave per row and query head, D / 64 dims a lane.
-// Lane r holds range r's maximum and sum; the outputs of the first two ranges are loaded beside them.
-template <unsigned D>
+// Lane r holds range r's maximum and sum; the outputs of the first two ranges are loaded beside them.  `rows` partial rows;
+// ByTile: those of the divided tiles.
+template <unsigned D, bool ByTile>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkAttnArgs a, uint32_t rows) {
   constexpr unsigned J = D / 64;
   using vec = float __attribute__((ext_vector_type(J)));
   using hvec = _Float16 __attribute__((ext_vector_type(J)));
   const unsigned lane = threadIdx.x & 63u;
-  const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
-  if (row >= rows) return;
-  const std::size_t base = static_cast<std::size_t>(row) * a.ranges;
+  const uint32_t part_row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
+  if (part_row >= rows) return;
+  uint32_t row = part_row;
+  if constexpr (ByTile) {
+    const uint32_t item = a.whole + part_row / a.tile_rows, row_of_tile = part_row % a.tile_rows;
+    const uint32_t row_tile = a.tiles - 1 - item / a.kv_heads, hk = item % a.kv_heads;
+    uint32_t of_sequence = 0xffffffffu, first_row = 0;  // a lane a sequence, one of which has the tile
+    for (uint32_t from = 0; from < a.list.count; from += 64) {
+      const uint32_t i = min(from + lane, a.list.count - 1), heads = (a.list.first[i + 1] - a.list.first[i]) * a.group;
+      const uint32_t here = (row_tile - a.first_tile[i]) * kRows + row_of_tile;
+      const uint64_t found = __ballot(from + lane < a.list.count && row_tile >= a.first_tile[i] && here < heads);
+      if (found == 0) continue;
+      const int at = __ffsll(static_cast<unsigned long long>(found)) - 1;
+      of_sequence = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(here), at));
+      first_row = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(a.list.first[i]), at));
+    }
+    if (of_sequence == 0xffffffffu) return;  // behind the rows of a sequence's last tile
+    row = (first_row + of_sequence / a.group) * a.q_heads + hk * a.group + of_sequence % a.group;
+  }
+  const std::size_t base = static_cast<std::size_t>(part_row) * a.ranges;
   const float* parts = a.partial_o + base * D + J * lane;
   // Many rows: complete ones are not worth the loads that cover the look.
-  if (rows > kJoinRows && __builtin_amdgcn_readfirstlane(__float_as_int(a.partial_ml[2 * base + 1])) == __float_as_int(kWritten)) return;
+  if ((ByTile || rows > kJoinRows) && __builtin_amdgcn_readfirstlane(__float_as_int(a.partial_ml[2 * base + 1])) == __float_as_int(kWritten)) return;
   vec g = {};
   if (a.gate != nullptr) g = *reinterpret_cast<const vec*>(a.gate + static_cast<std::size_t>(row) * 2 * D + D + J * lane);
   const vec first[2] = {*reinterpret_cast<const vec*>(parts), *reinterpret_cast<const vec*>(parts + D)};
@@ -1321,7 +1356,7 @@ int32_t read_heads(const gfxinfer_kv_pages* pages, uint32_t q_heads) {
 }
 
 struct ChunkShape {
-  uint32_t tiles, ranges, whole;
+  uint32_t tiles, ranges, whole, tile_rows;
 };
 
 // Row tiles, and the ranges that the longest sequence's positions are divided into: one and a half workgroups
@@ -1343,6 +1378,7 @@ ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads
     first_tile[order[e]] = s.tiles;
     s.tiles += (tokens(order[e]) * group + kRows - 1) / kRows;
   }
+  s.tile_rows = std::min(kRows, tokens(order[0]) * group);
   const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift, items = static_cast<uint64_t>(s.tiles) * kv_heads;
   const uint64_t places = (head_size == 128 ? kResident<128> : kResident<256>) * kComputeUnits;
   const uint64_t most = std::max<uint64_t>(1, capacity / ((head_size == 128 ? kTile<128> : kTile<256>) * kLeastSteps));
@@ -1356,9 +1392,15 @@ ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads
   return s;
 }
 
-std::size_t chunk_bytes(const ChunkShape& s, const ChunkList& list, uint32_t q_heads, uint32_t head_size) {
+// Rows with parts, see partial_row: at most kRows for each place.  (Below 2^18, so a launch holds a wave for each, and below
+// 2^24 workgroups for the items, of which there are at most 2^30 / kRows and one for each sequence and KV head.)
+uint32_t partial_rows(const ChunkShape& s, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads) {
   if (s.ranges == 1) return 0;
-  return static_cast<std::size_t>(list.first[kMaxChunks]) * q_heads * s.ranges * (head_size + 2) * sizeof(float);
+  return s.whole == 0 ? list.first[kMaxChunks] * q_heads : (s.tiles * kv_heads - s.whole) * s.tile_rows;
+}
+
+std::size_t chunk_bytes(const ChunkShape& s, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads, uint32_t head_size) {
+  return static_cast<std::size_t>(partial_rows(s, list, q_heads, kv_heads)) * s.ranges * (head_size + 2) * sizeof(float);
 }
 
 // How the rows of the long chunks are divided: workgroups along the positions, and parts of the rows.
@@ -1408,7 +1450,8 @@ extern "C" size_t gfxinfer_kv_pages_chunk_attention_workspace_bytes(const gfxinf
     // The slots do not matter here: every entry names the first one.
     const std::vector<uint32_t> any(std::min(count, kMaxChunks + 1), 0u);
     if (const int32_t s = read_chunks(a.pages, any.data(), tokens, count, false, a.list); s != GFXI_OK) return s;
-    bytes = chunk_bytes(chunk_shape(a.pages, a.list, q_heads, pages->kv_heads, pages->head_size, a.first_tile), a.list, q_heads, pages->head_size);
+    const ChunkShape shape = chunk_shape(a.pages, a.list, q_heads, pages->kv_heads, pages->head_size, a.first_tile);
+    bytes = chunk_bytes(shape, a.list, q_heads, pages->kv_heads, pages->head_size);
     return GFXI_OK;
   });
   return bytes;
@@ -1431,20 +1474,18 @@ extern "C" int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pa
     }
     const uint32_t head_size = pages->head_size, kv_heads = pages->kv_heads;
     const ChunkShape shape = chunk_shape(a.pages, a.list, q_heads, kv_heads, head_size, a.first_tile);
-    const std::size_t need = chunk_bytes(shape, a.list, q_heads, head_size);
+    const std::size_t need = chunk_bytes(shape, a.list, q_heads, kv_heads, head_size);
     if (need != 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need)) {
       return fail(GFXI_INVALID_ARGUMENT, "chunk attention workspace is null, not 16-byte aligned or too small");
     }
-    const uint64_t items = static_cast<uint64_t>(shape.tiles) * shape.ranges * kv_heads;
-    const std::size_t rows = static_cast<std::size_t>(a.list.first[kMaxChunks]) * q_heads;
-    if (items > (1u << 30)) return fail(GFXI_INVALID_ARGUMENT, "chunk attention over too many rows for one launch");
+    const uint32_t items = shape.tiles * kv_heads, rows = partial_rows(shape, a.list, q_heads, kv_heads);
     a.query = reinterpret_cast<const __half*>(query);
     a.gate = gate;
     a.output = reinterpret_cast<__half*>(output);
     a.log_sums = log_sums;
     if (need != 0) {
       a.partial_o = workspace;
-      a.partial_ml = a.partial_o + rows * shape.ranges * head_size;
+      a.partial_ml = a.partial_o + static_cast<std::size_t>(rows) * shape.ranges * head_size;
     }
     a.layer = layer;
     a.q_heads = q_heads;
@@ -1453,14 +1494,20 @@ extern "C" int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pa
     a.ranges = shape.ranges;
     a.tiles = shape.tiles;
     a.whole = shape.whole;
+    a.tile_rows = shape.tile_rows;
     a.scale = kLog2E / std::sqrt(static_cast<float>(head_size));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid(static_cast<unsigned>(items)), block(kWaves * 64), join(static_cast<unsigned>((rows + 3) / 4));
+    const dim3 grid(items + (items - shape.whole) * (shape.ranges - 1)), block(kWaves * 64), join((rows + 3) / 4);
     if (head_size == 128) hipLaunchKernelGGL(chunk_attention_kernel<128>, grid, block, 0, st, a);
     else hipLaunchKernelGGL(chunk_attention_kernel<256>, grid, block, 0, st, a);
     if (const int32_t s = launch_status("chunk attention launch failed"); s != GFXI_OK || a.ranges == 1) return s;
-    if (head_size == 128) hipLaunchKernelGGL(chunk_join_kernel<128>, join, dim3(256), 0, st, a, static_cast<uint32_t>(rows));
-    else hipLaunchKernelGGL(chunk_join_kernel<256>, join, dim3(256), 0, st, a, static_cast<uint32_t>(rows));
+    if (shape.whole == 0) {
+      if (head_size == 128) hipLaunchKernelGGL((chunk_join_kernel<128, false>), join, dim3(256), 0, st, a, rows);
+      else hipLaunchKernelGGL((chunk_join_kernel<256, false>), join, dim3(256), 0, st, a, rows);
+    } else {
+      if (head_size == 128) hipLaunchKernelGGL((chunk_join_kernel<128, true>), join, dim3(256), 0, st, a, rows);
+      else hipLaunchKernelGGL((chunk_join_kernel<256, true>), join, dim3(256), 0, st, a, rows);
+    }
     return launch_status("chunk attention join launch failed");
   });
 }

@@ -734,7 +734,9 @@ int32_t gfxinfer_launch_kv_pages_gated_attention(const gfxinfer_kv_pages* pages,
  * token.  A call lists at most 256 sequences and has at most 2^20 rows. */
 
 /* Bytes of device workspace (16-byte aligned) of gfxinfer_launch_kv_pages_chunk_attention; 0
- * where it needs none and for invalid arguments.  Calls that may run at once need one each. */
+ * where it needs none and for invalid arguments.  Calls that may run at once need one each.
+ * More tokens may need less (what fills the GPU is not divided), so a workspace for several
+ * calls takes the most that any of them needs; no call needs more than 104 MB. */
 size_t gfxinfer_kv_pages_chunk_attention_workspace_bytes(const gfxinfer_kv_pages* pages, const uint32_t* tokens,
                                                          uint32_t count, uint32_t q_heads);
 
