@@ -100,7 +100,7 @@ __device__ __forceinline__ uint32_t partial_row(const ChunkAttnArgs& a, uint32_t
 constexpr uint32_t kLeastSteps = 2;
 
 // The listed sequence of a row tile, and the steps of a range: ranges are of equal length for all
-// sequences, the longest one is divided into as many as the launch allows and the others into as few
+// sequences, the longest one with new tokens is divided into as many as the launch allows and the others into as few
 // as hold them.  The list and the lengths take one round of loads each, a lane a sequence; the first pages of the
 // sequence's table come beside its length.
 struct Listed {
@@ -121,7 +121,7 @@ __device__ __forceinline__ Listed find_listed(const ChunkAttnArgs& a, uint32_t r
     auto take = [&](uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), at)); };
     if (here != 0) window.start(a.pages, take(slot), 0);
     const uint32_t length = min(committed, a.pages.stride << a.pages.page_shift);
-    most = max(most, length + tokens);
+    most = max(most, tokens != 0 ? length + tokens : 0);
     if (here != 0) found = Listed{take(slot), take(length), take(row), take(tokens), take(tile), 0};
   }
 #pragma unroll

@@ -752,7 +752,7 @@ size_t gfxinfer_kv_pages_chunk_attention_workspace_bytes(const gfxinfer_kv_pages
  * The weights beside a row's largest (up to 15 of them, within 2 nats) together lose at most
  * 2^-7 of their sum, 2^-10 where their scores spread by up to 3 nats.  Sums are fp32.
  * Where a row's positions are cut for different workgroups, and so the order of its fp32
- * additions, depends on the token counts and lengths of all listed sequences: equal calls give
+ * additions, depends on the token counts and lengths of all sequences listed with tokens: equal calls give
  * equal bits, a row beside other sequences may differ in the last ones. */
 int32_t gfxinfer_launch_kv_pages_chunk_attention(const gfxinfer_kv_pages* pages, uint32_t layer, const uint16_t* query,
                                                  const float* gate, uint16_t* output, float* log_sums,

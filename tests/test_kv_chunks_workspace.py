@@ -49,3 +49,19 @@ def test_parts_of_the_rest_stay_in_the_workspace(device, gx, heads, page, length
         which = [i for i in range(len(tokens)) if tokens[i]]
         c.check(host(out), host(sums), which if len(which) < 10 else which[::9] + which[-1:])
         assert bool((work[size:] == 0xff).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(40, 8, 128), (24, 4, 256)])
+def test_sequences_without_tokens_change_nothing(device, gx, heads):
+    """A long one listed with no new tokens: the others are divided as without it, so their results have the same bits."""
+    from gpu_util import say
+    from test_kv_chunks_gpu import Chunks
+    say("idle sequences", heads)
+    c = Chunks(np.random.default_rng(6), heads, 64, [600, 1100, 9000, 200], [1, 3, 0, 1])
+    with_it = c.run(gx)
+    c.check(*with_it, [0, 1, 3])
+    c.tokens = [1, 3, 1]
+    without = c.run(gx, listed=[0, 1, 3])
+    for a, b in zip(with_it, without):
+        assert np.array_equal(a, b)
