@@ -1363,6 +1363,8 @@ struct ChunkShape {
 // for each place (two at head size 256), as far as full tables hold so many.  Where there are tiles for all places, those that
 // make whole rounds are not divided, and the rest only as far as it fills one more round: parts cost a trip through memory
 // (2048 tokens on 30000 in 640 tiles: 1369 us, all of them in two ranges 1412; 3000 on 8000 at head size 256: 912, undivided 1096).
+// Not so if sequences decode, each tile of as many positions as its sequence has and few rows' parts: 64 on 200 .. 4090 128 us,
+// undivided 139, of 400 .. 600 beside one of 30000 225 and 387, without that one 37 and 31.
 constexpr uint64_t kMostOfRest = 4;
 ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads, uint32_t kv_heads, uint32_t head_size,
                        uint32_t* first_tile) {
@@ -1382,7 +1384,7 @@ ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads
   const uint64_t capacity = static_cast<uint64_t>(p.stride) << p.page_shift, items = static_cast<uint64_t>(s.tiles) * kv_heads;
   const uint64_t places = (head_size == 128 ? kResident<128> : kResident<256>) * kComputeUnits;
   const uint64_t most = std::max<uint64_t>(1, capacity / ((head_size == 128 ? kTile<128> : kTile<256>) * kLeastSteps));
-  if (items < places) {
+  if (items < places || s.tile_rows <= 32) {
     s.ranges = static_cast<uint32_t>(std::clamp<uint64_t>((places * (head_size == 128 ? 3 : 4) / 2 + items - 1) / items, 1, most));
   } else {
     s.whole = static_cast<uint32_t>(items / places * places);

@@ -65,3 +65,12 @@ def test_sequences_without_tokens_change_nothing(device, gx, heads):
     without = c.run(gx, listed=[0, 1, 3])
     for a, b in zip(with_it, without):
         assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("heads,count", [((40, 8, 128), 64), ((40, 8, 128), 95), ((24, 4, 256), 64), ((24, 4, 256), 100)])
+def test_decoding_sequences_are_divided(gx, cache, heads, count):  # noqa: F811
+    """One more workgroup a place is worth it where lengths differ: a long sequence among 64 was a single range."""
+    q_heads, cache.kv_heads, cache.head_size = heads
+    cache.page_tokens, cache.table_stride, cache.sequences = 64, 1024, 256
+    size = gx.kv_pages_chunk_attention_workspace_bytes(cache, [1] * count, q_heads)
+    assert size >= 2 * count * q_heads * (heads[2] + 2) * 4
