@@ -6,7 +6,7 @@
 // The rows of a sequence and KV head are one tall matrix, in tiles of 128: a workgroup takes a tile
 // and a range of positions, each of its four waves 32 of the rows, and a K / V row staged in LDS
 // serves them all.  A second launch joins the ranges of a tile.  (Equal shares of all work, one a
-// workgroup and cut anywhere, were slower: 2048 tokens on 30000 1630 us, not 1403.  Workgroups that
+// workgroup and cut anywhere, took 16 % longer: 2048 tokens on 30000.  Workgroups that
 // go over the same positions of a head at the same time read them through one L2, those shares
 // did not.)
 //
@@ -20,10 +20,10 @@
 // the exponentials alone take a wave's vector unit nearly as long as both products take the
 // matrix unit.
 //
-// 2048 tokens on 30000, 40 x 8 x 128: 1369 us, 950 TFLOP/s (a large fp16 product: 1.28 PFLOP/s); the matrix units
-// are busy 48 % of the time, waits take 23 % of the waves'.  24 x 4 x 256: 1842 us, 848 TFLOP/s: the outputs of 32 rows
-// leave room for one wave a SIMD, and nothing covers its waits.  31 sequences that decode on 200 .. 4090 and a chunk of
-// 509: 77 us, 3.7 TB/s.  Eight that decode on up to 600: 13.4 us, two launches of dependent reads.
+// 2048 tokens on 30000, 40 x 8 x 128: 1355 us, 960 TFLOP/s (a large fp16 product: 1.28 PFLOP/s; other cards up to 1445 us); the
+// matrix units are busy 48 % of the time, waits take 23 % of the waves'.  24 x 4 x 256: 1850 to 1910 us, 830 TFLOP/s: the outputs of
+// 32 rows leave room for one wave a SIMD, and nothing covers its waits.  31 sequences that decode on 200 .. 4090 and a chunk
+// of 509: 78 us, 3.6 TB/s.  Eight that decode on up to 600: 14.7 us, two launches of dependent reads.
 #include <algorithm>
 #include <array>
 #include <cmath>
@@ -54,8 +54,8 @@ constexpr unsigned kResident = D == 128 ? 2 : 1;
 
 // A row's weights are 2^(score - m + kLift), scores in units of log2.  m is a maximum of the row so far that moves up
 // once it is passed by kRise, so weights stay below 2^15.  Tiles of more than 32 rows carry a weight as one fp16
-// number: 11 bits, half the size of the output's own rounding, where a second product for 22 bits would take half
-// as much again of the matrix units' time.  Tiles of at most 32 rows wait for memory and carry pairs.
+// number: 11 bits, half the size of the output's own rounding.  A second product for 22 bits takes 40 % longer (2048 tokens on
+// 30000 2025 us, on the same card 1445).  Tiles of at most 32 rows wait for memory and carry pairs.
 //
 // fp16 rounds weights below 2^kSmall by 2^-25 and drops those below that.  Beside peaks whose values are near zero they
 // may be all that carries the output (26 nats below a peak, 42 % of 4096 of them was lost).  So a row is open until
@@ -600,7 +600,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   if (few) {
     _Float16* lds[kWaves] = {k0, k1, v0, v1};
     // (Few rows are left to the join even if one range holds them: its waves divide the gate among more
-    // lanes, eight decoding sequences 12.9 us, not 14.4.)
+    // lanes, eight decoding sequences a tenth less.)
     attend_few<D>(a, Range{slot, end, from, to, hk, least_visible}, q, visible, lds, found, limit, window, o, m, l);
     if (out_row != 0xffffffffu) write_row<D, D / 128>(a, out_row, partial_row(a, item, n, out_row), range, !joined, joined, o, wave, 4, m, l, wave == 0 && h == 0);
     return;
@@ -701,7 +701,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   };
   // The outputs and queries belong into the accumulation registers: left to itself the compiler counts them
   // among the others and reads every operand right before its product (4 prompts of 300 on 1500..6000:
-  // 226 us, not 211), or moves all of them there and back where maxima might move (204, not 182).
+  // 7 % more), or moves all of them there and back where maxima might move (12 % more).
   auto keep_outputs = [&]() __attribute__((always_inline)) {
     if constexpr (D == 256) {
 #pragma unroll
@@ -1042,7 +1042,7 @@ __global__ __launch_bounds__(256) void few_weight_kernel(WeightArgs a) {
   float* weights = a.weights.weight + static_cast<std::size_t>(slot) * capacity;
   const uint32_t length = committed(pg, slot), end = min(length + tokens, capacity);
   // (Pages and weights are not asked for before the length is there: half of the workgroups have no
-  // positions, 19.9 us, not 18.6.)
+  // positions, 7 % more.)
   for (uint32_t at = blockIdx.x * 32; at < end; at += gridDim.x * 32) {
     const int32_t page = table_page(pg, slot, (at + n) >> pg.page_shift);
     const bool there = at + n < end && page >= 0;
@@ -1362,7 +1362,8 @@ struct ChunkShape {
 // Row tiles, and the ranges that the longest sequence's positions are divided into: one and a half workgroups
 // for each place (two at head size 256), as far as full tables hold so many.  Where there are tiles for all places, those that
 // make whole rounds are not divided, and the rest only as far as it fills one more round: parts cost a trip through memory
-// (2048 tokens on 30000 in 640 tiles: 1369 us, all of them in two ranges 1412; 3000 on 8000 at head size 256: 912, undivided 1096).
+// (2048 tokens on 30000 in 640 tiles: all of them in two ranges take 3 % longer; 3000 on 8000 at head size 256: 919 us, undivided 20 %
+// longer).
 // Not so if sequences decode, each tile of as many positions as its sequence has and few rows' parts: 64 on 200 .. 4090 128 us,
 // undivided 139, of 400 .. 600 beside one of 30000 225 and 387, without that one 37 and 31.
 constexpr uint64_t kMostOfRest = 4;
@@ -1371,7 +1372,7 @@ ChunkShape chunk_shape(const KvPages& p, const ChunkList& list, uint32_t q_heads
   ChunkShape s{};
   const uint32_t group = q_heads / kv_heads;
   // Tiles run from the last to the first: sequences with few new tokens get the last ones.  (31 that decode and a
-  // chunk behind them in the list: 88 us, in the list's order, with the chunk's tiles first, 93.)
+  // chunk behind them in the list: in the list's order, with the chunk's tiles first, 6 % longer.)
   std::array<uint16_t, kMaxChunks> order;
   std::iota(order.begin(), order.begin() + list.count, uint16_t{0});
   auto tokens = [&](uint32_t i) { return list.first[i + 1] - list.first[i]; };

@@ -418,8 +418,9 @@ __global__ __launch_bounds__(kGrantThreads) void grant_kernel(EvictArgs a) {
   grant_pages(a, lds);
 }
 
-// Both for up to four sequences whose tables hold at most 1024 rows, a launch less, which is the host's time (four
-// sequences, a row each, with all calls of the step: 31.2 us, not 36.0; replayed from a graph 23.2 and 21.8).
+// Both for up to four sequences whose tables hold at most 1024 rows, a launch less, which is the host's time: four
+// sequences, a row each, with all calls of the step take 32.7 us, not 36.4.  On the GPU it is the slower one, 10.7 us for 6.8 and
+// 2.0: replayed from a graph the step takes 27.2 us, not 25.9.
 
 __global__ __launch_bounds__(kGrantThreads) void select_grant_kernel(EvictArgs a) {
   __shared__ SelectShared<kSmallThreads> chosen[kSmallSequences];
@@ -607,7 +608,7 @@ extern "C" int32_t gfxinfer_launch_kv_pages_evict(const gfxinfer_kv_pages* pages
     a.status = status;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     // A wave's instructions are what the choice takes its time with, and sixteen waves share a CU's four vector
-    // units: tables of few rows take four (501 rows: 8.5 us, with sixteen 11.1).
+    // units: tables of few rows take four (501 rows: three quarters of the time with sixteen).
     const bool small = capacity_of(a.pages) <= kSmallThreads * kSelectKeys;
     if (small && count <= kSmallSequences) {
       hipLaunchKernelGGL(select_grant_kernel, dim3(1), dim3(kGrantThreads), 0, st, a);

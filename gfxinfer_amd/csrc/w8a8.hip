@@ -225,7 +225,7 @@ __device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0
 // Few tokens: the weights are streamed once.  A workgroup holds 16 R channels and 16 T tokens; its
 // waves divide K, each with a ring of Depth stages of 128 bytes in LDS for itself, and add their sums
 // at the end.  Loads cover whole lines of memory, eight rows of 128 bytes each: straight into the
-// registers of an operand they would be sixteen rows of 64 (17408 x 5120, one token: 27 us, not 21).
+// registers of an operand they would be sixteen rows of 64 (17408 x 5120, one token: 29 % longer).
 // Piece c of row r lies in slot c ^ (r / 2 % 8), see below.
 template <unsigned T, unsigned R, unsigned Waves, unsigned Depth>
 __global__ __launch_bounds__(Waves * 64) void w8a8_few_kernel(ProductArgs a) {
@@ -544,8 +544,8 @@ ProductShape best_shape(std::size_t rows, std::size_t columns, std::size_t token
 
 // Tiles of 256 x 256 take the least time for their size, but a last round of few of them takes as long as a full
 // one, and so does a tile with few tokens.  So where they pad the tokens no further than tiles of 128 would, they take the channels
-// that make whole rounds, and the others follow in the shape that is best for them.  17408 x 5120 with 4096 tokens: 419 us, in one
-// launch of 256 x 128 457; 34816 x 5120 with 509 tokens 120, not 151; 5120 x 5120 with 8192 tokens 234, not 247.  With more
+// that make whole rounds, and the others follow in the shape that is best for them.  17408 x 5120 with 4096 tokens: 393 us, in one
+// launch of 256 x 128 9 % more; 34816 x 5120 with 509 tokens 120, not 151; 5120 x 5120 with 8192 tokens 234, not 247.  With more
 // padding (34816 x 5120 and 300 tokens) it took 111 us and one launch 97; where more than half a round is left it is about even
 // (27392 x 5120 with 1024 tokens 199 and 203, 34816 x 5120 with 768 200 and 186).
 ProductShape product_shape(std::size_t rows, std::size_t columns, std::size_t tokens) {

@@ -731,7 +731,8 @@ int32_t gfxinfer_launch_kv_pages_gated_attention(const gfxinfer_kv_pages* pages,
  *     reserve, begin; per layer: append, chunk_attention, weights_add; advance, evict
  * Every listed sequence brings its own number of new tokens (host list; 0 is allowed, a call
  * has at least one), and their rows are packed: sequence by sequence in list order, token by
- * token.  A call lists at most 256 sequences and has at most 2^20 rows. */
+ * token.  A call with token counts lists at most 256 sequences and has at most 2^20 rows;
+ * eviction, which has none, lists at most 512. */
 
 /* Bytes of device workspace (16-byte aligned) of gfxinfer_launch_kv_pages_chunk_attention; 0
  * where it needs none and for invalid arguments.  Calls that may run at once need one each.
@@ -830,7 +831,8 @@ size_t gfxinfer_w8a8_gemm_workspace_bytes(size_t rows, size_t columns, size_t to
 
 /* weights int8 [rows][columns], weight_scales fp32 [rows], codes int8 [tokens][columns], scales
  * fp32 [tokens] -> output [tokens][rows], GFXI_F32 or GFXI_F16 (rounded once from fp32).  Codes
- * and output 16-byte aligned; columns a multiple of 16 below 2^17, rows and tokens 1..2^24. */
+ * and output 16-byte aligned; columns a multiple of 16 below 2^17, rows and tokens 1..2^24 (with
+ * both so large that a launch does not hold the tiles the call is refused). */
 int32_t gfxinfer_launch_w8a8_gemm(const int8_t* weights, const float* weight_scales, const int8_t* codes,
                                   const float* scales, void* output, int32_t output_type, size_t rows, size_t columns,
                                   size_t tokens, void* workspace, size_t workspace_bytes, void* stream);
