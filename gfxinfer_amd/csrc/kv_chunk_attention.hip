@@ -142,20 +142,26 @@ __device__ __forceinline__ float sum_over_halves(float v) {
   return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
-// A row's maximum, and whether its small weights may matter.  What is seldom needed lies in LDS: registers, scalar ones
-// too, are all taken.
+// What a row has found of weights beside its peaks.
+struct Found {
+  float others;  // the sum of weights below 2^kPeak as far as it was looked for
+  float small;   // 1: small weights were met on the way
+};
+__device__ __forceinline__ Found& found_at(Found& found) { return found; }
+__device__ __forceinline__ Found& found_at(Found* found) { return *found; }
+
+// A row's maximum, and whether its small weights may matter.  Place: Found, or Found* in LDS where registers, scalar ones
+// too, are all taken.  (The compiler lets a read of LDS wait for all loads into LDS that are on their way: where few rows wait
+// for them anyway it cost a tenth of the time.)
+template <typename Place>
 struct Peaks {
-  struct Found {
-    float others;  // the sum of weights below 2^kPeak as far as it was looked for
-    float small;   // 1: small weights were met on the way
-  };
   float m;
-  Found* found;
+  Place found;
   bool looks;  // a row of the wave looks for more
 
   __device__ __forceinline__ void clear() {
     m = -INFINITY;
-    *found = Found{0.0F, 0.0F};
+    found_at(found) = Found{0.0F, 0.0F};
     looks = false;
   }
   __device__ __forceinline__ bool moves(float top) const { return __any(!(top <= m + kRise)) || looks; }
@@ -172,7 +178,7 @@ struct Peaks {
     // From nothing to something: there is nothing to scale yet.
     const float factor = next == m || m == -INFINITY ? 1.0F : rescale_factor(m, next);
     if constexpr (Look) {
-      Found now = *found;
+      Found now = found_at(found);
       const float all = sum_over_halves(before) * factor;
       // After a rise by so much none of the weights so far is a peak.
       now.others = m != -INFINITY && next - m >= kLift + kRise - kPeak ? all : now.others * factor;
@@ -191,14 +197,14 @@ struct Peaks {
         if (small) now.small = 1.0F;
         looks = !__all(has(kAmple, now.others, all, positions));
       }
-      *found = now;
+      found_at(found) = now;
     }
     m = next;
     return factor;
   }
   // Rows that do not have enough where small weights were met, a bit a lane.
-  __device__ __forceinline__ uint64_t open(float all, uint32_t positions) const {
-    const Found now = *found;
+  __device__ __forceinline__ uint64_t open(float all, uint32_t positions) {
+    const Found now = found_at(found);
     const uint64_t small = __ballot(now.small != 0.0F);
     return (small | small >> 32 | small << 32) & ~__ballot(has(1.0F, now.others, sum_over_halves(all), positions));
   }
@@ -261,7 +267,7 @@ __device__ __forceinline__ void read_tiles(unsigned place, unsigned first, h8 (&
 // maxima and sums.
 template <unsigned D>
 __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& w, const h8 (&q)[D / 16], uint32_t visible,
-                                           _Float16* (&lds)[kWaves], Peaks::Found* found, const Limits& limit, PageWindow& window, f16v (&o)[D / 32], float& m, float& l) {
+                                           _Float16* (&lds)[kWaves], const Limits& limit, PageWindow& window, f16v (&o)[D / 32], float& m, float& l) {
   constexpr unsigned kBlock = 32, kLoadRows = 512 / D, kLoads = kBlock / kLoadRows;
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned n = lane & 31u, h = lane >> 5;
@@ -295,7 +301,7 @@ __device__ __forceinline__ void attend_few(const ChunkAttnArgs& a, const Range& 
                                                static_cast<int>((row0 & 15u) * row_bytes), 0, 0);
     }
   };
-  Peaks row{-INFINITY, found + 64 * wave + lane, false};
+  Peaks<Found> row{-INFINITY, Found{0.0F, 0.0F}, false};
   // A weight is high + low, both rounded to nearest: off by 2^-23 of itself, or by 2^-25 if that is more.
   auto rest_of = [](float x, _Float16 high) __attribute__((always_inline)) { return static_cast<_Float16>(x - static_cast<float>(high)); };
   // What a row sees of the wave's blocks: whole ones, and one in part.
@@ -540,7 +546,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   __shared__ __align__(1024) _Float16 k1[kPart];
   __shared__ __align__(1024) _Float16 v0[kPart];
   __shared__ __align__(1024) _Float16 v1[kPart];
-  __shared__ Peaks::Found found[kWaves * 64];
+  __shared__ Found found[kWaves * 64];
   __shared__ float2 taken_scores[kWaves * 64];
   __shared__ uint32_t again[kWaves];       // the wave's rows met an infinity or NaN
   __shared__ uint32_t strange_tiles[32];   // bit x % 1024: a tile x holds infinities or NaNs among its values
@@ -601,7 +607,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
     _Float16* lds[kWaves] = {k0, k1, v0, v1};
     // (Few rows are left to the join even if one range holds them: its waves divide the gate among more
     // lanes, eight decoding sequences a tenth less.)
-    attend_few<D>(a, Range{slot, end, from, to, hk, least_visible}, q, visible, lds, found, limit, window, o, m, l);
+    attend_few<D>(a, Range{slot, end, from, to, hk, least_visible}, q, visible, lds, limit, window, o, m, l);
     if (out_row != 0xffffffffu) write_row<D, D / 128>(a, out_row, partial_row(a, item, n, out_row), range, !joined, joined, o, wave, 4, m, l, wave == 0 && h == 0);
     return;
   }
@@ -610,7 +616,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident<D>) void chunk_attention_ker
   const __half* values = pg.value + layer_row;
   const uint32_t in_page = (1u << pg.page_shift) - 1;
   f16v s[kSub], s_next[kSub];
-  Peaks peaks{-INFINITY, found + threadIdx.x, false};
+  Peaks<Found*> peaks{-INFINITY, found + threadIdx.x, false};
   auto find_pages = [&](uint32_t x) __attribute__((always_inline)) {
     TilePages<D> p;
     p.missing = 0;
