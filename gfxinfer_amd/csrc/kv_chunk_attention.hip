@@ -151,8 +151,8 @@ __device__ __forceinline__ Found& found_at(Found& found) { return found; }
 __device__ __forceinline__ Found& found_at(Found* found) { return *found; }
 
 // A row's maximum, and whether its small weights may matter.  Place: Found, or Found* in LDS where registers, scalar ones
-// too, are all taken.  (The compiler lets a read of LDS wait for all loads into LDS that are on their way: where few rows wait
-// for them anyway it cost a tenth of the time.)
+// too, are all taken.  (The compiler lets a read of LDS wait for all loads into LDS that are on their way: it takes
+// tiles of few rows 1 to 3 % of their time.)
 template <typename Place>
 struct Peaks {
   float m;
